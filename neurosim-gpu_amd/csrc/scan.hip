@@ -1,0 +1,388 @@
+// Selective state space scan (gfx950): forward over whole signals, and one tick.
+//
+//   dt = softplus(delta + bias);  h[t] = exp(dt A) h[t-1] + dt x B[t]
+//   y[t] = (sum_s C[t] h[t] + D x) silu(z)
+//
+// Per (tick, channel, state) one exp2, three multiplies or adds of the update and one of
+// the sum, against 8 bytes (bf16) per (tick, channel): the vector ALU bounds it, at 16
+// states by about two to one over HBM.
+//
+// Few columns and channels leave most of the card idle, so time is then cut into chunks
+// scanned side by side: a first pass gives every chunk's end state from zero and its
+// summed time step, whose exponential is the chunk's decay exp(A sum dt); the chunks are
+// joined in order; a second pass runs them from their true start.  It costs the update
+// twice, so it is taken only where workgroups are few (ns_scan_chunks).
+#include "ns_scan.h"
+
+namespace ns {
+
+// What a thread keeps of its (tick, channel) items from the elementwise work to the output.
+template <int kItems>
+struct ScanItems {
+  float skip[kItems], gate[kItems];
+};
+
+template <class T, int kItems>
+struct ScanRaw {
+  T x[kItems], delta[kItems], z[kItems];
+};
+
+// Requests a tile's inputs: thread (wavefront w, lane l) takes ticks w, w+4, ... of channel l.
+template <class T, int kItems, bool kEnds>
+__device__ __forceinline__ void request(const ScanIn<T>& in, const ScanPlace& p, int64_t t,
+                                        int64_t end, ScanRaw<T, kItems>& raw) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int i = 0; i < kItems; ++i) {
+    const int64_t tick = t + wave + 4 * i;
+    raw.x[i] = raw.delta[i] = raw.z[i] = static_cast<T>(0.0f);
+    if (tick < end && lane < p.own) {
+      raw.x[i] = in.x.row(tick, p.b)[p.n0 + lane];
+      raw.delta[i] = in.delta.row(tick, p.b)[p.n0 + lane];
+      if (!kEnds && in.z.data) raw.z[i] = in.z.row(tick, p.b)[p.n0 + lane];
+    }
+  }
+}
+
+// kEnds: the first pass of a chunked scan, which keeps only end states and summed steps.
+template <class T, int R, bool kEnds>
+__global__ __launch_bounds__(kThreads) void scan_forward(ScanShape s, ScanIn<T> in, Signal<T> y,
+                                                         const float* start, float* out_state,
+                                                         float* checkpoints, float* ends,
+                                                         float* steps) {
+  constexpr int CT = kTile<R>, kItems = CT / 4;
+  __shared__ float2 step_of[CT][kScanChannels];          // dt, dt * x
+  __shared__ float write[CT][4 * R], read[CT][4 * R];
+  __shared__ float sums[CT][kScanChannels];
+  const ScanPlace p = scan_place(s);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int q = threadIdx.x & 3, channel = threadIdx.x >> 2;
+  const bool own = channel < p.own;
+  const int64_t n = p.n0 + (own ? channel : 0), line = p.b * s.channels + n;
+  const int64_t length = column_ticks(in.lengths, p.b, s.ticks);
+  const int64_t end = length < p.t1 ? length : p.t1;
+
+  float rate[R], h[R];
+  lane_row<R>(in.rates, n, q, s.states, own, rate);
+#pragma unroll
+  for (int r = 0; r < R; ++r) rate[r] *= kLog2e;
+  if (kEnds) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) h[r] = 0.0f;
+  } else if (p.c > 0) {
+    load_lane<R>(ends + (p.c * s.batch * s.channels + line) * (4 * R) + q * R, h);
+  } else {
+    lane_row<R>(start, line, q, s.states, own, h);
+  }
+  const float bias = in.delta_bias && lane < p.own ? in.delta_bias[p.n0 + lane] : 0.0f;
+  const float skip = in.skip && lane < p.own ? in.skip[p.n0 + lane] : 0.0f;
+  float total = 0.0f;
+
+  ScanRaw<T, kItems> raw;
+  request<T, kItems, kEnds>(in, p, p.t0, end, raw);
+  for (int64_t t = p.t0; t < p.t1; t += CT) {
+    if (!kEnds && checkpoints && own) {
+      const int64_t tile = t / CT;
+      store_lane<R>(checkpoints + (tile * s.batch * s.channels + line) * (4 * R) + q * R, h);
+    }
+    ScanItems<kItems> items;
+    if (t < end) {
+#pragma unroll
+      for (int i = 0; i < kItems; ++i) {
+        const int tick = wave + 4 * i;
+        const float x = static_cast<float>(raw.x[i]);
+        float dt = time_step(static_cast<float>(raw.delta[i]) + bias, s.softplus);
+        dt = t + tick < end && lane < p.own ? dt : 0.0f;
+        step_of[tick][lane] = make_float2(dt, dt * x);
+        if (!kEnds) {
+          const float z = static_cast<float>(raw.z[i]);
+          items.skip[i] = skip * x;
+          items.gate[i] = in.z.data ? z * sigmoid(z) : 1.0f;
+        }
+      }
+      stage_shared<T, R, CT>(in.write, s, p, t, end, write);
+      if (!kEnds) stage_shared<T, R, CT>(in.read, s, p, t, end, read);
+      request<T, kItems, kEnds>(in, p, t + CT, end, raw);
+      __syncthreads();
+#pragma unroll
+      for (int tick = 0; tick < CT; ++tick) {
+        const float2 d = step_of[tick][channel];
+        float sum = 0.0f;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const float decay = __builtin_amdgcn_exp2f(d.x * rate[r]);
+          h[r] = fmaf(decay, h[r], d.y * write[tick][q * R + r]);
+          if (!kEnds) sum = fmaf(read[tick][q * R + r], h[r], sum);
+        }
+        if (kEnds) total += d.x;
+        else sums[tick][channel] = quad_sum(sum);
+      }
+      __syncthreads();
+    }
+    if (!kEnds) {
+#pragma unroll
+      for (int i = 0; i < kItems; ++i) {
+        const int tick = wave + 4 * i;
+        if (t + tick < p.t1 && lane < p.own)
+          y.row(t + tick, p.b)[p.n0 + lane] = static_cast<T>(
+              t + tick < end ? (sums[tick][lane] + items.skip[i]) * items.gate[i] : 0.0f);
+      }
+    }
+  }
+  if (kEnds) {
+    if (own) {
+      store_lane<R>(ends + (p.c * s.batch * s.channels + line) * (4 * R) + q * R, h);
+      if (q == 0) steps[p.c * s.batch * s.channels + line] = total;
+    }
+  } else if (p.c == s.chunks - 1 && own && out_state) {
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (q * R + r < s.states) out_state[line * s.states + q * R + r] = h[r];
+  }
+}
+
+// One lane per (column, channel, padded state): walks the chunks in order, leaving in
+// place of each chunk's own end the state (or adjoint) it starts from.
+__global__ __launch_bounds__(kThreads) void join_kernel(ScanShape s, int64_t padded,
+                                                        const float* rates, const float* start,
+                                                        float* ends, const float* steps,
+                                                        bool reverse) {
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  const int64_t lines = s.batch * s.channels;
+  if (id >= lines * padded) return;
+  const int64_t line = id / padded, state = id - line * padded;
+  const bool real = state < s.states;
+  const float rate = real ? rates[line % s.channels * s.states + state] * kLog2e : 0.0f;
+  float carry = real && start ? start[line * s.states + state] : 0.0f;
+  constexpr int kAhead = 8;
+  for (int64_t first = 0; first < s.chunks; first += kAhead) {
+    float own[kAhead], step[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (first + u < s.chunks) {
+        const int64_t c = reverse ? s.chunks - 1 - first - u : first + u;
+        own[u] = ends[(c * lines + line) * padded + state];
+        step[u] = steps[c * lines + line];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (first + u < s.chunks) {
+        const int64_t c = reverse ? s.chunks - 1 - first - u : first + u;
+        ends[(c * lines + line) * padded + state] = carry;
+        carry = fmaf(__builtin_amdgcn_exp2f(step[u] * rate), carry, own[u]);
+      }
+    }
+  }
+}
+
+// One tick, the states updated in place.  Bound by the states' bytes, each read and
+// written once; a channel's four lanes read neighbouring floats.
+template <class T, int R>
+__global__ __launch_bounds__(kThreads) void scan_step(ScanShape s, ScanIn<T> in, Signal<T> y,
+                                                      float* state) {
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  const int64_t line = id >> 2;
+  const int q = threadIdx.x & 3;
+  if (line >= s.batch * s.channels) return;
+  const int64_t b = line / s.channels, n = line - b * s.channels, group = n / s.group_channels;
+  const float x = static_cast<float>(in.x.row(0, b)[n]);
+  const float bias = in.delta_bias ? in.delta_bias[n] : 0.0f;
+  const T* writes = in.write.row(0, b) + group * s.states;
+  const T* reads = in.read.row(0, b) + group * s.states;
+  float rate[R], h[R], write[R], read[R];
+  lane_row<R>(in.rates, n, q, s.states, true, rate);
+  lane_row<R>(state, line, q, s.states, true, h);
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int k = q * R + r;
+    write[r] = k < s.states ? static_cast<float>(writes[k]) : 0.0f;
+    read[r] = k < s.states ? static_cast<float>(reads[k]) : 0.0f;
+  }
+  const float dt = time_step(static_cast<float>(in.delta.row(0, b)[n]) + bias, s.softplus);
+  float sum = 0.0f;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    h[r] = fmaf(__builtin_amdgcn_exp2f(dt * (rate[r] * kLog2e)), h[r], dt * x * write[r]);
+    sum = fmaf(read[r], h[r], sum);
+    if (q * R + r < s.states) state[line * s.states + q * R + r] = h[r];
+  }
+  sum = quad_sum(sum);
+  if (q == 0) {
+    sum += in.skip ? in.skip[n] * x : 0.0f;
+    if (in.z.data) {
+      const float z = static_cast<float>(in.z.row(0, b)[n]);
+      sum *= z * sigmoid(z);
+    }
+    y.row(0, b)[n] = static_cast<T>(sum);
+  }
+}
+
+ScanShape scan_shape(const ns_scan_args* a) {
+  ScanShape s{};
+  s.ticks = a->ticks;
+  s.batch = a->batch;
+  s.channels = a->channels;
+  s.groups = a->groups;
+  s.group_channels = a->channels / a->groups;
+  s.group_blocks = (s.group_channels + kScanChannels - 1) / kScanChannels;
+  const int64_t tile = tile_of(lane_states(a->states));
+  const int64_t tiles = (a->ticks + tile - 1) / tile;
+  const int64_t wanted = a->chunks > 1 ? a->chunks : 1;
+  const int64_t per = tiles > 0 ? (tiles + wanted - 1) / wanted : 1;
+  s.chunk = per * tile;
+  s.chunks = tiles > 0 ? (tiles + per - 1) / per : 1;
+  s.states = a->states;
+  s.softplus = a->softplus;
+  return s;
+}
+
+int check_scan(const ns_scan_args* a) {
+  if (!a) return fail("scan arguments are required");
+  if (a->ticks < 0 || a->batch < 0 || a->channels <= 0)
+    return fail("a signal is [T, B, N] with N > 0");
+  if (a->groups < 1 || a->channels % a->groups)
+    return fail("the groups must divide the channels");
+  if (a->states < 1 || a->states > NS_SCAN_MAX_STATES)
+    return fail("a channel has 1 to %d states", NS_SCAN_MAX_STATES);
+  if (a->type != NS_TYPE_F32 && a->type != NS_TYPE_BF16 && a->type != NS_TYPE_F16)
+    return fail("unknown element type");
+  if (a->chunks < 1) return fail("a scan has at least one chunk");
+  if (!a->rates) return fail("the decay rates are required");
+  if (a->batch && a->ticks &&
+      (!a->x.data || !a->delta.data || !a->write.data || !a->read.data))
+    return fail("x, delta, B and C are required");
+  return NS_OK;
+}
+
+int scan_grid(const ScanShape& s, dim3* grid) {
+  const int64_t groups = s.groups * s.group_blocks * s.batch * s.chunks;
+  if (groups > INT32_MAX) return fail("the signal is too large for one launch");
+  *grid = dim3(static_cast<unsigned>(groups));
+  return NS_OK;
+}
+
+namespace {
+
+int launched(const char* what) {
+  const hipError_t err = hipGetLastError();
+  return err == hipSuccess ? NS_OK : fail_launch(what, err);
+}
+
+template <class T, int R>
+int run_forward(const ns_scan_args* a, hipStream_t stream) {
+  const ScanShape s = scan_shape(a);
+  dim3 grid;
+  if (int rc = scan_grid(s, &grid)) return rc;
+  const ScanIn<T> in = scan_in<T>(a);
+  const Signal<T> y = signal<T>(a->y);
+  float* steps = a->ends ? a->ends + s.chunks * s.batch * s.channels * (4 * R) : nullptr;
+  if (s.chunks > 1) {
+    scan_forward<T, R, true><<<grid, dim3(kThreads), 0, stream>>>(s, in, y, nullptr, nullptr,
+                                                                  nullptr, a->ends, steps);
+    if (int rc = launched("scan chunks")) return rc;
+    if (int rc = join_chunks(a, a->ends, a->state, false, stream)) return rc;
+  }
+  scan_forward<T, R, false><<<grid, dim3(kThreads), 0, stream>>>(
+      s, in, y, a->state, a->out_state, a->checkpoints, a->ends, nullptr);
+  return launched("scan");
+}
+
+template <class T, int R>
+int run_step(const ns_scan_args* a, hipStream_t stream) {
+  const ScanShape s = scan_shape(a);
+  const int64_t groups = (s.batch * s.channels * 4 + kThreads - 1) / kThreads;
+  if (groups > INT32_MAX) return fail("the signal is too large for one launch");
+  scan_step<T, R><<<dim3(static_cast<unsigned>(groups)), dim3(kThreads), 0, stream>>>(
+      s, scan_in<T>(a), signal<T>(a->y), a->out_state);
+  return launched("scan step");
+}
+
+template <class T>
+int run(const ns_scan_args* a, bool step, hipStream_t stream) {
+  switch (lane_states(a->states)) {
+    case 1: return step ? run_step<T, 1>(a, stream) : run_forward<T, 1>(a, stream);
+    case 2: return step ? run_step<T, 2>(a, stream) : run_forward<T, 2>(a, stream);
+    case 4: return step ? run_step<T, 4>(a, stream) : run_forward<T, 4>(a, stream);
+    case 8: return step ? run_step<T, 8>(a, stream) : run_forward<T, 8>(a, stream);
+    default: return step ? run_step<T, 16>(a, stream) : run_forward<T, 16>(a, stream);
+  }
+}
+
+int run_types(const ns_scan_args* a, bool step, void* stream) {
+  auto queue = static_cast<hipStream_t>(stream);
+  if (a->type == NS_TYPE_F32) return run<float>(a, step, queue);
+  if (a->type == NS_TYPE_BF16) return run<__bf16>(a, step, queue);
+  return run<_Float16>(a, step, queue);
+}
+
+}  // namespace
+
+int join_chunks(const ns_scan_args* a, float* ends, const float* start, bool reverse, void* stream) {
+  const ScanShape s = scan_shape(a);
+  const int64_t padded = 4 * lane_states(a->states), lines = s.batch * s.channels;
+  const int64_t groups = (lines * padded + kThreads - 1) / kThreads;
+  if (groups > INT32_MAX) return fail("the signal is too large for one launch");
+  join_kernel<<<dim3(static_cast<unsigned>(groups)), dim3(kThreads), 0,
+                static_cast<hipStream_t>(stream)>>>(s, padded, a->rates, start, ends,
+                                                    ends + s.chunks * lines * padded, reverse);
+  return launched("scan join");
+}
+
+}  // namespace ns
+
+extern "C" {
+
+int32_t ns_scan_chunks(int64_t ticks, int64_t batch, int64_t channels, int64_t groups,
+                       int32_t states, int32_t backward) {
+  if (ticks <= 0 || batch <= 0 || channels <= 0 || groups <= 0 || states <= 0 ||
+      states > NS_SCAN_MAX_STATES)
+    return 1;
+  (void)backward;
+  const int64_t per = channels / groups;
+  const int64_t blocks = groups * ((per + ns::kScanChannels - 1) / ns::kScanChannels) * batch;
+  const int64_t tile = ns::tile_of(ns::lane_states(states));
+  const int64_t tiles = (ticks + tile - 1) / tile;
+  if (blocks >= 512 || tiles < 8) return 1;
+  int64_t chunks = 2048 / blocks;
+  if (chunks > tiles / 4) chunks = tiles / 4;
+  return static_cast<int32_t>(chunks < 2 ? 1 : chunks);
+}
+
+int64_t ns_scan_checkpoint_floats(const ns_scan_args* a) {
+  ns::clear_error();
+  if (ns::check_scan(a) != NS_OK) return -1;
+  const int64_t r = ns::lane_states(a->states), tile = ns::tile_of(r);
+  return (a->ticks + tile - 1) / tile * a->batch * a->channels * 4 * r;
+}
+
+int64_t ns_scan_chunk_floats(const ns_scan_args* a) {
+  ns::clear_error();
+  if (ns::check_scan(a) != NS_OK) return -1;
+  const ns::ScanShape s = ns::scan_shape(a);
+  if (s.chunks <= 1) return 0;
+  return s.chunks * s.batch * s.channels * (4 * ns::lane_states(a->states) + 1);
+}
+
+int ns_scan_forward(const ns_scan_args* a, void* stream) {
+  ns::clear_error();
+  if (int rc = ns::check_scan(a)) return rc;
+  if (a->batch == 0) return NS_OK;
+  if (a->ticks && !a->y.data) return ns::fail("the output signal is required");
+  if (ns::scan_shape(a).chunks > 1 && !a->ends)
+    return ns::fail("a chunked scan needs its workspace");
+  return ns::run_types(a, false, stream);
+}
+
+int ns_scan_step(const ns_scan_args* a, void* stream) {
+  ns::clear_error();
+  if (int rc = ns::check_scan(a)) return rc;
+  if (a->ticks != 1 || a->lengths) return ns::fail("a step is one tick of every column");
+  if (a->batch == 0) return NS_OK;
+  if (!a->y.data) return ns::fail("the output signal is required");
+  if (!a->out_state || a->state != a->out_state)
+    return ns::fail("a step updates its state in place");
+  return ns::run_types(a, true, stream);
+}
+
+}  // extern "C"
