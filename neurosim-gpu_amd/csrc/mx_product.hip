@@ -20,71 +20,324 @@ struct MxView {
   int64_t rows, blocks;
 };
 
-struct MxOperand {
-  v4i codes;
-  int scale;
+// Geometry of a tile kernel: WM x WN wavefronts, each MI x NJ results of 16x16; K goes in
+// stages of KS steps of 128 values.
+template <int kMI, int kNJ, int kWM, int kWN, int kKS>
+struct Tile {
+  static constexpr int MI = kMI, NJ = kNJ, WM = kWM, WN = kWN, KS = kKS;
+  static constexpr int rows_m = 16 * MI * WM, rows_n = 16 * NJ * WN, rows = rows_m + rows_n;
+  static constexpr int subs = rows / 16;                   // 16-row strips, a's then b's
+  static constexpr int threads = 64 * WM * WN;
+  static constexpr int loads = rows * KS * 4 / threads;    // 16-byte pieces per thread and stage
+  static constexpr int scale_rows = (rows + threads - 1) / threads;
+  static_assert(rows * KS * 4 % threads == 0, "whole pieces per thread");
+  static_assert(rows_m % (threads / 8) == 0, "a load instruction reads one operand");
+  static_assert(KS == 2, "a stage's scales of a row are one 8-byte word");
 };
 
-// Block `block` of row `row` (past the matrix: zeros, scale 1).
-__device__ __forceinline__ MxOperand load_block(const MxView& m, int64_t row, int64_t block,
-                                                int64_t stop) {
-  MxOperand o{{0, 0, 0, 0}, 127};
-  if (row < m.rows && block < stop) {
-    o.codes = *reinterpret_cast<const v4i*>(m.codes + (row * m.blocks + block) * 16);
-    o.scale = m.scales[row * m.blocks + block];
-  }
-  return o;
+// One stage's operands in LDS.  Codes: rows of 8 blocks, 128 bytes, a whole cache line each,
+// with block k of row r at place k ^ (r % 8): the eight lanes that LDS serves at a time read
+// one block of eight rows, and so find them in eight different places.  Scale bytes of (step 0, step 1) as one 16-bit word per (wavefront row, lane, strip), so a
+// lane reads all its strips' scales at once and the instruction picks the byte it needs.
+template <class G>
+struct Stage {
+  v4i codes[G::rows * 8];
+  uint16_t scales_a[G::WM][64][G::MI];
+  uint16_t scales_b[G::WN][64][G::NJ];
+};
+
+// The rows a tile reads of one operand, as a buffer whose reads past its end give zeros.
+struct MxPanel {
+  __amdgpu_buffer_rsrc_t codes;
+  const uint8_t* scales;       // of the panel's first row
+  int blocks;
+  int last;                    // last row
+  uint32_t row_bytes;
+};
+
+__device__ __forceinline__ uint32_t uniform(uint32_t v) {
+  return __builtin_amdgcn_readfirstlane(v);
 }
 
-__device__ __forceinline__ v4f mx_mfma(const MxOperand& a, const MxOperand& b, v4f c) {
-  const v8i wide_a = {a.codes[0], a.codes[1], a.codes[2], a.codes[3], 0, 0, 0, 0};
-  const v8i wide_b = {b.codes[0], b.codes[1], b.codes[2], b.codes[3], 0, 0, 0, 0};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide_a, wide_b, c, 4, 4, 0, a.scale, 0,
-                                                          b.scale);
+__device__ __forceinline__ MxPanel panel(const MxView& m, int64_t row, int rows) {
+  const uint32_t own = uniform(static_cast<uint32_t>(m.rows - row < rows ? m.rows - row : rows));
+  const uint32_t row_bytes = uniform(static_cast<uint32_t>(m.blocks) * 16);
+  const uint64_t base = reinterpret_cast<uint64_t>(m.codes + row * row_bytes);
+  const uint64_t low = uniform(static_cast<uint32_t>(base)), high = uniform(base >> 32);
+  return MxPanel{__builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(high << 32 | low), 0,
+                                                   static_cast<int>(own * row_bytes), 0x00020000),
+                 m.scales + row * m.blocks, static_cast<int>(m.blocks), static_cast<int>(own) - 1,
+                 row_bytes};
 }
 
-// One wavefront per 32x32 tile and part of K.
-template <class T>
-__global__ __launch_bounds__(kThreads) void product_tiles(MxView a, MxView b, const float* bias,
-                                                          T* out, int64_t stride, int64_t tiles_n,
-                                                          int64_t tiles, int64_t splits,
-                                                          float* partials) {
-  const int lane = threadIdx.x & 63;
-  const int64_t id = static_cast<int64_t>(blockIdx.x) * (kThreads / 64) + (threadIdx.x >> 6);
-  if (id >= tiles * splits) return;
-  const int64_t split = id / tiles, tile = id - split * tiles;
-  const int64_t m0 = tile / tiles_n * 32, n0 = tile % tiles_n * 32;
-  const int64_t steps = (a.blocks + 3) / 4, per = (steps + splits - 1) / splits;
-  const int64_t first = split * per * 4;
-  int64_t stop = first + per * 4;
-  stop = stop < a.blocks ? stop : a.blocks;
-  v4f sum[2][2] = {};
-  for (int64_t block = first; block < stop; block += 4) {
-    MxOperand x[2], y[2];
+// Requests stage `block` .. of both panels' codes straight into LDS, eight rows of 128 bytes
+// per instruction: lane l fills place l%8 of row l/8.  Rows that do not exist read as zeros;
+// so do, in a row's last, partial stage (kWhole false), blocks from `stop` on.  (With 16 rows
+// of 64 bytes per instruction, in the order the fragments are read in, the product of 4096 x
+// 4096 by 32768 took 377 us: the L1 fetched every line twice.)
+template <bool kWhole>
+__device__ __forceinline__ void read_piece(const MxPanel& m, bool inside, uint32_t row,
+                                           uint32_t column, v4i* to) {
+  const uint32_t offset = kWhole || inside ? row * m.row_bytes + column : 0xFFFFFFF0u;
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(
+      m.codes, reinterpret_cast<__attribute__((address_space(3))) void*>(reinterpret_cast<uintptr_t>(to)),
+      16, static_cast<int>(offset), 0, 0, 0);
+}
+
+template <class G, bool kWhole>
+__device__ __forceinline__ void request_codes(const MxPanel& a, const MxPanel& b, int block, int stop,
+                                              int wave, int lane, Stage<G>& to) {
+  constexpr int kPerRound = G::threads / 8;                // rows per load instruction of all waves
+  const int at = block + ((lane & 7) ^ (lane >> 3));
+  const uint32_t row = 8 * wave + (lane >> 3), column = static_cast<uint32_t>(at) * 16;
+  const bool inside = at < stop;
+  constexpr int kLoadsA = G::rows_m / kPerRound;           // the first ones are a's
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      x[i] = load_block(a, m0 + 16 * i + (lane & 15), block + (lane >> 4), stop);
-      y[i] = load_block(b, n0 + 16 * i + (lane & 15), block + (lane >> 4), stop);
-    }
+  for (int i = 0; i < kLoadsA; ++i)
+    read_piece<kWhole>(a, inside, row + kPerRound * i, column, &to.codes[i * G::threads + 64 * wave]);
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+  for (int i = kLoadsA; i < G::loads; ++i)
+    read_piece<kWhole>(b, inside, row + kPerRound * (i - kLoadsA), column,
+                       &to.codes[i * G::threads + 64 * wave]);
+}
+
+// A thread's rows' scale bytes of a stage (past K: scale 1).
+template <class G>
+struct Scales {
+  uint32_t word[G::scale_rows][2];
+};
+
+template <class G, bool kWhole>
+__device__ __forceinline__ void request_scales(const MxPanel& a, const MxPanel& b, int block,
+                                               int stop, Scales<G>& next) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) sum[i][j] = mx_mfma(x[i], y[j], sum[i][j]);
-  }
+  for (int i = 0; i < G::scale_rows; ++i) {
+    const int piece = i * G::threads + static_cast<int>(threadIdx.x);
+    if (G::rows % G::threads == 0 || piece < G::rows) {
+      const bool of_a = piece < G::rows_m;
+      const int own = of_a ? piece : piece - G::rows_m, end = of_a ? a.last : b.last;
+      // A row that does not exist reads the last one's: its results are not stored.
+      const uint8_t* from = (of_a ? a.scales : b.scales) +
+                            static_cast<int64_t>(own < end ? own : end) * a.blocks + block;
+      if constexpr (kWhole) {
+        __builtin_memcpy(next.word[i], from, 8);
+      } else {
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+        for (int w = 0; w < 2; ++w) {
+          next.word[i][w] = 0;
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int64_t m = m0 + 16 * i + 4 * (lane >> 4) + r, n = n0 + 16 * j + (lane & 15);
-        if (m < a.rows && n < b.rows) {
-          if (splits > 1)
-            partials[(split * a.rows + m) * b.rows + n] = sum[i][j][r];
-          else
-            out[m * stride + n] = static_cast<T>(sum[i][j][r] + (bias ? bias[n] : 0.0f));
+          for (int k = 0; k < 4; ++k)
+            next.word[i][w] |= (block + 4 * w + k < stop ? from[4 * w + k] : 127u) << (8 * k);
         }
       }
+    }
+  }
+}
+
+template <class G>
+__device__ __forceinline__ void place_scales(const Scales<G>& next, Stage<G>& to) {
+#pragma unroll
+  for (int i = 0; i < G::scale_rows; ++i) {
+    const int row = i * G::threads + static_cast<int>(threadIdx.x);
+    if (G::rows % G::threads == 0 || row < G::rows) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint16_t two = static_cast<uint16_t>((next.word[i][0] >> (8 * k) & 255u) |
+                                                   (next.word[i][1] >> (8 * k) & 255u) << 8);
+        const int strip = row >> 4, lane = 16 * k + (row & 15);
+        if (row < G::rows_m)
+          to.scales_a[strip / G::MI][lane][strip % G::MI] = two;
+        else
+          to.scales_b[(strip - G::rows_m / 16) / G::NJ][lane][(strip - G::rows_m / 16) % G::NJ] = two;
+      }
+    }
+  }
+}
+
+// y^T strips: with b's rows as the instruction's first operand, a lane's four results are
+// four neighbouring columns of one row of y.
+template <int kByteA, int kByteB>
+__device__ __forceinline__ v4f mx_mfma(v4i a, v4i b, v4f c, int scale_a, int scale_b) {
+  const v8i wide_a = {a[0], a[1], a[2], a[3], 0, 0, 0, 0};
+  const v8i wide_b = {b[0], b[1], b[2], b[3], 0, 0, 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide_a, wide_b, c, 4, 4, kByteA, scale_a,
+                                                          kByteB, scale_b);
+}
+
+template <int kStrips>
+__device__ __forceinline__ void load_scales(const uint16_t* from, int (&to)[(kStrips + 1) / 2]) {
+  to[(kStrips + 1) / 2 - 1] = 0;
+  __builtin_memcpy(to, from, 2 * kStrips);
+}
+
+// A wavefront's operands of a stage.
+template <class G>
+struct Fragments {
+  v4i a[G::KS][G::MI], b[G::KS][G::NJ];
+  int scale_a[(G::MI + 1) / 2], scale_b[(G::NJ + 1) / 2];
+};
+
+template <class G>
+__device__ __forceinline__ void read_fragments(const Stage<G>& from, int wm, int wn, int lane,
+                                               Fragments<G>& f) {
+  load_scales<G::MI>(from.scales_a[wm][lane], f.scale_a);
+  load_scales<G::NJ>(from.scales_b[wn][lane], f.scale_b);
+#pragma unroll
+  for (int s = 0; s < G::KS; ++s) {
+    const int place = (4 * s + (lane >> 4)) ^ (lane & 7);
+#pragma unroll
+    for (int i = 0; i < G::MI; ++i)
+      f.a[s][i] = from.codes[((wm * G::MI + i) * 16 + (lane & 15)) * 8 + place];
+#pragma unroll
+    for (int j = 0; j < G::NJ; ++j)
+      f.b[s][j] = from.codes[(G::rows_m + (wn * G::NJ + j) * 16 + (lane & 15)) * 8 + place];
+  }
+}
+
+template <class G, int S = 0, int J = 0, int I = 0>
+__device__ __forceinline__ void multiply(const Fragments<G>& f, v4f (&sum)[G::MI][G::NJ]) {
+  sum[I][J] = mx_mfma<2 * (J & 1) + S, 2 * (I & 1) + S>(f.b[S][J], f.a[S][I], sum[I][J],
+                                                        f.scale_b[J / 2], f.scale_a[I / 2]);
+  if constexpr (I + 1 < G::MI)
+    multiply<G, S, J, I + 1>(f, sum);
+  else if constexpr (J + 1 < G::NJ)
+    multiply<G, S, J + 1, 0>(f, sum);
+  else if constexpr (S + 1 < G::KS)
+    multiply<G, S + 1, 0, 0>(f, sum);
+}
+
+// A wavefront's results, from row m0, column n0, of which `rows` and `columns` exist.  They
+// go strip by strip (16 rows) through LDS, so that each store instruction writes whole lines
+// of eight rows or more; rows are padded by 16 bytes against bank conflicts.  (Stored from the
+// registers, 32 bytes a row, the 8192^3 product spent 75 us of 418 on it.)
+template <class G, class T>
+struct Strip {
+  static constexpr int kWide = 16 / sizeof(T);                        // values per lane and store
+  static constexpr int kLanes = 16 * G::NJ / kWide;                   // lanes per row
+  static constexpr int kRows = 64 / kLanes < 16 ? 64 / kLanes : 16;   // rows per store
+  T values[16][16 * G::NJ + kWide];
+};
+
+template <class G, class T>
+__device__ __forceinline__ void store_tiles(T* to, int64_t stride, const v4f (&sum)[G::MI][G::NJ],
+                                            const float* bias, int64_t rows, int64_t columns, int lane,
+                                            Strip<G, T>& strip) {
+  using S = Strip<G, T>;
+  const int row = lane / S::kLanes, column = lane % S::kLanes * S::kWide;
+  const bool wide = column + S::kWide <= columns;
+#pragma unroll
+  for (int i = 0; i < G::MI; ++i) {
+#pragma unroll
+    for (int j = 0; j < G::NJ; ++j) {
+      Pack<T, 4> y;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int n = 16 * j + 4 * (lane >> 4) + r;
+        y.v[r] = static_cast<T>(sum[i][j][r] + (bias && n < columns ? bias[n] : 0.0f));
+      }
+      __builtin_memcpy(&strip.values[lane & 15][16 * j + 4 * (lane >> 4)], &y, sizeof(y));
+    }
+#pragma unroll
+    for (int r = 0; r < 16; r += S::kRows) {
+      if (row >= S::kRows || 16 * i + r + row >= rows) continue;
+      T* at = to + (16 * i + r + row) * stride + column;
+      Pack<T, S::kWide> y;
+      __builtin_memcpy(&y, &strip.values[r + row][column], sizeof(y));
+      if (wide) {
+        store_pack<T, S::kWide>(at, y);
+      } else {
+#pragma unroll
+        for (int k = 0; k < S::kWide; ++k)
+          if (column + k < columns) at[k] = y.v[k];
+      }
+    }
+  }
+}
+
+// All this wavefront's loads have arrived, those into LDS too.
+__device__ __forceinline__ void wait_all() { __builtin_amdgcn_s_waitcnt(0); }
+
+// Keeps the sums' computation before what follows in the program.
+template <class G>
+__device__ __forceinline__ void hold(v4f (&sum)[G::MI][G::NJ]) {
+#pragma unroll
+  for (int i = 0; i < G::MI; ++i)
+#pragma unroll
+    for (int j = 0; j < G::NJ; ++j) asm volatile("" : "+v"(sum[i][j]));
+}
+
+// Tiles of y, one workgroup per tile and part of K.  Two stages of LDS: while one is
+// multiplied, the next one is loaded.
+template <class G, class T>
+__global__ __launch_bounds__(G::threads) void product_tiles(MxView a, MxView b, const float* bias,
+                                                            T* out, int64_t stride, uint32_t tiles_m,
+                                                            uint32_t tiles_n, uint32_t splits,
+                                                            float* partials) {
+  __shared__ union {
+    Stage<G> stages[2];
+    Strip<G, T> strip[G::WM * G::WN];
+    Strip<G, float> partial[G::WM * G::WN];
+  } lds;
+  Stage<G>(&stages)[2] = lds.stages;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int wm = wave / G::WN, wn = wave % G::WN;
+  // Divisions run on the vector ALU; their results are the same in every lane, and have to
+  // be known as such for the panels' buffers.
+  const uint32_t split = uniform(blockIdx.x / (tiles_m * tiles_n));
+  const uint32_t tile = blockIdx.x - split * (tiles_m * tiles_n);
+  const uint32_t tile_m = uniform(tile / tiles_n), tile_n = tile - tile_m * tiles_n;
+  const int64_t m0 = static_cast<int64_t>(tile_m) * G::rows_m;
+  const int64_t n0 = static_cast<int64_t>(tile_n) * G::rows_n;
+  const int blocks = static_cast<int>(a.blocks);           // at most 2^18
+  const int all = (blocks + 4 * G::KS - 1) / (4 * G::KS);
+  const int per = static_cast<int>(uniform((all + splits - 1u) / splits));
+  const int first = static_cast<int>(split) * per * (4 * G::KS);
+  const int stop = first + per * (4 * G::KS) < blocks ? first + per * (4 * G::KS) : blocks;
+  const MxPanel pa = panel(a, m0, G::rows_m), pb = panel(b, n0, G::rows_n);
+  v4f sum[G::MI][G::NJ] = {};
+  Scales<G> next;
+  Fragments<G> f;
+  const int whole_stop = first + (stop - first) / (4 * G::KS) * (4 * G::KS);
+  int now = 0;
+  if (first < whole_stop) {
+    request_codes<G, true>(pa, pb, first, stop, wave, lane, stages[0]);
+    request_scales<G, true>(pa, pb, first, stop, next);
+    place_scales<G>(next, stages[0]);
+  }
+  for (int block = first; block < whole_stop; block += 4 * G::KS) {
+    // The stage's codes and scales have arrived, and the other stage is read to its end.
+    wait_all();
+    __syncthreads();
+    read_fragments<G>(stages[now], wm, wn, lane, f);
+    // The last whole stage requests itself again, which nothing reads.
+    const int ahead = block + 4 * G::KS < whole_stop ? block + 4 * G::KS : block;
+    now ^= 1;
+    request_codes<G, true>(pa, pb, ahead, stop, wave, lane, stages[now]);
+    request_scales<G, true>(pa, pb, ahead, stop, next);
+    multiply<G>(f, sum);
+    hold<G>(sum);
+    place_scales<G>(next, stages[now]);
+  }
+  if (whole_stop < stop) {
+    wait_all();
+    __syncthreads();
+    request_codes<G, false>(pa, pb, whole_stop, stop, wave, lane, stages[now]);
+    request_scales<G, false>(pa, pb, whole_stop, stop, next);
+    place_scales<G>(next, stages[now]);
+    wait_all();
+    __syncthreads();
+    read_fragments<G>(stages[now], wm, wn, lane, f);
+    multiply<G>(f, sum);
+  }
+  const int64_t m = m0 + 16 * wm * G::MI, n = n0 + 16 * wn * G::NJ;
+  __syncthreads();                                         // the stages are read to their end
+  if (splits > 1) {
+    store_tiles<G, float>(partials + (split * a.rows + m) * b.rows + n, b.rows, sum, nullptr,
+                          a.rows - m, b.rows - n, lane, lds.partial[wave]);
+  } else {
+    store_tiles<G, T>(out + m * stride + n, stride, sum, bias ? bias + n : nullptr, a.rows - m,
+                      b.rows - n, lane, lds.strip[wave]);
+  }
 }
 
 // The parts of K added in order.
@@ -109,20 +362,38 @@ MxView view(const ns_mx_matrix& m) {
   return MxView{m.codes, m.scales, m.rows, (m.columns + NS_MX_BLOCK - 1) / NS_MX_BLOCK};
 }
 
+using Large = Tile<8, 4, 2, 4, 2>;   // 256 x 256
+using Small = Tile<2, 2, 2, 2, 2>;   // 64 x 64
+
+// The tile for M x N: large ones where they fill the card.
+bool large_tiles(int64_t m, int64_t n) {
+  return (m + 255) / 256 * ((n + 255) / 256) >= 128;
+}
+
+template <class G, class T>
+int run_tiles(const ns_mx_product_args* p, hipStream_t stream) {
+  const MxView a = view(p->a), b = view(p->b);
+  const int64_t tiles_m = (a.rows + G::rows_m - 1) / G::rows_m;
+  const int64_t tiles_n = (b.rows + G::rows_n - 1) / G::rows_n;
+  const int64_t groups = tiles_m * tiles_n * p->splits;
+  if (groups > INT32_MAX) return fail("the product is too large for one launch");
+  product_tiles<G, T><<<dim3(static_cast<unsigned>(groups)), dim3(G::threads), 0, stream>>>(
+      a, b, p->bias, static_cast<T*>(p->out), p->stride, static_cast<uint32_t>(tiles_m),
+      static_cast<uint32_t>(tiles_n), static_cast<uint32_t>(p->splits), p->partials);
+  return launched("product");
+}
+
 template <class T>
 int run(const ns_mx_product_args* p, hipStream_t stream) {
-  const MxView a = view(p->a), b = view(p->b);
-  const int64_t tiles_n = (b.rows + 31) / 32, tiles = (a.rows + 31) / 32 * tiles_n;
-  const int64_t groups = (tiles * p->splits + 3) / 4;
-  if (groups > INT32_MAX) return fail("the product is too large for one launch");
-  product_tiles<T><<<dim3(static_cast<unsigned>(groups)), dim3(kThreads), 0, stream>>>(
-      a, b, p->bias, static_cast<T*>(p->out), p->stride, tiles_n, tiles, p->splits, p->partials);
-  if (int rc = launched("product")) return rc;
+  const int64_t rows = p->a.rows, columns = p->b.rows;
+  if (int rc = large_tiles(rows, columns) ? run_tiles<Large, T>(p, stream)
+                                          : run_tiles<Small, T>(p, stream))
+    return rc;
   if (p->splits == 1) return NS_OK;
-  const int64_t adds = (a.rows * b.rows + kThreads - 1) / kThreads;
+  const int64_t adds = (rows * columns + kThreads - 1) / kThreads;
   if (adds > INT32_MAX) return fail("the product is too large for one launch");
   add_splits<T><<<dim3(static_cast<unsigned>(adds)), dim3(kThreads), 0, stream>>>(
-      p->partials, p->splits, a.rows, b.rows, p->bias, static_cast<T*>(p->out), p->stride);
+      p->partials, p->splits, rows, columns, p->bias, static_cast<T*>(p->out), p->stride);
   return launched("product parts");
 }
 
@@ -141,12 +412,14 @@ extern "C" {
 
 int32_t ns_mx_product_splits(int64_t m, int64_t n, int64_t k) {
   if (m <= 0 || n <= 0 || k <= 0) return 1;
-  const int64_t tiles = (m + 31) / 32 * ((n + 31) / 32), steps = (k + 127) / 128;
-  int64_t splits = 4096 / tiles;
-  if (splits > steps / 4) splits = steps / 4;
+  const int64_t stages = (k + 255) / 256;
+  if (ns::large_tiles(m, n)) return 1;
+  const int64_t tiles = (m + 63) / 64 * ((n + 63) / 64);
+  int64_t splits = 1024 / tiles;
+  if (splits > stages / 2) splits = stages / 2;
   if (splits < 1) splits = 1;
-  const int64_t per = (steps + splits - 1) / splits;   // no empty part
-  return static_cast<int32_t>((steps + per - 1) / per);
+  const int64_t per = (stages + splits - 1) / splits;   // no empty part
+  return static_cast<int32_t>((stages + per - 1) / per);
 }
 
 int ns_mx_product(const ns_mx_product_args* p, void* stream) {
@@ -155,6 +428,8 @@ int ns_mx_product(const ns_mx_product_args* p, void* stream) {
   if (int rc = ns::check_operand(p->a, "a")) return rc;
   if (int rc = ns::check_operand(p->b, "b")) return rc;
   if (p->a.columns != p->b.columns) return ns::fail("the operands need the same number of columns");
+  // A tile's rows of codes are addressed in 31 bits.
+  if (p->a.columns > (1 << 23)) return ns::fail("a product takes at most 2^23 columns");
   if (p->splits < 1) return ns::fail("a product has at least one part");
   if (p->a.rows == 0 || p->b.rows == 0) return NS_OK;
   if (!p->out) return ns::fail("the output is required");
