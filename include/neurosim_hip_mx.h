@@ -39,19 +39,25 @@ int ns_mx_quantize(const ns_mx_matrix* matrix, const void* x, int64_t stride, in
 int ns_mx_dequantize(const ns_mx_matrix* matrix, void* out, int64_t stride, int32_t type,
                      void* stream);
 
-/* y[m*stride + n] = sum_k a[m,k] b[n,k] + bias[n], summed in float32, rounded to `type`. */
+/* y[m*stride + n] = sum_k a[m,k] b[n,k] + bias[n], summed in float32, rounded to `type`.
+ * With float rows `x` for a, they are quantised first (a.codes and a.scales are then not
+ * read: the workspace holds them). */
 typedef struct ns_mx_product_args {
-  ns_mx_matrix a, b;           /* M rows and N rows of K columns */
+  ns_mx_matrix a, b;           /* M rows and N rows of K columns (K up to NS_MX_MAX_COLUMNS) */
   const float* bias;           /* [N] or NULL */
   void* out;
   int64_t stride;
   int32_t type;                /* NS_TYPE_* of out */
-  int32_t splits;              /* K split over this many workgroups: ns_mx_product_splits, or 1 */
-  float* partials;             /* workspace float32 [splits][M][N] (splits > 1) */
+  int32_t x_type;              /* NS_TYPE_* of x */
+  const void* x;               /* optional: a's rows as floats, x[m*x_stride + k] */
+  int64_t x_stride;
+  void* workspace;             /* ns_mx_product_bytes bytes, 16-byte aligned */
 } ns_mx_product_args;
 
-/* Parts worth cutting K into (1: none). */
-int32_t ns_mx_product_splits(int64_t m, int64_t n, int64_t k);
+#define NS_MX_MAX_COLUMNS (1 << 23)
+
+/* Bytes of a product's workspace, with float rows for a or without (0: none needed). */
+int64_t ns_mx_product_bytes(int64_t m, int64_t n, int64_t k, int32_t float_rows);
 int ns_mx_product(const ns_mx_product_args* args, void* stream);
 
 #ifdef __cplusplus

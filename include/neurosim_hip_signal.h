@@ -82,7 +82,7 @@ typedef struct ns_scan_args {
   int32_t states;              /* S, 1 .. NS_SCAN_MAX_STATES */
   int32_t type;                /* NS_TYPE_* of x, delta, z, B, C, y (states, A, D float32) */
   int32_t softplus;
-  int32_t chunks;              /* time chunks scanned side by side: ns_scan_chunks, or 1 */
+  int32_t chunks;              /* time chunks scanned side by side (ns_scan_plan) */
   ns_signal x, delta, z, y;    /* z optional */
   ns_signal write, read;       /* B and C: [T, B, G, S], (g, s) at g*S + s of a column */
   const float* rates;          /* A [N][S] */
@@ -91,9 +91,9 @@ typedef struct ns_scan_args {
   const float* state;          /* h before the first tick [B][N][S], or NULL: zeros */
   float* out_state;            /* h after each column's last tick [B][N][S] */
   const int32_t* lengths;
-  float* checkpoints;          /* optional, ns_scan_checkpoint_floats: h before every tile of
+  float* checkpoints;          /* optional workspace (ns_scan_plan): h before every tile of
                                   ticks, kept for ns_scan_backward */
-  float* ends;                 /* workspace of ns_scan_chunk_floats floats (chunks > 1) */
+  float* ends;                 /* workspace (ns_scan_plan; chunks > 1) */
   /* ns_scan_backward only (checkpoints required): */
   ns_signal dy;
   const float* dout_state;     /* gradient of out_state, or NULL: zeros */
@@ -103,15 +103,14 @@ typedef struct ns_scan_args {
   float* drates;               /* dA [N][S] */
   float* dskip;                /* dD [N] (written also without D) */
   float* ddelta_bias;          /* [N] (written also without a bias) */
-  float* partials;             /* workspace of ns_scan_backward_floats floats */
+  float* partials;             /* workspace (ns_scan_plan) */
 } ns_scan_args;
 
-/* Time chunks worth scanning side by side (1: none). */
-int32_t ns_scan_chunks(int64_t ticks, int64_t batch, int64_t channels, int64_t groups,
-                       int32_t states, int32_t backward);
-int64_t ns_scan_checkpoint_floats(const ns_scan_args* args);
-int64_t ns_scan_chunk_floats(const ns_scan_args* args);
-int64_t ns_scan_backward_floats(const ns_scan_args* args);
+/* What a scan of this shape needs, `backward` or forward: sizes[0] time chunks worth scanning
+ * side by side (1: none), and the floats of `ends` [1] (0 for one chunk), `checkpoints` [2]
+ * and `partials` [3] with that many chunks. */
+int ns_scan_plan(int64_t ticks, int64_t batch, int64_t channels, int64_t groups, int32_t states,
+                 int32_t backward, int64_t* sizes);
 int ns_scan_forward(const ns_scan_args* args, void* stream);
 /* One tick (ticks == 1, no lengths): `out_state` is the state itself, updated in place. */
 int ns_scan_step(const ns_scan_args* args, void* stream);

@@ -370,36 +370,62 @@ bool large_tiles(int64_t m, int64_t n) {
   return (m + 255) / 256 * ((n + 255) / 256) >= 128;
 }
 
+// Parts that K is cut into where tiles are few: enough for four workgroups per compute
+// unit, of two stages at least.
+int64_t parts_of_k(int64_t m, int64_t n, int64_t k) {
+  if (m <= 0 || n <= 0 || k <= 0 || large_tiles(m, n)) return 1;
+  const int64_t stages = (k + 255) / 256, tiles = (m + 63) / 64 * ((n + 63) / 64);
+  int64_t parts = 1024 / tiles;
+  if (parts > stages / 2) parts = stages / 2;
+  if (parts < 1) parts = 1;
+  const int64_t per = (stages + parts - 1) / parts;   // no empty part
+  return (stages + per - 1) / per;
+}
+
+// The workspace: a's codes and scales (float rows), then the parts' sums.
+struct Workspace {
+  int64_t scales, partials, bytes;
+};
+
+Workspace workspace_of(int64_t m, int64_t n, int64_t k, bool float_rows) {
+  const int64_t blocks = (k + NS_MX_BLOCK - 1) / NS_MX_BLOCK, parts = parts_of_k(m, n, k);
+  Workspace w{};
+  w.scales = float_rows ? m * blocks * 16 : 0;
+  w.partials = float_rows ? (m * blocks * 17 + 15) / 16 * 16 : 0;
+  w.bytes = w.partials + (parts > 1 ? parts * m * n * 4 : 0);
+  return w;
+}
+
 template <class G, class T>
-int run_tiles(const ns_mx_product_args* p, hipStream_t stream) {
+int run_tiles(const ns_mx_product_args* p, int64_t parts, float* partials, hipStream_t stream) {
   const MxView a = view(p->a), b = view(p->b);
   const int64_t tiles_m = (a.rows + G::rows_m - 1) / G::rows_m;
   const int64_t tiles_n = (b.rows + G::rows_n - 1) / G::rows_n;
-  const int64_t groups = tiles_m * tiles_n * p->splits;
+  const int64_t groups = tiles_m * tiles_n * parts;
   if (groups > INT32_MAX) return fail("the product is too large for one launch");
   product_tiles<G, T><<<dim3(static_cast<unsigned>(groups)), dim3(G::threads), 0, stream>>>(
       a, b, p->bias, static_cast<T*>(p->out), p->stride, static_cast<uint32_t>(tiles_m),
-      static_cast<uint32_t>(tiles_n), static_cast<uint32_t>(p->splits), p->partials);
+      static_cast<uint32_t>(tiles_n), static_cast<uint32_t>(parts), partials);
   return launched("product");
 }
 
 template <class T>
-int run(const ns_mx_product_args* p, hipStream_t stream) {
+int run(const ns_mx_product_args* p, float* partials, hipStream_t stream) {
   const int64_t rows = p->a.rows, columns = p->b.rows;
-  if (int rc = large_tiles(rows, columns) ? run_tiles<Large, T>(p, stream)
-                                          : run_tiles<Small, T>(p, stream))
+  const int64_t parts = parts_of_k(rows, columns, p->a.columns);
+  if (int rc = large_tiles(rows, columns) ? run_tiles<Large, T>(p, parts, partials, stream)
+                                          : run_tiles<Small, T>(p, parts, partials, stream))
     return rc;
-  if (p->splits == 1) return NS_OK;
+  if (parts == 1) return NS_OK;
   const int64_t adds = (rows * columns + kThreads - 1) / kThreads;
   if (adds > INT32_MAX) return fail("the product is too large for one launch");
   add_splits<T><<<dim3(static_cast<unsigned>(adds)), dim3(kThreads), 0, stream>>>(
-      p->partials, p->splits, rows, columns, p->bias, static_cast<T*>(p->out), p->stride);
+      partials, parts, rows, columns, p->bias, static_cast<T*>(p->out), p->stride);
   return launched("product parts");
 }
 
 int check_operand(const ns_mx_matrix& m, const char* what) {
-  if (m.rows < 0 || m.columns < 0) return fail("%s: rows and columns must not be negative", what);
-  if (m.rows && m.columns && (!m.codes || !m.scales))
+  if (m.columns && (!m.codes || !m.scales))
     return fail("%s: codes and scales are required", what);
   if (reinterpret_cast<uintptr_t>(m.codes) % 16) return fail("%s: codes must be 16-byte aligned", what);
   return NS_OK;
@@ -410,35 +436,42 @@ int check_operand(const ns_mx_matrix& m, const char* what) {
 
 extern "C" {
 
-int32_t ns_mx_product_splits(int64_t m, int64_t n, int64_t k) {
-  if (m <= 0 || n <= 0 || k <= 0) return 1;
-  const int64_t stages = (k + 255) / 256;
-  if (ns::large_tiles(m, n)) return 1;
-  const int64_t tiles = (m + 63) / 64 * ((n + 63) / 64);
-  int64_t splits = 1024 / tiles;
-  if (splits > stages / 2) splits = stages / 2;
-  if (splits < 1) splits = 1;
-  const int64_t per = (stages + splits - 1) / splits;   // no empty part
-  return static_cast<int32_t>((stages + per - 1) / per);
+int64_t ns_mx_product_bytes(int64_t m, int64_t n, int64_t k, int32_t float_rows) {
+  if (m <= 0 || n <= 0 || k <= 0) return 0;
+  return ns::workspace_of(m, n, k, float_rows != 0).bytes;
 }
 
-int ns_mx_product(const ns_mx_product_args* p, void* stream) {
+int ns_mx_product(const ns_mx_product_args* args, void* stream) {
   ns::clear_error();
-  if (!p) return ns::fail("product arguments are required");
-  if (int rc = ns::check_operand(p->a, "a")) return rc;
-  if (int rc = ns::check_operand(p->b, "b")) return rc;
-  if (p->a.columns != p->b.columns) return ns::fail("the operands need the same number of columns");
+  if (!args) return ns::fail("product arguments are required");
+  ns_mx_product_args p = *args;
+  const int64_t m = p.a.rows, n = p.b.rows, k = p.a.columns;
+  if (p.a.columns != p.b.columns) return ns::fail("the operands need the same number of columns");
   // A tile's rows of codes are addressed in 31 bits.
-  if (p->a.columns > (1 << 23)) return ns::fail("a product takes at most 2^23 columns");
-  if (p->splits < 1) return ns::fail("a product has at least one part");
-  if (p->a.rows == 0 || p->b.rows == 0) return NS_OK;
-  if (!p->out) return ns::fail("the output is required");
-  if (p->splits > 1 && !p->partials) return ns::fail("a split product needs its workspace");
+  if (k > NS_MX_MAX_COLUMNS) return ns::fail("a product takes at most %d columns", NS_MX_MAX_COLUMNS);
+  if (m < 0 || n < 0 || k < 0) return ns::fail("rows and columns must not be negative");
+  if (m == 0 || n == 0) return NS_OK;
+  if (k > 0) {
+    const ns::Workspace w = ns::workspace_of(m, n, k, p.x != nullptr);
+    auto* space = static_cast<uint8_t*>(p.workspace);
+    if (w.bytes && (!space || reinterpret_cast<uintptr_t>(space) % 16))
+      return ns::fail("the product needs its workspace, 16-byte aligned");
+    if (p.x) {
+      p.a.codes = space;
+      p.a.scales = space + w.scales;
+      if (int rc = ns_mx_quantize(&p.a, p.x, p.x_stride, p.x_type, stream)) return rc;
+    }
+    p.workspace = space + w.partials;
+  }
+  if (int rc = ns::check_operand(p.a, "a")) return rc;
+  if (int rc = ns::check_operand(p.b, "b")) return rc;
+  if (!p.out) return ns::fail("the output is required");
   auto queue = static_cast<hipStream_t>(stream);
-  switch (p->type) {
-    case NS_TYPE_F32: return ns::run<float>(p, queue);
-    case NS_TYPE_BF16: return ns::run<__bf16>(p, queue);
-    case NS_TYPE_F16: return ns::run<_Float16>(p, queue);
+  auto* partials = static_cast<float*>(p.workspace);
+  switch (p.type) {
+    case NS_TYPE_F32: return ns::run<float>(&p, partials, queue);
+    case NS_TYPE_BF16: return ns::run<__bf16>(&p, partials, queue);
+    case NS_TYPE_F16: return ns::run<_Float16>(&p, partials, queue);
     default: return ns::fail("unknown element type");
   }
 }

@@ -218,6 +218,18 @@ __global__ __launch_bounds__(kThreads) void scan_step(ScanShape s, ScanIn<T> in,
   }
 }
 
+// Time chunks worth scanning side by side.
+int64_t worth_chunks(const ns_scan_args* a, bool backward) {
+  (void)backward;
+  if (a->ticks <= 0 || a->batch <= 0) return 1;
+  const int64_t per = a->channels / a->groups;
+  const int64_t blocks = a->groups * ((per + kScanChannels - 1) / kScanChannels) * a->batch;
+  const int64_t tile = tile_of(lane_states(a->states)), tiles = (a->ticks + tile - 1) / tile;
+  if (blocks >= 512 || tiles < 8) return 1;
+  const int64_t chunks = 2048 / blocks < tiles / 4 ? 2048 / blocks : tiles / 4;
+  return chunks < 2 ? 1 : chunks;
+}
+
 ScanShape scan_shape(const ns_scan_args* a) {
   ScanShape s{};
   s.ticks = a->ticks;
@@ -237,14 +249,19 @@ ScanShape scan_shape(const ns_scan_args* a) {
   return s;
 }
 
-int check_scan(const ns_scan_args* a) {
-  if (!a) return fail("scan arguments are required");
+int check_shape(const ns_scan_args* a) {
   if (a->ticks < 0 || a->batch < 0 || a->channels <= 0)
     return fail("a signal is [T, B, N] with N > 0");
   if (a->groups < 1 || a->channels % a->groups)
     return fail("the groups must divide the channels");
   if (a->states < 1 || a->states > NS_SCAN_MAX_STATES)
     return fail("a channel has 1 to %d states", NS_SCAN_MAX_STATES);
+  return NS_OK;
+}
+
+int check_scan(const ns_scan_args* a) {
+  if (!a) return fail("scan arguments are required");
+  if (int rc = check_shape(a)) return rc;
   if (a->type != NS_TYPE_F32 && a->type != NS_TYPE_BF16 && a->type != NS_TYPE_F16)
     return fail("unknown element type");
   if (a->chunks < 1) return fail("a scan has at least one chunk");
@@ -333,35 +350,28 @@ int join_chunks(const ns_scan_args* a, float* ends, const float* start, bool rev
 
 extern "C" {
 
-int32_t ns_scan_chunks(int64_t ticks, int64_t batch, int64_t channels, int64_t groups,
-                       int32_t states, int32_t backward) {
-  if (ticks <= 0 || batch <= 0 || channels <= 0 || groups <= 0 || states <= 0 ||
-      states > NS_SCAN_MAX_STATES)
-    return 1;
-  (void)backward;
-  const int64_t per = channels / groups;
-  const int64_t blocks = groups * ((per + ns::kScanChannels - 1) / ns::kScanChannels) * batch;
-  const int64_t tile = ns::tile_of(ns::lane_states(states));
-  const int64_t tiles = (ticks + tile - 1) / tile;
-  if (blocks >= 512 || tiles < 8) return 1;
-  int64_t chunks = 2048 / blocks;
-  if (chunks > tiles / 4) chunks = tiles / 4;
-  return static_cast<int32_t>(chunks < 2 ? 1 : chunks);
-}
-
-int64_t ns_scan_checkpoint_floats(const ns_scan_args* a) {
+int ns_scan_plan(int64_t ticks, int64_t batch, int64_t channels, int64_t groups, int32_t states,
+                 int32_t backward, int64_t* sizes) {
   ns::clear_error();
-  if (ns::check_scan(a) != NS_OK) return -1;
-  const int64_t r = ns::lane_states(a->states), tile = ns::tile_of(r);
-  return (a->ticks + tile - 1) / tile * a->batch * a->channels * 4 * r;
-}
-
-int64_t ns_scan_chunk_floats(const ns_scan_args* a) {
-  ns::clear_error();
-  if (ns::check_scan(a) != NS_OK) return -1;
-  const ns::ScanShape s = ns::scan_shape(a);
-  if (s.chunks <= 1) return 0;
-  return s.chunks * s.batch * s.channels * (4 * ns::lane_states(a->states) + 1);
+  static const float present = 0.0f;
+  ns_scan_args a{};
+  a.ticks = ticks;
+  a.batch = batch;
+  a.channels = channels;
+  a.groups = groups;
+  a.states = states;
+  a.chunks = 1;
+  a.rates = &present;
+  if (!sizes) return ns::fail("the sizes' place is required");
+  if (int rc = ns::check_shape(&a)) return rc;
+  a.chunks = static_cast<int32_t>(ns::worth_chunks(&a, backward != 0));
+  const ns::ScanShape s = ns::scan_shape(&a);
+  const int64_t r = ns::lane_states(states), tile = ns::tile_of(r), lines = batch * channels;
+  sizes[0] = s.chunks;
+  sizes[1] = s.chunks > 1 ? s.chunks * lines * (4 * r + 1) : 0;
+  sizes[2] = (ticks + tile - 1) / tile * lines * 4 * r;
+  sizes[3] = ns::scan_part_floats(&a);
+  return NS_OK;
 }
 
 int ns_scan_forward(const ns_scan_args* a, void* stream) {

@@ -399,16 +399,15 @@ int run(const ns_scan_args* a, hipStream_t stream) {
 }
 
 }  // namespace
+
+int64_t scan_part_floats(const ns_scan_args* a) {
+  const PartSizes sizes = part_sizes(a);
+  return sizes.rates + 2 * sizes.lines + sizes.shared;
+}
+
 }  // namespace ns
 
 extern "C" {
-
-int64_t ns_scan_backward_floats(const ns_scan_args* a) {
-  ns::clear_error();
-  if (ns::check_scan(a) != NS_OK) return -1;
-  const ns::PartSizes sizes = ns::part_sizes(a);
-  return sizes.rates + 2 * sizes.lines + sizes.shared;
-}
 
 int ns_scan_backward(const ns_scan_args* a, void* stream) {
   ns::clear_error();

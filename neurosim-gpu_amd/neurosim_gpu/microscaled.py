@@ -20,25 +20,21 @@ include/neurosim_hip_mx.h; calls run on the current stream and never synchronise
 from __future__ import annotations
 
 import ctypes
-from dataclasses import dataclass
+import struct
 from functools import lru_cache
 
 import torch
 
-from .native import _raise_on, load_library
-from .signal_ops import TYPES, _needs_grad, on_device
+from .native import load_library
+from .signal_ops import TYPES, _needs_grad, call
 
 MX_BLOCK = 32                        # NS_MX_BLOCK
 _i32, _i64, _ptr = ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p
 
-
-class _Matrix(ctypes.Structure):
-    _fields_ = [("rows", _i64), ("columns", _i64), ("codes", _ptr), ("scales", _ptr)]
-
-
-class _ProductArgs(ctypes.Structure):
-    _fields_ = [("a", _Matrix), ("b", _Matrix), ("bias", _ptr), ("out", _ptr), ("stride", _i64),
-                ("type", _i32), ("splits", _i32), ("partials", _ptr)]
+# The C argument structs, packed: ns_mx_matrix (rows, columns, codes, scales), and
+# ns_mx_product_args (a; b; bias, out; stride; types; x; its stride; workspace).
+_MATRIX = struct.Struct("=2q2Q")
+_PRODUCT = struct.Struct("=2q2Q 2q2Q 2Q q 2i Q q Q")
 
 
 @lru_cache(maxsize=1)
@@ -46,37 +42,33 @@ def _library() -> ctypes.CDLL:
     lib = load_library()
     for name in ("ns_mx_quantize", "ns_mx_dequantize"):
         fn = getattr(lib, name)
-        fn.restype = ctypes.c_int
-        fn.argtypes = [ctypes.POINTER(_Matrix), _ptr, _i64, _i32, _ptr]
-    lib.ns_mx_product.restype = ctypes.c_int
-    lib.ns_mx_product.argtypes = [ctypes.POINTER(_ProductArgs), _ptr]
-    lib.ns_mx_product_splits.restype = _i32
-    lib.ns_mx_product_splits.argtypes = [_i64, _i64, _i64]
+        fn.restype, fn.argtypes = ctypes.c_int, [_ptr, _ptr, _i64, _i32, _ptr]
+    lib.ns_mx_product.restype, lib.ns_mx_product.argtypes = ctypes.c_int, [_ptr, _ptr]
+    lib.ns_mx_product_bytes.restype = _i64
+    lib.ns_mx_product_bytes.argtypes = [_i64, _i64, _i64, _i32]
     return lib
 
 
-@dataclass(frozen=True)
 class MXTensor:
     """Quantised rows: ``codes`` uint8 [..., blocks * 16] and ``scales`` uint8 [..., blocks] of
     rows of ``columns`` values, blocks = ceil(columns / 32)."""
 
-    codes: torch.Tensor
-    scales: torch.Tensor
-    columns: int
+    __slots__ = ("codes", "scales", "columns")
 
-    def __post_init__(self) -> None:
-        blocks = -(-self.columns // MX_BLOCK)
-        for value, what, width in ((self.codes, "codes", blocks * (MX_BLOCK // 2)),
-                                   (self.scales, "scales", blocks)):
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, columns: int) -> None:
+        blocks = (columns + MX_BLOCK - 1) // MX_BLOCK
+        for value, what, width in ((codes, "codes", blocks * (MX_BLOCK // 2)),
+                                   (scales, "scales", blocks)):
             if (not isinstance(value, torch.Tensor) or value.dtype != torch.uint8
                     or value.dim() < 1 or value.shape[-1] != width):
-                raise ValueError(f"{what} must be uint8 [..., {width}] for {self.columns} columns")
+                raise ValueError(f"{what} must be uint8 [..., {width}] for {columns} columns")
             if not value.is_contiguous():
                 raise ValueError(f"{what} must be contiguous")
-        if self.codes.shape[:-1] != self.scales.shape[:-1] or self.codes.device != self.scales.device:
+        if codes.shape[:-1] != scales.shape[:-1] or codes.device != scales.device:
             raise ValueError("codes and scales need the same rows on the same device")
-        if self.codes.data_ptr() % 16:
+        if codes.data_ptr() % 16:
             raise ValueError("codes must be 16-byte aligned")
+        self.codes, self.scales, self.columns = codes, scales, columns
 
     @property
     def shape(self) -> torch.Size:
@@ -86,99 +78,109 @@ class MXTensor:
     def device(self) -> torch.device:
         return self.codes.device
 
+    def __repr__(self) -> str:
+        return f"MXTensor(shape={list(self.shape)}, device={self.device})"
+
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         return mx_dequantize(self, dtype)
 
 
-def _rows(value: MXTensor) -> int:
-    return value.scales.shape[:-1].numel()
+def _rows(lead) -> int:
+    rows = 1
+    for size in lead:
+        rows *= size
+    return rows
 
 
-def _matrix(value: MXTensor) -> _Matrix:
-    return _Matrix(_rows(value), value.columns,
-                   value.codes.data_ptr() if value.codes.numel() else None,
-                   value.scales.data_ptr() if value.scales.numel() else None)
+def _float_rows(x: torch.Tensor, rows: int, columns: int) -> torch.Tensor:
+    """x as [rows, columns] with dense rows (a copy where they are not)."""
+    if x.dim() != 2:
+        x = x.reshape(rows, columns)
+    return x if columns <= 1 or x.stride(1) == 1 else x.contiguous()
 
 
-def _stream(device: torch.device):
-    return torch.cuda.current_stream(device).cuda_stream
+def _check_floats(x) -> None:
+    if not isinstance(x, torch.Tensor) or x.dim() < 1 or x.dtype not in TYPES:
+        raise ValueError("quantisation takes [..., K] tensors of float32, bfloat16 or float16")
+    if not x.is_cuda:
+        raise ValueError("quantisation needs its input on a GPU")
+    if _needs_grad(x):
+        raise ValueError("quantisation gives no gradients; detach its input")
 
 
 def mx_quantize(x: torch.Tensor) -> MXTensor:
     """``x`` [..., K] (float32, bfloat16 or float16, on a GPU) quantised along its last dimension."""
-    if not isinstance(x, torch.Tensor) or x.dim() < 1 or x.dtype not in TYPES:
-        raise ValueError("quantisation takes [..., K] tensors of float32, bfloat16 or float16")
-    if x.device.type != "cuda":
-        raise ValueError("quantisation needs its input on a GPU")
-    if _needs_grad(x):
-        raise ValueError("quantisation gives no gradients; detach its input")
-    rows, columns = x.shape[:-1].numel(), x.shape[-1]
-    blocks = -(-columns // MX_BLOCK)
-    flat = x.detach().reshape(rows, columns) if x.dim() != 2 else x.detach()
-    if columns > 1 and flat.stride(1) != 1:
-        flat = flat.contiguous()
-    storage = torch.empty(rows * blocks * 17, dtype=torch.uint8, device=x.device)
-    out = MXTensor(storage[:rows * blocks * 16].view(*x.shape[:-1], blocks * 16),
-                   storage[rows * blocks * 16:].view(*x.shape[:-1], blocks), columns)
-    lib, matrix = _library(), _matrix(out)
-    with on_device(x.device):
-        _raise_on(lib.ns_mx_quantize(ctypes.byref(matrix), flat.data_ptr() or None, flat.stride(0),
-                                     TYPES[x.dtype], _stream(x.device)), lib)
-    return out
+    _check_floats(x)
+    *lead, columns = x.shape
+    rows, blocks, device = _rows(lead), (columns + MX_BLOCK - 1) // MX_BLOCK, x.device
+    flat = _float_rows(x, rows, columns)
+    codes = torch.empty((*lead, blocks * 16), dtype=torch.uint8, device=device)
+    scales = torch.empty((*lead, blocks), dtype=torch.uint8, device=device)
+    matrix = _MATRIX.pack(rows, columns, codes.data_ptr(), scales.data_ptr())
+    call(_library().ns_mx_quantize, device, matrix, flat.data_ptr(), flat.stride(0), TYPES[x.dtype])
+    return MXTensor(codes, scales, columns)
 
 
 def mx_dequantize(value: MXTensor, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """The values of quantised rows, rounded to ``dtype`` (exact in float32 and bfloat16)."""
-    if not isinstance(value, MXTensor) or value.device.type != "cuda":
+    if not isinstance(value, MXTensor) or not value.codes.is_cuda:
         raise ValueError("reading back needs an MXTensor on a GPU")
     if dtype not in TYPES:
         raise ValueError("values are read back as float32, bfloat16 or float16")
-    out = torch.empty(value.shape, dtype=dtype, device=value.device)
-    lib, matrix = _library(), _matrix(value)
-    with on_device(value.device):
-        _raise_on(lib.ns_mx_dequantize(ctypes.byref(matrix), out.data_ptr() or None, value.columns,
-                                       TYPES[dtype], _stream(value.device)), lib)
+    codes, scales, columns = value.codes, value.scales, value.columns
+    lead, device = codes.shape[:-1], codes.device
+    out = torch.empty((*lead, columns), dtype=dtype, device=device)
+    matrix = _MATRIX.pack(_rows(lead), columns, codes.data_ptr(), scales.data_ptr())
+    call(_library().ns_mx_dequantize, device, matrix, out.data_ptr(), columns, TYPES[dtype])
     return out
 
 
 def mx_product(x: torch.Tensor | MXTensor, weight: MXTensor, *, bias: torch.Tensor | None = None,
                dtype: torch.dtype | None = None) -> torch.Tensor:
-    """``x @ weight.T + bias`` of quantised rows: x [..., K], weight [N, K], result [..., N].
+    """``x @ weight.T + bias`` of quantised rows: x [..., K], weight [N, K], result [..., N]
+    (K up to 2^23).
 
     A float ``x`` is quantised on the way.  Sums are float32; the result is rounded once to
     ``dtype`` (x's own for a float x, else float32)."""
     if not isinstance(weight, MXTensor) or weight.codes.dim() != 2:
         raise ValueError("weight must be an MXTensor of [N, K]")
-    if isinstance(x, torch.Tensor):
+    columns, outputs, device = weight.columns, weight.codes.shape[0], weight.codes.device
+    floats = isinstance(x, torch.Tensor)
+    if floats:
+        _check_floats(x)
+        *lead, width = x.shape
         dtype = dtype or x.dtype
-        if x.dim() >= 1 and x.shape[-1] != weight.columns:
-            raise ValueError(f"x has {x.shape[-1]} columns, the weight {weight.columns}")
-        x = mx_quantize(x)
-    elif not isinstance(x, MXTensor):
+    elif isinstance(x, MXTensor):
+        lead, width = x.codes.shape[:-1], x.columns
+        dtype = dtype or torch.float32
+    else:
         raise ValueError("x must be a float tensor or an MXTensor")
-    dtype = dtype or torch.float32
+    if width != columns:
+        raise ValueError(f"x has {width} columns, the weight {columns}")
     if dtype not in TYPES:
         raise ValueError("a product is float32, bfloat16 or float16")
-    if x.columns != weight.columns:
-        raise ValueError(f"x has {x.columns} columns, the weight {weight.columns}")
-    if x.device != weight.device or weight.device.type != "cuda":
+    if x.device != device or not weight.codes.is_cuda:
         raise ValueError("x and the weight must be on the same GPU")
-    rows, outputs = _rows(x), weight.codes.shape[0]
     if bias is not None:
         if (not isinstance(bias, torch.Tensor) or bias.shape != (outputs,)
-                or bias.dtype != torch.float32 or bias.device != weight.device):
+                or bias.dtype != torch.float32 or bias.device != device):
             raise ValueError("bias must be float32 [N] on the weight's device")
         if _needs_grad(bias):
             raise ValueError("a 4-bit product gives no gradients")
-        bias = bias.detach().contiguous()
-    out = torch.empty((*x.shape[:-1], outputs), dtype=dtype, device=weight.device)
-    lib = _library()
-    splits = lib.ns_mx_product_splits(rows, outputs, weight.columns)
-    partials = (torch.empty(splits * rows * outputs, dtype=torch.float32, device=weight.device)
-                if splits > 1 else None)
-    args = _ProductArgs(_matrix(x), _matrix(weight), bias.data_ptr() if bias is not None else None,
-                        out.data_ptr() or None, outputs, TYPES[dtype], splits,
-                        partials.data_ptr() if partials is not None else None)
-    with on_device(weight.device):
-        _raise_on(lib.ns_mx_product(ctypes.byref(args), _stream(weight.device)), lib)
+        bias = bias.contiguous()
+    rows, lib = _rows(lead), _library()
+    out = torch.empty((*lead, outputs), dtype=dtype, device=device)
+    size = lib.ns_mx_product_bytes(rows, outputs, columns, floats)
+    work = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+    if floats and size:
+        flat = _float_rows(x, rows, columns)
+        a, rest = (0, 0), (TYPES[x.dtype], flat.data_ptr(), flat.stride(0))
+    else:
+        a = (0, 0) if floats else (x.codes.data_ptr(), x.scales.data_ptr())
+        rest = (0, 0, 0)
+    args = _PRODUCT.pack(rows, columns, *a, outputs, columns, weight.codes.data_ptr(),
+                         weight.scales.data_ptr(), 0 if bias is None else bias.data_ptr(),
+                         out.data_ptr(), outputs, TYPES[dtype], *rest,
+                         0 if work is None else work.data_ptr())
+    call(lib.ns_mx_product, device, args)
     return out

@@ -23,103 +23,77 @@ outputs and workspaces from torch, and never synchronise.
 from __future__ import annotations
 
 import ctypes
-from contextlib import nullcontext
+import struct
 from functools import lru_cache
 
 import torch
 from torch.autograd.function import once_differentiable
 
-from .native import _raise_on, load_library
+from .native import _RAW_STREAM, _raise_on, load_library
 
 MAX_TAPS, MAX_STATES = 8, 64         # NS_CONV_MAX_TAPS, NS_SCAN_MAX_STATES
 TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # NS_TYPE_*
 
+# The C argument structs, packed in one go: a call's host time is most of a small call.
+# ns_conv_args: shape; x; weight, bias; history; lengths; y, out_history, dy, dout_history,
+# dx, dhistory; partials, dweight.
+_CONV = struct.Struct("=3q4i Q2q 2Q Q2q Q Q2q Q2q Q2q Q2q Q2q Q2q 2Q")
+_CONV_FORWARD = struct.Struct("=3q4i Q2q 2Q Q2q Q Q2q Q2q 112x")
+# ns_scan_args: shape; x, delta, z, y; B, C; A, D, delta_bias, state, out_state, lengths,
+# checkpoints, ends; dy; dout_state; dx, ddelta, dz, dB, dC; dstate, dA, dD, ddelta_bias,
+# partials.
+_SCAN = struct.Struct("=4q4i Q2q Q2q Q2q Q2q Q2q Q2q 8Q Q2q Q Q2q Q2q Q2q Q2q Q2q 5Q")
+_SCAN_FORWARD = struct.Struct("=4q4i Q2q Q2q Q2q Q2q Q2q Q2q 8Q 192x")
+_ABSENT = (0, 0, 0)
+
 _i32, _i64, _ptr = ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p
-
-
-class _Signal(ctypes.Structure):
-    _fields_ = [("data", _ptr), ("stride_t", _i64), ("stride_b", _i64)]
-
-
-class _ConvArgs(ctypes.Structure):
-    _fields_ = [("ticks", _i64), ("batch", _i64), ("channels", _i64), ("taps", _i32),
-                ("type", _i32), ("silu", _i32), ("chunk", _i32), ("x", _Signal),
-                ("weight", _ptr), ("bias", _ptr), ("history", _Signal), ("lengths", _ptr),
-                ("y", _Signal), ("out_history", _Signal), ("dy", _Signal),
-                ("dout_history", _Signal), ("dx", _Signal), ("dhistory", _Signal),
-                ("partials", _ptr), ("dweight", _ptr)]
-
-
-class _ScanArgs(ctypes.Structure):
-    _fields_ = [("ticks", _i64), ("batch", _i64), ("channels", _i64), ("groups", _i64),
-                ("states", _i32), ("type", _i32), ("softplus", _i32), ("chunks", _i32),
-                ("x", _Signal), ("delta", _Signal), ("z", _Signal), ("y", _Signal),
-                ("write", _Signal), ("read", _Signal), ("rates", _ptr), ("skip", _ptr),
-                ("delta_bias", _ptr), ("state", _ptr), ("out_state", _ptr), ("lengths", _ptr),
-                ("checkpoints", _ptr), ("ends", _ptr), ("dy", _Signal), ("dout_state", _ptr),
-                ("dx", _Signal), ("ddelta", _Signal), ("dz", _Signal), ("dwrite", _Signal),
-                ("dread", _Signal), ("dstate", _ptr), ("drates", _ptr), ("dskip", _ptr),
-                ("ddelta_bias", _ptr), ("partials", _ptr)]
+_Sizes = _i64 * 4
 
 
 @lru_cache(maxsize=1)
 def _library() -> ctypes.CDLL:
     lib = load_library()
-    for name, kind in (("ns_conv_forward", _ConvArgs), ("ns_conv_step", _ConvArgs),
-                       ("ns_conv_backward", _ConvArgs), ("ns_scan_forward", _ScanArgs),
-                       ("ns_scan_step", _ScanArgs), ("ns_scan_backward", _ScanArgs)):
+    for name in ("ns_conv_forward", "ns_conv_step", "ns_conv_backward", "ns_scan_forward",
+                 "ns_scan_step", "ns_scan_backward"):
         fn = getattr(lib, name)
-        fn.restype, fn.argtypes = ctypes.c_int, [ctypes.POINTER(kind), _ptr]
-    for name, kind in (("ns_conv_backward_floats", _ConvArgs),
-                       ("ns_scan_checkpoint_floats", _ScanArgs),
-                       ("ns_scan_chunk_floats", _ScanArgs),
-                       ("ns_scan_backward_floats", _ScanArgs)):
-        fn = getattr(lib, name)
-        fn.restype, fn.argtypes = _i64, [ctypes.POINTER(kind)]
-    lib.ns_conv_chunk.restype = _i64
-    lib.ns_conv_chunk.argtypes = [_i64, _i64, _i64, _i32, _i32]
-    lib.ns_scan_chunks.restype = _i32
-    lib.ns_scan_chunks.argtypes = [_i64, _i64, _i64, _i64, _i32, _i32]
+        fn.restype, fn.argtypes = ctypes.c_int, [_ptr, _ptr]
+    lib.ns_conv_backward_floats.restype = _i64
+    lib.ns_conv_backward_floats.argtypes = [_ptr]
+    lib.ns_scan_plan.restype = ctypes.c_int
+    lib.ns_scan_plan.argtypes = [_i64, _i64, _i64, _i64, _i32, _i32, _ptr]
     return lib
 
 
-def on_device(device: torch.device):
-    """A guard that makes ``device`` current where it is not."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return nullcontext()
-    return torch.cuda.device(device)
+def call(fn, device: torch.device, *args) -> None:
+    """A library function with ``device`` current, on torch's current stream (its last
+    argument)."""
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        code = fn(*args, _RAW_STREAM(index))
+    else:
+        with torch.cuda.device(device):
+            code = fn(*args, _RAW_STREAM(index))
+    if code:
+        _raise_on(code, load_library())
 
 
-def _call(name: str, args, device: torch.device) -> None:
-    lib = _library()
-    with on_device(device):
-        stream = torch.cuda.current_stream(device).cuda_stream
-        _raise_on(getattr(lib, name)(ctypes.byref(args), stream), lib)
+def _address(value: torch.Tensor | None) -> int:
+    return 0 if value is None else value.data_ptr()
 
 
-def _floats(name: str, args, device: torch.device):
-    """A workspace of the size ``name`` gives (None: none needed)."""
-    lib = _library()
-    count = getattr(lib, name)(ctypes.byref(args))
-    if count < 0:
-        _raise_on(1, lib)
-    return torch.empty(count, dtype=torch.float32, device=device) if count else None
-
-
-def _address(value: torch.Tensor | None):
-    return None if value is None or value.numel() == 0 else value.data_ptr()
-
-
-def _signal(value: torch.Tensor | None) -> _Signal:
-    if value is None or value.numel() == 0:
-        return _Signal(None, 0, 0)
-    return _Signal(value.data_ptr(), value.stride(0), value.stride(1))
+def _signal(value: torch.Tensor | None) -> tuple[int, int, int]:
+    """(address, tick stride, column stride); an empty tensor's address is 0."""
+    if value is None:
+        return _ABSENT
+    return value.data_ptr(), value.stride(0), value.stride(1)
 
 
 def _unit_channels(value: torch.Tensor | None, inner: int = 1):
     """``value`` with its last ``inner`` dimensions dense (a copy where they are not)."""
     if value is None:
         return None
+    if value.is_contiguous():
+        return value
     width = 1
     for k in range(1, inner + 1):
         if value.shape[-k] != 1 and value.stride(-k) != width:
@@ -131,7 +105,7 @@ def _unit_channels(value: torch.Tensor | None, inner: int = 1):
 def _check_signal(x, what: str, dims: int) -> None:
     if not isinstance(x, torch.Tensor) or x.dim() != dims:
         raise ValueError(f"{what} must be a {'[T, B, N]' if dims == 3 else '[B, N]'} tensor")
-    if x.device.type != "cuda":
+    if not x.is_cuda:
         raise ValueError(f"{what} must be on a GPU")
     if x.dtype not in TYPES:
         raise ValueError(f"{what} must be float32, bfloat16 or float16")
@@ -139,14 +113,11 @@ def _check_signal(x, what: str, dims: int) -> None:
         raise ValueError(f"{what} has no channels")
 
 
-def _check_like(value, like: torch.Tensor, shape, what: str, dtype=None) -> None:
-    if value is None:
-        return
-    if not isinstance(value, torch.Tensor) or tuple(value.shape) != tuple(shape):
+def _check_like(value, what: str, shape: tuple, device: torch.device, dtype) -> None:
+    if not isinstance(value, torch.Tensor) or value.shape != shape:
         raise ValueError(f"{what} must be a tensor of shape {list(shape)}")
-    if value.device != like.device:
+    if value.device != device:
         raise ValueError(f"{what} must be on the signal's device")
-    dtype = dtype or like.dtype
     if value.dtype != dtype:
         raise ValueError(f"{what} must be {str(dtype).removeprefix('torch.')}")
 
@@ -170,11 +141,15 @@ def _master(value: torch.Tensor | None):
 
 
 def _dense(value: torch.Tensor | None):
-    return None if value is None else value.detach().contiguous()
+    return value if value is None or value.is_contiguous() else value.contiguous()
 
 
 def _needs_grad(*values) -> bool:
-    return torch.is_grad_enabled() and any(v is not None and v.requires_grad for v in values)
+    if torch.is_grad_enabled():
+        for value in values:
+            if value is not None and value.requires_grad:
+                return True
+    return False
 
 
 # ---- convolution ---------------------------------------------------------------------
@@ -184,35 +159,36 @@ _ACTIVATIONS = {None: 0, "silu": 1}
 
 def _check_conv(x, weight, bias, history, activation, dims: int) -> None:
     _check_signal(x, "x", dims)
-    channels = x.shape[-1]
+    shape, device = x.shape, x.device
+    channels = shape[-1]
     if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or weight.shape[0] != channels:
         raise ValueError("weight must be a [N, W] tensor")
-    if not 1 <= weight.shape[1] <= MAX_TAPS:
+    taps = weight.shape[1]
+    if not 1 <= taps <= MAX_TAPS:
         raise ValueError(f"a convolution has 1 to {MAX_TAPS} taps")
-    for value, what, shape in ((weight, "weight", weight.shape), (bias, "bias", (channels,))):
-        _check_like(value, x, shape, what, dtype=getattr(value, "dtype", None))
-        if value is not None and value.dtype not in TYPES:
-            raise ValueError(f"{what} must be float32, bfloat16 or float16")
-    _check_like(history, x, (weight.shape[1] - 1, x.shape[-2], channels), "history")
+    if weight.device != device:
+        raise ValueError("weight must be on the signal's device")
+    if weight.dtype not in TYPES:
+        raise ValueError("weight must be float32, bfloat16 or float16")
+    if bias is not None:
+        dtype = getattr(bias, "dtype", None)
+        _check_like(bias, "bias", (channels,), device, dtype if dtype in TYPES else torch.float32)
+    if history is not None:
+        _check_like(history, "history", (taps - 1, shape[-2], channels), device, x.dtype)
     if activation not in _ACTIVATIONS:
         raise ValueError("activation must be 'silu' or None")
 
 
-def _conv_args(x, weight, bias, history, lengths, silu) -> _ConvArgs:
-    args = _ConvArgs(*x.shape, weight.shape[1], TYPES[x.dtype], silu)
-    args.x, args.history = _signal(x), _signal(history)
-    args.weight, args.bias = _address(weight), _address(bias)
-    args.lengths = _address(lengths)
-    return args
-
-
-def _conv_forward(x, weight, bias, history, lengths, silu):
-    """(y, last inputs) of detached dense operands."""
-    args = _conv_args(x, weight, bias, history, lengths, silu)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    last = torch.empty((weight.shape[1] - 1, *x.shape[1:]), dtype=x.dtype, device=x.device)
-    args.y, args.out_history = _signal(y), _signal(last)
-    _call("ns_conv_forward", args, x.device)
+def _conv_forward(x, weight, bias, history, lengths, silu, chunk=0):
+    """(y, last inputs) of dense operands."""
+    ticks, batch, n = x.shape
+    taps, device = weight.shape[1], x.device
+    y = torch.empty((ticks, batch, n), dtype=x.dtype, device=device)
+    last = torch.empty((taps - 1, batch, n), dtype=x.dtype, device=device)
+    args = _CONV_FORWARD.pack(ticks, batch, n, taps, TYPES[x.dtype], silu, chunk, *_signal(x),
+                              weight.data_ptr(), _address(bias), *_signal(history),
+                              _address(lengths), *_signal(y), *_signal(last))
+    call(_library().ns_conv_forward, device, args)
     return y, last
 
 
@@ -228,21 +204,24 @@ class _CausalConv(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy, dlast):
         x, weight, bias, history, lengths = ctx.saved_tensors
-        wants = ctx.needs_input_grad
-        channels, taps = weight.shape
-        args = _conv_args(x, weight, bias, history, lengths, ctx.silu)
+        wants, device = ctx.needs_input_grad, x.device
+        (ticks, batch, channels), taps = x.shape, weight.shape[1]
         dy, dlast = _unit_channels(dy), _unit_channels(dlast)
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if wants[0] else None
-        dhistory = (torch.empty(history.shape, dtype=x.dtype, device=x.device)
+        dx = torch.empty(x.shape, dtype=x.dtype, device=device) if wants[0] else None
+        dhistory = (torch.empty(history.shape, dtype=x.dtype, device=device)
                     if history is not None and wants[3] else None)
-        sums = torch.empty(channels * (taps + 1), dtype=torch.float32, device=x.device)
-        partials = _floats("ns_conv_backward_floats", args, x.device)
-        args.dy, args.dout_history = _signal(dy), _signal(dlast)
-        args.dx, args.dhistory = _signal(dx), _signal(dhistory)
-        args.partials, args.dweight = _address(partials), sums.data_ptr()
-        _call("ns_conv_backward", args, x.device)
+        lib, count = _library(), channels * (taps + 1)
+        head = (ticks, batch, channels, taps, TYPES[x.dtype], ctx.silu, 0, *_signal(x),
+                weight.data_ptr(), _address(bias), *_signal(history), _address(lengths))
+        parts = lib.ns_conv_backward_floats(_CONV.pack(*head, *_ABSENT * 6, 0, 0))
+        if parts < 0:
+            _raise_on(1, lib)
+        sums = torch.empty(count + parts, dtype=torch.float32, device=device)
+        args = _CONV.pack(*head, *_ABSENT, *_ABSENT, *_signal(dy), *_signal(dlast), *_signal(dx),
+                          *_signal(dhistory), sums.data_ptr() + 4 * count, sums.data_ptr())
+        call(lib.ns_conv_backward, device, args)
         return (dx, sums[:channels * taps].view(channels, taps) if wants[1] else None,
-                sums[channels * taps:] if bias is not None and wants[2] else None, dhistory,
+                sums[channels * taps:count] if bias is not None and wants[2] else None, dhistory,
                 None, None)
 
 
@@ -270,21 +249,30 @@ def causal_conv_step(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor |
     _check_conv(x, weight, bias, history, activation, 2)
     if _needs_grad(x, weight, bias, history):
         raise ValueError("a step gives no gradients; use causal_conv")
-    if history is None or (weight.shape[1] > 1 and not _own_elements(history)):
+    batch, n = x.shape
+    taps = weight.shape[1]
+    if history is None or (taps > 1 and not _own_elements(history)):
         raise ValueError("history must be a [W-1, B, N] tensor with dense channels, updated in place")
-    weight, bias, x = _dense(_master(weight)), _dense(_master(bias)), _unit_channels(x)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    args = _conv_args(x.unsqueeze(0), weight, bias, history, None, _ACTIVATIONS[activation])
-    args.out_history, args.y = args.history, _signal(y.unsqueeze(0))
-    _call("ns_conv_step", args, x.device)
+    if weight.dtype != torch.float32 or not weight.is_contiguous():
+        weight = _dense(_master(weight))
+    if bias is not None and (bias.dtype != torch.float32 or bias.stride(0) != 1):
+        bias = _dense(_master(bias))
+    if n > 1 and x.stride(1) != 1:
+        x = x.contiguous()
+    y = torch.empty((batch, n), dtype=x.dtype, device=x.device)
+    carried = _signal(history)
+    args = _CONV_FORWARD.pack(1, batch, n, taps, TYPES[x.dtype], _ACTIVATIONS[activation], 0,
+                              x.data_ptr(), 0, x.stride(0), weight.data_ptr(), _address(bias),
+                              *carried, 0, y.data_ptr(), 0, n, *carried)
+    call(_library().ns_conv_step, x.device, args)
     return y
 
 
 def _own_elements(value: torch.Tensor) -> bool:
     """Channels dense and no two elements the same memory."""
-    rows, columns, n = value.shape
-    if value.numel() == 0:
+    if value.is_contiguous() or value.numel() == 0:
         return True
+    rows, columns, n = value.shape
     if n > 1 and value.stride(2) != 1:
         return False
     near, far = sorted((s, c) for s, c in ((value.stride(0), rows), (value.stride(1), columns))
@@ -300,7 +288,7 @@ def _own_elements(value: torch.Tensor) -> bool:
 def _check_scan(x, delta, A, B, C, D, z, delta_bias, state, dims: int) -> tuple[int, int]:
     """(groups, states) of valid operands."""
     _check_signal(x, "x", dims)
-    lead, channels = tuple(x.shape[:-1]), x.shape[-1]
+    *lead, channels = x.shape
     if not isinstance(A, torch.Tensor) or A.dim() != 2 or A.shape[0] != channels:
         raise ValueError("A must be a [N, S] tensor")
     states = A.shape[1]
@@ -308,34 +296,36 @@ def _check_scan(x, delta, A, B, C, D, z, delta_bias, state, dims: int) -> tuple[
         raise ValueError(f"a channel has 1 to {MAX_STATES} states")
     if not isinstance(B, torch.Tensor) or B.dim() not in (dims, dims + 1):
         raise ValueError("B must be [T, B, S] or [T, B, G, S] (without T for a step)")
-    groups = B.shape[-2] if B.dim() == dims + 1 else 1
+    grouped = B.dim() == dims + 1
+    groups = B.shape[-2] if grouped else 1
     if groups == 0 or channels % groups:
         raise ValueError("the groups of B and C must divide the channels")
-    shared = (*lead, groups, states) if B.dim() == dims + 1 else (*lead, states)
-    for value, what, shape, dtype in (
-            (delta, "delta", x.shape, x.dtype), (z, "z", x.shape, x.dtype),
-            (B, "B", shared, x.dtype), (C, "C", shared, x.dtype),
-            (A, "A", A.shape, torch.float32), (D, "D", (channels,), torch.float32),
-            (delta_bias, "delta_bias", (channels,), torch.float32),
-            (state, "state", (x.shape[-2], channels, states), torch.float32)):
-        if value is None and what in ("delta", "C"):
-            raise ValueError(f"{what} is required")
-        _check_like(value, x, shape, what, dtype=dtype)
+    device, dtype, full = x.device, x.dtype, (*lead, channels)
+    shared = (*lead, groups, states) if grouped else (*lead, states)
+    if delta is None or C is None:
+        raise ValueError(f"{'delta' if delta is None else 'C'} is required")
+    _check_like(delta, "delta", full, device, dtype)
+    _check_like(B, "B", shared, device, dtype)
+    _check_like(C, "C", shared, device, dtype)
+    _check_like(A, "A", (channels, states), device, torch.float32)
+    if z is not None:
+        _check_like(z, "z", full, device, dtype)
+    if D is not None:
+        _check_like(D, "D", (channels,), device, torch.float32)
+    if delta_bias is not None:
+        _check_like(delta_bias, "delta_bias", (channels,), device, torch.float32)
+    if state is not None:
+        _check_like(state, "state", (lead[-1], channels, states), device, torch.float32)
     return groups, states
 
 
-def _scan_args(x, delta, A, B, C, D, z, delta_bias, lengths, softplus, groups) -> _ScanArgs:
-    args = _ScanArgs(*x.shape, groups, A.shape[1], TYPES[x.dtype], int(softplus), 1)
-    args.x, args.delta, args.z = _signal(x), _signal(delta), _signal(z)
-    args.write, args.read = _signal(B), _signal(C)
-    args.rates, args.skip, args.delta_bias = _address(A), _address(D), _address(delta_bias)
-    args.lengths = _address(lengths)
-    return args
-
-
-def _chunks(args: _ScanArgs, backward: bool) -> int:
-    return _library().ns_scan_chunks(args.ticks, args.batch, args.channels, args.groups,
-                                     args.states, int(backward))
+def _plan(shape, groups: int, states: int, backward: bool):
+    """(chunks of time, floats of the chunk, checkpoint and partial workspaces)."""
+    lib, sizes = _library(), _Sizes()
+    code = lib.ns_scan_plan(*shape, groups, states, backward, ctypes.addressof(sizes))
+    if code:
+        _raise_on(code, lib)
+    return sizes
 
 
 def _dense_scan(x, delta, A, B, C, D, z, delta_bias):
@@ -346,64 +336,69 @@ def _dense_scan(x, delta, A, B, C, D, z, delta_bias):
 
 def _scan_forward(operands, state, lengths, softplus, groups, keep: bool):
     """(y, final state, checkpoints or None) of dense operands."""
-    x, A = operands[0], operands[2]
-    args = _scan_args(*operands, lengths, softplus, groups)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    final = torch.empty((x.shape[1], *A.shape), dtype=torch.float32, device=x.device)
-    args.y, args.state, args.out_state = _signal(y), _address(state), _address(final)
-    args.chunks = _chunks(args, False)
-    ends = _floats("ns_scan_chunk_floats", args, x.device)
-    checkpoints = _floats("ns_scan_checkpoint_floats", args, x.device) if keep else None
-    args.ends, args.checkpoints = _address(ends), _address(checkpoints)
-    _call("ns_scan_forward", args, x.device)
-    return y, final, checkpoints
+    x, delta, A, B, C, D, z, delta_bias = operands
+    ticks, batch, n = x.shape
+    states, device = A.shape[1], x.device
+    y = torch.empty((ticks, batch, n), dtype=x.dtype, device=device)
+    final = torch.empty((batch, n, states), dtype=torch.float32, device=device)
+    chunks, ends_floats, kept_floats, _ = _plan(x.shape, groups, states, False)
+    ends = torch.empty(ends_floats, dtype=torch.float32, device=device) if ends_floats else None
+    kept = torch.empty(kept_floats, dtype=torch.float32, device=device) if keep else None
+    args = _SCAN_FORWARD.pack(
+        ticks, batch, n, groups, states, TYPES[x.dtype], softplus, chunks, *_signal(x),
+        *_signal(delta), *_signal(z), *_signal(y), *_signal(B), *_signal(C), A.data_ptr(),
+        _address(D), _address(delta_bias), _address(state), final.data_ptr(), _address(lengths),
+        _address(kept), _address(ends))
+    call(_library().ns_scan_forward, device, args)
+    return y, final, kept
 
 
 class _SelectiveScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, delta, A, B, C, D, z, delta_bias, state, lengths, softplus, groups):
         operands = _dense_scan(x, delta, A, B, C, D, z, delta_bias)
-        start = _dense(state)
-        y, final, checkpoints = _scan_forward(operands, start, lengths, softplus, groups, True)
-        ctx.save_for_backward(*operands, lengths, checkpoints)
+        y, final, kept = _scan_forward(operands, _dense(state), lengths, softplus, groups, True)
+        ctx.save_for_backward(*operands, lengths, kept)
         ctx.softplus, ctx.groups = softplus, groups
         return y, final
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dfinal):
-        *operands, lengths, checkpoints = ctx.saved_tensors
+        *operands, lengths, kept = ctx.saved_tensors
         x, delta, A, B, C, D, z, delta_bias = operands
-        wants = ctx.needs_input_grad
+        wants, device = ctx.needs_input_grad, x.device
+        ticks, batch, n = x.shape
         dfinal = dfinal.contiguous()
-        if x.shape[0] == 0 or x.shape[1] == 0:        # no tick: the state passes through
+        if ticks == 0 or batch == 0:                  # no tick: the state passes through
             zeros = [torch.zeros_like(v) if v is not None and w else None
                      for v, w in zip(operands, wants)]
             return (*zeros, dfinal if wants[8] else None, None, None, None)
-        args = _scan_args(*operands, lengths, ctx.softplus, ctx.groups)
-        dy = _unit_channels(dy)
+        dy, states = _unit_channels(dy), A.shape[1]
+        chunks, ends_floats, _, part_floats = _plan(x.shape, ctx.groups, states, True)
 
         def like(value):
             return None if value is None else torch.empty(value.shape, dtype=value.dtype,
-                                                          device=x.device)
+                                                          device=device)
 
-        dx, ddelta, dz, dB, dC, dA = (like(v) for v in (x, delta, z, B, C, A))
-        dskip, dbias = (torch.empty(x.shape[2], dtype=torch.float32, device=x.device)
-                        for _ in range(2))
-        dstate = torch.empty_like(dfinal) if wants[8] else None
-        args.dy, args.dout_state = _signal(dy), _address(dfinal)
-        args.dx, args.ddelta, args.dz = _signal(dx), _signal(ddelta), _signal(dz)
-        args.dwrite, args.dread, args.dstate = _signal(dB), _signal(dC), _address(dstate)
-        args.drates, args.dskip, args.ddelta_bias = (dA.data_ptr(), dskip.data_ptr(),
-                                                     dbias.data_ptr())
-        args.chunks = _chunks(args, True)
-        ends = _floats("ns_scan_chunk_floats", args, x.device)
-        partials = _floats("ns_scan_backward_floats", args, x.device)
-        args.ends, args.partials = _address(ends), _address(partials)
-        args.checkpoints = checkpoints.data_ptr()
-        _call("ns_scan_backward", args, x.device)
-        grads = (dx, ddelta, dA, dB, dC, dskip if D is not None else None, dz,
-                 dbias if delta_bias is not None else None, dstate)
+        dx, ddelta, dz, dB, dC = like(x), like(delta), like(z), like(B), like(C)
+        dstate = like(dfinal) if wants[8] else None
+        # The parameters' gradients and the workspaces share one allocation.
+        sums = torch.empty(n * (states + 2), dtype=torch.float32, device=device)
+        work = torch.empty(part_floats + ends_floats, dtype=torch.float32, device=device)
+        rates, skips = sums.data_ptr(), sums.data_ptr() + 4 * n * states
+        args = _SCAN.pack(
+            ticks, batch, n, ctx.groups, states, TYPES[x.dtype], ctx.softplus, chunks,
+            *_signal(x), *_signal(delta), *_signal(z), *_ABSENT, *_signal(B), *_signal(C),
+            A.data_ptr(), _address(D), _address(delta_bias), 0, 0, _address(lengths),
+            kept.data_ptr(), work.data_ptr() + 4 * part_floats if ends_floats else 0,
+            *_signal(dy), dfinal.data_ptr(), *_signal(dx), *_signal(ddelta), *_signal(dz),
+            *_signal(dB), *_signal(dC), _address(dstate), rates, skips, skips + 4 * n,
+            work.data_ptr())
+        call(_library().ns_scan_backward, device, args)
+        grads = (dx, ddelta, sums[:n * states].view(n, states), dB, dC,
+                 sums[n * states:n * (states + 1)] if D is not None else None, dz,
+                 sums[n * (states + 1):] if delta_bias is not None else None, dstate)
         return (*(g if w else None for g, w in zip(grads, wants)), None, None, None)
 
 
@@ -438,16 +433,19 @@ def selective_scan_step(x: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B
     """One tick of ``selective_scan``: ``x``, ``delta``, ``z`` [B, N], ``B`` and ``C`` [B, S]
     or [B, G, S], y [B, N]; ``state`` [B, N, S] (float32, contiguous) is updated in place.
     Keeps nothing for gradients."""
-    groups, _ = _check_scan(x, delta, A, B, C, D, z, delta_bias, state, 2)
+    groups, states = _check_scan(x, delta, A, B, C, D, z, delta_bias, state, 2)
     if _needs_grad(x, delta, A, B, C, D, z, delta_bias, state):
         raise ValueError("a step gives no gradients; use selective_scan")
     if state is None or not state.is_contiguous():
         raise ValueError("state must be a contiguous [B, N, S] tensor, updated in place")
-    operands = _dense_scan(x, delta, A, B, C, D, z, delta_bias)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    ticked = [v if i in (2, 5, 7) or v is None else v.unsqueeze(0) for i, v in enumerate(operands)]
-    args = _scan_args(*ticked, None, softplus, groups)
-    args.state = args.out_state = _address(state)
-    args.y = _signal(y.unsqueeze(0))
-    _call("ns_scan_step", args, x.device)
+    x, delta, A, B, C, D, z, delta_bias = _dense_scan(x, delta, A, B, C, D, z, delta_bias)
+    batch, n = x.shape
+    y = torch.empty((batch, n), dtype=x.dtype, device=x.device)
+    args = _SCAN_FORWARD.pack(
+        1, batch, n, groups, states, TYPES[x.dtype], softplus, 1, x.data_ptr(), 0, x.stride(0),
+        delta.data_ptr(), 0, delta.stride(0),
+        *(_ABSENT if z is None else (z.data_ptr(), 0, z.stride(0))), y.data_ptr(), 0, n,
+        B.data_ptr(), 0, B.stride(0), C.data_ptr(), 0, C.stride(0), A.data_ptr(), _address(D),
+        _address(delta_bias), state.data_ptr(), state.data_ptr(), 0, 0, 0)
+    call(_library().ns_scan_step, x.device, args)
     return y

@@ -8,8 +8,6 @@ whether it rounds or truncates), is within K 2^-23 times the sum of the terms' s
 
 from __future__ import annotations
 
-import ctypes
-
 import pytest
 import torch
 
@@ -236,7 +234,9 @@ def test_refusals(gpu):
     refuses("contiguous", MXTensor, weight.codes.t().contiguous().t(), weight.scales, 64)
     refuses("same rows", MXTensor, weight.codes, weight.scales[:3], 64)
     lib = microscaled._library()
-    args = microscaled._ProductArgs()
-    args.a, args.b = microscaled._Matrix(2, 32, None, None), microscaled._Matrix(2, 32, None, None)
-    assert lib.ns_mx_product(ctypes.byref(args), None) == 1
+    args = microscaled._PRODUCT.pack(2, 32, 0, 0, 2, 32, 0, 0, 0, 0, 2, 0, 0, 0, 0, 0)
+    assert lib.ns_mx_product(args, None) == 1
     assert b"codes and scales are required" in lib.ns_last_error()
+    args = microscaled._PRODUCT.pack(2, 2 ** 24, 0, 0, 2, 2 ** 24, 0, 0, 0, 0, 2, 0, 0, 0, 0, 0)
+    assert lib.ns_mx_product(args, None) == 1
+    assert b"at most 8388608 columns" in lib.ns_last_error()

@@ -168,13 +168,9 @@ def test_conv_chunks_do_not_change_results(gpu):
     draw = Draw(gpu, 8)
     operands = conv_operands(draw, 90, 2, 20, 4, torch.float32)
     want, last = causal_conv(**operands)
-    x, lib = operands["x"], signal_ops._library()
     for chunk in (1, 4, 7, 90, 1000):
-        y, history = torch.empty_like(want), torch.empty_like(last)
-        args = signal_ops._conv_args(x, operands["weight"], operands["bias"], operands["history"],
-                                     None, 1)
-        args.chunk, args.y, args.out_history = chunk, signal_ops._signal(y), signal_ops._signal(history)
-        signal_ops._call("ns_conv_forward", args, x.device)
+        y, history = signal_ops._conv_forward(operands["x"], operands["weight"], operands["bias"],
+                                              operands["history"], None, 1, chunk)
         assert torch.equal(y, want) and torch.equal(history, last), chunk
 
 
@@ -265,8 +261,8 @@ def test_scan_lengths(gpu, S):
 def test_scan_in_chunks_of_time(gpu, S, ragged):
     """A long signal of few channels: time is cut into chunks scanned side by side."""
     draw, T, B, N = Draw(gpu, 60 + S), 260, 2, 5
-    assert signal_ops._library().ns_scan_chunks(T, B, N, 1, S, 0) > 1
-    assert signal_ops._library().ns_scan_chunks(T, B, N, 1, S, 1) > 1
+    assert signal_ops._plan((T, B, N), 1, S, False)[0] > 1
+    assert signal_ops._plan((T, B, N), 1, S, True)[0] > 1
     operands = scan_operands(draw, T, B, N, S, 1, torch.float32)
     lengths = torch.tensor([T, 100], device=gpu) if ragged else None
     check_scan(operands, lengths, True, draw(T, B, N), draw(B, N, S))
