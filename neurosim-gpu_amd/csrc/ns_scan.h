@@ -35,7 +35,8 @@ struct ScanShape {
   int64_t group_channels, group_blocks;   // N/G; workgroups per group
   int64_t chunks, chunk;                  // chunks of `chunk` ticks (whole tiles)
   int32_t states, softplus;
-};
+};   // below 2^31: ticks (the scalar unit compares 32 bits), and batch times groups times
+     // group_blocks times chunks (scan_grid)
 
 template <class T>
 struct ScanIn {
@@ -46,25 +47,83 @@ struct ScanIn {
   const int32_t* lengths;
 };
 
+// A value that is the same in every lane of a wavefront, known as such to the compiler:
+// what is addressed by it alone is then computed once, on the scalar unit.
+__device__ __forceinline__ uint32_t uniform(uint32_t v) {
+  return __builtin_amdgcn_readfirstlane(v);
+}
+
 // A workgroup's place: channels n0 .. n0 + own - 1 of a group, column, chunk.
 struct ScanPlace {
-  int64_t n0, own, group, b, c, t0, t1;
+  int64_t n0;
+  int own, t0, t1, end;        // ticks [t0, t1), of which [t0, end) belong to the column
+  uint32_t group, block, b, c;
 };
 
-__device__ __forceinline__ ScanPlace scan_place(const ScanShape& s) {
+__device__ __forceinline__ ScanPlace scan_place(const ScanShape& s, const int32_t* lengths) {
   ScanPlace p;
-  const int64_t blocks = s.groups * s.group_blocks;
-  const int64_t line = blockIdx.x / blocks, block = blockIdx.x - line * blocks;
-  p.c = line / s.batch;
-  p.b = line - p.c * s.batch;
-  p.group = block / s.group_blocks;
-  const int64_t first = (block - p.group * s.group_blocks) * kScanChannels;
+  const uint32_t group_blocks = static_cast<uint32_t>(s.group_blocks);
+  const uint32_t blocks = static_cast<uint32_t>(s.groups) * group_blocks;
+  const uint32_t line = uniform(blockIdx.x / blocks), block = blockIdx.x - line * blocks;
+  p.c = uniform(line / static_cast<uint32_t>(s.batch));
+  p.b = line - p.c * static_cast<uint32_t>(s.batch);
+  p.group = uniform(block / group_blocks);
+  p.block = block - p.group * group_blocks;
+  const int64_t first = static_cast<int64_t>(p.block) * kScanChannels;
   p.n0 = p.group * s.group_channels + first;
   const int64_t left = s.group_channels - first;
-  p.own = left < kScanChannels ? left : kScanChannels;
-  p.t0 = p.c * s.chunk;
-  p.t1 = p.t0 + s.chunk < s.ticks ? p.t0 + s.chunk : s.ticks;
+  p.own = static_cast<int>(left < kScanChannels ? left : kScanChannels);
+  const int ticks = static_cast<int>(s.ticks), chunk = static_cast<int>(s.chunk);
+  p.t0 = static_cast<int>(p.c) * chunk;
+  p.t1 = ticks - p.t0 < chunk ? ticks : p.t0 + chunk;
+  const int length = static_cast<int>(uniform(static_cast<uint32_t>(column_ticks(lengths, p.b, ticks))));
+  p.end = length < p.t1 ? length : p.t1;
   return p;
+}
+
+// Element `lane_bytes` bytes past an address that is the same in every lane: the address
+// stays in scalar registers and the lane's part is one 32-bit offset, shared by all signals.
+template <class T>
+__device__ __forceinline__ const T& at_lane(const T* uniform_base, uint32_t lane_bytes) {
+  return *reinterpret_cast<const T*>(reinterpret_cast<const char*>(uniform_base) + lane_bytes);
+}
+template <class T>
+__device__ __forceinline__ T& at_lane(T* uniform_base, uint32_t lane_bytes) {
+  return *reinterpret_cast<T*>(reinterpret_cast<char*>(uniform_base) + lane_bytes);
+}
+
+// One tile of a signal at a workgroup's channels: wavefront w, lane l has ticks w, w+4, ...
+// of channel l.  Ticks outside [t0, end) and channels not owned read a neighbour's value,
+// which is never used: no branches between the loads.
+template <class T, int kItems>
+__device__ __forceinline__ void load_items(const Signal<T>& from, const ScanPlace& p, int t, int wave,
+                                           uint32_t lane_bytes, T (&to)[kItems]) {
+  const T* base = from.data + p.b * from.sb + p.n0;
+#pragma unroll
+  for (int i = 0; i < kItems; ++i) {
+    int tick = t + wave + 4 * i;
+    tick = tick < p.end ? tick : p.end - 1;
+    tick = tick > p.t0 ? tick : p.t0;
+    to[i] = at_lane(base + tick * from.st, lane_bytes);
+  }
+}
+
+// The lane part of a channel's address (a channel not owned: the last one's).
+template <class T>
+__device__ __forceinline__ uint32_t lane_bytes(const ScanPlace& p, int lane) {
+  return static_cast<uint32_t>(lane < p.own ? lane : p.own - 1) * sizeof(T);
+}
+
+// Has `v` computed here: the compiler otherwise moves such work to its later use, and keeps
+// its several inputs in registers across a tile's ticks instead of this one value.
+__device__ __forceinline__ void settle(float& v) { asm volatile("" : "+v"(v)); }
+
+// The thread's number, computed anew: what depends on it (places in LDS and in rows) is
+// then not kept in registers across a tile's ticks.
+__device__ __forceinline__ int fresh_thread() {
+  int thread = static_cast<int>(threadIdx.x);
+  asm volatile("" : "+v"(thread));
+  return thread;
 }
 
 // Sum over the four lanes of a channel, in every one of them (quad permutations 1032, 2301).
@@ -80,15 +139,17 @@ __device__ __forceinline__ float time_step(float raw, bool soft) { return soft ?
 // The tile's B or C rows (padded with zeros past S and past the column's end) into LDS.
 template <class T, int R, int kTicks>
 __device__ __forceinline__ void stage_shared(const Signal<T>& from, const ScanShape& s,
-                                             const ScanPlace& p, int64_t t, int64_t end,
+                                             const ScanPlace& p, int t, int thread,
                                              float (*to)[4 * R]) {
+  const T* base = from.data + p.b * from.sb + t * from.st + p.group * s.states;
 #pragma unroll
-  for (int i = threadIdx.x; i < kTicks * 4 * R; i += kThreads) {
-    const int tick = i / (4 * R), state = i % (4 * R);
-    float v = 0.0f;
-    if (state < s.states && t + tick < end)
-      v = static_cast<float>(from.row(t + tick, p.b)[p.group * s.states + state]);
-    to[tick][state] = v;
+  for (int first = 0; first < kTicks * 4 * R; first += kThreads) {
+    const int i = first + thread, tick = i / (4 * R), state = i % (4 * R);
+    if (kTicks * 4 * R % kThreads == 0 || i < kTicks * 4 * R) {
+      const bool inside = state < s.states && t + tick < p.end;
+      const T v = base[inside ? tick * from.st + state : 0];
+      to[tick][state] = inside ? static_cast<float>(v) : 0.0f;
+    }
   }
 }
 
@@ -103,16 +164,28 @@ __device__ __forceinline__ void lane_row(const float* table, int64_t n, int q, i
   }
 }
 
-// Places of a lane's R floats in the padded [line][N][4R] workspaces.
+// A lane's R floats of a padded [line][N][4R] workspace at a workgroup's channels.
 template <int R>
-__device__ __forceinline__ void load_lane(const float* from, float (&out)[R]) {
-#pragma unroll
-  for (int r = 0; r < R; ++r) out[r] = from[r];
+struct LaneStates {
+  float v[R];
+};
+template <int R>
+__device__ __forceinline__ uint32_t lane_states_bytes(int channel, int q) {
+  return static_cast<uint32_t>((channel * 4 + q) * R) * 4;
 }
 template <int R>
-__device__ __forceinline__ void store_lane(float* to, const float (&v)[R]) {
+__device__ __forceinline__ void load_lane(const float* uniform_base, uint32_t bytes, float (&out)[R]) {
+  LaneStates<R> v;
+  __builtin_memcpy(&v, &at_lane(uniform_base, bytes), sizeof(v));
 #pragma unroll
-  for (int r = 0; r < R; ++r) to[r] = v[r];
+  for (int r = 0; r < R; ++r) out[r] = v.v[r];
+}
+template <int R>
+__device__ __forceinline__ void store_lane(float* uniform_base, uint32_t bytes, const float (&v)[R]) {
+  LaneStates<R> out;
+#pragma unroll
+  for (int r = 0; r < R; ++r) out.v[r] = v[r];
+  __builtin_memcpy(&at_lane(uniform_base, bytes), &out, sizeof(out));
 }
 
 template <class T>

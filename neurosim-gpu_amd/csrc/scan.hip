@@ -27,21 +27,12 @@ struct ScanRaw {
   T x[kItems], delta[kItems], z[kItems];
 };
 
-// Requests a tile's inputs: thread (wavefront w, lane l) takes ticks w, w+4, ... of channel l.
 template <class T, int kItems, bool kEnds>
-__device__ __forceinline__ void request(const ScanIn<T>& in, const ScanPlace& p, int64_t t,
-                                        int64_t end, ScanRaw<T, kItems>& raw) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int i = 0; i < kItems; ++i) {
-    const int64_t tick = t + wave + 4 * i;
-    raw.x[i] = raw.delta[i] = raw.z[i] = static_cast<T>(0.0f);
-    if (tick < end && lane < p.own) {
-      raw.x[i] = in.x.row(tick, p.b)[p.n0 + lane];
-      raw.delta[i] = in.delta.row(tick, p.b)[p.n0 + lane];
-      if (!kEnds && in.z.data) raw.z[i] = in.z.row(tick, p.b)[p.n0 + lane];
-    }
-  }
+__device__ __forceinline__ void request(const ScanIn<T>& in, const ScanPlace& p, int t, int wave,
+                                        uint32_t bytes, ScanRaw<T, kItems>& raw) {
+  load_items<T, kItems>(in.x, p, t, wave, bytes, raw.x);
+  load_items<T, kItems>(in.delta, p, t, wave, bytes, raw.delta);
+  if (!kEnds && in.z.data) load_items<T, kItems>(in.z, p, t, wave, bytes, raw.z);
 }
 
 // kEnds: the first pass of a chunked scan, which keeps only end states and summed steps.
@@ -54,13 +45,13 @@ __global__ __launch_bounds__(kThreads) void scan_forward(ScanShape s, ScanIn<T> 
   __shared__ float2 step_of[CT][kScanChannels];          // dt, dt * x
   __shared__ float write[CT][4 * R], read[CT][4 * R];
   __shared__ float sums[CT][kScanChannels];
-  const ScanPlace p = scan_place(s);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const ScanPlace p = scan_place(s, in.lengths);
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int q = threadIdx.x & 3, channel = threadIdx.x >> 2;
   const bool own = channel < p.own;
   const int64_t n = p.n0 + (own ? channel : 0), line = p.b * s.channels + n;
-  const int64_t length = column_ticks(in.lengths, p.b, s.ticks);
-  const int64_t end = length < p.t1 ? length : p.t1;
+  const int64_t first_line = p.b * s.channels + p.n0, lines = s.batch * s.channels;
+  const uint32_t bytes = lane_bytes<T>(p, lane), state_bytes = lane_states_bytes<R>(channel, q);
 
   float rate[R], h[R];
   lane_row<R>(in.rates, n, q, s.states, own, rate);
@@ -70,7 +61,7 @@ __global__ __launch_bounds__(kThreads) void scan_forward(ScanShape s, ScanIn<T> 
 #pragma unroll
     for (int r = 0; r < R; ++r) h[r] = 0.0f;
   } else if (p.c > 0) {
-    load_lane<R>(ends + (p.c * s.batch * s.channels + line) * (4 * R) + q * R, h);
+    load_lane<R>(ends + (p.c * lines + first_line) * (4 * R), own ? state_bytes : 0, h);
   } else {
     lane_row<R>(start, line, q, s.states, own, h);
   }
@@ -78,31 +69,37 @@ __global__ __launch_bounds__(kThreads) void scan_forward(ScanShape s, ScanIn<T> 
   const float skip = in.skip && lane < p.own ? in.skip[p.n0 + lane] : 0.0f;
   float total = 0.0f;
 
-  ScanRaw<T, kItems> raw;
-  request<T, kItems, kEnds>(in, p, p.t0, end, raw);
-  for (int64_t t = p.t0; t < p.t1; t += CT) {
-    if (!kEnds && checkpoints && own) {
-      const int64_t tile = t / CT;
-      store_lane<R>(checkpoints + (tile * s.batch * s.channels + line) * (4 * R) + q * R, h);
+  ScanRaw<T, kItems> raw{};
+  if (p.t0 < p.end) request<T, kItems, kEnds>(in, p, p.t0, wave, bytes, raw);
+  const int64_t tile_floats = lines * (4 * R);
+  float* checkpoint = checkpoints ? checkpoints + p.t0 / CT * tile_floats + first_line * (4 * R)
+                                  : nullptr;
+  for (int t = p.t0; t < p.t1; t += CT) {
+    if (!kEnds && checkpoints) {
+      if (own) store_lane<R>(checkpoint, state_bytes, h);
+      checkpoint += tile_floats;
     }
     ScanItems<kItems> items;
-    if (t < end) {
+    if (t < p.end) {
 #pragma unroll
       for (int i = 0; i < kItems; ++i) {
         const int tick = wave + 4 * i;
-        const float x = static_cast<float>(raw.x[i]);
+        const bool live = t + tick < p.end && lane < p.own;
+        const float x = live ? static_cast<float>(raw.x[i]) : 0.0f;
         float dt = time_step(static_cast<float>(raw.delta[i]) + bias, s.softplus);
-        dt = t + tick < end && lane < p.own ? dt : 0.0f;
+        dt = live ? dt : 0.0f;
         step_of[tick][lane] = make_float2(dt, dt * x);
         if (!kEnds) {
           const float z = static_cast<float>(raw.z[i]);
           items.skip[i] = skip * x;
           items.gate[i] = in.z.data ? z * sigmoid(z) : 1.0f;
+          settle(items.skip[i]);
+          settle(items.gate[i]);
         }
       }
-      stage_shared<T, R, CT>(in.write, s, p, t, end, write);
-      if (!kEnds) stage_shared<T, R, CT>(in.read, s, p, t, end, read);
-      request<T, kItems, kEnds>(in, p, t + CT, end, raw);
+      stage_shared<T, R, CT>(in.write, s, p, t, static_cast<int>(threadIdx.x), write);
+      if (!kEnds) stage_shared<T, R, CT>(in.read, s, p, t, static_cast<int>(threadIdx.x), read);
+      request<T, kItems, kEnds>(in, p, t + CT, wave, bytes, raw);
       __syncthreads();
 #pragma unroll
       for (int tick = 0; tick < CT; ++tick) {
@@ -124,15 +121,15 @@ __global__ __launch_bounds__(kThreads) void scan_forward(ScanShape s, ScanIn<T> 
       for (int i = 0; i < kItems; ++i) {
         const int tick = wave + 4 * i;
         if (t + tick < p.t1 && lane < p.own)
-          y.row(t + tick, p.b)[p.n0 + lane] = static_cast<T>(
-              t + tick < end ? (sums[tick][lane] + items.skip[i]) * items.gate[i] : 0.0f);
+          at_lane(y.row(t + tick, p.b) + p.n0, bytes) = static_cast<T>(
+              t + tick < p.end ? (sums[tick][lane] + items.skip[i]) * items.gate[i] : 0.0f);
       }
     }
   }
   if (kEnds) {
     if (own) {
-      store_lane<R>(ends + (p.c * s.batch * s.channels + line) * (4 * R) + q * R, h);
-      if (q == 0) steps[p.c * s.batch * s.channels + line] = total;
+      store_lane<R>(ends + (p.c * lines + first_line) * (4 * R), state_bytes, h);
+      if (q == 0) steps[p.c * lines + line] = total;
     }
   } else if (p.c == s.chunks - 1 && own && out_state) {
 #pragma unroll
@@ -252,6 +249,7 @@ ScanShape scan_shape(const ns_scan_args* a) {
 int check_shape(const ns_scan_args* a) {
   if (a->ticks < 0 || a->batch < 0 || a->channels <= 0)
     return fail("a signal is [T, B, N] with N > 0");
+  if (a->ticks > INT32_MAX - 64) return fail("a scan takes fewer than 2^31 ticks");
   if (a->groups < 1 || a->channels % a->groups)
     return fail("the groups must divide the channels");
   if (a->states < 1 || a->states > NS_SCAN_MAX_STATES)

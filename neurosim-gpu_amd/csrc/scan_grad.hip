@@ -35,7 +35,7 @@ struct ScanOut {
   float* rate_parts;    // [chunks*B][N][S]
   float* skip_parts;    // [chunks*B][N]
   float* bias_parts;    // [chunks*B][N]
-  float* shared_parts;  // [group_blocks][T][B][G][2][4R]: dC, dB
+  float* shared_parts;  // [group_blocks][B][G][T][2][4R]: dC, dB
 };
 
 template <class T, int kItems>
@@ -45,21 +45,12 @@ struct GradRaw {
 
 template <class T, int kItems, bool kEnds>
 __device__ __forceinline__ void request(const ScanIn<T>& in, const Signal<T>& dy,
-                                        const ScanPlace& p, int64_t t, int64_t end,
+                                        const ScanPlace& p, int t, int wave, uint32_t bytes,
                                         GradRaw<T, kItems>& raw) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int i = 0; i < kItems; ++i) {
-    const int64_t tick = t + wave + 4 * i;
-    raw.x[i] = raw.delta[i] = raw.z[i] = raw.dy[i] = static_cast<T>(0.0f);
-    if (t >= p.t0 && tick < end && lane < p.own) {
-      const int64_t n = p.n0 + lane;
-      if (!kEnds) raw.x[i] = in.x.row(tick, p.b)[n];
-      raw.delta[i] = in.delta.row(tick, p.b)[n];
-      raw.dy[i] = dy.row(tick, p.b)[n];
-      if (in.z.data) raw.z[i] = in.z.row(tick, p.b)[n];
-    }
-  }
+  if (!kEnds) load_items<T, kItems>(in.x, p, t, wave, bytes, raw.x);
+  load_items<T, kItems>(in.delta, p, t, wave, bytes, raw.delta);
+  load_items<T, kItems>(dy, p, t, wave, bytes, raw.dy);
+  if (in.z.data) load_items<T, kItems>(in.z, p, t, wave, bytes, raw.z);
 }
 
 // A chunk's own adjoint at its start from zero at its end, and its summed time step.
@@ -70,13 +61,13 @@ __global__ __launch_bounds__(kThreads) void scan_adjoint_ends(ScanShape s, ScanI
   constexpr int CT = kTile<R>, kItems = CT / 4;
   __shared__ float2 step_of[CT][kScanChannels];          // dt, gy
   __shared__ float read[CT][4 * R];
-  const ScanPlace p = scan_place(s);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const ScanPlace p = scan_place(s, in.lengths);
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int q = threadIdx.x & 3, channel = threadIdx.x >> 2;
   const bool own = channel < p.own;
   const int64_t n = p.n0 + (own ? channel : 0), line = p.b * s.channels + n;
-  const int64_t length = column_ticks(in.lengths, p.b, s.ticks);
-  const int64_t end = length < p.t1 ? length : p.t1;
+  const int64_t first_line = p.b * s.channels + p.n0, lines = s.batch * s.channels;
+  const uint32_t bytes = lane_bytes<T>(p, lane), state_bytes = lane_states_bytes<R>(channel, q);
   float rate[R], g[R];
   lane_row<R>(in.rates, n, q, s.states, own, rate);
 #pragma unroll
@@ -86,22 +77,23 @@ __global__ __launch_bounds__(kThreads) void scan_adjoint_ends(ScanShape s, ScanI
   }
   const float bias = in.delta_bias && lane < p.own ? in.delta_bias[p.n0 + lane] : 0.0f;
   float total = 0.0f;
-  if (end > p.t0) {
-    const int64_t last = p.t0 + (end - 1 - p.t0) / CT * CT;
-    GradRaw<T, kItems> raw;
-    request<T, kItems, true>(in, dy, p, last, end, raw);
-    for (int64_t t = last; t >= p.t0; t -= CT) {
+  if (p.end > p.t0) {
+    const int last = p.t0 + (p.end - 1 - p.t0) / CT * CT;
+    GradRaw<T, kItems> raw{};
+    request<T, kItems, true>(in, dy, p, last, wave, bytes, raw);
+    for (int t = last; t >= p.t0; t -= CT) {
 #pragma unroll
       for (int i = 0; i < kItems; ++i) {
         const int tick = wave + 4 * i;
+        const bool live = t + tick < p.end && lane < p.own;
         const float z = static_cast<float>(raw.z[i]);
-        float dt = time_step(static_cast<float>(raw.delta[i]) + bias, s.softplus);
-        dt = t + tick < end && lane < p.own ? dt : 0.0f;
+        const float dt = time_step(static_cast<float>(raw.delta[i]) + bias, s.softplus);
         const float gate = in.z.data ? z * sigmoid(z) : 1.0f;
-        step_of[tick][lane] = make_float2(dt, static_cast<float>(raw.dy[i]) * gate);
+        step_of[tick][lane] = make_float2(live ? dt : 0.0f,
+                                          live ? static_cast<float>(raw.dy[i]) * gate : 0.0f);
       }
-      stage_shared<T, R, CT>(in.read, s, p, t, end, read);
-      request<T, kItems, true>(in, dy, p, t - CT, end, raw);
+      stage_shared<T, R, CT>(in.read, s, p, t, static_cast<int>(threadIdx.x), read);
+      request<T, kItems, true>(in, dy, p, t - CT, wave, bytes, raw);
       __syncthreads();
 #pragma unroll
       for (int tick = CT - 1; tick >= 0; --tick) {
@@ -115,8 +107,8 @@ __global__ __launch_bounds__(kThreads) void scan_adjoint_ends(ScanShape s, ScanI
     }
   }
   if (own) {
-    store_lane<R>(ends + (p.c * s.batch * s.channels + line) * (4 * R) + q * R, g);
-    if (q == 0) steps[p.c * s.batch * s.channels + line] = total;
+    store_lane<R>(ends + (p.c * lines + first_line) * (4 * R), state_bytes, g);
+    if (q == 0) steps[p.c * lines + line] = total;
   }
 }
 
@@ -142,30 +134,29 @@ __device__ __forceinline__ float row_quads(float v) {
 }
 
 template <class T, int R>
-__global__ __launch_bounds__(kThreads) void scan_backward(ScanShape s, ScanIn<T> in, ScanUp<T> up,
+__global__ __launch_bounds__(kThreads, 2) void scan_backward(ScanShape s, ScanIn<T> in, ScanUp<T> up,
                                                           ScanOut<T> out, const float* checkpoints,
                                                           const float* ends) {
   constexpr int CT = kTile<R>, kItems = CT / 4, SP = 4 * R;
-  __shared__ float4 step_of[CT][kScanChannels];          // dt, dt * x, gy
+  __shared__ float4 step_of[CT][kScanChannels];          // dt, dt * x, gy, x
   __shared__ float write[CT][SP], read[CT][SP];
   __shared__ float sum_y[CT][kScanChannels], sum_w[CT][kScanChannels], sum_f[CT][kScanChannels];
   __shared__ float parts[4][CT][2 * SP];                 // per wavefront: dC, dB
-  const ScanPlace p = scan_place(s);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const ScanPlace p = scan_place(s, in.lengths);
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int q = threadIdx.x & 3, channel = threadIdx.x >> 2;
   const bool own = channel < p.own;
   const int64_t n = p.n0 + (own ? channel : 0), line = p.b * s.channels + n;
-  const int64_t length = column_ticks(in.lengths, p.b, s.ticks);
-  const int64_t end = length < p.t1 ? length : p.t1;
-  const int64_t block = (p.n0 - p.group * s.group_channels) / kScanChannels;
+  const int64_t first_line = p.b * s.channels + p.n0, lines = s.batch * s.channels;
+  const uint32_t bytes = lane_bytes<T>(p, lane), state_bytes = lane_states_bytes<R>(channel, q);
+  // The workgroup's sums for dC and dB: [T][2][4R] of its block, column and group.
   float* shared = out.shared_parts +
-                  (block * s.ticks * s.batch * s.groups + p.b * s.groups + p.group) * (2 * SP);
-  const int64_t shared_t = s.batch * s.groups * (2 * SP);
+                  ((p.block * s.batch + p.b) * s.groups + p.group) * s.ticks * (2 * SP);
 
   float rate[R], g[R], drate[R];
   lane_row<R>(in.rates, n, q, s.states, own, rate);
   if (p.c < s.chunks - 1) {
-    load_lane<R>(ends + (p.c * s.batch * s.channels + line) * SP + q * R, g);
+    load_lane<R>(ends + (p.c * lines + first_line) * SP, own ? state_bytes : 0, g);
   } else {
     lane_row<R>(up.dout_state, line, q, s.states, own, g);
   }
@@ -179,50 +170,53 @@ __global__ __launch_bounds__(kThreads) void scan_backward(ScanShape s, ScanIn<T>
   const float skip = in.skip && lane < p.own ? in.skip[p.n0 + lane] : 0.0f;
   float dskip = 0.0f, dbias = 0.0f;
 
-  const int64_t last = p.t0 + (p.t1 - 1 - p.t0) / CT * CT;
-  GradRaw<T, kItems> raw;
-  request<T, kItems, false>(in, up.dy, p, last, end, raw);
-  for (int64_t t = last; t >= p.t0; t -= CT) {
-    if (t >= end) {                       // past the column's end: zeros
+  const int last = p.t0 + (p.t1 - 1 - p.t0) / CT * CT;
+  const int64_t tile_floats = lines * SP;
+  const float* checkpoint = checkpoints + last / CT * tile_floats + first_line * SP;
+  GradRaw<T, kItems> raw{};
+  if (p.t0 < p.end) request<T, kItems, false>(in, up.dy, p, last, wave, bytes, raw);
+  for (int t = last; t >= p.t0; t -= CT, checkpoint -= tile_floats) {
+    const int thread = fresh_thread(), lane = thread & 63;
+    const uint32_t bytes = lane_bytes<T>(p, lane);
+    if (t >= p.end) {                       // past the column's end: zeros
 #pragma unroll
       for (int i = 0; i < kItems; ++i) {
-        const int64_t tick = t + wave + 4 * i;
+        const int tick = t + wave + 4 * i;
         if (tick < p.t1 && lane < p.own) {
           const T zero = static_cast<T>(0.0f);
-          out.dx.row(tick, p.b)[p.n0 + lane] = zero;
-          out.ddelta.row(tick, p.b)[p.n0 + lane] = zero;
-          if (in.z.data) out.dz.row(tick, p.b)[p.n0 + lane] = zero;
+          at_lane(out.dx.row(tick, p.b) + p.n0, bytes) = zero;
+          at_lane(out.ddelta.row(tick, p.b) + p.n0, bytes) = zero;
+          if (in.z.data) at_lane(out.dz.row(tick, p.b) + p.n0, bytes) = zero;
         }
       }
-      for (int i = threadIdx.x; i < CT * 2 * SP; i += kThreads)
-        if (t + i / (2 * SP) < p.t1) shared[(t + i / (2 * SP)) * shared_t + i % (2 * SP)] = 0.0f;
-      request<T, kItems, false>(in, up.dy, p, t - CT, end, raw);
+      for (int i = thread; i < CT * 2 * SP; i += kThreads)
+        if (t + i / (2 * SP) < p.t1) (shared + static_cast<int64_t>(t) * (2 * SP))[i] = 0.0f;
+      if (p.t0 < p.end) request<T, kItems, false>(in, up.dy, p, t - CT, wave, bytes, raw);
       continue;
     }
-    float item_x[kItems], item_sig[kItems], item_slope[kItems];
+    float item_sig[kItems], item_slope[kItems];
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
       const int tick = wave + 4 * i;
-      const bool live = t + tick < end && lane < p.own;
-      const float x = static_cast<float>(raw.x[i]), z = static_cast<float>(raw.z[i]);
-      const float dy = static_cast<float>(raw.dy[i]);
+      const bool live = t + tick < p.end && lane < p.own;
+      const float x = live ? static_cast<float>(raw.x[i]) : 0.0f, z = static_cast<float>(raw.z[i]);
+      const float dy = live ? static_cast<float>(raw.dy[i]) : 0.0f;
       const float soft = static_cast<float>(raw.delta[i]) + bias;
       const float dt = live ? time_step(soft, s.softplus) : 0.0f;
       const float gate = sigmoid(z);
       const float gy = in.z.data ? dy * (z * gate) : dy;
-      item_x[i] = x;
       item_sig[i] = s.softplus ? sigmoid(soft) : 1.0f;
       item_slope[i] = dy * (gate * (1.0f + z * (1.0f - gate)));
-      step_of[tick][lane] = make_float4(dt, dt * x, gy, 0.0f);
+      settle(item_sig[i]);
+      settle(item_slope[i]);
+      step_of[tick][lane] = make_float4(dt, dt * x, gy, x);
     }
-    stage_shared<T, R, CT>(in.write, s, p, t, end, write);
-    stage_shared<T, R, CT>(in.read, s, p, t, end, read);
-    request<T, kItems, false>(in, up.dy, p, t - CT, end, raw);
+    stage_shared<T, R, CT>(in.write, s, p, t, thread, write);
+    stage_shared<T, R, CT>(in.read, s, p, t, thread, read);
     float start[R], h[CT][R], a[CT][R];
 #pragma unroll
     for (int r = 0; r < R; ++r) start[r] = 0.0f;
-    if (own)
-      load_lane<R>(checkpoints + (t / CT * s.batch * s.channels + line) * SP + q * R, start);
+    if (own) load_lane<R>(checkpoint, state_bytes, start);
     __syncthreads();
 #pragma unroll
     for (int tick = 0; tick < CT; ++tick) {
@@ -235,59 +229,85 @@ __global__ __launch_bounds__(kThreads) void scan_backward(ScanShape s, ScanIn<T>
         sum = fmaf(read[tick][q * R + r], h[tick][r], sum);
       }
       sum_y[tick][channel] = quad_sum(sum);
+      if (tick % 4 == 3) __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
     for (int four = CT - 4; four >= 0; four -= 4) {
-      float value[4][2 * R];              // of ticks four .. four+3: dC and dB products
+      // Half the tile's registers are free by now: the next tile's inputs fit.
+      if (four == (CT > 4 ? 4 : 0))
+        request<T, kItems, false>(in, up.dy, p, t - CT, wave, bytes, raw);
+      constexpr int RG = R < 2 ? R : 2;   // states whose B and C of four ticks are held
+      float4 d[4];
+      float through[4] = {}, flow[4] = {};
 #pragma unroll
-      for (int k = 3; k >= 0; --k) {
-        const int tick = four + k;
-        const float4 d = step_of[tick][channel];
-        float through = 0.0f, flow = 0.0f;
+      for (int k = 0; k < 4; ++k) d[k] = step_of[four + k][channel];
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-          g[r] = fmaf(read[tick][q * R + r], d.z, g[r]);
-          value[k][r] = d.z * h[tick][r];
-          value[k][R + r] = g[r] * d.y;
-          through = fmaf(g[r], write[tick][q * R + r], through);
-          g[r] *= a[tick][r];
-          const float f = g[r] * (tick ? h[tick - 1][r] : start[r]);
-          flow = fmaf(f, rate[r], flow);
-          drate[r] = fmaf(f, d.x, drate[r]);
+      for (int r0 = 0; r0 < R; r0 += RG) {
+        float w[4][RG], c[4][RG], sum_c[RG], sum_b[RG];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          __builtin_memcpy(w[k], &write[four + k][q * R + r0], sizeof(w[k]));
+          __builtin_memcpy(c[k], &read[four + k][q * R + r0], sizeof(c[k]));
         }
-        sum_w[tick][channel] = quad_sum(through);
-        sum_f[tick][channel] = quad_sum(flow);
-      }
-      // Row k of the wavefront gets tick four + k, summed over the 16 channels.
 #pragma unroll
-      for (int v = 0; v < 2 * R; ++v) {
-        const float low = join16(join32(value[0][v], value[2][v]), join32(value[1][v], value[3][v]));
-        parts[wave][four + (lane >> 4)][v < R ? q * R + v : SP + q * R + v - R] = row_quads(low);
+        for (int r = 0; r < RG; ++r) {
+          const int rr = r0 + r;
+          float dc[4], db[4];
+#pragma unroll
+          for (int k = 3; k >= 0; --k) {
+            const int tick = four + k;
+            g[rr] = fmaf(c[k][r], d[k].z, g[rr]);
+            dc[k] = d[k].z * h[tick][rr];
+            db[k] = g[rr] * d[k].y;
+            through[k] = fmaf(g[rr], w[k][r], through[k]);
+            g[rr] *= a[tick][rr];
+            const float f = g[rr] * (tick ? h[tick - 1][rr] : start[rr]);
+            flow[k] = fmaf(f, rate[rr], flow[k]);
+            drate[rr] = fmaf(f, d[k].x, drate[rr]);
+          }
+          // Row k of the wavefront gets tick four + k, summed over the 16 channels.
+          sum_c[r] = row_quads(join16(join32(dc[0], dc[2]), join32(dc[1], dc[3])));
+          sum_b[r] = row_quads(join16(join32(db[0], db[2]), join32(db[1], db[3])));
+        }
+        float* part = &parts[wave][four + (lane >> 4)][q * R + r0];
+        __builtin_memcpy(part, sum_c, sizeof(sum_c));
+        __builtin_memcpy(part + SP, sum_b, sizeof(sum_b));
+        __builtin_amdgcn_sched_barrier(0);
       }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        sum_w[four + k][channel] = quad_sum(through[k]);
+        sum_f[four + k][channel] = quad_sum(flow[k]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
     __syncthreads();
+    const int later = fresh_thread(), out_lane = later & 63;
+    const uint32_t out_bytes = lane_bytes<T>(p, out_lane);
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
       const int tick = wave + 4 * i;
-      if (t + tick < p.t1 && lane < p.own) {
-        const float4 d = step_of[tick][lane];
-        const float through = sum_w[tick][lane], inner = sum_y[tick][lane] + skip * item_x[i];
+      if (t + tick < p.t1 && out_lane < p.own) {
+        const float4 d = step_of[tick][out_lane];
+        const float through = sum_w[tick][out_lane], inner = sum_y[tick][out_lane] + skip * d.w;
         const float dx = fmaf(d.x, through, skip * d.z);
-        const float dd = fmaf(sum_f[tick][lane], kLn2, item_x[i] * through) * item_sig[i];
-        const bool live = t + tick < end;
-        out.dx.row(t + tick, p.b)[p.n0 + lane] = static_cast<T>(live ? dx : 0.0f);
-        out.ddelta.row(t + tick, p.b)[p.n0 + lane] = static_cast<T>(live ? dd : 0.0f);
+        const float dd = fmaf(sum_f[tick][out_lane], kLn2, d.w * through) * item_sig[i];
+        const bool live = t + tick < p.end;
+        at_lane(out.dx.row(t + tick, p.b) + p.n0, out_bytes) = static_cast<T>(live ? dx : 0.0f);
+        at_lane(out.ddelta.row(t + tick, p.b) + p.n0, out_bytes) = static_cast<T>(live ? dd : 0.0f);
         if (in.z.data)
-          out.dz.row(t + tick, p.b)[p.n0 + lane] = static_cast<T>(live ? item_slope[i] * inner : 0.0f);
-        dskip += live ? d.z * item_x[i] : 0.0f;
+          at_lane(out.dz.row(t + tick, p.b) + p.n0, out_bytes) = static_cast<T>(live ? item_slope[i] * inner : 0.0f);
+        dskip += live ? d.z * d.w : 0.0f;
         dbias += live ? dd : 0.0f;
       }
     }
-    for (int i = threadIdx.x; i < CT * 2 * SP; i += kThreads) {
-      const int tick = i / (2 * SP), v = i % (2 * SP);
-      if (t + tick < p.t1)
-        shared[(t + tick) * shared_t + v] = (parts[0][tick][v] + parts[1][tick][v]) +
-                                            (parts[2][tick][v] + parts[3][tick][v]);
+#pragma unroll
+    for (int first = 0; first < CT * 2 * SP; first += kThreads) {
+      const uint32_t i = first + later;
+      const float* sums = &parts[0][0][0];
+      if (i < CT * 2 * SP && t + static_cast<int>(i / (2 * SP)) < p.t1)
+        at_lane(shared + static_cast<int64_t>(t) * (2 * SP), 4 * i) =
+            (sums[i] + sums[i + CT * 2 * SP]) + (sums[i + 2 * CT * 2 * SP] + sums[i + 3 * CT * 2 * SP]);
     }
     __syncthreads();                      // before the next tile overwrites LDS
   }
@@ -313,7 +333,7 @@ __global__ __launch_bounds__(kThreads) void scan_backward(ScanShape s, ScanIn<T>
   }
 }
 
-// dC and dB: the workgroups' sums added in order, one lane per (tick, column, group, state).
+// dC and dB: the workgroups' sums added in order, one lane per (column, group, tick, state).
 template <class T>
 __global__ __launch_bounds__(kThreads) void add_shared(ScanShape s, int32_t padded,
                                                        const float* __restrict__ parts,
@@ -327,9 +347,9 @@ __global__ __launch_bounds__(kThreads) void add_shared(ScanShape s, int32_t padd
 #pragma unroll
     for (int u = 0; u < 4; ++u) four[u] += parts[(block + u) * total + id];
   for (; block < s.group_blocks; ++block) four[0] += parts[block * total + id];
-  const int64_t pair = id / (2 * padded), state = id - pair * (2 * padded);
-  const int64_t line = pair / s.groups, group = pair - line * s.groups;
-  const int64_t t = line / s.batch, b = line - t * s.batch;
+  const int64_t tick = id / (2 * padded), state = id - tick * (2 * padded);
+  const int64_t line = tick / s.ticks, t = tick - line * s.ticks;
+  const int64_t b = line / s.groups, group = line - b * s.groups;
   const int64_t own = state < padded ? state : state - padded;
   if (own < s.states)
     (state < padded ? dread : dwrite).row(t, b)[group * s.states + own] =
