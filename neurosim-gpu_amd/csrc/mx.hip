@@ -13,11 +13,6 @@ namespace {
 
 constexpr int kLaneValues = 8;
 
-template <class T>
-struct Eight {
-  T v[kLaneValues];
-};
-
 // Eight values of a row from k (zeros past K).
 template <class T>
 __device__ __forceinline__ void load_eight(const T* row, int64_t k, int64_t width, float (&out)[8]) {
@@ -52,63 +47,99 @@ __device__ __forceinline__ float scale_value(uint32_t byte) {
   return __builtin_bit_cast(float, byte ? byte << 23 : 0x00400000u);
 }
 
-template <class T>
-__global__ __launch_bounds__(kThreads) void quantize(const T* x, int64_t stride, int64_t rows,
-                                                     int64_t width, int64_t blocks, uint8_t* codes,
-                                                     uint8_t* scales) {
-  const int64_t id = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  const int64_t block = id >> 2;
-  const int part = threadIdx.x & 3;
-  if (block >= rows * blocks) return;               // whole quads
-  const int64_t row = block / blocks, k = (block - row * blocks) * NS_MX_BLOCK + part * kLaneValues;
-  float v[8];
-  load_eight(x + row * stride, k, width, v);
-  uint32_t peak = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t size = __builtin_bit_cast(uint32_t, v[i]) & 0x7FFFFFFFu;
-    peak = size > peak ? size : peak;
-  }
-  const uint32_t byte = scale_byte(quad_max(peak));
-  uint32_t packed = 0;
-  if (byte != 255u) {
-    // The conversion divides by the scale, rounds to nearest even and saturates.
-    const float unit = scale_value(byte);
-    packed = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(packed, v[0], v[1], unit, 0);
-    packed = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(packed, v[2], v[3], unit, 1);
-    packed = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(packed, v[4], v[5], unit, 2);
-    packed = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(packed, v[6], v[7], unit, 3);
-  }
-  reinterpret_cast<uint32_t*>(codes)[id] = packed;
-  if (part == 0) scales[block] = static_cast<uint8_t>(byte);
+// Pieces (of eight values) per thread, a workgroup's width apart: several requests on their
+// way at a time.  Places are counted in I, 32 bits where the pieces allow: a 64-bit division
+// per piece would cost more than the rest of its work.
+constexpr int kPieces = 4;
+
+template <class I>
+struct Piece {
+  I block, row;
+  int64_t k;
+  bool inside;
+};
+
+template <class I>
+__device__ __forceinline__ Piece<I> piece_at(I first, int i, I total, I blocks) {
+  Piece<I> p;
+  const I id = first + i * kThreads + threadIdx.x;
+  p.inside = id < total;
+  p.block = (p.inside ? id : 0) >> 2;
+  p.row = p.block / blocks;
+  p.k = static_cast<int64_t>(p.block - p.row * blocks) * NS_MX_BLOCK + (threadIdx.x & 3) * kLaneValues;
+  return p;
 }
 
-template <class T>
-__global__ __launch_bounds__(kThreads) void dequantize(const uint8_t* codes, const uint8_t* scales,
-                                                       int64_t rows, int64_t width, int64_t blocks,
-                                                       T* out, int64_t stride) {
-  const int64_t id = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  const int64_t block = id >> 2;
-  if (block >= rows * blocks) return;
-  const int64_t row = block / blocks,
-                k = (block - row * blocks) * NS_MX_BLOCK + (threadIdx.x & 3) * kLaneValues;
-  const uint32_t packed = reinterpret_cast<const uint32_t*>(codes)[id], byte = scales[block];
-  const float unit = byte == 255u ? __builtin_nanf("") : scale_value(byte);
-  Pack<T, 8> v;
+template <class T, class I>
+__global__ __launch_bounds__(kThreads) void quantize(const T* x, int64_t stride, I total,
+                                                     int64_t width, I blocks, uint8_t* codes,
+                                                     uint8_t* scales) {
+  const I first = static_cast<I>(blockIdx.x) * (kPieces * kThreads);
+  Piece<I> at[kPieces];
+  float v[kPieces][8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    // Codes to values with a unit scale, then one multiply: exact in float32.
-    const ns_v2f two = e2m1_pair(packed >> (8 * i) & 255u);
-    v.v[2 * i] = static_cast<T>(two.x * unit);
-    v.v[2 * i + 1] = static_cast<T>(two.y * unit);
+  for (int i = 0; i < kPieces; ++i) {
+    at[i] = piece_at<I>(first, i, total, blocks);
+    load_eight(x + at[i].row * stride, at[i].k, width, v[i]);
   }
-  T* to = out + row * stride + k;
-  if (k + kLaneValues <= width) {
-    store_pack<T, 8>(to, v);
-  } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (k + i < width) to[i] = v.v[i];
+  for (int i = 0; i < kPieces; ++i) {
+    uint32_t peak = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const uint32_t size = __builtin_bit_cast(uint32_t, v[i][k]) & 0x7FFFFFFFu;
+      peak = size > peak ? size : peak;
+    }
+    const uint32_t byte = scale_byte(quad_max(peak));    // whole quads are inside or not
+    // The conversion divides by the scale, rounds to nearest even and saturates.
+    const float unit = scale_value(byte);
+    uint32_t packed = 0;
+    packed = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(packed, v[i][0], v[i][1], unit, 0);
+    packed = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(packed, v[i][2], v[i][3], unit, 1);
+    packed = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(packed, v[i][4], v[i][5], unit, 2);
+    packed = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(packed, v[i][6], v[i][7], unit, 3);
+    if (byte == 255u) packed = 0;
+    if (at[i].inside) {
+      reinterpret_cast<uint32_t*>(codes)[first + i * kThreads + threadIdx.x] = packed;
+      if ((threadIdx.x & 3) == 0) scales[at[i].block] = static_cast<uint8_t>(byte);
+    }
+  }
+}
+
+template <class T, class I>
+__global__ __launch_bounds__(kThreads) void dequantize(const uint8_t* codes, const uint8_t* scales,
+                                                       I total, int64_t width, I blocks, T* out,
+                                                       int64_t stride) {
+  const I first = static_cast<I>(blockIdx.x) * (kPieces * kThreads);
+  Piece<I> at[kPieces];
+  uint32_t packed[kPieces], byte[kPieces];
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i) {
+    at[i] = piece_at<I>(first, i, total, blocks);
+    packed[i] = reinterpret_cast<const uint32_t*>(codes)[at[i].block * 4 + (threadIdx.x & 3)];
+    byte[i] = scales[at[i].block];
+  }
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i) {
+    const float unit = byte[i] == 255u ? __builtin_nanf("") : scale_value(byte[i]);
+    Pack<T, 8> v;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      // Codes to values with a unit scale, then one multiply: exact in float32.
+      const ns_v2f two = e2m1_pair(packed[i] >> (8 * k) & 255u);
+      v.v[2 * k] = static_cast<T>(two.x * unit);
+      v.v[2 * k + 1] = static_cast<T>(two.y * unit);
+    }
+    if (!at[i].inside) continue;
+    T* to = out + at[i].row * stride + at[i].k;
+    if (at[i].k + kLaneValues <= width) {
+      // Past the caches: the values are several times their codes, and evict them otherwise.
+      stream_pack<T, 8>(to, v);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (at[i].k + k < width) to[k] = v.v[k];
+    }
   }
 }
 
@@ -121,25 +152,29 @@ int check_matrix(const ns_mx_matrix* m) {
   return NS_OK;
 }
 
-int rows_grid(const ns_mx_matrix* m, dim3* grid) {
-  const int64_t blocks = (m->columns + NS_MX_BLOCK - 1) / NS_MX_BLOCK;
-  const int64_t groups = (m->rows * blocks * 4 + kThreads - 1) / kThreads;
-  if (groups > INT32_MAX) return fail("the matrix is too large for one launch");
-  *grid = dim3(static_cast<unsigned>(groups));
-  return NS_OK;
+template <class T, class I>
+void launch_rows(const ns_mx_matrix* m, void* x, int64_t stride, bool back, int64_t total,
+                 int64_t blocks, hipStream_t stream) {
+  const dim3 grid(static_cast<unsigned>((total + kPieces * kThreads - 1) / (kPieces * kThreads)));
+  if (back)
+    dequantize<T, I><<<grid, dim3(kThreads), 0, stream>>>(
+        m->codes, m->scales, static_cast<I>(total), m->columns, static_cast<I>(blocks),
+        static_cast<T*>(x), stride);
+  else
+    quantize<T, I><<<grid, dim3(kThreads), 0, stream>>>(
+        static_cast<const T*>(x), stride, static_cast<I>(total), m->columns, static_cast<I>(blocks),
+        m->codes, m->scales);
 }
 
 template <class T>
 int run_rows(const ns_mx_matrix* m, void* x, int64_t stride, bool back, hipStream_t stream) {
-  dim3 grid;
-  if (int rc = rows_grid(m, &grid)) return rc;
-  const int64_t blocks = (m->columns + NS_MX_BLOCK - 1) / NS_MX_BLOCK;
-  if (back)
-    dequantize<T><<<grid, dim3(kThreads), 0, stream>>>(m->codes, m->scales, m->rows, m->columns,
-                                                       blocks, static_cast<T*>(x), stride);
+  const int64_t blocks = (m->columns + NS_MX_BLOCK - 1) / NS_MX_BLOCK, total = m->rows * blocks * 4;
+  if (total / (kPieces * kThreads) >= INT32_MAX) return fail("the matrix is too large for one launch");
+  // The last workgroup's pieces too have to be counted within I.
+  if (total <= UINT32_MAX - kPieces * kThreads)
+    launch_rows<T, uint32_t>(m, x, stride, back, total, blocks, stream);
   else
-    quantize<T><<<grid, dim3(kThreads), 0, stream>>>(static_cast<const T*>(x), stride, m->rows,
-                                                     m->columns, blocks, m->codes, m->scales);
+    launch_rows<T, int64_t>(m, x, stride, back, total, blocks, stream);
   const hipError_t err = hipGetLastError();
   return err == hipSuccess ? NS_OK : fail_launch(back ? "dequantise" : "quantise", err);
 }

@@ -340,15 +340,132 @@ __global__ __launch_bounds__(G::threads) void product_tiles(MxView a, MxView b, 
   }
 }
 
-// The parts of K added in order.
+// Few rows of a (up to 16): bound by b's bytes, each read once.  A wavefront takes 16 columns of y (rows
+// of b) straight from memory to registers, four stages of K requested ahead; where columns
+// are few, the four wavefronts of a workgroup take a quarter of K each and meet in LDS.  A sum over K may take its blocks in any
+// order, as long as both operands do: lane l takes blocks 2(l/16) and 2(l/16) + 1 of a
+// stage for its two steps, so that four lanes read a whole line of a row and a row's two
+// scale bytes are one 16-bit word.
+struct RowPanel {
+  __amdgpu_buffer_rsrc_t codes;
+  const uint8_t* scales;       // of the lane's row
+  uint32_t row_offset;
+  int blocks;
+};
+
+// Rows row .. row + 15 of an operand (past its last row: none).
+__device__ __forceinline__ RowPanel row_panel(const MxView& m, int64_t row, int lane) {
+  const MxPanel p = panel(m, row < m.rows ? row : m.rows - 1, row < m.rows ? 16 : 0);
+  const int own = (lane & 15) < p.last ? (lane & 15) : p.last > 0 ? p.last : 0;
+  return RowPanel{p.codes, p.scales + static_cast<int64_t>(own) * p.blocks,
+                  static_cast<uint32_t>(lane & 15) * p.row_bytes, p.blocks};
+}
+
+struct RowStage {
+  v4i codes[2];
+  int scales;                  // byte 0: first step, byte 1: second
+};
+
+// Blocks and rows that do not exist read as zeros with scale 1.
+__device__ __forceinline__ void load_row_stage(const RowPanel& p, int block, RowStage& to) {
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    const uint32_t offset = block + s < p.blocks ? p.row_offset + (block + s) * 16u : 0xFFFFFFF0u;
+    to.codes[s] = __builtin_bit_cast(
+        v4i, __builtin_amdgcn_raw_buffer_load_b128(p.codes, static_cast<int>(offset), 0, 0));
+  }
+  if (p.blocks >= 2) {
+    // The row's last word holds the last block's byte second.
+    const int at = block < p.blocks - 2 ? block : p.blocks - 2;
+    uint16_t two;
+    __builtin_memcpy(&two, p.scales + at, 2);
+    to.scales = block <= p.blocks - 2 ? two : block == p.blocks - 1 ? two >> 8 | 127 << 8 : 0x7F7F;
+  } else {
+    to.scales = block == 0 ? p.scales[0] | 127 << 8 : 0x7F7F;
+  }
+}
+
+constexpr int kRowsAhead = 4;   // stages
+
+// KW wavefronts of a workgroup share a strip of 16 columns, a part of K each.
+template <int KW, class T>
+__global__ __launch_bounds__(kThreads) void product_rows(MxView a, MxView b, const float* bias,
+                                                         T* out, int64_t stride, uint32_t groups,
+                                                         uint32_t splits, float* partials) {
+  constexpr int kWaves = kThreads / 64;
+  __shared__ v4f sums[kWaves][64];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const uint32_t split = uniform(blockIdx.x / groups), group = blockIdx.x - split * groups;
+  const int64_t n0 = (static_cast<int64_t>(group) * (kWaves / KW) + wave / KW) * 16;
+  const RowPanel pa = row_panel(a, 0, lane), pb = row_panel(b, n0, lane);
+  const int blocks = static_cast<int>(a.blocks), stages = (blocks + 7) / 8;
+  const uint32_t parts = splits * KW, part = split * KW + wave % KW;
+  const int per = static_cast<int>(uniform((stages + parts - 1) / parts));
+  const int first = static_cast<int>(part) * per;
+  const int stop = first + per < stages ? first + per : stages;
+
+  v4f sum = {};
+  RowStage x[kRowsAhead], y[kRowsAhead];
+  const int mine = 2 * (lane >> 4);
+  // A stage past the end reads as zeros.
+  const auto load = [&](int stage, int to) __attribute__((always_inline)) {
+    const int block = 8 * (stage < stop ? stage : stages) + mine;
+    load_row_stage(pb, block, y[to]);
+    load_row_stage(pa, block, x[to]);
+  };
+  if (first < stop) {
+#pragma unroll
+    for (int u = 0; u < kRowsAhead; ++u) load(first + u, u);
+  }
+  for (int stage = first; stage < stop; stage += kRowsAhead) {
+#pragma unroll
+    for (int u = 0; u < kRowsAhead; ++u) {
+      sum = mx_mfma<0, 0>(y[u].codes[0], x[u].codes[0], sum, y[u].scales, x[u].scales);
+      sum = mx_mfma<1, 1>(y[u].codes[1], x[u].codes[1], sum, y[u].scales, x[u].scales);
+      if (stage + kRowsAhead < stop) load(stage + kRowsAhead + u, u);
+    }
+  }
+  sums[wave][lane] = sum;
+  __syncthreads();
+  // KW = 1: a wavefront stores its own strip; else all threads join the parts of the one.
+  const int thread = KW == 1 ? lane : static_cast<int>(threadIdx.x);
+  constexpr int kAtOnce = KW == 1 ? 4 : 16;
+  const int column = thread & 15;
+  const int64_t n = n0 + column;
+#pragma unroll
+  for (int r = 0; r < 16; r += kAtOnce) {
+    const int m = r + (thread >> 4), from = (column >> 2) * 16 + m;   // the lane that holds it
+    float total = 0.0f;
+#pragma unroll
+    for (int w = 0; w < KW; ++w)
+      total += reinterpret_cast<const float*>(&sums[KW == 1 ? wave : w][from])[column & 3];
+    if (m < a.rows && n < b.rows) {
+      if (splits > 1)
+        partials[(split * a.rows + m) * b.rows + n] = total;
+      else
+        out[m * stride + n] = static_cast<T>(total + (bias ? bias[n] : 0.0f));
+    }
+  }
+}
+
+// The parts of K added in order, eight requested at a time.
 template <class T>
 __global__ __launch_bounds__(kThreads) void add_splits(const float* __restrict__ partials,
-                                                       int64_t splits, int64_t rows, int64_t columns,
-                                                       const float* bias, T* out, int64_t stride) {
+                                                       uint32_t splits, int64_t rows,
+                                                       int64_t columns, const float* bias, T* out,
+                                                       int64_t stride) {
   const int64_t id = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
   if (id >= rows * columns) return;
   float sum = 0.0f;
-  for (int64_t k = 0; k < splits; ++k) sum += partials[k * rows * columns + id];
+  constexpr uint32_t kAhead = 8;
+  for (uint32_t k = 0; k < splits; k += kAhead) {
+    float v[kAhead];
+#pragma unroll
+    for (uint32_t u = 0; u < kAhead; ++u)
+      v[u] = partials[(k + u < splits ? k + u : k) * rows * columns + id];
+#pragma unroll
+    for (uint32_t u = 0; u < kAhead; ++u) sum += k + u < splits ? v[u] : 0.0f;
+  }
   const int64_t m = id / columns, n = id - m * columns;
   out[m * stride + n] = static_cast<T>(sum + (bias ? bias[n] : 0.0f));
 }
@@ -365,19 +482,44 @@ MxView view(const ns_mx_matrix& m) {
 using Large = Tile<8, 4, 2, 4, 2>;   // 256 x 256
 using Small = Tile<2, 2, 2, 2, 2>;   // 64 x 64
 
-// The tile for M x N: large ones where they fill the card.
-bool large_tiles(int64_t m, int64_t n) {
-  return (m + 255) / 256 * ((n + 255) / 256) >= 128;
+constexpr int64_t kFewRows = 16;     // product_rows
+
+// Which kernel multiplies M x N.  us, 64 x 64 tiles against 256 x 256: 4096^3 86 / 51;
+// 2048 x 4096 by 1024 (128 large tiles, half the compute units) 16.7 / 17.7; 2048^3 (64) 13.8 /
+// 21.  product_rows against 64 x 64 tiles: 1 x 50,000 by 1024 8.6 / 12.7, 16 x 4096 by 4096 6.8 /
+// 10; its form for 32 rows took 68 for 32 x 50,000 by 4096, the tiles 38.
+enum class Kernel { kRows, kSmall, kLarge };
+Kernel kernel_of(int64_t m, int64_t n) {
+  if (m <= kFewRows) return Kernel::kRows;
+  return (m + 255) / 256 * ((n + 255) / 256) >= 192 ? Kernel::kLarge : Kernel::kSmall;
 }
 
-// Parts that K is cut into where tiles are few: enough for four workgroups per compute
-// unit, of two stages at least.
+// Wavefronts per strip of 16 columns in product_rows: one where the strips alone give every
+// SIMD one.
+int64_t waves_per_strip(int64_t n) { return n >= 16 * 1024 ? 1 : 4; }
+
+// Parts that K is cut into where workgroups are few.  A part's sums are written, read again
+// and cost a launch (4 us), so parts are long: rows, what a wavefront requests ahead; tiles,
+// eight stages, sixteen where the tiles alone give every compute unit one.  us, whole / cut:
+// 256 x 4096 by 4096 11.4 / 16.2 (2 parts of 8 stages), 1024 x 1024 by 8192 24.3 / 21.7 (2 of
+// 16), 64 x 8192 by 8192 18.1 (2 of 16) / 15.4 (4 of 8), 33 x 1000 by 50,000 15.5 (16 of 13) /
+// 14 (28 of 7).
 int64_t parts_of_k(int64_t m, int64_t n, int64_t k) {
-  if (m <= 0 || n <= 0 || k <= 0 || large_tiles(m, n)) return 1;
-  const int64_t stages = (k + 255) / 256, tiles = (m + 63) / 64 * ((n + 63) / 64);
-  int64_t parts = 1024 / tiles;
-  if (parts > stages / 2) parts = stages / 2;
-  if (parts < 1) parts = 1;
+  if (m <= 0 || n <= 0 || k <= 0) return 1;
+  const Kernel kernel = kernel_of(m, n);
+  if (kernel == Kernel::kLarge) return 1;
+  const int64_t stages = (k + 255) / 256;
+  int64_t parts, most;
+  if (kernel == Kernel::kRows) {
+    parts = 4096 / ((n + 15) / 16 * waves_per_strip(n));
+    most = stages / (waves_per_strip(n) * kRowsAhead);
+  } else {
+    const int64_t tiles = (m + 63) / 64 * ((n + 63) / 64);
+    parts = 512 / tiles;
+    most = stages / (tiles >= 256 ? 16 : 7);
+  }
+  if (parts > most) parts = most;
+  if (parts <= 1) return 1;
   const int64_t per = (stages + parts - 1) / parts;   // no empty part
   return (stages + per - 1) / per;
 }
@@ -410,17 +552,43 @@ int run_tiles(const ns_mx_product_args* p, int64_t parts, float* partials, hipSt
 }
 
 template <class T>
+int run_rows(const ns_mx_product_args* p, int64_t parts, float* partials, hipStream_t stream) {
+  const int64_t shared = waves_per_strip(p->b.rows), strips = (p->b.rows + 15) / 16;
+  const int64_t groups = (strips * shared + 3) / 4;
+  if (groups * parts > INT32_MAX) return fail("the product is too large for one launch");
+  const dim3 grid(static_cast<unsigned>(groups * parts));
+  const MxView a = view(p->a), b = view(p->b);
+  if (shared == 1)
+    product_rows<1, T><<<grid, dim3(kThreads), 0, stream>>>(
+        a, b, p->bias, static_cast<T*>(p->out), p->stride, static_cast<uint32_t>(groups),
+        static_cast<uint32_t>(parts), partials);
+  else
+    product_rows<4, T><<<grid, dim3(kThreads), 0, stream>>>(
+        a, b, p->bias, static_cast<T*>(p->out), p->stride, static_cast<uint32_t>(groups),
+        static_cast<uint32_t>(parts), partials);
+  return launched("product");
+}
+
+template <class T>
+int run_kernel(const ns_mx_product_args* p, int64_t parts, float* partials, hipStream_t stream) {
+  switch (kernel_of(p->a.rows, p->b.rows)) {
+    case Kernel::kLarge: return run_tiles<Large, T>(p, parts, partials, stream);
+    case Kernel::kSmall: return run_tiles<Small, T>(p, parts, partials, stream);
+    default: return run_rows<T>(p, parts, partials, stream);
+  }
+}
+
+template <class T>
 int run(const ns_mx_product_args* p, float* partials, hipStream_t stream) {
   const int64_t rows = p->a.rows, columns = p->b.rows;
   const int64_t parts = parts_of_k(rows, columns, p->a.columns);
-  if (int rc = large_tiles(rows, columns) ? run_tiles<Large, T>(p, parts, partials, stream)
-                                          : run_tiles<Small, T>(p, parts, partials, stream))
-    return rc;
+  if (int rc = run_kernel<T>(p, parts, partials, stream)) return rc;
   if (parts == 1) return NS_OK;
   const int64_t adds = (rows * columns + kThreads - 1) / kThreads;
   if (adds > INT32_MAX) return fail("the product is too large for one launch");
   add_splits<T><<<dim3(static_cast<unsigned>(adds)), dim3(kThreads), 0, stream>>>(
-      partials, parts, rows, columns, p->bias, static_cast<T*>(p->out), p->stride);
+      partials, static_cast<uint32_t>(parts), rows, columns, p->bias, static_cast<T*>(p->out),
+      p->stride);
   return launched("product parts");
 }
 

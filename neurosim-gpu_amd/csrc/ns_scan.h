@@ -136,31 +136,42 @@ __device__ __forceinline__ float quad_sum(float v) {
 // A channel's time step and its slope in delta.
 __device__ __forceinline__ float time_step(float raw, bool soft) { return soft ? softplus(raw) : raw; }
 
-// The tile's B or C rows (padded with zeros past S and past the column's end) into LDS.
-template <class T, int R, int kTicks>
-__device__ __forceinline__ void stage_shared(const Signal<T>& from, const ScanShape& s,
-                                             const ScanPlace& p, int t, int thread,
-                                             float (*to)[4 * R]) {
-  const T* base = from.data + p.b * from.sb + t * from.st + p.group * s.states;
-#pragma unroll
-  for (int first = 0; first < kTicks * 4 * R; first += kThreads) {
-    const int i = first + thread, tick = i / (4 * R), state = i % (4 * R);
-    if (kTicks * 4 * R % kThreads == 0 || i < kTicks * 4 * R) {
-      const bool inside = state < s.states && t + tick < p.end;
-      const T v = base[inside ? tick * from.st + state : 0];
-      to[tick][state] = inside ? static_cast<float>(v) : 0.0f;
-    }
-  }
+// A tile's B or C rows, one value per thread: requested with the tile's other inputs, and
+// put into LDS (padded with zeros past S and past the column's end) when the tile begins.
+template <class T, int R>
+__device__ __forceinline__ T load_shared(const Signal<T>& from, const ScanShape& s,
+                                         const ScanPlace& p, int t, int thread) {
+  static_assert(kTile<R> * 4 * R <= kThreads, "one value per thread");
+  const int tick = thread / (4 * R), state = thread % (4 * R);
+  const int start = t < p.t0 ? p.t0 : t < p.end ? t : p.end - 1;
+  const T* base = from.data + p.b * from.sb + start * from.st + p.group * s.states;
+  const bool inside = state < s.states && start + tick < p.end;
+  return base[inside ? tick * from.st + state : 0];
 }
 
-// A lane's R values of row n of a [N][S] table, zero past S and for channels not owned.
-template <int R>
-__device__ __forceinline__ void lane_row(const float* table, int64_t n, int q, int32_t states,
-                                         bool own, float (&out)[R]) {
+template <class T, int R>
+__device__ __forceinline__ void place_shared(T value, const ScanShape& s, const ScanPlace& p, int t,
+                                             int thread, float (*to)[4 * R]) {
+  const int tick = thread / (4 * R), state = thread % (4 * R);
+  if (kTile<R> * 4 * R == kThreads || tick < kTile<R>)
+    to[tick][state] = state < s.states && t + tick < p.end ? static_cast<float>(value) : 0.0f;
+}
+
+// A lane's R values of row n of a [N][S] table, zero past S and for channels not owned: one
+// wide load where the lanes' parts are whole.
+template <int R, class T = float>
+__device__ __forceinline__ void lane_row(const T* table, int64_t n, int q, int32_t states, bool own,
+                                         float (&out)[R]) {
+  if (table && states == 4 * R) {
+    const Pack<T, R> v = load_pack<T, R>(table + n * (4 * R) + q * R);
+#pragma unroll
+    for (int r = 0; r < R; ++r) out[r] = own ? static_cast<float>(v.v[r]) : 0.0f;
+    return;
+  }
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const int s = q * R + r;
-    out[r] = own && table && s < states ? table[n * states + s] : 0.0f;
+    out[r] = own && table && s < states ? static_cast<float>(table[n * states + s]) : 0.0f;
   }
 }
 

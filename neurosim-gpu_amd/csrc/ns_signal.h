@@ -46,6 +46,18 @@ __device__ __forceinline__ void store_pack(T* p, const Pack<T, V>& x) {
   __builtin_memcpy(p, &x, sizeof(x));
 }
 
+// The same past the caches (non-temporal), for what is not read again soon: 16 bytes or more.
+template <class T, int V>
+__device__ __forceinline__ void stream_pack(T* p, const Pack<T, V>& x) {
+  static_assert(sizeof(x) % 16 == 0, "whole 16-byte words");
+  typedef uint32_t word __attribute__((ext_vector_type(4), aligned(2)));
+  word w[sizeof(x) / 16];
+  __builtin_memcpy(w, &x, sizeof(x));
+#pragma unroll
+  for (unsigned i = 0; i < sizeof(x) / 16; ++i)
+    __builtin_nontemporal_store(w[i], reinterpret_cast<word*>(p) + i);
+}
+
 // 1 / (1 + exp(-x)); exp overflows to infinity for very negative x, whose reciprocal is 0.
 __device__ __forceinline__ float sigmoid(float x) {
   return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * x));

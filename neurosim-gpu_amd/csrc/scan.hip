@@ -24,15 +24,17 @@ struct ScanItems {
 
 template <class T, int kItems>
 struct ScanRaw {
-  T x[kItems], delta[kItems], z[kItems];
+  T x[kItems], delta[kItems], z[kItems], write, read;
 };
 
-template <class T, int kItems, bool kEnds>
-__device__ __forceinline__ void request(const ScanIn<T>& in, const ScanPlace& p, int t, int wave,
-                                        uint32_t bytes, ScanRaw<T, kItems>& raw) {
+template <class T, int R, int kItems, bool kEnds>
+__device__ __forceinline__ void request(const ScanIn<T>& in, const ScanShape& s, const ScanPlace& p,
+                                        int t, int wave, uint32_t bytes, ScanRaw<T, kItems>& raw) {
   load_items<T, kItems>(in.x, p, t, wave, bytes, raw.x);
   load_items<T, kItems>(in.delta, p, t, wave, bytes, raw.delta);
   if (!kEnds && in.z.data) load_items<T, kItems>(in.z, p, t, wave, bytes, raw.z);
+  raw.write = load_shared<T, R>(in.write, s, p, t, threadIdx.x);
+  if (!kEnds) raw.read = load_shared<T, R>(in.read, s, p, t, threadIdx.x);
 }
 
 // kEnds: the first pass of a chunked scan, which keeps only end states and summed steps.
@@ -69,12 +71,16 @@ __global__ __launch_bounds__(kThreads) void scan_forward(ScanShape s, ScanIn<T> 
   const float skip = in.skip && lane < p.own ? in.skip[p.n0 + lane] : 0.0f;
   float total = 0.0f;
 
-  ScanRaw<T, kItems> raw{};
-  if (p.t0 < p.end) request<T, kItems, kEnds>(in, p, p.t0, wave, bytes, raw);
+  // Two tiles of inputs are on their way: a tile's ticks take about as long as one request.
+  ScanRaw<T, kItems> even{}, odd{};
+  if (p.t0 < p.end) {
+    request<T, R, kItems, kEnds>(in, s, p, p.t0, wave, bytes, even);
+    request<T, R, kItems, kEnds>(in, s, p, p.t0 + CT, wave, bytes, odd);
+  }
   const int64_t tile_floats = lines * (4 * R);
   float* checkpoint = checkpoints ? checkpoints + p.t0 / CT * tile_floats + first_line * (4 * R)
                                   : nullptr;
-  for (int t = p.t0; t < p.t1; t += CT) {
+  const auto tile = [&](int t, ScanRaw<T, kItems>& raw) __attribute__((always_inline)) {
     if (!kEnds && checkpoints) {
       if (own) store_lane<R>(checkpoint, state_bytes, h);
       checkpoint += tile_floats;
@@ -97,9 +103,9 @@ __global__ __launch_bounds__(kThreads) void scan_forward(ScanShape s, ScanIn<T> 
           settle(items.gate[i]);
         }
       }
-      stage_shared<T, R, CT>(in.write, s, p, t, static_cast<int>(threadIdx.x), write);
-      if (!kEnds) stage_shared<T, R, CT>(in.read, s, p, t, static_cast<int>(threadIdx.x), read);
-      request<T, kItems, kEnds>(in, p, t + CT, wave, bytes, raw);
+      place_shared<T, R>(raw.write, s, p, t, threadIdx.x, write);
+      if (!kEnds) place_shared<T, R>(raw.read, s, p, t, threadIdx.x, read);
+      request<T, R, kItems, kEnds>(in, s, p, t + 2 * CT, wave, bytes, raw);
       __syncthreads();
 #pragma unroll
       for (int tick = 0; tick < CT; ++tick) {
@@ -125,6 +131,10 @@ __global__ __launch_bounds__(kThreads) void scan_forward(ScanShape s, ScanIn<T> 
               t + tick < p.end ? (sums[tick][lane] + items.skip[i]) * items.gate[i] : 0.0f);
       }
     }
+  };
+  for (int t = p.t0; t < p.t1; t += 2 * CT) {
+    tile(t, even);
+    if (t + CT < p.t1) tile(t + CT, odd);
   }
   if (kEnds) {
     if (own) {
@@ -182,37 +192,39 @@ __global__ __launch_bounds__(kThreads) void scan_step(ScanShape s, ScanIn<T> in,
   const int64_t line = id >> 2;
   const int q = threadIdx.x & 3;
   if (line >= s.batch * s.channels) return;
-  const int64_t b = line / s.channels, n = line - b * s.channels, group = n / s.group_channels;
-  const float x = static_cast<float>(in.x.row(0, b)[n]);
-  const float bias = in.delta_bias ? in.delta_bias[n] : 0.0f;
-  const T* writes = in.write.row(0, b) + group * s.states;
-  const T* reads = in.read.row(0, b) + group * s.states;
+  const uint32_t channels = static_cast<uint32_t>(s.channels);   // line: below 2^31
+  const uint32_t b = static_cast<uint32_t>(line) / channels;
+  const uint32_t n = static_cast<uint32_t>(line) - b * channels;
+  const uint32_t group = n / static_cast<uint32_t>(s.group_channels);
   float rate[R], h[R], write[R], read[R];
-  lane_row<R>(in.rates, n, q, s.states, true, rate);
   lane_row<R>(state, line, q, s.states, true, h);
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int k = q * R + r;
-    write[r] = k < s.states ? static_cast<float>(writes[k]) : 0.0f;
-    read[r] = k < s.states ? static_cast<float>(reads[k]) : 0.0f;
-  }
-  const float dt = time_step(static_cast<float>(in.delta.row(0, b)[n]) + bias, s.softplus);
+  lane_row<R>(in.rates, n, q, s.states, true, rate);
+  lane_row<R, T>(in.write.row(0, b), group, q, s.states, true, write);
+  lane_row<R, T>(in.read.row(0, b), group, q, s.states, true, read);
+  const float x = static_cast<float>(in.x.row(0, b)[n]);
+  const float raw = static_cast<float>(in.delta.row(0, b)[n]);
+  const float z = in.z.data ? static_cast<float>(in.z.row(0, b)[n]) : 0.0f;
+  const float bias = in.delta_bias ? in.delta_bias[n] : 0.0f;
+  const float skip = in.skip ? in.skip[n] : 0.0f;
+  const float dt = time_step(raw + bias, s.softplus);
   float sum = 0.0f;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     h[r] = fmaf(__builtin_amdgcn_exp2f(dt * (rate[r] * kLog2e)), h[r], dt * x * write[r]);
     sum = fmaf(read[r], h[r], sum);
-    if (q * R + r < s.states) state[line * s.states + q * R + r] = h[r];
   }
-  sum = quad_sum(sum);
-  if (q == 0) {
-    sum += in.skip ? in.skip[n] * x : 0.0f;
-    if (in.z.data) {
-      const float z = static_cast<float>(in.z.row(0, b)[n]);
-      sum *= z * sigmoid(z);
-    }
-    y.row(0, b)[n] = static_cast<T>(sum);
+  if (s.states == 4 * R) {
+    Pack<float, R> out;
+#pragma unroll
+    for (int r = 0; r < R; ++r) out.v[r] = h[r];
+    store_pack<float, R>(state + line * (4 * R) + q * R, out);
+  } else {
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (q * R + r < s.states) state[line * s.states + q * R + r] = h[r];
   }
+  sum = quad_sum(sum) + skip * x;
+  if (q == 0) y.row(0, b)[n] = static_cast<T>(in.z.data ? sum * (z * sigmoid(z)) : sum);
 }
 
 // Time chunks worth scanning side by side.
@@ -306,8 +318,8 @@ int run_forward(const ns_scan_args* a, hipStream_t stream) {
 template <class T, int R>
 int run_step(const ns_scan_args* a, hipStream_t stream) {
   const ScanShape s = scan_shape(a);
+  if (s.batch * s.channels > INT32_MAX) return fail("the signal is too large for one launch");
   const int64_t groups = (s.batch * s.channels * 4 + kThreads - 1) / kThreads;
-  if (groups > INT32_MAX) return fail("the signal is too large for one launch");
   scan_step<T, R><<<dim3(static_cast<unsigned>(groups)), dim3(kThreads), 0, stream>>>(
       s, scan_in<T>(a), signal<T>(a->y), a->out_state);
   return launched("scan step");

@@ -40,17 +40,20 @@ struct ScanOut {
 
 template <class T, int kItems>
 struct GradRaw {
-  T x[kItems], delta[kItems], z[kItems], dy[kItems];
+  T x[kItems], delta[kItems], z[kItems], dy[kItems], write, read;
 };
 
-template <class T, int kItems, bool kEnds>
-__device__ __forceinline__ void request(const ScanIn<T>& in, const Signal<T>& dy,
-                                        const ScanPlace& p, int t, int wave, uint32_t bytes,
+template <class T, int R, int kItems, bool kEnds>
+__device__ __forceinline__ void request(const ScanIn<T>& in, const ScanShape& s, const Signal<T>& dy,
+                                        const ScanPlace& p, int t, int wave, int thread,
                                         GradRaw<T, kItems>& raw) {
+  const uint32_t bytes = lane_bytes<T>(p, thread & 63);
   if (!kEnds) load_items<T, kItems>(in.x, p, t, wave, bytes, raw.x);
   load_items<T, kItems>(in.delta, p, t, wave, bytes, raw.delta);
   load_items<T, kItems>(dy, p, t, wave, bytes, raw.dy);
   if (in.z.data) load_items<T, kItems>(in.z, p, t, wave, bytes, raw.z);
+  if (!kEnds) raw.write = load_shared<T, R>(in.write, s, p, t, thread);
+  raw.read = load_shared<T, R>(in.read, s, p, t, thread);
 }
 
 // A chunk's own adjoint at its start from zero at its end, and its summed time step.
@@ -67,7 +70,7 @@ __global__ __launch_bounds__(kThreads) void scan_adjoint_ends(ScanShape s, ScanI
   const bool own = channel < p.own;
   const int64_t n = p.n0 + (own ? channel : 0), line = p.b * s.channels + n;
   const int64_t first_line = p.b * s.channels + p.n0, lines = s.batch * s.channels;
-  const uint32_t bytes = lane_bytes<T>(p, lane), state_bytes = lane_states_bytes<R>(channel, q);
+  const uint32_t state_bytes = lane_states_bytes<R>(channel, q);
   float rate[R], g[R];
   lane_row<R>(in.rates, n, q, s.states, own, rate);
 #pragma unroll
@@ -79,9 +82,10 @@ __global__ __launch_bounds__(kThreads) void scan_adjoint_ends(ScanShape s, ScanI
   float total = 0.0f;
   if (p.end > p.t0) {
     const int last = p.t0 + (p.end - 1 - p.t0) / CT * CT;
-    GradRaw<T, kItems> raw{};
-    request<T, kItems, true>(in, dy, p, last, wave, bytes, raw);
-    for (int t = last; t >= p.t0; t -= CT) {
+    GradRaw<T, kItems> even{}, odd{};
+    request<T, R, kItems, true>(in, s, dy, p, last, wave, threadIdx.x, even);
+    request<T, R, kItems, true>(in, s, dy, p, last - CT, wave, threadIdx.x, odd);
+    const auto tile = [&](int t, GradRaw<T, kItems>& raw) __attribute__((always_inline)) {
 #pragma unroll
       for (int i = 0; i < kItems; ++i) {
         const int tick = wave + 4 * i;
@@ -92,8 +96,8 @@ __global__ __launch_bounds__(kThreads) void scan_adjoint_ends(ScanShape s, ScanI
         step_of[tick][lane] = make_float2(live ? dt : 0.0f,
                                           live ? static_cast<float>(raw.dy[i]) * gate : 0.0f);
       }
-      stage_shared<T, R, CT>(in.read, s, p, t, static_cast<int>(threadIdx.x), read);
-      request<T, kItems, true>(in, dy, p, t - CT, wave, bytes, raw);
+      place_shared<T, R>(raw.read, s, p, t, threadIdx.x, read);
+      request<T, R, kItems, true>(in, s, dy, p, t - 2 * CT, wave, threadIdx.x, raw);
       __syncthreads();
 #pragma unroll
       for (int tick = CT - 1; tick >= 0; --tick) {
@@ -104,6 +108,10 @@ __global__ __launch_bounds__(kThreads) void scan_adjoint_ends(ScanShape s, ScanI
           g[r] = __builtin_amdgcn_exp2f(d.x * rate[r]) * fmaf(read[tick][q * R + r], d.y, g[r]);
       }
       __syncthreads();
+    };
+    for (int t = last; t >= p.t0; t -= 2 * CT) {
+      tile(t, even);
+      if (t - CT >= p.t0) tile(t - CT, odd);
     }
   }
   if (own) {
@@ -148,7 +156,7 @@ __global__ __launch_bounds__(kThreads, 2) void scan_backward(ScanShape s, ScanIn
   const bool own = channel < p.own;
   const int64_t n = p.n0 + (own ? channel : 0), line = p.b * s.channels + n;
   const int64_t first_line = p.b * s.channels + p.n0, lines = s.batch * s.channels;
-  const uint32_t bytes = lane_bytes<T>(p, lane), state_bytes = lane_states_bytes<R>(channel, q);
+  const uint32_t state_bytes = lane_states_bytes<R>(channel, q);
   // The workgroup's sums for dC and dB: [T][2][4R] of its block, column and group.
   float* shared = out.shared_parts +
                   ((p.block * s.batch + p.b) * s.groups + p.group) * s.ticks * (2 * SP);
@@ -174,7 +182,7 @@ __global__ __launch_bounds__(kThreads, 2) void scan_backward(ScanShape s, ScanIn
   const int64_t tile_floats = lines * SP;
   const float* checkpoint = checkpoints + last / CT * tile_floats + first_line * SP;
   GradRaw<T, kItems> raw{};
-  if (p.t0 < p.end) request<T, kItems, false>(in, up.dy, p, last, wave, bytes, raw);
+  if (p.t0 < p.end) request<T, R, kItems, false>(in, s, up.dy, p, last, wave, threadIdx.x, raw);
   for (int t = last; t >= p.t0; t -= CT, checkpoint -= tile_floats) {
     const int thread = fresh_thread(), lane = thread & 63;
     const uint32_t bytes = lane_bytes<T>(p, lane);
@@ -191,7 +199,8 @@ __global__ __launch_bounds__(kThreads, 2) void scan_backward(ScanShape s, ScanIn
       }
       for (int i = thread; i < CT * 2 * SP; i += kThreads)
         if (t + i / (2 * SP) < p.t1) (shared + static_cast<int64_t>(t) * (2 * SP))[i] = 0.0f;
-      if (p.t0 < p.end) request<T, kItems, false>(in, up.dy, p, t - CT, wave, bytes, raw);
+      if (p.t0 < p.end)
+        request<T, R, kItems, false>(in, s, up.dy, p, t - CT, wave, thread, raw);
       continue;
     }
     float item_sig[kItems], item_slope[kItems];
@@ -211,8 +220,8 @@ __global__ __launch_bounds__(kThreads, 2) void scan_backward(ScanShape s, ScanIn
       settle(item_slope[i]);
       step_of[tick][lane] = make_float4(dt, dt * x, gy, x);
     }
-    stage_shared<T, R, CT>(in.write, s, p, t, thread, write);
-    stage_shared<T, R, CT>(in.read, s, p, t, thread, read);
+    place_shared<T, R>(raw.write, s, p, t, thread, write);
+    place_shared<T, R>(raw.read, s, p, t, thread, read);
     float start[R], h[CT][R], a[CT][R];
 #pragma unroll
     for (int r = 0; r < R; ++r) start[r] = 0.0f;
@@ -235,7 +244,7 @@ __global__ __launch_bounds__(kThreads, 2) void scan_backward(ScanShape s, ScanIn
     for (int four = CT - 4; four >= 0; four -= 4) {
       // Half the tile's registers are free by now: the next tile's inputs fit.
       if (four == (CT > 4 ? 4 : 0))
-        request<T, kItems, false>(in, up.dy, p, t - CT, wave, bytes, raw);
+        request<T, R, kItems, false>(in, s, up.dy, p, t - CT, wave, fresh_thread(), raw);
       constexpr int RG = R < 2 ? R : 2;   // states whose B and C of four ticks are held
       float4 d[4];
       float through[4] = {}, flow[4] = {};
