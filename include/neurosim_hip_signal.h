@@ -57,15 +57,16 @@ typedef struct ns_conv_args {
   ns_signal dout_history;      /* gradient of out_history, or absent */
   ns_signal dx;                /* absent: not written */
   ns_signal dhistory;          /* absent: not written */
-  float* partials;             /* workspace of ns_conv_backward_floats floats */
-  float* dweight;              /* [N][W] and bias gradient [N] behind it: [N*(W+1)]; */
+  float* partials;             /* workspace (ns_conv_backward_floats) */
+  float* dweight;              /* [N][W], and the bias gradient [N] behind it */
 } ns_conv_args;
 
 /* Ticks per thread that ns_conv_forward (`backward` zero) and ns_conv_backward use. */
 int64_t ns_conv_chunk(int64_t ticks, int64_t batch, int64_t channels, int32_t type,
                       int32_t backward);
-/* Floats of ns_conv_backward's workspace. */
-int64_t ns_conv_backward_floats(const ns_conv_args* args);
+/* Floats of ns_conv_backward's workspace (with `chunk` 0). */
+int64_t ns_conv_backward_floats(int64_t ticks, int64_t batch, int64_t channels, int32_t taps,
+                                int32_t type);
 int ns_conv_forward(const ns_conv_args* args, void* stream);
 /* One tick (ticks == 1, no lengths), `out_history` the history itself, moved on in place. */
 int ns_conv_step(const ns_conv_args* args, void* stream);

@@ -402,11 +402,11 @@ int64_t ns_conv_chunk(int64_t ticks, int64_t batch, int64_t channels, int32_t ty
   return chunk < least ? least : (chunk > most ? most : chunk);
 }
 
-int64_t ns_conv_backward_floats(const ns_conv_args* a) {
-  ns::clear_error();
-  if (ns::check_conv(a) != NS_OK) return -1;
-  const ns::ConvShape s = ns::shape_of(a, true);
-  return s.chunks * s.batch * s.channels * (a->taps + 1);
+int64_t ns_conv_backward_floats(int64_t ticks, int64_t batch, int64_t channels, int32_t taps,
+                                int32_t type) {
+  if (ticks <= 0 || batch <= 0 || channels <= 0) return batch > 0 ? batch * channels * (taps + 1) : 0;
+  const int64_t chunk = ns_conv_chunk(ticks, batch, channels, type, 1);
+  return (ticks + chunk - 1) / chunk * batch * channels * (taps + 1);
 }
 
 int ns_conv_forward(const ns_conv_args* a, void* stream) {

@@ -4,6 +4,8 @@
 // mfma_scale 16x16x128, lane l holds row l%16 of an operand, block l/16 of four (16 bytes
 // of codes, one scale byte), so a lane's operand is one 16-byte load; the 16x16 result has
 // column l%16 and rows 4*(l/16) .. +3 in lane l's four registers.
+#include <cstddef>
+
 #include "ns_signal.h"
 #include "neurosim_hip_mx.h"
 
@@ -36,8 +38,8 @@ struct Tile {
 };
 
 // One stage's operands in LDS.  Codes: rows of 8 blocks, 128 bytes, a whole cache line each,
-// with block k of row r at place k ^ (r % 8): the eight lanes that LDS serves at a time read
-// one block of eight rows, and so find them in eight different places.  Scale bytes of (step 0, step 1) as one 16-bit word per (wavefront row, lane, strip), so a
+// with block k of row r at place k ^ (r/2 % 8): a fragment, blocks 4s .. 4s+3 of 16 rows, is then
+// read without bank conflicts (so it is with r % 8; blocks 0, 2, 4, 6 would conflict).  Scale bytes of (step 0, step 1) as one 16-bit word per (wavefront row, lane, strip), so a
 // lane reads all its strips' scales at once and the instruction picks the byte it needs.
 template <class G>
 struct Stage {
@@ -88,8 +90,9 @@ template <class G, bool kWhole>
 __device__ __forceinline__ void request_codes(const MxPanel& a, const MxPanel& b, int block, int stop,
                                               int wave, int lane, Stage<G>& to) {
   constexpr int kPerRound = G::threads / 8;                // rows per load instruction of all waves
-  const int at = block + ((lane & 7) ^ (lane >> 3));
-  const uint32_t row = 8 * wave + (lane >> 3), column = static_cast<uint32_t>(at) * 16;
+  const uint32_t row = 8 * wave + (lane >> 3);
+  const int at = block + static_cast<int>((lane & 7) ^ (row >> 1 & 7));
+  const uint32_t column = static_cast<uint32_t>(at) * 16;
   const bool inside = at < stop;
   constexpr int kLoadsA = G::rows_m / kPerRound;           // the first ones are a's
 #pragma unroll
@@ -184,7 +187,7 @@ __device__ __forceinline__ void read_fragments(const Stage<G>& from, int wm, int
   load_scales<G::NJ>(from.scales_b[wn][lane], f.scale_b);
 #pragma unroll
   for (int s = 0; s < G::KS; ++s) {
-    const int place = (4 * s + (lane >> 4)) ^ (lane & 7);
+    const int place = (4 * s + (lane >> 4)) ^ (lane >> 1 & 7);
 #pragma unroll
     for (int i = 0; i < G::MI; ++i)
       f.a[s][i] = from.codes[((wm * G::MI + i) * 16 + (lane & 15)) * 8 + place];
@@ -338,6 +341,179 @@ __global__ __launch_bounds__(G::threads) void product_tiles(MxView a, MxView b, 
     store_tiles<G, T>(out + m * stride + n, stride, sum, bias ? bias + n : nullptr, a.rows - m,
                       b.rows - n, lane, lds.strip[wave]);
   }
+}
+
+// Large tiles where rows of scales are whole 32-bit words (K a multiple of 128): scales too go
+// straight into LDS, nothing passes through registers on its way there, and the next stages
+// are requested two ahead.  A stage's buffer is free as soon as every wavefront has its
+// fragments in registers, so a second barrier there lets the stage after next be requested
+// before this one is multiplied: two stages' time for a request instead of three quarters of
+// one (8192^3: see below).  The requests are inline assembly because the compiler, which
+// cannot tell the two buffers apart, would wait for all of them before it reads either; they
+// write LDS only, no registers, and the waits below count them.
+struct alignas(16) WordPanel {
+  v4i codes, scales;           // buffer descriptors
+  uint32_t row_bytes, blocks;
+};
+
+__device__ __forceinline__ v4i describe(const uint8_t* base, uint32_t bytes) {
+  const uint64_t address = reinterpret_cast<uint64_t>(base);
+  return v4i{static_cast<int>(uniform(static_cast<uint32_t>(address))),
+             static_cast<int>(uniform(static_cast<uint32_t>(address >> 32))),
+             static_cast<int>(uniform(bytes)), 0x00020000};
+}
+
+__device__ __forceinline__ WordPanel word_panel(const MxView& m, int64_t row, int rows) {
+  const uint32_t own = static_cast<uint32_t>(m.rows - row < rows ? m.rows - row : rows);
+  const uint32_t blocks = uniform(static_cast<uint32_t>(m.blocks));
+  return WordPanel{describe(m.codes + row * m.blocks * 16, own * blocks * 16),
+                   describe(m.scales + row * m.blocks, own * blocks), blocks * 16, blocks};
+}
+
+// 16 bytes (4 bytes) per lane from `offset` of a buffer to LDS at `to` + 16 (4) * lane.
+__device__ __forceinline__ void to_lds_16(const v4i& buffer, uint32_t offset, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :: "s"(to), "v"(offset), "s"(buffer) : "memory");
+}
+__device__ __forceinline__ void to_lds_4(const v4i& buffer, uint32_t offset, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+               :: "s"(to), "v"(offset), "s"(buffer) : "memory");
+}
+
+template <class G>
+struct WordStage {
+  v4i codes[G::rows * 8];      // block 2g + s of row r at place (4s + g) ^ (r/2 % 8)
+  uint32_t scales[G::rows * 2];
+};
+
+template <class G>
+constexpr int kWordRequests = G::loads + G::rows * 2 / G::threads;   // per wavefront and stage
+
+template <class G>
+__device__ __forceinline__ void request_stage(const WordPanel& a, const WordPanel& b, int block,
+                                              int wave, int lane, uint32_t to) {
+  constexpr uint32_t kNone = 0xFFFFFFF0u;                  // past every buffer: reads as zeros
+  constexpr int kPerRound = G::threads / 8, kLoadsA = G::rows_m / kPerRound;
+  const uint32_t row = 8 * wave + (lane >> 3), own = (lane & 7) ^ (row >> 1 & 7);
+  const uint32_t at = block + (2 * (own & 3) | own >> 2);
+  const bool inside = at < a.blocks;
+#pragma unroll
+  for (int i = 0; i < G::loads; ++i) {
+    const WordPanel& m = i < kLoadsA ? a : b;
+    const uint32_t r = row + kPerRound * (i < kLoadsA ? i : i - kLoadsA);
+    to_lds_16(m.codes, inside ? r * m.row_bytes + at * 16 : kNone,
+              to + 16 * (i * G::threads + 64 * wave));
+  }
+  // Words 2r, 2r + 1 of LDS: row r's blocks 0-3 and 4-7.  A wavefront's words are all of one
+  // operand.
+  constexpr int kWords = G::rows * 2 / G::threads;
+  static_assert(G::rows_m * 2 % (64 * kWords) == 0, "a wavefront's scales are of one operand");
+  const bool of_a = wave < G::rows_m * 2 / (64 * kWords);
+  const v4i buffer = of_a ? a.scales : b.scales;
+#pragma unroll
+  for (int i = 0; i < kWords; ++i) {
+    const uint32_t word = (wave * kWords + i) * 64 + lane, half = block + 4 * (word & 1);
+    const uint32_t r = (word >> 1) - (of_a ? 0 : G::rows_m);
+    to_lds_4(buffer, half < a.blocks ? r * a.blocks + half : kNone,
+             to + static_cast<uint32_t>(offsetof(WordStage<G>, scales)) +
+                 4 * ((wave * kWords + i) * 64));
+  }
+}
+
+// A wavefront's operands of a stage; lane l's blocks are 2(l/16) and 2(l/16) + 1, so that its
+// two scale bytes are one 16-bit word.
+template <class G>
+struct WordFragments {
+  v4i a[2][G::MI], b[2][G::NJ];
+  int scale_a[G::MI], scale_b[G::NJ];
+};
+
+template <class G>
+__device__ __forceinline__ void read_fragments(const WordStage<G>& from, int wm, int wn, int lane,
+                                               WordFragments<G>& f) {
+  const int group = lane >> 4, row = lane & 15;
+  const auto* bytes = reinterpret_cast<const uint16_t*>(from.scales);
+#pragma unroll
+  for (int i = 0; i < G::MI; ++i)
+    f.scale_a[i] = bytes[((wm * G::MI + i) * 16 + row) * 4 + group];
+#pragma unroll
+  for (int j = 0; j < G::NJ; ++j)
+    f.scale_b[j] = bytes[(G::rows_m + (wn * G::NJ + j) * 16 + row) * 4 + group];
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    const int place = (4 * s + group) ^ (lane >> 1 & 7);
+#pragma unroll
+    for (int i = 0; i < G::MI; ++i)
+      f.a[s][i] = from.codes[((wm * G::MI + i) * 16 + row) * 8 + place];
+#pragma unroll
+    for (int j = 0; j < G::NJ; ++j)
+      f.b[s][j] = from.codes[(G::rows_m + (wn * G::NJ + j) * 16 + row) * 8 + place];
+  }
+}
+
+template <class G, int S>
+__device__ __forceinline__ void multiply(const WordFragments<G>& f, v4f (&sum)[G::MI][G::NJ]) {
+#pragma unroll
+  for (int j = 0; j < G::NJ; ++j)
+#pragma unroll
+    for (int i = 0; i < G::MI; ++i)
+      sum[i][j] = mx_mfma<S, S>(f.b[S][j], f.a[S][i], sum[i][j], f.scale_b[j], f.scale_a[i]);
+}
+
+// s_waitcnt: vmcnt in bits 0-3 and 14-15, expcnt 4-6, lgkmcnt 8-11.
+constexpr int wait_loads(int n) { return (n & 15) | (n >> 4) << 14 | 7 << 4 | 15 << 8; }
+constexpr int kWaitLds = 15 | 3 << 14 | 7 << 4;
+
+template <int kWait>
+__device__ __forceinline__ void wait_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(kWait);
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+template <class G, class T>
+__global__ __launch_bounds__(G::threads) void product_word_tiles(MxView a, MxView b,
+                                                                 const float* bias, T* out,
+                                                                 int64_t stride, uint32_t tiles_m,
+                                                                 uint32_t tiles_n) {
+  __shared__ union {
+    WordStage<G> stages[2];
+    Strip<G, T> strip[G::WM * G::WN];
+  } lds;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int wm = wave / G::WN, wn = wave % G::WN;
+  const uint32_t tile = blockIdx.x;
+  const uint32_t tile_m = uniform(tile / tiles_n), tile_n = tile - tile_m * tiles_n;
+  const int64_t m0 = static_cast<int64_t>(tile_m) * G::rows_m;
+  const int64_t n0 = static_cast<int64_t>(tile_n) * G::rows_n;
+  const WordPanel pa = word_panel(a, m0, G::rows_m), pb = word_panel(b, n0, G::rows_n);
+  const int stages = (static_cast<int>(pa.blocks) + 7) / 8;
+  uint32_t place[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    place[i] = uniform(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
+        (__attribute__((address_space(3))) void*)&lds.stages[i])));
+
+  v4f sum[G::MI][G::NJ] = {};
+  WordFragments<G> f;
+  request_stage<G>(pa, pb, 0, wave, lane, place[0]);
+  request_stage<G>(pa, pb, 8, wave, lane, place[1]);
+  // Stages past the last read as zeros, which nothing multiplies: every stage has as many
+  // requests behind it.
+  for (int stage = 0; stage < stages; ++stage) {
+    wait_barrier<wait_loads(kWordRequests<G>)>();          // this stage has arrived, for all
+    read_fragments<G>(lds.stages[stage & 1], wm, wn, lane, f);
+    wait_barrier<kWaitLds>();                              // and is read, by all
+    request_stage<G>(pa, pb, 8 * (stage + 2), wave, lane, stage & 1 ? place[1] : place[0]);
+    multiply<G, 0>(f, sum);
+    multiply<G, 1>(f, sum);
+    hold<G>(sum);
+  }
+  wait_barrier<wait_loads(0)>();                           // before LDS is used anew
+  const int64_t m = m0 + 16 * wm * G::MI, n = n0 + 16 * wn * G::NJ;
+  store_tiles<G, T>(out + m * stride + n, stride, sum, bias ? bias + n : nullptr, a.rows - m,
+                    b.rows - n, lane, lds.strip[wave]);
 }
 
 // Few rows of a (up to 16): bound by b's bytes, each read once.  A wavefront takes 16 columns of y (rows
@@ -551,6 +727,27 @@ int run_tiles(const ns_mx_product_args* p, int64_t parts, float* partials, hipSt
   return launched("product");
 }
 
+// Whether product_word_tiles takes the operands.
+bool word_scales(const ns_mx_product_args* p) {
+  return p->a.columns > 0 && (p->a.columns + NS_MX_BLOCK - 1) / NS_MX_BLOCK % 4 == 0 &&
+         reinterpret_cast<uintptr_t>(p->a.scales) % 4 == 0 &&
+         reinterpret_cast<uintptr_t>(p->b.scales) % 4 == 0;
+}
+
+template <class T>
+int run_large(const ns_mx_product_args* p, hipStream_t stream) {
+  using G = Large;
+  if (!word_scales(p)) return run_tiles<G, T>(p, 1, nullptr, stream);
+  const int64_t tiles_m = (p->a.rows + G::rows_m - 1) / G::rows_m;
+  const int64_t tiles_n = (p->b.rows + G::rows_n - 1) / G::rows_n;
+  if (tiles_m * tiles_n > INT32_MAX) return fail("the product is too large for one launch");
+  product_word_tiles<G, T><<<dim3(static_cast<unsigned>(tiles_m * tiles_n)), dim3(G::threads), 0,
+                             stream>>>(view(p->a), view(p->b), p->bias, static_cast<T*>(p->out),
+                                       p->stride, static_cast<uint32_t>(tiles_m),
+                                       static_cast<uint32_t>(tiles_n));
+  return launched("product");
+}
+
 template <class T>
 int run_rows(const ns_mx_product_args* p, int64_t parts, float* partials, hipStream_t stream) {
   const int64_t shared = waves_per_strip(p->b.rows), strips = (p->b.rows + 15) / 16;
@@ -572,7 +769,7 @@ int run_rows(const ns_mx_product_args* p, int64_t parts, float* partials, hipStr
 template <class T>
 int run_kernel(const ns_mx_product_args* p, int64_t parts, float* partials, hipStream_t stream) {
   switch (kernel_of(p->a.rows, p->b.rows)) {
-    case Kernel::kLarge: return run_tiles<Large, T>(p, parts, partials, stream);
+    case Kernel::kLarge: return run_large<T>(p, stream);
     case Kernel::kSmall: return run_tiles<Small, T>(p, parts, partials, stream);
     default: return run_rows<T>(p, parts, partials, stream);
   }

@@ -58,7 +58,7 @@ def _library() -> ctypes.CDLL:
         fn = getattr(lib, name)
         fn.restype, fn.argtypes = ctypes.c_int, [_ptr, _ptr]
     lib.ns_conv_backward_floats.restype = _i64
-    lib.ns_conv_backward_floats.argtypes = [_ptr]
+    lib.ns_conv_backward_floats.argtypes = [_i64, _i64, _i64, _i32, _i32]
     lib.ns_scan_plan.restype = ctypes.c_int
     lib.ns_scan_plan.argtypes = [_i64, _i64, _i64, _i64, _i32, _i32, _ptr]
     return lib
@@ -197,6 +197,7 @@ class _CausalConv(torch.autograd.Function):
     def forward(ctx, x, weight, bias, history, lengths, silu):
         operands = (_unit_channels(x), _dense(weight), _dense(bias), _unit_channels(history))
         ctx.save_for_backward(*operands, lengths)
+        ctx.set_materialize_grads(False)
         ctx.silu = silu
         return _conv_forward(*operands, lengths, silu)
 
@@ -206,18 +207,18 @@ class _CausalConv(torch.autograd.Function):
         x, weight, bias, history, lengths = ctx.saved_tensors
         wants, device = ctx.needs_input_grad, x.device
         (ticks, batch, channels), taps = x.shape, weight.shape[1]
-        dy, dlast = _unit_channels(dy), _unit_channels(dlast)
+        dy = torch.zeros_like(x) if dy is None else _unit_channels(dy)
+        dlast = _unit_channels(dlast)
         dx = torch.empty(x.shape, dtype=x.dtype, device=device) if wants[0] else None
         dhistory = (torch.empty(history.shape, dtype=x.dtype, device=device)
                     if history is not None and wants[3] else None)
         lib, count = _library(), channels * (taps + 1)
-        head = (ticks, batch, channels, taps, TYPES[x.dtype], ctx.silu, 0, *_signal(x),
-                weight.data_ptr(), _address(bias), *_signal(history), _address(lengths))
-        parts = lib.ns_conv_backward_floats(_CONV.pack(*head, *_ABSENT * 6, 0, 0))
-        if parts < 0:
-            _raise_on(1, lib)
+        parts = lib.ns_conv_backward_floats(ticks, batch, channels, taps, TYPES[x.dtype])
+        # The parameters' gradients and the workspace share one allocation.
         sums = torch.empty(count + parts, dtype=torch.float32, device=device)
-        args = _CONV.pack(*head, *_ABSENT, *_ABSENT, *_signal(dy), *_signal(dlast), *_signal(dx),
+        args = _CONV.pack(ticks, batch, channels, taps, TYPES[x.dtype], ctx.silu, 0, *_signal(x),
+                          weight.data_ptr(), _address(bias), *_signal(history), _address(lengths),
+                          *_ABSENT, *_ABSENT, *_signal(dy), *_signal(dlast), *_signal(dx),
                           *_signal(dhistory), sums.data_ptr() + 4 * count, sums.data_ptr())
         call(lib.ns_conv_backward, device, args)
         return (dx, sums[:channels * taps].view(channels, taps) if wants[1] else None,
@@ -359,6 +360,7 @@ class _SelectiveScan(torch.autograd.Function):
         operands = _dense_scan(x, delta, A, B, C, D, z, delta_bias)
         y, final, kept = _scan_forward(operands, _dense(state), lengths, softplus, groups, True)
         ctx.save_for_backward(*operands, lengths, kept)
+        ctx.set_materialize_grads(False)
         ctx.softplus, ctx.groups = softplus, groups
         return y, final
 
@@ -369,12 +371,12 @@ class _SelectiveScan(torch.autograd.Function):
         x, delta, A, B, C, D, z, delta_bias = operands
         wants, device = ctx.needs_input_grad, x.device
         ticks, batch, n = x.shape
-        dfinal = dfinal.contiguous()
+        dfinal, states = _dense(dfinal), A.shape[1]
         if ticks == 0 or batch == 0:                  # no tick: the state passes through
             zeros = [torch.zeros_like(v) if v is not None and w else None
                      for v, w in zip(operands, wants)]
             return (*zeros, dfinal if wants[8] else None, None, None, None)
-        dy, states = _unit_channels(dy), A.shape[1]
+        dy = torch.zeros_like(x) if dy is None else _unit_channels(dy)
         chunks, ends_floats, _, part_floats = _plan(x.shape, ctx.groups, states, True)
 
         def like(value):
@@ -382,7 +384,8 @@ class _SelectiveScan(torch.autograd.Function):
                                                           device=device)
 
         dx, ddelta, dz, dB, dC = like(x), like(delta), like(z), like(B), like(C)
-        dstate = like(dfinal) if wants[8] else None
+        dstate = (torch.empty((batch, n, states), dtype=torch.float32, device=device)
+                  if wants[8] else None)
         # The parameters' gradients and the workspaces share one allocation.
         sums = torch.empty(n * (states + 2), dtype=torch.float32, device=device)
         work = torch.empty(part_floats + ends_floats, dtype=torch.float32, device=device)
@@ -392,7 +395,7 @@ class _SelectiveScan(torch.autograd.Function):
             *_signal(x), *_signal(delta), *_signal(z), *_ABSENT, *_signal(B), *_signal(C),
             A.data_ptr(), _address(D), _address(delta_bias), 0, 0, _address(lengths),
             kept.data_ptr(), work.data_ptr() + 4 * part_floats if ends_floats else 0,
-            *_signal(dy), dfinal.data_ptr(), *_signal(dx), *_signal(ddelta), *_signal(dz),
+            *_signal(dy), _address(dfinal), *_signal(dx), *_signal(ddelta), *_signal(dz),
             *_signal(dB), *_signal(dC), _address(dstate), rates, skips, skips + 4 * n,
             work.data_ptr())
         call(_library().ns_scan_backward, device, args)

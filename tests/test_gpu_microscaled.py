@@ -127,6 +127,29 @@ def test_product(gpu, shape):
     assert torch.equal(mx_product(x, weight, bias=bias, dtype=dtype), y)
 
 
+@pytest.mark.parametrize("shape", [(3500, 3400, 128), (3400, 3500, 96), (3333, 3600, 384),
+                                   (3400, 3700, 1000), (3500, 3500, 640), (3329, 3585, 1024)])
+def test_product_of_many_rows(gpu, shape):
+    """The 256 x 256 tiles, K of one stage to several, whole and with a part of one, scale
+    rows of whole words (K a multiple of 128) and not; a sample of rows and columns."""
+    M, N, K = shape
+    x, weight = mx_quantize(rows(gpu, 40, M, K)), mx_quantize(rows(gpu, 41, N, K) / K ** 0.5)
+    bias, dtype = rows(gpu, 42, N), TYPES[K % 3]
+    y = mx_product(x, weight, bias=bias, dtype=dtype)
+    m = torch.cat((torch.arange(0, 40), torch.arange(250, 262), torch.arange(M - 40, M)))
+    n = torch.cat((torch.arange(0, 70), torch.arange(500, 530), torch.arange(N - 70, N)))
+    a = so.mx_values(so.unpack(x.codes.cpu()[m]), x.scales.cpu()[m], K)
+    b = so.mx_values(so.unpack(weight.codes.cpu()[n]), weight.scales.cpu()[n], K)
+    want = a @ b.t() + so.wide(bias)[n]
+    bound = (K + 2) * 2.0 ** -23 * (a.abs() @ b.abs().t() + so.wide(bias).abs()[n])
+    bound = bound + HALF_ULP[dtype] * (want.abs() + bound) + 2.0 ** -24 * (dtype == torch.float16)
+    assert ((y.cpu()[m][:, n].double() - want).abs() <= bound).all()
+    # The whole result against float32, to the bound of both sums and of one rounding more.
+    whole = x.dequantize() @ weight.dequantize().t() + bias
+    error = (y.float() - whole).norm() / whole.norm()
+    assert error <= 2 * (HALF_ULP[dtype] + K * 2.0 ** -23)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_product_keeps_leading_dimensions(gpu, dtype):
     x = rows(gpu, 8, 3, 5, 90, dtype=dtype)
