@@ -389,81 +389,137 @@ struct WordStage {
 template <class G>
 constexpr int kWordRequests = G::loads + G::rows * 2 / G::threads;   // per wavefront and stage
 
+// The requests of a stage, by number: the first G::loads are codes, eight rows of 128 bytes
+// each; the others scales, words 2r and 2r + 1 of LDS being row r's blocks 0-3 and 4-7.
 template <class G>
-__device__ __forceinline__ void request_stage(const WordPanel& a, const WordPanel& b, int block,
-                                              int wave, int lane, uint32_t to) {
-  constexpr uint32_t kNone = 0xFFFFFFF0u;                  // past every buffer: reads as zeros
-  constexpr int kPerRound = G::threads / 8, kLoadsA = G::rows_m / kPerRound;
-  const uint32_t row = 8 * wave + (lane >> 3), own = (lane & 7) ^ (row >> 1 & 7);
-  const uint32_t at = block + (2 * (own & 3) | own >> 2);
-  const bool inside = at < a.blocks;
-#pragma unroll
-  for (int i = 0; i < G::loads; ++i) {
-    const WordPanel& m = i < kLoadsA ? a : b;
-    const uint32_t r = row + kPerRound * (i < kLoadsA ? i : i - kLoadsA);
-    to_lds_16(m.codes, inside ? r * m.row_bytes + at * 16 : kNone,
-              to + 16 * (i * G::threads + 64 * wave));
-  }
-  // Words 2r, 2r + 1 of LDS: row r's blocks 0-3 and 4-7.  A wavefront's words are all of one
-  // operand.
-  constexpr int kWords = G::rows * 2 / G::threads;
-  static_assert(G::rows_m * 2 % (64 * kWords) == 0, "a wavefront's scales are of one operand");
-  const bool of_a = wave < G::rows_m * 2 / (64 * kWords);
-  const v4i buffer = of_a ? a.scales : b.scales;
-#pragma unroll
-  for (int i = 0; i < kWords; ++i) {
-    const uint32_t word = (wave * kWords + i) * 64 + lane, half = block + 4 * (word & 1);
-    const uint32_t r = (word >> 1) - (of_a ? 0 : G::rows_m);
-    to_lds_4(buffer, half < a.blocks ? r * a.blocks + half : kNone,
-             to + static_cast<uint32_t>(offsetof(WordStage<G>, scales)) +
-                 4 * ((wave * kWords + i) * 64));
-  }
-}
-
-// A wavefront's operands of a stage; lane l's blocks are 2(l/16) and 2(l/16) + 1, so that its
-// two scale bytes are one 16-bit word.
-template <class G>
-struct WordFragments {
-  v4i a[2][G::MI], b[2][G::NJ];
-  int scale_a[G::MI], scale_b[G::NJ];
+struct StageRequests {
+  uint32_t row, at, to;        // row and block of the lane's codes; LDS address of the stage
+  bool inside;
+  int block, wave, lane;
 };
 
 template <class G>
-__device__ __forceinline__ void read_fragments(const WordStage<G>& from, int wm, int wn, int lane,
-                                               WordFragments<G>& f) {
-  const int group = lane >> 4, row = lane & 15;
-  const auto* bytes = reinterpret_cast<const uint16_t*>(from.scales);
-#pragma unroll
-  for (int i = 0; i < G::MI; ++i)
-    f.scale_a[i] = bytes[((wm * G::MI + i) * 16 + row) * 4 + group];
-#pragma unroll
-  for (int j = 0; j < G::NJ; ++j)
-    f.scale_b[j] = bytes[(G::rows_m + (wn * G::NJ + j) * 16 + row) * 4 + group];
-#pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    const int place = (4 * s + group) ^ (lane >> 1 & 7);
-#pragma unroll
-    for (int i = 0; i < G::MI; ++i)
-      f.a[s][i] = from.codes[((wm * G::MI + i) * 16 + row) * 8 + place];
-#pragma unroll
-    for (int j = 0; j < G::NJ; ++j)
-      f.b[s][j] = from.codes[(G::rows_m + (wn * G::NJ + j) * 16 + row) * 8 + place];
+__device__ __forceinline__ StageRequests<G> stage_requests(const WordPanel& a, int block, int wave,
+                                                           int lane, uint32_t to) {
+  StageRequests<G> q;
+  q.row = 8 * wave + (lane >> 3);
+  const uint32_t own = (lane & 7) ^ (q.row >> 1 & 7);
+  q.at = block + (2 * (own & 3) | own >> 2);
+  q.inside = q.at < a.blocks;
+  q.to = to;
+  q.block = block;
+  q.wave = wave;
+  q.lane = lane;
+  return q;
+}
+
+template <class G, int I>
+__device__ __forceinline__ void request_piece(const WordPanel& a, const WordPanel& b,
+                                              const StageRequests<G>& q) {
+  constexpr uint32_t kNone = 0xFFFFFFF0u;                  // past every buffer: reads as zeros
+  constexpr int kPerRound = G::threads / 8, kLoadsA = G::rows_m / kPerRound;
+  if constexpr (I < G::loads) {
+    const WordPanel& m = I < kLoadsA ? a : b;
+    const uint32_t r = q.row + kPerRound * (I < kLoadsA ? I : I - kLoadsA);
+    to_lds_16(m.codes, q.inside ? r * m.row_bytes + q.at * 16 : kNone,
+              q.to + 16 * (I * G::threads + 64 * q.wave));
+  } else if constexpr (I < kWordRequests<G>) {
+    constexpr int i = I - G::loads, kWords = G::rows * 2 / G::threads;
+    static_assert(G::rows_m * 2 % G::threads == 0, "a request's scales are of one operand");
+    const bool of_a = i * G::threads < G::rows_m * 2;
+    const WordPanel& m = of_a ? a : b;
+    const uint32_t word = i * G::threads + 64 * q.wave + q.lane, half = q.block + 4 * (word & 1);
+    const uint32_t r = (word >> 1) - (of_a ? 0 : G::rows_m);
+    to_lds_4(m.scales, half < m.blocks ? r * m.blocks + half : kNone,
+             q.to + static_cast<uint32_t>(offsetof(WordStage<G>, scales)) +
+                 4 * (i * G::threads + 64 * q.wave));
+    (void)kWords;
   }
 }
 
-template <class G, int S>
-__device__ __forceinline__ void multiply(const WordFragments<G>& f, v4f (&sum)[G::MI][G::NJ]) {
+template <class G, int First, int Count>
+__device__ __forceinline__ void request_pieces(const WordPanel& a, const WordPanel& b,
+                                               const StageRequests<G>& q) {
+  if constexpr (Count > 0) {
+    request_piece<G, First>(a, b, q);
+    request_pieces<G, First + 1, Count - 1>(a, b, q);
+  }
+}
+
+// A wavefront's operands: of one step of a stage, and a stage's scales (byte s: step s).
+// Lane l's blocks are 2(l/16) and 2(l/16) + 1, so that its two scale bytes are one word.
+template <class G>
+struct StepFragments {
+  v4i a[G::MI], b[G::NJ];
+};
+template <class G>
+struct StageScales {
+  int a[G::MI / 2], b[G::NJ];  // a: two strips a register
+};
+
+// LDS addresses of a wavefront's first strips of a step, per lane; the other strips lie at
+// constant distances.
+struct StepBase {
+  uint32_t codes_a, codes_b, scales_a, scales_b;
+};
+
+template <class G>
+__device__ __forceinline__ StepBase step_base(uint32_t stage, int step, int wm, int wn, int lane) {
+  const uint32_t row = lane & 15, place = (4 * step + (lane >> 4)) ^ (lane >> 1 & 7);
+  const uint32_t codes = stage + (row * 8 + place) * 16;
+  const uint32_t scales = stage + static_cast<uint32_t>(offsetof(WordStage<G>, scales)) + row * 8 +
+                          2 * (lane >> 4);
+  StepBase base{codes + wm * (G::MI * 16 * 128), codes + (G::rows_m + wn * G::NJ * 16) * 128,
+                scales + wm * (G::MI * 16 * 8), scales + (G::rows_m + wn * G::NJ * 16) * 8};
+  // One register each, here: left to itself the compiler keeps every strip's.
+  asm volatile("" : "+v"(base.codes_a), "+v"(base.codes_b), "+v"(base.scales_a), "+v"(base.scales_b));
+  return base;
+}
+
+__device__ __forceinline__ v4i read_code(uint32_t base, int strip) {
+  return *(const __attribute__((address_space(3))) v4i*)static_cast<uintptr_t>(base + strip * (16 * 128));
+}
+__device__ __forceinline__ int read_scale(uint32_t base, int strip) {
+  return *(const __attribute__((address_space(3))) uint16_t*)static_cast<uintptr_t>(base + strip * (16 * 8));
+}
+
+// Multiplies column strip J of step S, reading strip J of the next step meanwhile (and, where
+// that begins a stage, its scales), and making requests First .. of the stage after.
+template <class G, int S, int J>
+__device__ __forceinline__ void column(StepFragments<G>& f, const StageScales<G>& scales,
+                                       const StepBase& from, StepFragments<G>& next,
+                                       StageScales<G>& next_scales, const WordPanel& pa,
+                                       const WordPanel& pb, const StageRequests<G>& q,
+                                       v4f (&sum)[G::MI][G::NJ]) {
+  constexpr int kPer = G::MI / G::NJ;                      // a's strips per column
+  static_assert(kPer == 2, "a column reads two strips of a");
+  int pair[2];
+  next.b[J] = read_code(from.codes_b, J);
 #pragma unroll
-  for (int j = 0; j < G::NJ; ++j)
+  for (int i = kPer * J; i < kPer * (J + 1); ++i) next.a[i] = read_code(from.codes_a, i);
+  if constexpr (S == 1) {
+    next_scales.b[J] = read_scale(from.scales_b, J);
+    pair[0] = read_scale(from.scales_a, kPer * J);
+    pair[1] = read_scale(from.scales_a, kPer * J + 1);
+    constexpr int kEach = (kWordRequests<G> + 1) / 2;      // all in the first two columns
+    request_pieces<G, kEach * J, J < 2 ? kEach : 0>(pa, pb, q);
+  }
+  // The empty statements keep the products of a column in its place: the compiler would gather
+  // them before the barrier, and wait there for operands that were to arrive meanwhile.
+  asm volatile("" : "+v"(f.b[J]));
 #pragma unroll
-    for (int i = 0; i < G::MI; ++i)
-      sum[i][j] = mx_mfma<S, S>(f.b[S][j], f.a[S][i], sum[i][j], f.scale_b[j], f.scale_a[i]);
+  for (int i = 0; i < G::MI; ++i)
+    sum[i][J] = i & 1 ? mx_mfma<S, 2 + S>(f.b[J], f.a[i], sum[i][J], scales.b[J], scales.a[i / 2])
+                      : mx_mfma<S, S>(f.b[J], f.a[i], sum[i][J], scales.b[J], scales.a[i / 2]);
+#pragma unroll
+  for (int i = 0; i < G::MI; ++i) asm volatile("" : "+v"(sum[i][J]));
+  if constexpr (S == 1) next_scales.a[J] = pair[0] | pair[1] << 16;
+  if constexpr (J + 1 < G::NJ)
+    column<G, S, J + 1>(f, scales, from, next, next_scales, pa, pb, q, sum);
 }
 
 // s_waitcnt: vmcnt in bits 0-3 and 14-15, expcnt 4-6, lgkmcnt 8-11.
 constexpr int wait_loads(int n) { return (n & 15) | (n >> 4) << 14 | 7 << 4 | 15 << 8; }
-constexpr int kWaitLds = 15 | 3 << 14 | 7 << 4;
-
 template <int kWait>
 __device__ __forceinline__ void wait_barrier() {
   asm volatile("" ::: "memory");
@@ -496,21 +552,35 @@ __global__ __launch_bounds__(G::threads) void product_word_tiles(MxView a, MxVie
         (__attribute__((address_space(3))) void*)&lds.stages[i])));
 
   v4f sum[G::MI][G::NJ] = {};
-  WordFragments<G> f;
-  request_stage<G>(pa, pb, 0, wave, lane, place[0]);
-  request_stage<G>(pa, pb, 8, wave, lane, place[1]);
-  // Stages past the last read as zeros, which nothing multiplies: every stage has as many
-  // requests behind it.
-  for (int stage = 0; stage < stages; ++stage) {
-    wait_barrier<wait_loads(kWordRequests<G>)>();          // this stage has arrived, for all
-    read_fragments<G>(lds.stages[stage & 1], wm, wn, lane, f);
-    wait_barrier<kWaitLds>();                              // and is read, by all
-    request_stage<G>(pa, pb, 8 * (stage + 2), wave, lane, stage & 1 ? place[1] : place[0]);
-    multiply<G, 0>(f, sum);
-    multiply<G, 1>(f, sum);
-    hold<G>(sum);
+  StepFragments<G> even, odd;  // operands of a stage's first and second step
+  StageScales<G> scales, next_scales;
+  request_pieces<G, 0, kWordRequests<G>>(pa, pb, stage_requests<G>(pa, 0, wave, lane, place[0]));
+  request_pieces<G, 0, kWordRequests<G>>(pa, pb, stage_requests<G>(pa, 8, wave, lane, place[1]));
+  wait_barrier<wait_loads(kWordRequests<G>)>();
+  const StepBase begin = step_base<G>(place[0], 0, wm, wn, lane);
+#pragma unroll
+  for (int i = 0; i < G::MI; ++i) {
+    even.a[i] = read_code(begin.codes_a, i);
+    if (i & 1) scales.a[i / 2] = read_scale(begin.scales_a, i - 1) | read_scale(begin.scales_a, i) << 16;
   }
-  wait_barrier<wait_loads(0)>();                           // before LDS is used anew
+#pragma unroll
+  for (int j = 0; j < G::NJ; ++j) {
+    even.b[j] = read_code(begin.codes_b, j);
+    scales.b[j] = read_scale(begin.scales_b, j);
+  }
+  // Stages past the last read as zeros and are not multiplied.
+  for (int stage = 0; stage < stages; ++stage) {
+    const uint32_t now = stage & 1 ? place[1] : place[0], then = stage & 1 ? place[0] : place[1];
+    const StageRequests<G> none{};
+    column<G, 0, 0>(even, scales, step_base<G>(now, 1, wm, wn, lane), odd, next_scales, pa, pb, none,
+                    sum);
+    // This stage is read by all, and the next one has arrived for all.
+    wait_barrier<0>();
+    column<G, 1, 0>(odd, scales, step_base<G>(then, 0, wm, wn, lane), even, next_scales, pa, pb,
+                    stage_requests<G>(pa, 8 * (stage + 2), wave, lane, now), sum);
+    scales = next_scales;
+  }
+  wait_barrier<0>();                                       // before LDS is used anew
   const int64_t m = m0 + 16 * wm * G::MI, n = n0 + 16 * wn * G::NJ;
   store_tiles<G, T>(out + m * stride + n, stride, sum, bias ? bias + n : nullptr, a.rows - m,
                     b.rows - n, lane, lds.strip[wave]);
@@ -736,8 +806,8 @@ bool word_scales(const ns_mx_product_args* p) {
 
 template <class T>
 int run_large(const ns_mx_product_args* p, hipStream_t stream) {
+  if (!word_scales(p)) return run_tiles<Large, T>(p, 1, nullptr, stream);
   using G = Large;
-  if (!word_scales(p)) return run_tiles<G, T>(p, 1, nullptr, stream);
   const int64_t tiles_m = (p->a.rows + G::rows_m - 1) / G::rows_m;
   const int64_t tiles_n = (p->b.rows + G::rows_n - 1) / G::rows_n;
   if (tiles_m * tiles_n > INT32_MAX) return fail("the product is too large for one launch");
