@@ -114,10 +114,6 @@ __device__ __forceinline__ uint32_t lane_bytes(const ScanPlace& p, int lane) {
   return static_cast<uint32_t>(lane < p.own ? lane : p.own - 1) * sizeof(T);
 }
 
-// Has `v` computed here: the compiler otherwise moves such work to its later use, and keeps
-// its several inputs in registers across a tile's ticks instead of this one value.
-__device__ __forceinline__ void settle(float& v) { asm volatile("" : "+v"(v)); }
-
 // The thread's number, computed anew: what depends on it (places in LDS and in rows) is
 // then not kept in registers across a tile's ticks.
 __device__ __forceinline__ int fresh_thread() {
@@ -133,8 +129,17 @@ __device__ __forceinline__ float quad_sum(float v) {
   return v;
 }
 
-// A channel's time step and its slope in delta.
-__device__ __forceinline__ float time_step(float raw, bool soft) { return soft ? softplus(raw) : raw; }
+// Has `v` computed here: the compiler otherwise moves such work to its later use, and keeps
+// its several inputs in registers across a tile's ticks instead of this one value.
+__device__ __forceinline__ void settle(float& v) { asm volatile("" : "+v"(v)); }
+
+// A channel's time step.  Computed both ways: a branch between a thread's items would keep
+// their chains of dependent operations from overlapping.
+__device__ __forceinline__ float time_step(float raw, bool soft) {
+  float smooth = softplus(raw);
+  settle(smooth);
+  return soft ? smooth : raw;
+}
 
 // A tile's B or C rows, one value per thread: requested with the tile's other inputs, and
 // put into LDS (padded with zeros past S and past the column's end) when the tile begins.

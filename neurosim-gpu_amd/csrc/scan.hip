@@ -97,8 +97,10 @@ __global__ __launch_bounds__(kThreads) void scan_forward(ScanShape s, ScanIn<T> 
         step_of[tick][lane] = make_float2(dt, dt * x);
         if (!kEnds) {
           const float z = static_cast<float>(raw.z[i]);
+          float gate = z * sigmoid(z);
+          settle(gate);
           items.skip[i] = skip * x;
-          items.gate[i] = in.z.data ? z * sigmoid(z) : 1.0f;
+          items.gate[i] = in.z.data ? gate : 1.0f;
           settle(items.skip[i]);
           settle(items.gate[i]);
         }

@@ -92,9 +92,10 @@ __global__ __launch_bounds__(kThreads) void scan_adjoint_ends(ScanShape s, ScanI
         const bool live = t + tick < p.end && lane < p.own;
         const float z = static_cast<float>(raw.z[i]);
         const float dt = time_step(static_cast<float>(raw.delta[i]) + bias, s.softplus);
-        const float gate = in.z.data ? z * sigmoid(z) : 1.0f;
-        step_of[tick][lane] = make_float2(live ? dt : 0.0f,
-                                          live ? static_cast<float>(raw.dy[i]) * gate : 0.0f);
+        float gate = z * sigmoid(z);
+        settle(gate);
+        const float gy = static_cast<float>(raw.dy[i]) * (in.z.data ? gate : 1.0f);
+        step_of[tick][lane] = make_float2(live ? dt : 0.0f, live ? gy : 0.0f);
       }
       place_shared<T, R>(raw.read, s, p, t, threadIdx.x, read);
       request<T, R, kItems, true>(in, s, dy, p, t - 2 * CT, wave, threadIdx.x, raw);
@@ -211,10 +212,13 @@ __global__ __launch_bounds__(kThreads, 2) void scan_backward(ScanShape s, ScanIn
       const float x = live ? static_cast<float>(raw.x[i]) : 0.0f, z = static_cast<float>(raw.z[i]);
       const float dy = live ? static_cast<float>(raw.dy[i]) : 0.0f;
       const float soft = static_cast<float>(raw.delta[i]) + bias;
-      const float dt = live ? time_step(soft, s.softplus) : 0.0f;
+      const float step = time_step(soft, s.softplus), dt = live ? step : 0.0f;
       const float gate = sigmoid(z);
-      const float gy = in.z.data ? dy * (z * gate) : dy;
-      item_sig[i] = s.softplus ? sigmoid(soft) : 1.0f;
+      float gated = dy * (z * gate), slope = sigmoid(soft);
+      settle(gated);
+      settle(slope);
+      const float gy = in.z.data ? gated : dy;
+      item_sig[i] = s.softplus ? slope : 1.0f;
       item_slope[i] = dy * (gate * (1.0f + z * (1.0f - gate)));
       settle(item_sig[i]);
       settle(item_slope[i]);
