@@ -221,7 +221,9 @@ struct Strip {
   T values[16][16 * G::NJ + kWide];
 };
 
-template <class G, class T>
+// kStream: past the caches, for results too large to be read again from there (8192^3 331 ->
+// 306 us, 8000 x 50,000 by 1024 497 -> 382).
+template <class G, class T, bool kStream>
 __device__ __forceinline__ void store_tiles(T* to, int64_t stride, const v4f (&sum)[G::MI][G::NJ],
                                             const float* bias, int64_t rows, int64_t columns, int lane,
                                             Strip<G, T>& strip) {
@@ -247,7 +249,10 @@ __device__ __forceinline__ void store_tiles(T* to, int64_t stride, const v4f (&s
       Pack<T, S::kWide> y;
       __builtin_memcpy(&y, &strip.values[r + row][column], sizeof(y));
       if (wide) {
-        store_pack<T, S::kWide>(at, y);
+        if constexpr (kStream)
+          stream_pack<T, S::kWide>(at, y);
+        else
+          store_pack<T, S::kWide>(at, y);
       } else {
 #pragma unroll
         for (int k = 0; k < S::kWide; ++k)
@@ -335,11 +340,11 @@ __global__ __launch_bounds__(G::threads) void product_tiles(MxView a, MxView b, 
   const int64_t m = m0 + 16 * wm * G::MI, n = n0 + 16 * wn * G::NJ;
   __syncthreads();                                         // the stages are read to their end
   if (splits > 1) {
-    store_tiles<G, float>(partials + (split * a.rows + m) * b.rows + n, b.rows, sum, nullptr,
+    store_tiles<G, float, false>(partials + (split * a.rows + m) * b.rows + n, b.rows, sum, nullptr,
                           a.rows - m, b.rows - n, lane, lds.partial[wave]);
   } else {
-    store_tiles<G, T>(out + m * stride + n, stride, sum, bias ? bias + n : nullptr, a.rows - m,
-                      b.rows - n, lane, lds.strip[wave]);
+    store_tiles<G, T, false>(out + m * stride + n, stride, sum, bias ? bias + n : nullptr,
+                             a.rows - m, b.rows - n, lane, lds.strip[wave]);
   }
 }
 
@@ -349,11 +354,12 @@ __global__ __launch_bounds__(G::threads) void product_tiles(MxView a, MxView b, 
 // stages' requests leave one by one between the products, so that neither LDS, nor the
 // requests' addresses, nor the barrier keep the matrix cores waiting for long: one barrier a
 // stage, after its first half, when all have read the stage to its end and the next one has
-// arrived.  8192^3 in bf16: 324 us, 3.40 PFLOP/s, 50% of the rate at which these instructions
-// issue from registers (6.8); 418 us with both steps' fragments read at once and two barriers'
-// worth of waits a stage, 336 with all requests right behind the barrier.  What bounds it is
-// the units' taking turns: per stage of 4700 cycles the matrix cores are busy 2050, the
-// texture units with the requests 2500, LDS 1100.
+// arrived.  8192^3 in bf16: 308 us, 3.57 PFLOP/s; 4096 x 4096 by 32768: 238 us, 4.61 PFLOP/s, 68%
+// of the rate at which these instructions issue from registers (6.8).  (On the way, the first
+// of them: 418 us with both steps' fragments read at once and a wait for all requests; 366
+// with two barriers a stage; 336 like this with all requests right behind the barrier; 324
+// spread.)  What bounds it is the units' taking turns: per stage of 4700 cycles (at 336 us) the
+// matrix cores are busy 2050, the texture units with the requests 2500, LDS 1100.
 // The requests are inline assembly because the compiler, which cannot tell the two buffers
 // apart, would wait for all of them before it reads either; they write LDS only, no registers,
 // and the barriers' waits count them.
@@ -546,8 +552,17 @@ __global__ __launch_bounds__(G::threads) void product_word_tiles(MxView a, MxVie
   } lds;
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int wm = wave / G::WN, wn = wave % G::WN;
-  const uint32_t tile = blockIdx.x;
-  const uint32_t tile_m = uniform(tile / tiles_n), tile_n = tile - tile_m * tiles_n;
+  // Workgroups are dealt to the XCDs in turn: each XCD gets a run of tiles, in bands of four
+  // rows, so that the 32 it multiplies at a time share four panels of a and eight of b in its
+  // L2 (4096 x 4096 by 32768 251 -> 238 us, 3000 x 50,000 by 4096 399 -> 359, against rows of
+  // tiles dealt one by one).
+  constexpr uint32_t kBand = 4;
+  const uint32_t share = tiles_m * tiles_n / kXcds;
+  const uint32_t tile = blockIdx.x < share * kXcds ? blockIdx.x % kXcds * share + blockIdx.x / kXcds
+                                                   : blockIdx.x;
+  const uint32_t band = uniform(tile / (kBand * tiles_n)), in_band = tile - band * kBand * tiles_n;
+  const uint32_t high = tiles_m - kBand * band < kBand ? tiles_m - kBand * band : kBand;
+  const uint32_t tile_n = uniform(in_band / high), tile_m = kBand * band + in_band - tile_n * high;
   const int64_t m0 = static_cast<int64_t>(tile_m) * G::rows_m;
   const int64_t n0 = static_cast<int64_t>(tile_n) * G::rows_n;
   const WordPanel pa = word_panel(a, m0, G::rows_m), pb = word_panel(b, n0, G::rows_n);
@@ -588,8 +603,8 @@ __global__ __launch_bounds__(G::threads) void product_word_tiles(MxView a, MxVie
   }
   wait_barrier<0>();                                       // before LDS is used anew
   const int64_t m = m0 + 16 * wm * G::MI, n = n0 + 16 * wn * G::NJ;
-  store_tiles<G, T>(out + m * stride + n, stride, sum, bias ? bias + n : nullptr, a.rows - m,
-                    b.rows - n, lane, lds.strip[wave]);
+  store_tiles<G, T, true>(out + m * stride + n, stride, sum, bias ? bias + n : nullptr, a.rows - m,
+                          b.rows - n, lane, lds.strip[wave]);
 }
 
 // Few rows of a (up to 16): bound by b's bytes, each read once.  A wavefront takes 16 columns of y (rows
