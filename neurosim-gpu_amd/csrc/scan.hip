@@ -11,7 +11,7 @@
 // scanned side by side: a first pass gives every chunk's end state from zero and its
 // summed time step, whose exponential is the chunk's decay exp(A sum dt); the chunks are
 // joined in order; a second pass runs them from their true start.  It costs the update
-// twice, so it is taken only where workgroups are few (ns_scan_chunks).
+// twice, so it is taken only where workgroups are few (worth_chunks).
 #include "ns_scan.h"
 
 namespace ns {
@@ -229,15 +229,23 @@ __global__ __launch_bounds__(kThreads) void scan_step(ScanShape s, ScanIn<T> in,
   if (q == 0) y.row(0, b)[n] = static_cast<T>(in.z.data ? sum * (z * sigmoid(z)) : sum);
 }
 
-// Time chunks worth scanning side by side.
-int64_t worth_chunks(const ns_scan_args* a, bool backward) {
-  (void)backward;
+// Time chunks worth scanning side by side: enough to fill the card, at least two tiles each.
+// Forward / backward, us, at 16 states in bf16:
+//   blocks (T, B, N)            1 chunk      8          16         32         64
+//   256  (2048, 8, 2048)        293 / 801    244 / 631  238 / 636
+//   64   (4096, 1, 4096)                                136 / 340  134 / 341
+//   32   (16384, 1, 2048)                                          262 / 651  249 / 642
+//   32   (256, 1, 2048)         40           18.7
+// Few tiles over many blocks do not pay: 256 blocks, forward with 1 and 4 chunks, 400 ticks
+// 64 and 60, 128 ticks 23 and 31.  With 512 blocks one chunk is faster than two, 369 / 1039
+// against 499 / 1254: every further pass costs the update again.
+int64_t worth_chunks(const ns_scan_args* a) {
   if (a->ticks <= 0 || a->batch <= 0) return 1;
   const int64_t per = a->channels / a->groups;
   const int64_t blocks = a->groups * ((per + kScanChannels - 1) / kScanChannels) * a->batch;
   const int64_t tile = tile_of(lane_states(a->states)), tiles = (a->ticks + tile - 1) / tile;
-  if (blocks >= 512 || tiles < 8) return 1;
-  const int64_t chunks = 2048 / blocks < tiles / 4 ? 2048 / blocks : tiles / 4;
+  if (blocks >= 512 || tiles < 8 + blocks / 16) return 1;
+  const int64_t chunks = 2048 / blocks < tiles / 2 ? 2048 / blocks : tiles / 2;
   return chunks < 2 ? 1 : chunks;
 }
 
@@ -376,7 +384,7 @@ int ns_scan_plan(int64_t ticks, int64_t batch, int64_t channels, int64_t groups,
   a.rates = &present;
   if (!sizes) return ns::fail("the sizes' place is required");
   if (int rc = ns::check_shape(&a)) return rc;
-  a.chunks = static_cast<int32_t>(ns::worth_chunks(&a, backward != 0));
+  a.chunks = static_cast<int32_t>(ns::worth_chunks(&a));
   const ns::ScanShape s = ns::scan_shape(&a);
   const int64_t r = ns::lane_states(states), tile = ns::tile_of(r), lines = batch * channels;
   sizes[0] = s.chunks;
