@@ -354,12 +354,14 @@ __global__ __launch_bounds__(G::threads) void product_tiles(MxView a, MxView b, 
 // stages' requests leave one by one between the products, so that neither LDS, nor the
 // requests' addresses, nor the barrier keep the matrix cores waiting for long: one barrier a
 // stage, after its first half, when all have read the stage to its end and the next one has
-// arrived.  8192^3 in bf16: 308 us, 3.57 PFLOP/s; 4096 x 4096 by 32768: 238 us, 4.61 PFLOP/s, 68%
-// of the rate at which these instructions issue from registers (6.8).  (On the way, the first
-// of them: 418 us with both steps' fragments read at once and a wait for all requests; 366
-// with two barriers a stage; 336 like this with all requests right behind the barrier; 324
-// spread.)  What bounds it is the units' taking turns: per stage of 4700 cycles (at 336 us) the
-// matrix cores are busy 2050, the texture units with the requests 2500, LDS 1100.
+// arrived.  On one card 8192^3 in bf16 takes 270 us, 4.07 PFLOP/s, 4096 x 4096 by 32768 264 us,
+// 4.16 PFLOP/s: 61% of the rate at which these instructions issue from registers (6.8).  (On
+// the way, the first of them on another card: 418 us with both steps' fragments read at once
+// and a wait for all requests; 366 with two barriers a stage; 336 like this with all requests
+// right behind the barrier; 324 spread; 304 with streamed results and bands of tiles.)  What
+// bounds it: of the second's 264 us the products alone, in this frame, take 189, with the
+// fragments' reads 219; the requests alone take 124 without those for scales, and slow the
+// rest down while they pass through the same LDS.
 // The requests are inline assembly because the compiler, which cannot tell the two buffers
 // apart, would wait for all of them before it reads either; they write LDS only, no registers,
 // and the barriers' waits count them.
@@ -392,72 +394,72 @@ __device__ __forceinline__ void to_lds_4(const v4i& buffer, uint32_t offset, uin
                :: "s"(to), "v"(offset), "s"(buffer) : "memory");
 }
 
+// Where row r keeps block k of a stage: place k ^ turn(r).  Four neighbouring lanes then ask
+// for 64 neighbouring bytes (blocks of one step side by side: requests alone 183 us instead
+// of 124, without scales), and the fragment reads, whose quarters hold rows 0-3 and 12-15 of
+// one block with rows 4-11 of the next but one, meet no bank twice: bit 2 of the turn tells
+// the two sets of rows apart.
+__device__ __forceinline__ uint32_t turn(uint32_t row) {
+  return (row >> 1 & 7) ^ (row & 4);
+}
+
 template <class G>
-struct WordStage {
-  v4i codes[G::rows * 8];      // block 2g + s of row r at place (4s + g) ^ (r/2 % 8)
-  uint32_t scales[G::rows * 2];
+struct WordStages {
+  v4i codes[2][G::rows * 8];
+  uint32_t scales[2][G::rows * 4];   // words 4r .. are row r's of two stages
 };
 
-template <class G>
-constexpr int kWordRequests = G::loads + G::rows * 2 / G::threads;   // per wavefront and stage
-
-// The requests of a stage, by number: the first G::loads are codes, eight rows of 128 bytes
-// each; the others scales, words 2r and 2r + 1 of LDS being row r's blocks 0-3 and 4-7.
-template <class G>
+// What a wavefront asks for: per stage G::loads pieces of codes, eight rows of 128 bytes each;
+// per two stages one piece of scales, 16 bytes of 64 rows (4 bytes of 32 rows a stage: 4096 x
+// 4096 by 32768 277 us instead of 264).
 struct StageRequests {
   uint32_t row, at, to;        // row and block of the lane's codes; LDS address of the stage
   bool inside;
-  int block, wave, lane;
+};
+struct ScaleRequests {
+  uint32_t block, wave, lane, to;
+  bool wanted;
 };
 
 template <class G>
-__device__ __forceinline__ StageRequests<G> stage_requests(const WordPanel& a, int block, int wave,
-                                                           int lane, uint32_t to) {
-  StageRequests<G> q;
+__device__ __forceinline__ StageRequests stage_requests(const WordPanel& a, int block, int wave,
+                                                        int lane, uint32_t to) {
+  StageRequests q;
   q.row = 8 * wave + (lane >> 3);
-  const uint32_t own = (lane & 7) ^ (q.row >> 1 & 7);
-  q.at = block + (2 * (own & 3) | own >> 2);
+  q.at = block + ((lane & 7) ^ turn(q.row));
   q.inside = q.at < a.blocks;
-  q.to = to;
-  q.block = block;
-  q.wave = wave;
-  q.lane = lane;
+  q.to = to + 16 * 64 * wave;
   return q;
 }
 
+constexpr uint32_t kNone = 0xFFFFFFF0u;                    // past every buffer: reads as zeros
+
 template <class G, int I>
-__device__ __forceinline__ void request_piece(const WordPanel& a, const WordPanel& b,
-                                              const StageRequests<G>& q) {
-  constexpr uint32_t kNone = 0xFFFFFFF0u;                  // past every buffer: reads as zeros
+__device__ __forceinline__ void request_codes(const WordPanel& a, const WordPanel& b,
+                                              const StageRequests& q) {
   constexpr int kPerRound = G::threads / 8, kLoadsA = G::rows_m / kPerRound;
-  if constexpr (I < G::loads) {
-    const WordPanel& m = I < kLoadsA ? a : b;
-    const uint32_t r = q.row + kPerRound * (I < kLoadsA ? I : I - kLoadsA);
-    to_lds_16(m.codes, q.inside ? r * m.row_bytes + q.at * 16 : kNone,
-              q.to + 16 * (I * G::threads + 64 * q.wave));
-  } else if constexpr (I < kWordRequests<G>) {
-    constexpr int i = I - G::loads, kWords = G::rows * 2 / G::threads;
-    static_assert(G::rows_m * 2 % G::threads == 0, "a request's scales are of one operand");
-    const bool of_a = i * G::threads < G::rows_m * 2;
-    const WordPanel& m = of_a ? a : b;
-    const uint32_t word = i * G::threads + 64 * q.wave + q.lane, half = q.block + 4 * (word & 1);
-    const uint32_t r = (word >> 1) - (of_a ? 0 : G::rows_m);
-    to_lds_4(m.scales, half < m.blocks ? r * m.blocks + half : kNone,
-             q.to + static_cast<uint32_t>(offsetof(WordStage<G>, scales)) +
-                 4 * (i * G::threads + 64 * q.wave));
-    (void)kWords;
-  }
+  const WordPanel& m = I < kLoadsA ? a : b;
+  const uint32_t r = q.row + kPerRound * (I < kLoadsA ? I : I - kLoadsA);
+  to_lds_16(m.codes, q.inside ? r * m.row_bytes + q.at * 16 : kNone, q.to + 16 * (I * G::threads));
 }
 
-template <class G, int First, int Count>
-__device__ __forceinline__ void request_pieces(const WordPanel& a, const WordPanel& b,
-                                               const StageRequests<G>& q) {
-  if constexpr (Count > 0) {
-    request_piece<G, First>(a, b, q);
-    request_pieces<G, First + 1, Count - 1>(a, b, q);
-  }
+// Scales of two stages.  Past a row's end these are the next row's, and are not used.
+template <class G>
+__device__ __forceinline__ void request_scales(const WordPanel& a, const WordPanel& b,
+                                               const ScaleRequests& q) {
+  static_assert(G::rows == G::threads && G::rows_m % 64 == 0, "one row per lane, of one operand");
+  const bool of_a = 64 * q.wave < G::rows_m;
+  const WordPanel& m = of_a ? a : b;
+  const uint32_t r = 64 * q.wave + q.lane - (of_a ? 0 : G::rows_m);
+  to_lds_16(m.scales, q.block < a.blocks ? r * a.blocks + q.block : kNone, q.to + 16 * 64 * q.wave);
 }
 
+template <class G, int I = 0>
+__device__ __forceinline__ void request_all_codes(const WordPanel& a, const WordPanel& b,
+                                                  const StageRequests& q) {
+  request_codes<G, I>(a, b, q);
+  if constexpr (I + 1 < G::loads) request_all_codes<G, I + 1>(a, b, q);
+}
 // A wavefront's operands: of one step of a stage, and a stage's scales (byte s: step s).
 // Lane l's blocks are 2(l/16) and 2(l/16) + 1, so that its two scale bytes are one word.
 template <class G>
@@ -476,13 +478,15 @@ struct StepBase {
 };
 
 template <class G>
-__device__ __forceinline__ StepBase step_base(uint32_t stage, int step, int wm, int wn, int lane) {
-  const uint32_t row = lane & 15, place = (4 * step + (lane >> 4)) ^ (lane >> 1 & 7);
+__device__ __forceinline__ StepBase step_base(uint32_t stage, uint32_t stage_scales, int step, int wm,
+                                              int wn, int lane) {
+  constexpr int kScaleBytes = 16;                          // per row
+  const uint32_t row = lane & 15, place = (2 * (lane >> 4) + step) ^ turn(row);
   const uint32_t codes = stage + (row * 8 + place) * 16;
-  const uint32_t scales = stage + static_cast<uint32_t>(offsetof(WordStage<G>, scales)) + row * 8 +
-                          2 * (lane >> 4);
+  const uint32_t scales = stage_scales + row * kScaleBytes + 2 * (lane >> 4);
   StepBase base{codes + wm * (G::MI * 16 * 128), codes + (G::rows_m + wn * G::NJ * 16) * 128,
-                scales + wm * (G::MI * 16 * 8), scales + (G::rows_m + wn * G::NJ * 16) * 8};
+                scales + wm * (G::MI * 16 * kScaleBytes),
+                scales + (G::rows_m + wn * G::NJ * 16) * kScaleBytes};
   // One register each, here: left to itself the compiler keeps every strip's.
   asm volatile("" : "+v"(base.codes_a), "+v"(base.codes_b), "+v"(base.scales_a), "+v"(base.scales_b));
   return base;
@@ -492,19 +496,21 @@ __device__ __forceinline__ v4i read_code(uint32_t base, int strip) {
   return *(const __attribute__((address_space(3))) v4i*)static_cast<uintptr_t>(base + strip * (16 * 128));
 }
 __device__ __forceinline__ int read_scale(uint32_t base, int strip) {
-  return *(const __attribute__((address_space(3))) uint16_t*)static_cast<uintptr_t>(base + strip * (16 * 8));
+  return *(const __attribute__((address_space(3))) uint16_t*)static_cast<uintptr_t>(base + strip * (16 * 16));
 }
 
 // Multiplies column strip J of step S, reading strip J of the next step meanwhile (and, where
-// that begins a stage, its scales), and making requests First .. of the stage after.
+// that begins a stage, its scales), and requesting codes of the stage after that (S 1) or the
+// scales of stages to come (S 0).
 template <class G, int S, int J>
 __device__ __forceinline__ void column(StepFragments<G>& f, const StageScales<G>& scales,
                                        const StepBase& from, StepFragments<G>& next,
                                        StageScales<G>& next_scales, const WordPanel& pa,
-                                       const WordPanel& pb, const StageRequests<G>& q,
-                                       v4f (&sum)[G::MI][G::NJ]) {
+                                       const WordPanel& pb, const StageRequests& q,
+                                       const ScaleRequests& to_come, int keep, v4f (&sum)[G::MI][G::NJ]) {
   constexpr int kPer = G::MI / G::NJ;                      // a's strips per column
   static_assert(kPer == 2, "a column reads two strips of a");
+  static_assert(G::loads == 2 * G::NJ, "a column requests two pieces");
   int pair[2];
   next.b[J] = read_code(from.codes_b, J);
 #pragma unroll
@@ -513,9 +519,10 @@ __device__ __forceinline__ void column(StepFragments<G>& f, const StageScales<G>
     next_scales.b[J] = read_scale(from.scales_b, J);
     pair[0] = read_scale(from.scales_a, kPer * J);
     pair[1] = read_scale(from.scales_a, kPer * J + 1);
-    request_pieces<G, 2 * J, 2>(pa, pb, q);
-  } else {
-    request_pieces<G, 2 * G::NJ + J, J < 2 ? 1 : 0>(pa, pb, q);
+    request_codes<G, 2 * J>(pa, pb, q);
+    request_codes<G, 2 * J + 1>(pa, pb, q);
+  } else if constexpr (J == 0) {
+    if (to_come.wanted) request_scales<G>(pa, pb, to_come);
   }
   // The empty statements keep the products of a column in its place: the compiler would gather
   // them before the barrier, and wait there for operands that were to arrive meanwhile.
@@ -526,9 +533,12 @@ __device__ __forceinline__ void column(StepFragments<G>& f, const StageScales<G>
                       : mx_mfma<S, S>(f.b[J], f.a[i], sum[i][J], scales.b[J], scales.a[i / 2]);
 #pragma unroll
   for (int i = 0; i < G::MI; ++i) asm volatile("" : "+v"(sum[i][J]));
-  if constexpr (S == 1) next_scales.a[J] = pair[0] | pair[1] << 16;
+  if constexpr (S == 1) {
+    next_scales.b[J] &= keep;
+    next_scales.a[J] = (pair[0] | pair[1] << 16) & keep;
+  }
   if constexpr (J + 1 < G::NJ)
-    column<G, S, J + 1>(f, scales, from, next, next_scales, pa, pb, q, sum);
+    column<G, S, J + 1>(f, scales, from, next, next_scales, pa, pb, q, to_come, keep, sum);
 }
 
 // s_waitcnt: vmcnt in bits 0-3 and 14-15, expcnt 4-6, lgkmcnt 8-11.
@@ -541,13 +551,18 @@ __device__ __forceinline__ void wait_barrier() {
   asm volatile("" ::: "memory");
 }
 
+__device__ __forceinline__ uint32_t lds_address(const void* at) {
+  return uniform(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
+      (__attribute__((address_space(3))) const void*)at)));
+}
+
 template <class G, class T>
 __global__ __launch_bounds__(G::threads) void product_word_tiles(MxView a, MxView b,
                                                                  const float* bias, T* out,
                                                                  int64_t stride, uint32_t tiles_m,
                                                                  uint32_t tiles_n) {
   __shared__ union {
-    WordStage<G> stages[2];
+    WordStages<G> stages;
     Strip<G, T> strip[G::WM * G::WN];
   } lds;
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
@@ -567,38 +582,50 @@ __global__ __launch_bounds__(G::threads) void product_word_tiles(MxView a, MxVie
   const int64_t n0 = static_cast<int64_t>(tile_n) * G::rows_n;
   const WordPanel pa = word_panel(a, m0, G::rows_m), pb = word_panel(b, n0, G::rows_n);
   const int stages = (static_cast<int>(pa.blocks) + 7) / 8;
-  uint32_t place[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-    place[i] = uniform(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
-        (__attribute__((address_space(3))) void*)&lds.stages[i])));
+  const uint32_t codes = lds_address(&lds.stages.codes), scales_at = lds_address(&lds.stages.scales);
+  constexpr uint32_t kCodes = sizeof(lds.stages.codes[0]), kScales = sizeof(lds.stages.scales[0]);
 
   v4f sum[G::MI][G::NJ] = {};
   StepFragments<G> even, odd;  // operands of a stage's first and second step
   StageScales<G> scales, next_scales;
-  request_pieces<G, 0, kWordRequests<G>>(pa, pb, stage_requests<G>(pa, 0, wave, lane, place[0]));
-  request_pieces<G, 0, kWordRequests<G>>(pa, pb, stage_requests<G>(pa, 8, wave, lane, place[1]));
-  wait_barrier<wait_loads(kWordRequests<G>)>();
-  const StepBase begin = step_base<G>(place[0], 0, wm, wn, lane);
+  request_all_codes<G>(pa, pb, stage_requests<G>(pa, 0, wave, lane, codes));
+  request_scales<G>(pa, pb, ScaleRequests{0, static_cast<uint32_t>(wave),
+                                                     static_cast<uint32_t>(lane), scales_at, true});
+  request_all_codes<G>(pa, pb, stage_requests<G>(pa, 8, wave, lane, codes + kCodes));
+  wait_barrier<wait_loads(G::loads)>();
+  const StepBase begin = step_base<G>(codes, scales_at, 0, wm, wn, lane);
+  const int keep = 2 * (lane >> 4) < static_cast<int>(pa.blocks) ? -1 : 0;
 #pragma unroll
   for (int i = 0; i < G::MI; ++i) {
     even.a[i] = read_code(begin.codes_a, i);
-    if (i & 1) scales.a[i / 2] = read_scale(begin.scales_a, i - 1) | read_scale(begin.scales_a, i) << 16;
+    if (i & 1)
+      scales.a[i / 2] =
+          (read_scale(begin.scales_a, i - 1) | read_scale(begin.scales_a, i) << 16) & keep;
   }
 #pragma unroll
   for (int j = 0; j < G::NJ; ++j) {
     even.b[j] = read_code(begin.codes_b, j);
-    scales.b[j] = read_scale(begin.scales_b, j);
+    scales.b[j] = read_scale(begin.scales_b, j) & keep;
   }
   // Stages past the last read as zeros and are not multiplied.
   for (int stage = 0; stage < stages; ++stage) {
-    const uint32_t now = stage & 1 ? place[1] : place[0], then = stage & 1 ? place[0] : place[1];
-    column<G, 0, 0>(even, scales, step_base<G>(now, 1, wm, wn, lane), odd, next_scales, pa, pb,
-                    stage_requests<G>(pa, 8 * (stage + 1), wave, lane, then), sum);
+    const uint32_t now = codes + (stage & 1 ? kCodes : 0), then = codes + (stage & 1 ? 0 : kCodes);
+    const int after = stage + 1;
+    // The other half of the scales is read to its end: the last barrier saw to it.
+    const ScaleRequests to_come{8u * (stage + 2), static_cast<uint32_t>(wave),
+                                static_cast<uint32_t>(lane),
+                                scales_at + ((stage & 2) ? 0 : kScales), !(stage & 1)};
+    column<G, 0, 0>(even, scales, step_base<G>(now, scales_at, 1, wm, wn, lane), odd, next_scales, pa,
+                    pb, StageRequests{}, to_come, 0, sum);
     // This stage is read by all, and the next one has arrived for all.
     wait_barrier<0>();
-    column<G, 1, 0>(odd, scales, step_base<G>(then, 0, wm, wn, lane), even, next_scales, pa, pb,
-                    stage_requests<G>(pa, 8 * (stage + 2), wave, lane, now), sum);
+    // Blocks past K have codes of zero, but their scales, another row's, may be NaN.
+    const int keep = 8 * after + 2 * (lane >> 4) < static_cast<int>(pa.blocks) ? -1 : 0;
+    column<G, 1, 0>(odd, scales,
+                    step_base<G>(then, scales_at + (after & 2 ? kScales : 0) + 8 * (after & 1), 0, wm,
+                                 wn, lane),
+                    even, next_scales, pa, pb, stage_requests<G>(pa, 8 * (stage + 2), wave, lane, now),
+                    to_come, keep, sum);
     scales = next_scales;
   }
   wait_barrier<0>();                                       // before LDS is used anew

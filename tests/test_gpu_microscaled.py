@@ -150,6 +150,19 @@ def test_product_of_many_rows(gpu, shape):
     assert error <= 2 * (HALF_ULP[dtype] + K * 2.0 ** -23)
 
 
+@pytest.mark.parametrize("K", [128, 256, 384, 640, 896])
+def test_blocks_without_numbers_stay_in_their_row(gpu, K):
+    """The 256 x 256 tiles ask for scales past a row's end; those, another row's, may be NaN."""
+    x, w = rows(gpu, 43, 3500, K), rows(gpu, 44, 3400, K) / K ** 0.5
+    want = mx_product(x, mx_quantize(w))
+    x[1::7, 0], w[2::5, 0] = float("nan"), float("nan")
+    got = mx_product(x, mx_quantize(w))
+    bad = torch.zeros_like(got, dtype=torch.bool)
+    bad[1::7], bad[:, 2::5] = True, True
+    assert torch.equal(got.isnan(), bad)
+    assert torch.equal(got[~bad], want[~bad])
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_product_keeps_leading_dimensions(gpu, dtype):
     x = rows(gpu, 8, 3, 5, 90, dtype=dtype)
