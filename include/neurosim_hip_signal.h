@@ -101,9 +101,8 @@ typedef struct ns_scan_args {
   ns_signal dx, ddelta, dz;    /* dz present exactly if z is */
   ns_signal dwrite, dread;     /* dB, dC */
   float* dstate;               /* gradient of state [B][N][S], or NULL */
-  float* drates;               /* dA [N][S] */
-  float* dskip;                /* dD [N] (written also without D) */
-  float* ddelta_bias;          /* [N] (written also without a bias) */
+  float* dparameters;          /* dA [N][S], then dD [N] and d(delta_bias) [N] (these are
+                                  written also without D and without a bias) */
   float* partials;             /* workspace (ns_scan_plan) */
 } ns_scan_args;
 

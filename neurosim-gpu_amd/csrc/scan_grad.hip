@@ -32,9 +32,7 @@ template <class T>
 struct ScanOut {
   Signal<T> dx, ddelta, dz;
   float* dstate;
-  float* rate_parts;    // [chunks*B][N][S]
-  float* skip_parts;    // [chunks*B][N]
-  float* bias_parts;    // [chunks*B][N]
+  float* parts;         // [chunks*B] of dA [N][S], dD [N], d(delta_bias) [N]
   float* shared_parts;  // [group_blocks][B][G][T][2][4R]: dC, dB
 };
 
@@ -324,13 +322,13 @@ __global__ __launch_bounds__(kThreads, 2) void scan_backward(ScanShape s, ScanIn
     }
     __syncthreads();                      // before the next tile overwrites LDS
   }
-  const int64_t part = p.c * s.batch + p.b;
+  float* const own_parts = out.parts + (p.c * s.batch + p.b) * s.channels * (s.states + 2);
   if (own) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const int state = q * R + r;
       if (state < s.states) {
-        out.rate_parts[(part * s.channels + n) * s.states + state] = drate[r];
+        own_parts[n * s.states + state] = drate[r];
         if (p.c == 0 && out.dstate) out.dstate[line * s.states + state] = g[r];
       }
     }
@@ -339,9 +337,9 @@ __global__ __launch_bounds__(kThreads, 2) void scan_backward(ScanShape s, ScanIn
   sum_w[wave][lane] = dbias;
   __syncthreads();
   if (wave == 0 && lane < p.own) {
-    out.skip_parts[part * s.channels + p.n0 + lane] =
+    own_parts[s.channels * s.states + p.n0 + lane] =
         (sum_y[0][lane] + sum_y[1][lane]) + (sum_y[2][lane] + sum_y[3][lane]);
-    out.bias_parts[part * s.channels + p.n0 + lane] =
+    own_parts[s.channels * (s.states + 1) + p.n0 + lane] =
         (sum_w[0][lane] + sum_w[1][lane]) + (sum_w[2][lane] + sum_w[3][lane]);
   }
 }
@@ -377,13 +375,12 @@ int launched(const char* what) {
 }
 
 struct PartSizes {
-  int64_t rates, lines, shared;
+  int64_t parameters, shared;
 };
 
 PartSizes part_sizes(const ns_scan_args* a) {
   const ScanShape s = scan_shape(a);
-  const int64_t parts = s.chunks * s.batch;
-  return PartSizes{parts * s.channels * s.states, parts * s.channels,
+  return PartSizes{s.chunks * s.batch * s.channels * (s.states + 2),
                    s.group_blocks * s.ticks * s.batch * s.groups * 8 * lane_states(s.states)};
 }
 
@@ -395,8 +392,7 @@ int run_backward(const ns_scan_args* a, hipStream_t stream) {
   const ScanIn<T> in = scan_in<T>(a);
   const PartSizes sizes = part_sizes(a);
   ScanOut<T> out{signal<T>(a->dx), signal<T>(a->ddelta), signal<T>(a->dz), a->dstate, a->partials,
-                 a->partials + sizes.rates, a->partials + sizes.rates + sizes.lines,
-                 a->partials + sizes.rates + 2 * sizes.lines};
+                 a->partials + sizes.parameters};
   const Signal<T> dy = signal<T>(a->dy);
   if (s.chunks > 1) {
     scan_adjoint_ends<T, R><<<grid, dim3(kThreads), 0, stream>>>(
@@ -407,10 +403,9 @@ int run_backward(const ns_scan_args* a, hipStream_t stream) {
   scan_backward<T, R><<<grid, dim3(kThreads), 0, stream>>>(
       s, in, ScanUp<T>{dy, a->dout_state}, out, a->checkpoints, a->ends);
   if (int rc = launched("scan backward")) return rc;
-  const int64_t parts = s.chunks * s.batch;
-  if (int rc = sum_partials(out.rate_parts, parts, s.channels * s.states, a->drates, stream)) return rc;
-  if (int rc = sum_partials(out.skip_parts, parts, s.channels, a->dskip, stream)) return rc;
-  if (int rc = sum_partials(out.bias_parts, parts, s.channels, a->ddelta_bias, stream)) return rc;
+  if (int rc = sum_partials(out.parts, s.chunks * s.batch, s.channels * (s.states + 2),
+                            a->dparameters, stream))
+    return rc;
   const int64_t values = s.ticks * s.batch * s.groups * 8 * R;
   const int64_t groups = (values + kThreads - 1) / kThreads;
   if (groups > INT32_MAX) return fail("the signal is too large for one launch");
@@ -435,7 +430,7 @@ int run(const ns_scan_args* a, hipStream_t stream) {
 
 int64_t scan_part_floats(const ns_scan_args* a) {
   const PartSizes sizes = part_sizes(a);
-  return sizes.rates + 2 * sizes.lines + sizes.shared;
+  return sizes.parameters + sizes.shared;
 }
 
 }  // namespace ns
@@ -445,7 +440,7 @@ extern "C" {
 int ns_scan_backward(const ns_scan_args* a, void* stream) {
   ns::clear_error();
   if (int rc = ns::check_scan(a)) return rc;
-  if (!a->drates || !a->dskip || !a->ddelta_bias)
+  if (!a->dparameters)
     return ns::fail("the gradients of the rates, skips and biases are required");
   if (a->batch && a->ticks) {
     if (!a->partials || !a->checkpoints) return ns::fail("the backward needs its workspaces");

@@ -40,10 +40,10 @@ TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # NS_TYPE_*
 _CONV = struct.Struct("=3q4i Q2q 2Q Q2q Q Q2q Q2q Q2q Q2q Q2q Q2q 2Q")
 _CONV_FORWARD = struct.Struct("=3q4i Q2q 2Q Q2q Q Q2q Q2q 112x")
 # ns_scan_args: shape; x, delta, z, y; B, C; A, D, delta_bias, state, out_state, lengths,
-# checkpoints, ends; dy; dout_state; dx, ddelta, dz, dB, dC; dstate, dA, dD, ddelta_bias,
-# partials.
-_SCAN = struct.Struct("=4q4i Q2q Q2q Q2q Q2q Q2q Q2q 8Q Q2q Q Q2q Q2q Q2q Q2q Q2q 5Q")
-_SCAN_FORWARD = struct.Struct("=4q4i Q2q Q2q Q2q Q2q Q2q Q2q 8Q 192x")
+# checkpoints, ends; dy; dout_state; dx, ddelta, dz, dB, dC; dstate, gradients of A, D and
+# delta_bias, partials.
+_SCAN = struct.Struct("=4q4i Q2q Q2q Q2q Q2q Q2q Q2q 8Q Q2q Q Q2q Q2q Q2q Q2q Q2q 3Q")
+_SCAN_FORWARD = struct.Struct("=4q4i Q2q Q2q Q2q Q2q Q2q Q2q 8Q 176x")
 _ABSENT = (0, 0, 0)
 
 _i32, _i64, _ptr = ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p
@@ -389,15 +389,13 @@ class _SelectiveScan(torch.autograd.Function):
         # The parameters' gradients and the workspaces share one allocation.
         sums = torch.empty(n * (states + 2), dtype=torch.float32, device=device)
         work = torch.empty(part_floats + ends_floats, dtype=torch.float32, device=device)
-        rates, skips = sums.data_ptr(), sums.data_ptr() + 4 * n * states
         args = _SCAN.pack(
             ticks, batch, n, ctx.groups, states, TYPES[x.dtype], ctx.softplus, chunks,
             *_signal(x), *_signal(delta), *_signal(z), *_ABSENT, *_signal(B), *_signal(C),
             A.data_ptr(), _address(D), _address(delta_bias), 0, 0, _address(lengths),
             kept.data_ptr(), work.data_ptr() + 4 * part_floats if ends_floats else 0,
             *_signal(dy), _address(dfinal), *_signal(dx), *_signal(ddelta), *_signal(dz),
-            *_signal(dB), *_signal(dC), _address(dstate), rates, skips, skips + 4 * n,
-            work.data_ptr())
+            *_signal(dB), *_signal(dC), _address(dstate), sums.data_ptr(), work.data_ptr())
         call(_library().ns_scan_backward, device, args)
         grads = (dx, ddelta, sums[:n * states].view(n, states), dB, dC,
                  sums[n * states:n * (states + 1)] if D is not None else None, dz,
