@@ -102,6 +102,13 @@ def _unit_channels(value: torch.Tensor | None, inner: int = 1):
     return value
 
 
+def _room(value: torch.Tensor) -> torch.Tensor:
+    """A dense tensor of ``value``'s shape and type (the short way costs a third)."""
+    if value.is_contiguous():
+        return torch.empty_like(value)
+    return torch.empty(value.shape, dtype=value.dtype, device=value.device)
+
+
 def _check_signal(x, what: str, dims: int) -> None:
     if not isinstance(x, torch.Tensor) or x.dim() != dims:
         raise ValueError(f"{what} must be a {'[T, B, N]' if dims == 3 else '[B, N]'} tensor")
@@ -183,7 +190,7 @@ def _conv_forward(x, weight, bias, history, lengths, silu, chunk=0):
     """(y, last inputs) of dense operands."""
     ticks, batch, n = x.shape
     taps, device = weight.shape[1], x.device
-    y = torch.empty((ticks, batch, n), dtype=x.dtype, device=device)
+    y = _room(x)
     last = torch.empty((taps - 1, batch, n), dtype=x.dtype, device=device)
     args = _CONV_FORWARD.pack(ticks, batch, n, taps, TYPES[x.dtype], silu, chunk, *_signal(x),
                               weight.data_ptr(), _address(bias), *_signal(history),
@@ -209,9 +216,8 @@ class _CausalConv(torch.autograd.Function):
         (ticks, batch, channels), taps = x.shape, weight.shape[1]
         dy = torch.zeros_like(x) if dy is None else _unit_channels(dy)
         dlast = _unit_channels(dlast)
-        dx = torch.empty(x.shape, dtype=x.dtype, device=device) if wants[0] else None
-        dhistory = (torch.empty(history.shape, dtype=x.dtype, device=device)
-                    if history is not None and wants[3] else None)
+        dx = _room(x) if wants[0] else None
+        dhistory = _room(history) if history is not None and wants[3] else None
         lib, count = _library(), channels * (taps + 1)
         parts = lib.ns_conv_backward_floats(ticks, batch, channels, taps, TYPES[x.dtype])
         # The parameters' gradients and the workspace share one allocation.
@@ -260,7 +266,7 @@ def causal_conv_step(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor |
         bias = _dense(_master(bias))
     if n > 1 and x.stride(1) != 1:
         x = x.contiguous()
-    y = torch.empty((batch, n), dtype=x.dtype, device=x.device)
+    y = _room(x)
     carried = _signal(history)
     args = _CONV_FORWARD.pack(1, batch, n, taps, TYPES[x.dtype], _ACTIVATIONS[activation], 0,
                               x.data_ptr(), 0, x.stride(0), weight.data_ptr(), _address(bias),
@@ -340,7 +346,7 @@ def _scan_forward(operands, state, lengths, softplus, groups, keep: bool):
     x, delta, A, B, C, D, z, delta_bias = operands
     ticks, batch, n = x.shape
     states, device = A.shape[1], x.device
-    y = torch.empty((ticks, batch, n), dtype=x.dtype, device=device)
+    y = _room(x)
     final = torch.empty((batch, n, states), dtype=torch.float32, device=device)
     chunks, ends_floats, kept_floats, _ = _plan(x.shape, groups, states, False)
     ends = torch.empty(ends_floats, dtype=torch.float32, device=device) if ends_floats else None
@@ -379,11 +385,8 @@ class _SelectiveScan(torch.autograd.Function):
         dy = torch.zeros_like(x) if dy is None else _unit_channels(dy)
         chunks, ends_floats, _, part_floats = _plan(x.shape, ctx.groups, states, True)
 
-        def like(value):
-            return None if value is None else torch.empty(value.shape, dtype=value.dtype,
-                                                          device=device)
-
-        dx, ddelta, dz, dB, dC = like(x), like(delta), like(z), like(B), like(C)
+        dx, ddelta, dB, dC = _room(x), _room(delta), _room(B), _room(C)
+        dz = None if z is None else _room(z)
         dstate = (torch.empty((batch, n, states), dtype=torch.float32, device=device)
                   if wants[8] else None)
         # The parameters' gradients and the workspaces share one allocation.
@@ -441,7 +444,7 @@ def selective_scan_step(x: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B
         raise ValueError("state must be a contiguous [B, N, S] tensor, updated in place")
     x, delta, A, B, C, D, z, delta_bias = _dense_scan(x, delta, A, B, C, D, z, delta_bias)
     batch, n = x.shape
-    y = torch.empty((batch, n), dtype=x.dtype, device=x.device)
+    y = _room(x)
     args = _SCAN_FORWARD.pack(
         1, batch, n, groups, states, TYPES[x.dtype], softplus, 1, x.data_ptr(), 0, x.stride(0),
         delta.data_ptr(), 0, delta.stride(0),
