@@ -114,11 +114,13 @@ def mx_quantize(x: torch.Tensor) -> MXTensor:
     *lead, columns = x.shape
     rows, blocks, device = _rows(lead), (columns + MX_BLOCK - 1) // MX_BLOCK, x.device
     flat = _float_rows(x, rows, columns)
-    codes = torch.empty((*lead, blocks * 16), dtype=torch.uint8, device=device)
-    scales = torch.empty((*lead, blocks), dtype=torch.uint8, device=device)
+    codes = x.new_empty((*lead, blocks * 16), dtype=torch.uint8)
+    scales = x.new_empty((*lead, blocks), dtype=torch.uint8)
     matrix = _MATRIX.pack(rows, columns, codes.data_ptr(), scales.data_ptr())
     call(_library().ns_mx_quantize, device, matrix, flat.data_ptr(), flat.stride(0), TYPES[x.dtype])
-    return MXTensor(codes, scales, columns)
+    result = MXTensor.__new__(MXTensor)              # as made here, without checks
+    result.codes, result.scales, result.columns = codes, scales, columns
+    return result
 
 
 def mx_dequantize(value: MXTensor, dtype: torch.dtype = torch.float32) -> torch.Tensor:
@@ -129,7 +131,7 @@ def mx_dequantize(value: MXTensor, dtype: torch.dtype = torch.float32) -> torch.
         raise ValueError("values are read back as float32, bfloat16 or float16")
     codes, scales, columns = value.codes, value.scales, value.columns
     lead, device = codes.shape[:-1], codes.device
-    out = torch.empty((*lead, columns), dtype=dtype, device=device)
+    out = codes.new_empty((*lead, columns), dtype=dtype)
     matrix = _MATRIX.pack(_rows(lead), columns, codes.data_ptr(), scales.data_ptr())
     call(_library().ns_mx_dequantize, device, matrix, out.data_ptr(), columns, TYPES[dtype])
     return out
@@ -169,9 +171,9 @@ def mx_product(x: torch.Tensor | MXTensor, weight: MXTensor, *, bias: torch.Tens
             raise ValueError("a 4-bit product gives no gradients")
         bias = bias.contiguous()
     rows, lib = _rows(lead), _library()
-    out = torch.empty((*lead, outputs), dtype=dtype, device=device)
+    out = weight.codes.new_empty((*lead, outputs), dtype=dtype)
     size = lib.ns_mx_product_bytes(rows, outputs, columns, floats)
-    work = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+    work = out.new_empty(size, dtype=torch.uint8) if size else None
     if floats and size:
         flat = _float_rows(x, rows, columns)
         a, rest = (0, 0), (TYPES[x.dtype], flat.data_ptr(), flat.stride(0))
