@@ -1,6 +1,7 @@
 // Microscaled 4-bit rows (gfx950): quantising float rows, and reading them back.
 //
-// Both are one pass over memory.  Four neighbouring lanes share a block of 32 values,
+// Both are one pass over memory: 16384 x 8192 in bf16 (340 MB) 57 us to quantise, 48 to read
+// back, 6 and 7 TB/s.  Four neighbouring lanes share a block of 32 values,
 // eight values each, so a wavefront's loads and stores are whole runs of a row; the
 // block's largest magnitude is joined over its lanes by two DPP steps.  Magnitudes are
 // compared as integers: on non-negative floats the order is the same, and infinities and

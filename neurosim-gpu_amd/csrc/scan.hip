@@ -3,15 +3,21 @@
 //   dt = softplus(delta + bias);  h[t] = exp(dt A) h[t-1] + dt x B[t]
 //   y[t] = (sum_s C[t] h[t] + D x) silu(z)
 //
-// Per (tick, channel, state) one exp2, three multiplies or adds of the update and one of
-// the sum, against 8 bytes (bf16) per (tick, channel): the vector ALU bounds it, at 16
-// states by about two to one over HBM.
+// Per (tick, channel, state) one exp2 (two issue slots), three multiplies or adds of the update
+// and one of the sum, against 8 bytes (bf16) per (tick, channel): the vector ALU bounds it, at
+// 16 states by about two to one over HBM.  T=2048, B=8, N=4096, S=16 in bf16: 377 us, of which
+// those six slots alone take 192 at the card's 33.5e12 lanes/s and the elementwise part (two
+// exp, a log, a reciprocal and their like per tick and channel) about 80.  (With inputs two
+// tiles ahead 412, with the elementwise part of a thread's items overlapping 377; a tile's
+// ticks beside the next one's elementwise part, in two halves of LDS, 375 and so left out.)
 //
 // Few columns and channels leave most of the card idle, so time is then cut into chunks
 // scanned side by side: a first pass gives every chunk's end state from zero and its
 // summed time step, whose exponential is the chunk's decay exp(A sum dt); the chunks are
 // joined in order; a second pass runs them from their true start.  It costs the update
-// twice, so it is taken only where workgroups are few (worth_chunks).
+// twice, so it is taken only where workgroups are few (worth_chunks).  T=16384, B=1, N=2048,
+// S=16 in bf16, 64 chunks: 107 us for the ends, 13 for the join, 160 for the outputs; in one
+// chunk the 32 workgroups would take 40 us per 256 ticks.
 #include "ns_scan.h"
 
 namespace ns {
@@ -151,33 +157,38 @@ __global__ __launch_bounds__(kThreads) void scan_forward(ScanShape s, ScanIn<T> 
 }
 
 // One lane per (column, channel, padded state): walks the chunks in order, leaving in
-// place of each chunk's own end the state (or adjoint) it starts from.
-__global__ __launch_bounds__(kThreads) void join_kernel(ScanShape s, int64_t padded,
-                                                        const float* rates, const float* start,
-                                                        float* ends, const float* steps,
-                                                        bool reverse) {
-  const int64_t id = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  const int64_t lines = s.batch * s.channels;
-  if (id >= lines * padded) return;
-  const int64_t line = id / padded, state = id - line * padded;
-  const bool real = state < s.states;
-  const float rate = real ? rates[line % s.channels * s.states + state] * kLog2e : 0.0f;
+// place of each chunk's own end the state (or adjoint) it starts from.  `blocks` workgroups
+// to a column.  Reads past the last chunk are the last one's again, so that all of a round
+// are requested without a branch between them.  64 chunks of 2048 channels with 16 states (17
+// MB that another XCD has just written): 13 us, all 64 requested at once 11.
+__global__ __launch_bounds__(kThreads) void join_kernel(ScanShape s, uint32_t blocks,
+                                                        uint32_t padded, const float* rates,
+                                                        const float* start, float* ends,
+                                                        const float* steps, bool reverse) {
+  const uint32_t b = uniform(blockIdx.x / blocks);
+  const int64_t at = static_cast<int64_t>(blockIdx.x - b * blocks) * kThreads + threadIdx.x;
+  if (at >= s.channels * padded) return;
+  const uint32_t state = static_cast<uint32_t>(at) & (padded - 1);   // a power of two
+  const int64_t channel = at >> (31 - __builtin_clz(padded)), lines = s.batch * s.channels;
+  const int64_t line = b * s.channels + channel;
+  const bool real = state < static_cast<uint32_t>(s.states);
+  const float rate = real ? rates[channel * s.states + state] * kLog2e : 0.0f;
   float carry = real && start ? start[line * s.states + state] : 0.0f;
-  constexpr int kAhead = 8;
-  for (int64_t first = 0; first < s.chunks; first += kAhead) {
+  const int chunks = static_cast<int>(s.chunks);
+  constexpr int kAhead = 16;
+  for (int first = 0; first < chunks; first += kAhead) {
     float own[kAhead], step[kAhead];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      if (first + u < s.chunks) {
-        const int64_t c = reverse ? s.chunks - 1 - first - u : first + u;
-        own[u] = ends[(c * lines + line) * padded + state];
-        step[u] = steps[c * lines + line];
-      }
+      const int k = first + u < chunks ? first + u : chunks - 1;
+      const int64_t c = reverse ? chunks - 1 - k : k;
+      own[u] = ends[(c * lines + line) * padded + state];
+      step[u] = steps[c * lines + line];
     }
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      if (first + u < s.chunks) {
-        const int64_t c = reverse ? s.chunks - 1 - first - u : first + u;
+      if (first + u < chunks) {
+        const int64_t c = reverse ? chunks - 1 - first - u : first + u;
         ends[(c * lines + line) * padded + state] = carry;
         carry = fmaf(__builtin_amdgcn_exp2f(step[u] * rate), carry, own[u]);
       }
@@ -186,7 +197,8 @@ __global__ __launch_bounds__(kThreads) void join_kernel(ScanShape s, int64_t pad
 }
 
 // One tick, the states updated in place.  Bound by the states' bytes, each read and
-// written once; a channel's four lanes read neighbouring floats.
+// written once; a channel's four lanes read neighbouring floats.  B=32, N=4096, S=16: 6.4 us
+// for 18 MB, of which a launch takes 2.
 template <class T, int R>
 __global__ __launch_bounds__(kThreads) void scan_step(ScanShape s, ScanIn<T> in, Signal<T> y,
                                                       float* state) {
@@ -358,11 +370,12 @@ int run_types(const ns_scan_args* a, bool step, void* stream) {
 int join_chunks(const ns_scan_args* a, float* ends, const float* start, bool reverse, void* stream) {
   const ScanShape s = scan_shape(a);
   const int64_t padded = 4 * lane_states(a->states), lines = s.batch * s.channels;
-  const int64_t groups = (lines * padded + kThreads - 1) / kThreads;
-  if (groups > INT32_MAX) return fail("the signal is too large for one launch");
-  join_kernel<<<dim3(static_cast<unsigned>(groups)), dim3(kThreads), 0,
-                static_cast<hipStream_t>(stream)>>>(s, padded, a->rates, start, ends,
-                                                    ends + s.chunks * lines * padded, reverse);
+  const int64_t blocks = (s.channels * padded + kThreads - 1) / kThreads;
+  if (s.batch * blocks > INT32_MAX) return fail("the signal is too large for one launch");
+  join_kernel<<<dim3(static_cast<unsigned>(s.batch * blocks)), dim3(kThreads), 0,
+                static_cast<hipStream_t>(stream)>>>(
+      s, static_cast<uint32_t>(blocks), static_cast<uint32_t>(padded), a->rates, start, ends,
+      ends + s.chunks * lines * padded, reverse);
   return launched("scan join");
 }
 
