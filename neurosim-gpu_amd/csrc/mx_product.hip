@@ -277,8 +277,7 @@ __device__ __forceinline__ void hold(v4f (&sum)[G::MI][G::NJ]) {
 
 // Tiles of y, one workgroup per tile and part of K.  Two stages of LDS: while one is
 // multiplied, the next one is loaded.  33 x 1000 by 50,000 (64 x 64 tiles, 28 parts): 10 us,
-// and 4 for the parts' sums.  256 x 256 tiles are for large products whose rows
-// of scales are no whole words: 8192 x 8192 by 8160 425 us.
+// and 4 for the parts' sums.
 template <class G, class T>
 __global__ __launch_bounds__(G::threads) void product_tiles(MxView a, MxView b, const float* bias,
                                                             T* out, int64_t stride, uint32_t tiles_m,
@@ -351,8 +350,9 @@ __global__ __launch_bounds__(G::threads) void product_tiles(MxView a, MxView b, 
   }
 }
 
-// Large tiles where rows of scales are whole 32-bit words (K a multiple of 128): scales too go
-// straight into LDS, nothing passes through registers on its way there.  Half a stage (one step
+// Large tiles.  Scales too go straight into LDS, nothing passes through registers on its way
+// there; their rows have to be whole 32-bit words, and where they are not (K no multiple of
+// 128) pad_scales lays them out so first.  Half a stage (one step
 // of 128 values) is multiplied while the fragments of the next half are read and the next
 // stages' requests leave one by one between the products, so that neither LDS, nor the
 // requests' addresses, nor the barrier keep the matrix cores waiting for long: one barrier a
@@ -370,7 +370,7 @@ __global__ __launch_bounds__(G::threads) void product_tiles(MxView a, MxView b, 
 // and the barriers' waits count them.
 struct alignas(16) WordPanel {
   v4i codes, scales;           // buffer descriptors
-  uint32_t row_bytes, blocks;
+  uint32_t row_bytes, blocks, scale_bytes;   // a row's codes, blocks, and scales with their padding
 };
 
 __device__ __forceinline__ v4i describe(const uint8_t* base, uint32_t bytes) {
@@ -382,9 +382,9 @@ __device__ __forceinline__ v4i describe(const uint8_t* base, uint32_t bytes) {
 
 __device__ __forceinline__ WordPanel word_panel(const MxView& m, int64_t row, int rows) {
   const uint32_t own = static_cast<uint32_t>(m.rows - row < rows ? m.rows - row : rows);
-  const uint32_t blocks = uniform(static_cast<uint32_t>(m.blocks));
+  const uint32_t blocks = uniform(static_cast<uint32_t>(m.blocks)), scales = (blocks + 3) & ~3u;
   return WordPanel{describe(m.codes + row * m.blocks * 16, own * blocks * 16),
-                   describe(m.scales + row * m.blocks, own * blocks), blocks * 16, blocks};
+                   describe(m.scales + row * scales, own * scales), blocks * 16, blocks, scales};
 }
 
 // 16 bytes (4 bytes) per lane from `offset` of a buffer to LDS at `to` + 16 (4) * lane.
@@ -446,7 +446,7 @@ __device__ __forceinline__ void request_codes(const WordPanel& a, const WordPane
   to_lds_16(m.codes, q.inside ? r * m.row_bytes + q.at * 16 : kNone, q.to + 16 * (I * G::threads));
 }
 
-// Scales of two stages.  Past a row's end these are the next row's, and are not used.
+// Scales of two stages.  Past a row's words these are the next row's, and are not used.
 template <class G>
 __device__ __forceinline__ void request_scales(const WordPanel& a, const WordPanel& b,
                                                const ScaleRequests& q) {
@@ -454,7 +454,7 @@ __device__ __forceinline__ void request_scales(const WordPanel& a, const WordPan
   const bool of_a = 64 * q.wave < G::rows_m;
   const WordPanel& m = of_a ? a : b;
   const uint32_t r = 64 * q.wave + q.lane - (of_a ? 0 : G::rows_m);
-  to_lds_16(m.scales, q.block < a.blocks ? r * a.blocks + q.block : kNone, q.to + 16 * 64 * q.wave);
+  to_lds_16(m.scales, q.block < a.blocks ? r * a.scale_bytes + q.block : kNone, q.to + 16 * 64 * q.wave);
 }
 
 template <class G, int I = 0>
@@ -552,6 +552,23 @@ __device__ __forceinline__ void wait_barrier() {
   __builtin_amdgcn_s_waitcnt(kWait);
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
+}
+
+// Both operands' rows of scales, a's then b's, in whole words with zeros behind them; a
+// wavefront per row.  For 8192 x 8192 by 8160 PADUS us, and the product 425 -> PRODUS: it was left
+// to tiles like the small ones, 256 x 256 and with scales through registers.
+__global__ __launch_bounds__(kThreads) void pad_scales(MxView a, MxView b, uint32_t* out) {
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / 64) + (threadIdx.x >> 6);
+  if (row >= a.rows + b.rows) return;
+  const uint8_t* from = row < a.rows ? a.scales + row * a.blocks : b.scales + (row - a.rows) * b.blocks;
+  const int64_t words = (a.blocks + 3) / 4;
+  for (int64_t w = threadIdx.x & 63; w < words; w += 64) {
+    uint32_t word = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (4 * w + k < a.blocks) word |= static_cast<uint32_t>(from[4 * w + k]) << (8 * k);
+    out[row * words + w] = word;
+  }
 }
 
 __device__ __forceinline__ uint32_t lds_address(const void* at) {
@@ -823,17 +840,21 @@ int64_t parts_of_k(int64_t m, int64_t n, int64_t k) {
   return (stages + per - 1) / per;
 }
 
-// The workspace: a's codes and scales (float rows), then the parts' sums.
+// The workspace: a's codes and scales (float rows), then the parts' sums, or both operands'
+// scales in whole words.
 struct Workspace {
-  int64_t scales, partials, bytes;
+  int64_t scales, rest, bytes;
 };
+
+int64_t word_bytes(int64_t blocks) { return (blocks + 3) / 4 * 4; }
 
 Workspace workspace_of(int64_t m, int64_t n, int64_t k, bool float_rows) {
   const int64_t blocks = (k + NS_MX_BLOCK - 1) / NS_MX_BLOCK, parts = parts_of_k(m, n, k);
   Workspace w{};
   w.scales = float_rows ? m * blocks * 16 : 0;
-  w.partials = float_rows ? (m * blocks * 17 + 15) / 16 * 16 : 0;
-  w.bytes = w.partials + (parts > 1 ? parts * m * n * 4 : 0);
+  w.rest = float_rows ? (m * blocks * 17 + 15) / 16 * 16 : 0;
+  w.bytes = w.rest + (parts > 1 ? parts * m * n * 4 : 0);
+  if (kernel_of(m, n) == Kernel::kLarge) w.bytes += (m + n) * word_bytes(blocks);
   return w;
 }
 
@@ -850,23 +871,27 @@ int run_tiles(const ns_mx_product_args* p, int64_t parts, float* partials, hipSt
   return launched("product");
 }
 
-// Whether product_word_tiles takes the operands.
-bool word_scales(const ns_mx_product_args* p) {
-  return p->a.columns > 0 && (p->a.columns + NS_MX_BLOCK - 1) / NS_MX_BLOCK % 4 == 0 &&
-         reinterpret_cast<uintptr_t>(p->a.scales) % 4 == 0 &&
-         reinterpret_cast<uintptr_t>(p->b.scales) % 4 == 0;
-}
-
 template <class T>
-int run_large(const ns_mx_product_args* p, hipStream_t stream) {
-  if (!word_scales(p)) return run_tiles<Large, T>(p, 1, nullptr, stream);
+int run_large(const ns_mx_product_args* p, void* words, hipStream_t stream) {
   using G = Large;
-  const int64_t tiles_m = (p->a.rows + G::rows_m - 1) / G::rows_m;
-  const int64_t tiles_n = (p->b.rows + G::rows_n - 1) / G::rows_n;
-  if (tiles_m * tiles_n > INT32_MAX) return fail("the product is too large for one launch");
+  MxView a = view(p->a), b = view(p->b);
+  const int64_t tiles_m = (a.rows + G::rows_m - 1) / G::rows_m;
+  const int64_t tiles_n = (b.rows + G::rows_n - 1) / G::rows_n;
+  const int64_t copies = (a.rows + b.rows + kThreads / 64 - 1) / (kThreads / 64);
+  if (tiles_m * tiles_n > INT32_MAX || copies > INT32_MAX)
+    return fail("the product is too large for one launch");
+  if (a.blocks % 4 || reinterpret_cast<uintptr_t>(a.scales) % 4 ||
+      reinterpret_cast<uintptr_t>(b.scales) % 4) {
+    auto* to = static_cast<uint8_t*>(words);
+    pad_scales<<<dim3(static_cast<unsigned>(copies)), dim3(kThreads), 0, stream>>>(
+        a, b, static_cast<uint32_t*>(words));
+    if (int rc = launched("product scales")) return rc;
+    a.scales = to;
+    b.scales = to + a.rows * word_bytes(a.blocks);
+  }
   product_word_tiles<G, T><<<dim3(static_cast<unsigned>(tiles_m * tiles_n)), dim3(G::threads), 0,
-                             stream>>>(view(p->a), view(p->b), p->bias, static_cast<T*>(p->out),
-                                       p->stride, static_cast<uint32_t>(tiles_m),
+                             stream>>>(a, b, p->bias, static_cast<T*>(p->out), p->stride,
+                                       static_cast<uint32_t>(tiles_m),
                                        static_cast<uint32_t>(tiles_n));
   return launched("product");
 }
@@ -891,8 +916,9 @@ int run_rows(const ns_mx_product_args* p, int64_t parts, float* partials, hipStr
 
 template <class T>
 int run_kernel(const ns_mx_product_args* p, int64_t parts, float* partials, hipStream_t stream) {
-  switch (kernel_of(p->a.rows, p->b.rows)) {
-    case Kernel::kLarge: return run_large<T>(p, stream);
+  const Kernel kernel = kernel_of(p->a.rows, p->b.rows);
+  switch (p->a.columns || kernel == Kernel::kRows ? kernel : Kernel::kSmall) {
+    case Kernel::kLarge: return run_large<T>(p, partials, stream);
     case Kernel::kSmall: return run_tiles<Small, T>(p, parts, partials, stream);
     default: return run_rows<T>(p, parts, partials, stream);
   }
@@ -949,7 +975,7 @@ int ns_mx_product(const ns_mx_product_args* args, void* stream) {
       p.a.scales = space + w.scales;
       if (int rc = ns_mx_quantize(&p.a, p.x, p.x_stride, p.x_type, stream)) return rc;
     }
-    p.workspace = space + w.partials;
+    p.workspace = space + w.rest;
   }
   if (int rc = ns::check_operand(p.a, "a")) return rc;
   if (int rc = ns::check_operand(p.b, "b")) return rc;

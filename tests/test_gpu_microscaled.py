@@ -150,7 +150,7 @@ def test_product_of_many_rows(gpu, shape):
     assert error <= 2 * (HALF_ULP[dtype] + K * 2.0 ** -23)
 
 
-@pytest.mark.parametrize("K", [128, 256, 384, 640, 896])
+@pytest.mark.parametrize("K", [96, 128, 160, 256, 384, 500, 640, 705, 896])
 def test_blocks_without_numbers_stay_in_their_row(gpu, K):
     """The 256 x 256 tiles ask for scales past a row's end; those, another row's, may be NaN."""
     x, w = rows(gpu, 43, 3500, K), rows(gpu, 44, 3400, K) / K ** 0.5
@@ -161,6 +161,18 @@ def test_blocks_without_numbers_stay_in_their_row(gpu, K):
     bad[1::7], bad[:, 2::5] = True, True
     assert torch.equal(got.isnan(), bad)
     assert torch.equal(got[~bad], want[~bad])
+
+
+def test_scales_at_any_address(gpu):
+    """Rows of scales need no alignment; few rows, small tiles and large ones."""
+    for M, N, K in ((2, 300, 256), (100, 300, 256), (3500, 3400, 256), (3500, 3400, 200)):
+        x, w = mx_quantize(rows(gpu, 45, M, K)), mx_quantize(rows(gpu, 46, N, K))
+        moved = []
+        for q in (x, w):
+            scales = torch.empty(q.scales.numel() + 1, dtype=torch.uint8, device=gpu)[1:]
+            moved.append(MXTensor(q.codes, scales.view(q.scales.shape).copy_(q.scales), K))
+        assert moved[0].scales.data_ptr() % 4 == 1
+        assert torch.equal(mx_product(*moved), mx_product(x, w))
 
 
 @pytest.mark.parametrize("dtype", TYPES)
