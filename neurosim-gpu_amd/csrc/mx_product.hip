@@ -210,6 +210,12 @@ __device__ __forceinline__ void multiply(const Fragments<G>& f, v4f (&sum)[G::MI
     multiply<G, S + 1, 0, 0>(f, sum);
 }
 
+// What a wavefront's lanes have written to LDS is read by others of them: no read or write
+// moves past this in the program (in LDS they stay in order by themselves).  kPath tells ways
+// apart that differ in how they store only: the compiler would join them to one of the two.
+template <int kPath>
+__device__ __forceinline__ void lanes_meet() { asm volatile("" :: "i"(kPath) : "memory"); }
+
 // A wavefront's results, from row m0, column n0, of which `rows` and `columns` exist.  They
 // go strip by strip (16 rows) through LDS, so that each store instruction writes whole lines
 // of eight rows or more; rows are padded by 16 bytes against bank conflicts.  (Stored from the
@@ -223,7 +229,9 @@ struct Strip {
 };
 
 // kStream: past the caches, for results too large to be read again from there (8192^3 331 ->
-// 306 us, 8000 x 50,000 by 1024 497 -> 382).
+// 306 us, 8000 x 50,000 by 1024 497 -> 382), where every lane writes whole halves of 32 bytes
+// that no other store shares (5000 rows by 700, us past and through the caches: 31,040 columns
+// 128 / 134; 31,016, 16 bytes off a line, 171 / 139; 31,013 194 / 144).
 template <class G, class T, bool kStream>
 __device__ __forceinline__ void store_tiles(T* to, int64_t stride, const v4f (&sum)[G::MI][G::NJ],
                                             const float* bias, int64_t rows, int64_t columns, int lane,
@@ -243,6 +251,7 @@ __device__ __forceinline__ void store_tiles(T* to, int64_t stride, const v4f (&s
       }
       __builtin_memcpy(&strip.values[lane & 15][16 * j + 4 * (lane >> 4)], &y, sizeof(y));
     }
+    lanes_meet<kStream>();
 #pragma unroll
     for (int r = 0; r < 16; r += S::kRows) {
       if (row >= S::kRows || 16 * i + r + row >= rows) continue;
@@ -250,16 +259,14 @@ __device__ __forceinline__ void store_tiles(T* to, int64_t stride, const v4f (&s
       Pack<T, S::kWide> y;
       __builtin_memcpy(&y, &strip.values[r + row][column], sizeof(y));
       if (wide) {
-        if constexpr (kStream)
-          stream_pack<T, S::kWide>(at, y);
-        else
-          store_pack<T, S::kWide>(at, y);
+        stream_pack<T, S::kWide, kStream>(at, y);
       } else {
 #pragma unroll
         for (int k = 0; k < S::kWide; ++k)
           if (column + k < columns) at[k] = y.v[k];
       }
     }
+    lanes_meet<kStream>();
   }
 }
 
@@ -650,8 +657,12 @@ __global__ __launch_bounds__(G::threads) void product_word_tiles(MxView a, MxVie
   }
   wait_barrier<0>();                                       // before LDS is used anew
   const int64_t m = m0 + 16 * wm * G::MI, n = n0 + 16 * wn * G::NJ;
-  store_tiles<G, T, true>(out + m * stride + n, stride, sum, bias ? bias + n : nullptr, a.rows - m,
-                          b.rows - n, lane, lds.strip[wave]);
+  T* const to = out + m * stride + n;
+  const float* const more = bias ? bias + n : nullptr;
+  if ((reinterpret_cast<uintptr_t>(out) | stride * sizeof(T)) % 32 == 0)
+    store_tiles<G, T, true>(to, stride, sum, more, a.rows - m, b.rows - n, lane, lds.strip[wave]);
+  else
+    store_tiles<G, T, false>(to, stride, sum, more, a.rows - m, b.rows - n, lane, lds.strip[wave]);
 }
 
 // Few rows of a (up to 16): bound by b's bytes, each read once.  A wavefront takes 16 columns

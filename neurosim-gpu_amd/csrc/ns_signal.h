@@ -46,8 +46,9 @@ __device__ __forceinline__ void store_pack(T* p, const Pack<T, V>& x) {
   __builtin_memcpy(p, &x, sizeof(x));
 }
 
-// The same past the caches (non-temporal), for what is not read again soon: 16 bytes or more.
-template <class T, int V>
+// The same in 16-byte words, kStream: past the caches (non-temporal), for what is not read
+// again soon.
+template <class T, int V, bool kStream = true>
 __device__ __forceinline__ void stream_pack(T* p, const Pack<T, V>& x) {
   static_assert(sizeof(x) % 16 == 0, "whole 16-byte words");
   typedef uint32_t word __attribute__((ext_vector_type(4), aligned(2)));
@@ -55,7 +56,10 @@ __device__ __forceinline__ void stream_pack(T* p, const Pack<T, V>& x) {
   __builtin_memcpy(w, &x, sizeof(x));
 #pragma unroll
   for (unsigned i = 0; i < sizeof(x) / 16; ++i)
-    __builtin_nontemporal_store(w[i], reinterpret_cast<word*>(p) + i);
+    if constexpr (kStream)
+      __builtin_nontemporal_store(w[i], reinterpret_cast<word*>(p) + i);
+    else
+      reinterpret_cast<word*>(p)[i] = w[i];
 }
 
 // 1 / (1 + exp(-x)); exp overflows to infinity for very negative x, whose reciprocal is 0.
