@@ -1,11 +1,13 @@
 // Microscaled 4-bit rows (gfx950): quantising float rows, and reading them back.
 //
 // Both are one pass over memory: 16384 x 8192 in bf16 (340 MB) 57 us to quantise, 48 to read
-// back, 6 and 7 TB/s.  Four neighbouring lanes share a block of 32 values,
-// eight values each, so a wavefront's loads and stores are whole runs of a row; the
+// back, 6 and 7 TB/s.  Quantising, four neighbouring lanes share a block of 32 values, eight
+// values each, so a wavefront's loads and stores are whole runs of a row; the
 // block's largest magnitude is joined over its lanes by two DPP steps.  Magnitudes are
 // compared as integers: on non-negative floats the order is the same, and infinities and
 // NaN come out on top.
+#include <type_traits>
+
 #include "ns_signal.h"
 #include "neurosim_hip_mx.h"
 
@@ -48,7 +50,7 @@ __device__ __forceinline__ float scale_value(uint32_t byte) {
   return __builtin_bit_cast(float, byte ? byte << 23 : 0x00400000u);
 }
 
-// Pieces (of eight values) per thread, a workgroup's width apart: several requests on their
+// Pieces (of a few values of a block) per thread, a workgroup's width apart: several requests on their
 // way at a time.  Places are counted in I, 32 bits where the pieces allow: a 64-bit division
 // per piece would cost more than the rest of its work.
 constexpr int kPieces = 4;
@@ -60,14 +62,16 @@ struct Piece {
   bool inside;
 };
 
-template <class I>
+template <class I, int kValues = kLaneValues>
 __device__ __forceinline__ Piece<I> piece_at(I first, int i, I total, I blocks) {
   Piece<I> p;
   const I id = first + i * kThreads + threadIdx.x;
   p.inside = id < total;
-  p.block = (p.inside ? id : 0) >> 2;
+  constexpr int kLanes = NS_MX_BLOCK / kValues;            // per block
+  p.block = (p.inside ? id : 0) / kLanes;
   p.row = p.block / blocks;
-  p.k = static_cast<int64_t>(p.block - p.row * blocks) * NS_MX_BLOCK + (threadIdx.x & 3) * kLaneValues;
+  p.k = static_cast<int64_t>(p.block - p.row * blocks) * NS_MX_BLOCK +
+        (threadIdx.x & (kLanes - 1)) * kValues;
   return p;
 }
 
@@ -107,25 +111,31 @@ __global__ __launch_bounds__(kThreads) void quantize(const T* x, int64_t stride,
   }
 }
 
-template <class T, class I>
+// A piece is 16 bytes of the values, so that a wavefront's store is one run of a row (eight
+// values a piece in float32 too: 226 us instead of 85 for 16384 x 8192).  kStream: past the
+// caches, the values being several times their codes.
+template <class T, class I, bool kStream>
 __global__ __launch_bounds__(kThreads) void dequantize(const uint8_t* codes, const uint8_t* scales,
                                                        I total, int64_t width, I blocks, T* out,
                                                        int64_t stride) {
+  constexpr int kValues = 16 / sizeof(T);
+  typedef std::conditional_t<kValues == 8, uint32_t, uint16_t> Codes;
   const I first = static_cast<I>(blockIdx.x) * (kPieces * kThreads);
   Piece<I> at[kPieces];
   uint32_t packed[kPieces], byte[kPieces];
 #pragma unroll
   for (int i = 0; i < kPieces; ++i) {
-    at[i] = piece_at<I>(first, i, total, blocks);
-    packed[i] = reinterpret_cast<const uint32_t*>(codes)[at[i].block * 4 + (threadIdx.x & 3)];
+    at[i] = piece_at<I, kValues>(first, i, total, blocks);
+    const I id = first + i * kThreads + threadIdx.x;
+    packed[i] = reinterpret_cast<const Codes*>(codes)[at[i].inside ? id : 0];
     byte[i] = scales[at[i].block];
   }
 #pragma unroll
   for (int i = 0; i < kPieces; ++i) {
     const float unit = byte[i] == 255u ? __builtin_nanf("") : scale_value(byte[i]);
-    Pack<T, 8> v;
+    Pack<T, kValues> v;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < kValues / 2; ++k) {
       // Codes to values with a unit scale, then one multiply: exact in float32.
       const ns_v2f two = e2m1_pair(packed[i] >> (8 * k) & 255u);
       v.v[2 * k] = static_cast<T>(two.x * unit);
@@ -133,12 +143,11 @@ __global__ __launch_bounds__(kThreads) void dequantize(const uint8_t* codes, con
     }
     if (!at[i].inside) continue;
     T* to = out + at[i].row * stride + at[i].k;
-    if (at[i].k + kLaneValues <= width) {
-      // Past the caches: the values are several times their codes, and evict them otherwise.
-      stream_pack<T, 8>(to, v);
+    if (at[i].k + kValues <= width) {
+      stream_pack<T, kValues, kStream>(to, v);
     } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
+      for (int k = 0; k < kValues; ++k)
         if (at[i].k + k < width) to[k] = v.v[k];
     }
   }
@@ -157,19 +166,26 @@ template <class T, class I>
 void launch_rows(const ns_mx_matrix* m, void* x, int64_t stride, bool back, int64_t total,
                  int64_t blocks, hipStream_t stream) {
   const dim3 grid(static_cast<unsigned>((total + kPieces * kThreads - 1) / (kPieces * kThreads)));
-  if (back)
-    dequantize<T, I><<<grid, dim3(kThreads), 0, stream>>>(
-        m->codes, m->scales, static_cast<I>(total), m->columns, static_cast<I>(blocks),
-        static_cast<T*>(x), stride);
-  else
+  if (back) {
+    // us, past the caches and through them: 16384 x 8192 in bf16 49 / 60, float32 85 / 112; where
+    // two stores share a piece of 32 bytes, the same (16384 x 8191 65 / 65, float32 127 / 127).
+    const bool whole = (reinterpret_cast<uintptr_t>(x) | stride * sizeof(T)) % 32 == 0;
+    const auto kernel = whole ? dequantize<T, I, true> : dequantize<T, I, false>;
+    kernel<<<grid, dim3(kThreads), 0, stream>>>(m->codes, m->scales, static_cast<I>(total),
+                                                m->columns, static_cast<I>(blocks),
+                                                static_cast<T*>(x), stride);
+  } else {
     quantize<T, I><<<grid, dim3(kThreads), 0, stream>>>(
         static_cast<const T*>(x), stride, static_cast<I>(total), m->columns, static_cast<I>(blocks),
         m->codes, m->scales);
+  }
 }
 
 template <class T>
 int run_rows(const ns_mx_matrix* m, void* x, int64_t stride, bool back, hipStream_t stream) {
-  const int64_t blocks = (m->columns + NS_MX_BLOCK - 1) / NS_MX_BLOCK, total = m->rows * blocks * 4;
+  const int64_t blocks = (m->columns + NS_MX_BLOCK - 1) / NS_MX_BLOCK;
+  const int64_t lanes = NS_MX_BLOCK / (back ? 16 / static_cast<int>(sizeof(T)) : kLaneValues);
+  const int64_t total = m->rows * blocks * lanes;
   if (total / (kPieces * kThreads) >= INT32_MAX) return fail("the matrix is too large for one launch");
   // The last workgroup's pieces too have to be counted within I.
   if (total <= UINT32_MAX - kPieces * kThreads)
