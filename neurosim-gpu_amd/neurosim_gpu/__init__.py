@@ -4,7 +4,9 @@ The package keeps the public API of NeuroSim-GPU's dendritic mainline
 (DendriticDynamics, the matrix and PELS runtimes, their native variants,
 SparseTopology / random_topology, precision codecs, checkpoint/resume) and runs
 the native tick as hand-written HIP kernels behind the C ABI declared in
-include/neurosim_hip.h (library: neurosim_gpu/_lib/libneurosim_hip.so).
+include/neurosim_hip.h (library: neurosim_gpu/_lib/libneurosim_hip.so).  Around the network
+stand the operators of a signal path, in the same library: causal convolution, selective
+scan and products of microscaled 4-bit rows (signal_ops, microscaled, signal_encoder).
 """
 
 from .checkpoint import (capture_runtime, load_runtime_checkpoint, restore_runtime,

@@ -47,6 +47,20 @@ def test_codes_and_values(gpu, shape, dtype):
     assert torch.equal(q.dequantize(torch.float16).cpu(), want.to(torch.float16))
 
 
+@pytest.mark.parametrize("width", [2048, 2046, 2044, 2040])
+def test_values_of_long_rows(gpu, width):
+    """Rows on and off lines of 32 bytes; the values against the oracle's of a sample of rows."""
+    x = rows(gpu, 47, 700, width)
+    q = mx_quantize(x)
+    some = torch.tensor([0, 1, 2, 350, 698, 699])
+    want = so.mx_values(so.unpack(q.codes.cpu()[some]), q.scales.cpu()[some], width)
+    for dtype in TYPES:
+        assert torch.equal(mx_dequantize(q, dtype).cpu()[some], want.to(dtype))
+    whole = mx_dequantize(q)
+    assert torch.equal(mx_dequantize(q, torch.bfloat16).float(), whole)
+    assert ((whole - x).abs().amax() <= x.abs().amax() / 4)      # a step of a block's top values
+
+
 def test_every_rounding(gpu):
     """Every multiple of 1/64 of a block's unit, both signs, at scales over the whole range."""
     grid = torch.arange(0, 8 * 64, dtype=torch.float64) / 64
@@ -128,7 +142,8 @@ def test_product(gpu, shape):
 
 
 @pytest.mark.parametrize("shape", [(3500, 3400, 128), (3400, 3500, 96), (3333, 3600, 384),
-                                   (3400, 3700, 1000), (3500, 3500, 640), (3329, 3585, 1024)])
+                                   (3400, 3700, 1000), (3500, 3500, 640), (3329, 3585, 1024),
+                                   (3500, 3456, 1000), (3400, 3456, 33)])
 def test_product_of_many_rows(gpu, shape):
     """The 256 x 256 tiles, K of one stage to several, whole and with a part of one, scale
     rows of whole words (K a multiple of 128) and not; a sample of rows and columns."""
