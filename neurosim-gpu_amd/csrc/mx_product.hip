@@ -665,14 +665,13 @@ __global__ __launch_bounds__(G::threads) void product_word_tiles(MxView a, MxVie
     store_tiles<G, T, false>(to, stride, sum, more, a.rows - m, b.rows - n, lane, lds.strip[wave]);
 }
 
-// Few rows of a (up to 16): bound by b's bytes, each read once.  A wavefront takes 16 columns
-// of y (rows of b) straight from memory to registers, four stages of K requested ahead; where
-// columns are few, the four wavefronts of a workgroup take a quarter of K each and meet in LDS.
+// Few rows of a (up to 16) and few columns: bound by b's bytes, each read once, and by the way
+// from a request to its use.  A workgroup takes 16 columns of y (rows of b) straight from
+// memory to registers, four stages of K requested ahead; its four wavefronts take a quarter of
+// K each and meet in LDS.
 // A sum over K may take its blocks in any order, as long as both operands do: lane l takes
 // blocks 2(l/16) and 2(l/16) + 1 of a stage for its two steps, so that four lanes read a whole
-// line of a row and a row's two scale bytes are one 16-bit word.  1 x 50,000 by 1024 takes
-// 9.1 us, 27 MB of b: 2 us of launch, the rest one round of 3125 wavefronts, each with four
-// requests in flight, then the tail.
+// line of a row and a row's two scale bytes are one 16-bit word.  16 x 4096 by 4096 takes 6 us with its call.
 struct RowPanel {
   __amdgpu_buffer_rsrc_t codes;
   const uint8_t* scales;       // of the lane's row
@@ -713,20 +712,20 @@ __device__ __forceinline__ void load_row_stage(const RowPanel& p, int block, Row
 }
 
 constexpr int kRowsAhead = 4;   // stages
+constexpr int kWaves = kThreads / 64;
 
-// KW wavefronts of a workgroup share a strip of 16 columns, a part of K each.
-template <int KW, class T>
+// A workgroup's wavefronts share a strip of 16 columns, a part of K each.
+template <class T>
 __global__ __launch_bounds__(kThreads) void product_rows(MxView a, MxView b, const float* bias,
                                                          T* out, int64_t stride, uint32_t groups,
                                                          uint32_t splits, float* partials) {
-  constexpr int kWaves = kThreads / 64;
   __shared__ v4f sums[kWaves][64];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const uint32_t split = uniform(blockIdx.x / groups), group = blockIdx.x - split * groups;
-  const int64_t n0 = (static_cast<int64_t>(group) * (kWaves / KW) + wave / KW) * 16;
+  const int64_t n0 = static_cast<int64_t>(group) * 16;
   const RowPanel pa = row_panel(a, 0, lane), pb = row_panel(b, n0, lane);
   const int blocks = static_cast<int>(a.blocks), stages = (blocks + 7) / 8;
-  const uint32_t parts = splits * KW, part = split * KW + wave % KW;
+  const uint32_t parts = splits * kWaves, part = split * kWaves + wave;
   const int per = static_cast<int>(uniform((stages + parts - 1) / parts));
   const int first = static_cast<int>(part) * per;
   const int stop = first + per < stages ? first + per : stages;
@@ -754,24 +753,18 @@ __global__ __launch_bounds__(kThreads) void product_rows(MxView a, MxView b, con
   }
   sums[wave][lane] = sum;
   __syncthreads();
-  // KW = 1: a wavefront stores its own strip; else all threads join the parts of the one.
-  const int thread = KW == 1 ? lane : static_cast<int>(threadIdx.x);
-  constexpr int kAtOnce = KW == 1 ? 4 : 16;
-  const int column = thread & 15;
+  const int column = threadIdx.x & 15, m = threadIdx.x >> 4;
+  const int from = (column >> 2) * 16 + m;                 // the lane that holds it
   const int64_t n = n0 + column;
+  float total = 0.0f;
 #pragma unroll
-  for (int r = 0; r < 16; r += kAtOnce) {
-    const int m = r + (thread >> 4), from = (column >> 2) * 16 + m;   // the lane that holds it
-    float total = 0.0f;
-#pragma unroll
-    for (int w = 0; w < KW; ++w)
-      total += reinterpret_cast<const float*>(&sums[KW == 1 ? wave : w][from])[column & 3];
-    if (m < a.rows && n < b.rows) {
-      if (splits > 1)
-        partials[(split * a.rows + m) * b.rows + n] = total;
-      else
-        out[m * stride + n] = static_cast<T>(total + (bias ? bias[n] : 0.0f));
-    }
+  for (int w = 0; w < kWaves; ++w)
+    total += reinterpret_cast<const float*>(&sums[w][from])[column & 3];
+  if (m < a.rows && n < b.rows) {
+    if (splits > 1)
+      partials[(split * a.rows + m) * b.rows + n] = total;
+    else
+      out[m * stride + n] = static_cast<T>(total + (bias ? bias[n] : 0.0f));
   }
 }
 
@@ -811,19 +804,20 @@ using Small = Tile<2, 2, 2, 2, 2>;   // 64 x 64
 
 constexpr int64_t kFewRows = 16;     // product_rows
 
-// Which kernel multiplies M x N.  us, 64 x 64 tiles against 256 x 256: 4096^3 86 / 51;
+// Which kernel multiplies M x N by K.  us, 64 x 64 tiles against 256 x 256: 4096^3 86 / 51;
 // 2048 x 4096 by 1024 (128 large tiles, half the compute units) 16.7 / 17.7; 2048^3 (64) 13.8 /
-// 21.  product_rows against 64 x 64 tiles: 1 x 50,000 by 1024 8.6 / 12.7, 16 x 4096 by 4096 6.8 /
-// 10; its form for 32 rows took 68 for 32 x 50,000 by 4096, the tiles 38.
+// 21.  One small tile high or wide, the large ones are mostly empty: 33 x 50,000 by 1024 8.0 /
+// 13.2, by 4096 23 / 29, 64 x 50,000 by 4096 29 / 30, 50,000 x 64 by 1024 8.2 / 17.7; two high,
+// 128 x 50,000 by 1024 15.6 / 16.3, by 4096 47 / 32.  product_rows saves small tiles the cut of
+// K and its launch where both have few columns and not too many of K: product_rows / tiles, 16 x
+// 4096 by 4096 6.0 / 9.5, 1 x 12,000 by 6000 8.6 / 13; but 1 x 50,000 by 1024 8.5 / 6.8, 16 x
+// 50,000 by 1024 13.2 / 7.1, 16 x 8192 by 16,384 26 / 17, 1 x 1000 by 50,000 11.3 / 10.1.
 enum class Kernel { kRows, kSmall, kLarge };
-Kernel kernel_of(int64_t m, int64_t n) {
-  if (m <= kFewRows) return Kernel::kRows;
+Kernel kernel_of(int64_t m, int64_t n, int64_t k) {
+  if (m <= kFewRows && n < 16 * 1024 && k <= 8 * 1024) return Kernel::kRows;
+  if (m <= Small::rows_m || n <= Small::rows_n) return Kernel::kSmall;
   return (m + 255) / 256 * ((n + 255) / 256) >= 192 ? Kernel::kLarge : Kernel::kSmall;
 }
-
-// Wavefronts per strip of 16 columns in product_rows: one where the strips alone give every
-// SIMD one.
-int64_t waves_per_strip(int64_t n) { return n >= 16 * 1024 ? 1 : 4; }
 
 // Parts that K is cut into where workgroups are few.  A part's sums are written, read again
 // and cost a launch (4 us), so parts are long: rows, what a wavefront requests ahead; tiles,
@@ -833,13 +827,13 @@ int64_t waves_per_strip(int64_t n) { return n >= 16 * 1024 ? 1 : 4; }
 // 14 (28 of 7).
 int64_t parts_of_k(int64_t m, int64_t n, int64_t k) {
   if (m <= 0 || n <= 0 || k <= 0) return 1;
-  const Kernel kernel = kernel_of(m, n);
+  const Kernel kernel = kernel_of(m, n, k);
   if (kernel == Kernel::kLarge) return 1;
   const int64_t stages = (k + 255) / 256;
   int64_t parts, most;
   if (kernel == Kernel::kRows) {
-    parts = 4096 / ((n + 15) / 16 * waves_per_strip(n));
-    most = stages / (waves_per_strip(n) * kRowsAhead);
+    parts = 4096 / ((n + 15) / 16 * kWaves);
+    most = stages / (kWaves * kRowsAhead);
   } else {
     const int64_t tiles = (m + 63) / 64 * ((n + 63) / 64);
     parts = 512 / tiles;
@@ -865,7 +859,7 @@ Workspace workspace_of(int64_t m, int64_t n, int64_t k, bool float_rows) {
   w.scales = float_rows ? m * blocks * 16 : 0;
   w.rest = float_rows ? (m * blocks * 17 + 15) / 16 * 16 : 0;
   w.bytes = w.rest + (parts > 1 ? parts * m * n * 4 : 0);
-  if (kernel_of(m, n) == Kernel::kLarge) w.bytes += (m + n) * word_bytes(blocks);
+  if (kernel_of(m, n, k) == Kernel::kLarge) w.bytes += (m + n) * word_bytes(blocks);
   return w;
 }
 
@@ -909,25 +903,16 @@ int run_large(const ns_mx_product_args* p, void* words, hipStream_t stream) {
 
 template <class T>
 int run_rows(const ns_mx_product_args* p, int64_t parts, float* partials, hipStream_t stream) {
-  const int64_t shared = waves_per_strip(p->b.rows), strips = (p->b.rows + 15) / 16;
-  const int64_t groups = (strips * shared + 3) / 4;
-  if (groups * parts > INT32_MAX) return fail("the product is too large for one launch");
-  const dim3 grid(static_cast<unsigned>(groups * parts));
-  const MxView a = view(p->a), b = view(p->b);
-  if (shared == 1)
-    product_rows<1, T><<<grid, dim3(kThreads), 0, stream>>>(
-        a, b, p->bias, static_cast<T*>(p->out), p->stride, static_cast<uint32_t>(groups),
-        static_cast<uint32_t>(parts), partials);
-  else
-    product_rows<4, T><<<grid, dim3(kThreads), 0, stream>>>(
-        a, b, p->bias, static_cast<T*>(p->out), p->stride, static_cast<uint32_t>(groups),
-        static_cast<uint32_t>(parts), partials);
+  const int64_t strips = (p->b.rows + 15) / 16;
+  product_rows<T><<<dim3(static_cast<unsigned>(strips * parts)), dim3(kThreads), 0, stream>>>(
+      view(p->a), view(p->b), p->bias, static_cast<T*>(p->out), p->stride,
+      static_cast<uint32_t>(strips), static_cast<uint32_t>(parts), partials);
   return launched("product");
 }
 
 template <class T>
 int run_kernel(const ns_mx_product_args* p, int64_t parts, float* partials, hipStream_t stream) {
-  const Kernel kernel = kernel_of(p->a.rows, p->b.rows);
+  const Kernel kernel = kernel_of(p->a.rows, p->b.rows, p->a.columns);
   switch (p->a.columns || kernel == Kernel::kRows ? kernel : Kernel::kSmall) {
     case Kernel::kLarge: return run_large<T>(p, partials, stream);
     case Kernel::kSmall: return run_tiles<Small, T>(p, parts, partials, stream);
