@@ -28,7 +28,6 @@ template <int kMI, int kNJ, int kWM, int kWN, int kKS>
 struct Tile {
   static constexpr int MI = kMI, NJ = kNJ, WM = kWM, WN = kWN, KS = kKS;
   static constexpr int rows_m = 16 * MI * WM, rows_n = 16 * NJ * WN, rows = rows_m + rows_n;
-  static constexpr int subs = rows / 16;                   // 16-row strips, a's then b's
   static constexpr int threads = 64 * WM * WN;
   static constexpr int loads = rows * KS * 4 / threads;    // 16-byte pieces per thread and stage
   static constexpr int scale_rows = (rows + threads - 1) / threads;
@@ -394,14 +393,10 @@ __device__ __forceinline__ WordPanel word_panel(const MxView& m, int64_t row, in
                    describe(m.scales + row * scales, own * scales), blocks * 16, blocks, scales};
 }
 
-// 16 bytes (4 bytes) per lane from `offset` of a buffer to LDS at `to` + 16 (4) * lane.
+// 16 bytes per lane from `offset` of a buffer to LDS at `to` + 16 * lane.
 __device__ __forceinline__ void to_lds_16(const v4i& buffer, uint32_t offset, uint32_t to) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-               :: "s"(to), "v"(offset), "s"(buffer) : "memory");
-}
-__device__ __forceinline__ void to_lds_4(const v4i& buffer, uint32_t offset, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
-               :: "s"(to), "v"(offset), "s"(buffer) : "memory");
+               :: "s"(to), "v"(offset), "s"(buffer) : "memory", "m0");
 }
 
 // Where row r keeps block k of a stage: place k ^ turn(r).  Four neighbouring lanes then ask
