@@ -346,7 +346,10 @@ __global__ __launch_bounds__(G::threads) void product_tiles(MxView a, MxView b, 
     multiply<G>(f, sum);
   }
   const int64_t m = m0 + 16 * wm * G::MI, n = n0 + 16 * wn * G::NJ;
-  __syncthreads();                                         // the stages are read to their end
+  // LDS is used anew: the stages are read to their end, and the last requests, which nothing
+  // reads, have arrived.
+  wait_all();
+  __syncthreads();
   if (splits > 1) {
     store_tiles<G, float, false>(partials + (split * a.rows + m) * b.rows + n, b.rows, sum, nullptr,
                           a.rows - m, b.rows - n, lane, lds.partial[wave]);

@@ -303,3 +303,18 @@ def test_refusals(gpu):
     args = microscaled._PRODUCT.pack(2, 2 ** 24, 0, 0, 2, 2 ** 24, 0, 0, 0, 0, 2, 0, 0, 0, 0, 0)
     assert lib.ns_mx_product(args, None) == 1
     assert b"at most 8388608 columns" in lib.ns_last_error()
+
+
+@pytest.mark.parametrize("shape", [(17, 64, 256), (64, 64, 1792), (20, 130, 2048), (300, 500, 1024),
+                                   (40, 100, 20_000), (33, 200, 50_000), (70, 90, 50_176)])
+def test_small_tiles_of_whole_and_many_stages(gpu, shape):
+    """The 64 x 64 tiles where K ends with a whole stage of 256 (their last requests then bring
+    nothing that is read, into the LDS that the results pass through), and where it is cut into
+    many parts, of whole stages and not."""
+    M, N, K = shape
+    x, weight = mx_quantize(rows(gpu, 50, M, K)), mx_quantize(rows(gpu, 51, N, K) / K ** 0.5)
+    bias = rows(gpu, 52, N)
+    for dtype in TYPES:
+        y = check_product(x, weight, bias, dtype)
+        for _ in range(3):
+            assert torch.equal(mx_product(x, weight, bias=bias, dtype=dtype), y)
