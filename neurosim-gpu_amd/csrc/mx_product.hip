@@ -396,10 +396,11 @@ __device__ __forceinline__ WordPanel word_panel(const MxView& m, int64_t row, in
                    describe(m.scales + row * scales, own * scales), blocks * 16, blocks, scales};
 }
 
-// 16 bytes per lane from `offset` of a buffer to LDS at `to` + 16 * lane.
+// 16 bytes per lane from `offset` of a buffer to LDS at `to` + 16 * lane.  The address is in m0,
+// which the compiler sets; a request right behind that needs one wait state.
 __device__ __forceinline__ void to_lds_16(const v4i& buffer, uint32_t offset, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-               :: "s"(to), "v"(offset), "s"(buffer) : "memory", "m0");
+  asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :: "{m0}"(to), "v"(offset), "s"(buffer) : "memory");
 }
 
 // Where row r keeps block k of a stage: place k ^ turn(r).  Four neighbouring lanes then ask
