@@ -28,6 +28,7 @@ from functools import lru_cache
 
 import torch
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
 from .native import _RAW_STREAM, _raise_on, load_library
 
@@ -151,6 +152,13 @@ def _dense(value: torch.Tensor | None):
     return value if value is None or value.is_contiguous() else value.contiguous()
 
 
+def _moved_on(carried: torch.Tensor) -> None:
+    """Tells autograd that a kernel has written ``carried`` in place: a backward that saved its
+    earlier values then refuses.  Inference tensors keep no version."""
+    if not carried.is_inference():
+        increment_version(carried)
+
+
 def _needs_grad(*values) -> bool:
     if torch.is_grad_enabled():
         for value in values:
@@ -252,7 +260,8 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None
 def causal_conv_step(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
                      history: torch.Tensor, activation: str | None = "silu") -> torch.Tensor:
     """One tick of ``causal_conv``: ``x`` [B, N] to y [B, N], ``history`` [W-1, B, N]
-    moved on by it in place.  Keeps nothing for gradients."""
+    moved on by it in place.  Keeps nothing for gradients; a backward that saved the history
+    as it was refuses."""
     _check_conv(x, weight, bias, history, activation, 2)
     if _needs_grad(x, weight, bias, history):
         raise ValueError("a step gives no gradients; use causal_conv")
@@ -272,6 +281,7 @@ def causal_conv_step(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor |
                               x.data_ptr(), 0, x.stride(0), weight.data_ptr(), _address(bias),
                               *carried, 0, y.data_ptr(), 0, n, *carried)
     call(_library().ns_conv_step, x.device, args)
+    _moved_on(history)
     return y
 
 
@@ -436,7 +446,7 @@ def selective_scan_step(x: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B
                         softplus: bool = True, state: torch.Tensor) -> torch.Tensor:
     """One tick of ``selective_scan``: ``x``, ``delta``, ``z`` [B, N], ``B`` and ``C`` [B, S]
     or [B, G, S], y [B, N]; ``state`` [B, N, S] (float32, contiguous) is updated in place.
-    Keeps nothing for gradients."""
+    Keeps nothing for gradients; a backward that saved the state as it was refuses."""
     groups, states = _check_scan(x, delta, A, B, C, D, z, delta_bias, state, 2)
     if _needs_grad(x, delta, A, B, C, D, z, delta_bias, state):
         raise ValueError("a step gives no gradients; use selective_scan")
@@ -452,4 +462,5 @@ def selective_scan_step(x: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B
         B.data_ptr(), 0, B.stride(0), C.data_ptr(), 0, C.stride(0), A.data_ptr(), _address(D),
         _address(delta_bias), state.data_ptr(), state.data_ptr(), 0, 0, 0)
     call(_library().ns_scan_step, x.device, args)
+    _moved_on(state)
     return y

@@ -511,3 +511,49 @@ def test_refusals(gpu):
     refuses("in place", selective_scan_step, **{**step, "state": None})
     refuses("in place", selective_scan_step, **{**step, "state": draw(2, 5, 6).transpose(1, 2)})
     refuses("no gradients", selective_scan_step, **{**step, "A": good["A"].clone().requires_grad_()})
+
+
+def test_steps_move_the_version_of_what_they_update(gpu):
+    """A step writes its history or state in place; a backward that kept the earlier values
+    refuses, as after torch's own in-place operations."""
+    draw = Draw(gpu, 20)
+    conv = conv_operands(draw, 6, 2, 10, 4, torch.float32)
+    wide_history = draw(3, 2, 14)
+    for history in (conv["history"], wide_history[..., 2:12]):
+        weight = conv["weight"].clone().requires_grad_()
+        y, _ = causal_conv(conv["x"], weight, history=history)
+        with torch.no_grad():
+            before = history._version
+            causal_conv_step(conv["x"][0], weight, history=history)
+            assert history._version > before
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+    assert wide_history._version == history._version
+
+    scan = scan_operands(draw, 6, 2, 10, 5, 2, torch.float32)
+    state, factor = scan.pop("state"), draw(2, 10, 5).requires_grad_()
+    product = (state * factor).sum()
+    selective_scan_step(**{k: v[0] if k in ("x", "delta", "z", "B", "C") else v
+                           for k, v in scan.items()}, state=state)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        product.backward()
+
+
+def test_steps_of_inference_tensors(gpu):
+    """They keep no version, and are updated like any other."""
+    draw = Draw(gpu, 21)
+    conv = conv_operands(draw, 1, 2, 10, 4, torch.float32)
+    scan = scan_operands(draw, 1, 2, 10, 5, 1, torch.float32)
+    want_y, want_history = causal_conv(**conv)
+    now = {k: v[0] if k in ("x", "delta", "z", "B", "C") else v for k, v in scan.items()
+           if k != "state"}
+    mine = scan["state"].clone()
+    want_s = selective_scan_step(**now, state=mine)
+    with torch.inference_mode():
+        history, state = conv["history"].clone(), scan["state"].clone()
+        y = causal_conv_step(conv["x"][0], conv["weight"], conv["bias"], history=history)
+        s = selective_scan_step(**now, state=state)
+        assert torch.equal(y, want_y[0]) and torch.equal(history, want_history)
+        assert torch.equal(s, want_s) and torch.equal(state, mine)
+        assert causal_conv_step(conv["x"][0], conv["weight"][:, :1].contiguous(),
+                                history=history[:0]).shape == (2, 10)
