@@ -156,6 +156,14 @@ __global__ __launch_bounds__(kThreads) void scan_forward(ScanShape s, ScanIn<T> 
   }
 }
 
+// 2^exponent carry, also where 2^exponent alone has no float32: growing states (positive
+// rates) multiply by more than that over a chunk, which a carry of zero or a tiny one bears as
+// it does tick by tick.  Beyond 2^+-1000 any carry but zero is past float32's range.
+__device__ __forceinline__ float over_chunk(float carry, float exponent) {
+  const float bounded = fminf(fmaxf(exponent, -1000.0f), 1000.0f), whole = rintf(bounded);
+  return __builtin_ldexpf(__builtin_amdgcn_exp2f(bounded - whole) * carry, static_cast<int>(whole));
+}
+
 // One lane per (column, channel, padded state): walks the chunks in order, leaving in
 // place of each chunk's own end the state (or adjoint) it starts from.  `blocks` workgroups
 // to a column.  Reads past the last chunk are the last one's again, so that all of a round
@@ -190,7 +198,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(ScanShape s, uint32_t bl
       if (first + u < chunks) {
         const int64_t c = reverse ? chunks - 1 - first - u : first + u;
         ends[(c * lines + line) * padded + state] = carry;
-        carry = fmaf(__builtin_amdgcn_exp2f(step[u] * rate), carry, own[u]);
+        carry = over_chunk(carry, step[u] * rate) + own[u];
       }
     }
   }

@@ -557,3 +557,56 @@ def test_steps_of_inference_tensors(gpu):
         assert torch.equal(s, want_s) and torch.equal(state, mine)
         assert causal_conv_step(conv["x"][0], conv["weight"][:, :1].contiguous(),
                                 history=history[:0]).shape == (2, 10)
+
+
+GROWN_T, GROWN_N = 300, 5
+
+
+def growing_operands(draw, S, step):
+    """Rates of 2.5 to 4 and time steps of ``step`` [T, 1, N]; and the ticks of a chunk, over
+    which a step of 1 a tick would multiply by more than float32 holds."""
+    T, N = GROWN_T, GROWN_N
+    chunks, tiles = signal_ops._plan((T, 1, N), 1, S, False)[0], -(-T // 16)
+    ticks = -(-tiles // chunks) * 16
+    assert chunks > 2 and 2.5 * ticks > 89
+    operands = scan_operands(draw, T, 1, N, S, 1, torch.float32)
+    rates = 2.5 + 1.5 * torch.rand(N, S, generator=draw.g)
+    operands |= {"A": rates.to(draw.gpu), "delta": torch.log(torch.expm1(step)).to(draw.gpu),
+                 "delta_bias": None, "state": None}
+    return operands, ticks
+
+
+@pytest.mark.parametrize("S", [4, 16])
+def test_growth_over_chunks_that_hold_nothing(gpu, S):
+    """A state of zero stays zero, however much a chunk would multiply it by, until the last
+    ticks drive it; and so does an adjoint, until the first ticks."""
+    draw, T, N, driven = Draw(gpu, 80 + S), GROWN_T, GROWN_N, 9
+    operands, _ = growing_operands(draw, S, torch.full((T, 1, N), 1.0))
+    x = operands["x"].clone()
+    operands["x"][:T - driven] = 0
+    check_scan(operands)
+
+    operands["x"] = x.zero_()
+    dy = draw(T, 1, N)
+    dy[driven:] = 0
+    inputs = leaves(operands)
+    y, _ = selective_scan(**inputs)
+    got = gradients((y,), inputs, (dy,))
+    grads = so.scan(**operands, dy=dy)[1]
+    size = so.scan(**operands, dy=dy, magnitude=True)[1]
+    for name, value in got.items():
+        close(value, grads[name], size[name], 2 * (70 * T + 20) + S + 60 + T + N, f"d{name}")
+    assert float(got["x"][0].abs().max()) > 0
+
+
+def test_growth_of_small_states_over_a_chunk(gpu):
+    """A chunk that multiplies by more than float32 holds, on a state and a gradient of the
+    final state that are small enough to bear it; the other chunks' steps are tiny."""
+    draw, T, N, S = Draw(gpu, 90), GROWN_T, GROWN_N, 16
+    step = torch.full((T, 1, N), 1e-13, dtype=torch.float64)
+    operands, ticks = growing_operands(draw, S, step)
+    step[ticks:2 * ticks] = 100 / (4.0 * ticks)             # A sum(dt) of 62 to 100
+    operands["delta"] = torch.log(torch.expm1(step)).float().to(gpu)
+    operands["x"].zero_()
+    operands["state"] = (draw(1, N, S).abs() + 0.1) * 1e-30
+    check_scan(operands, None, True, draw(T, 1, N) * 1e-30, draw(1, N, S) * 1e-30)
