@@ -12,12 +12,12 @@ float32 and each output is rounded once.
   ``dt = softplus(delta + delta_bias)``.
 
 Both take and return the state that carries a signal on (``history``, ``state``), give
-native gradients of every tensor input, and have a one-tick form that updates the carried
-state in place.  ``lengths`` gives columns their own number of ticks: past it outputs and
-gradients are zero, the carried state stays that of the column's last tick, and what the
-inputs hold there is never used.  The kernels are csrc/conv.hip, scan.hip, scan_grad.hip
-behind include/neurosim_hip_signal.h; calls run on the current stream, allocate their
-outputs and workspaces from torch, and never synchronise.
+native gradients of every tensor input (forward-mode derivatives are refused), and have a
+one-tick form that updates the carried state in place.  ``lengths`` gives columns their own
+number of ticks: past it outputs and gradients are zero, the carried state stays that of the
+column's last tick, and what the inputs hold there is never used.  The kernels are
+csrc/conv.hip, scan.hip, scan_grad.hip behind include/neurosim_hip_signal.h; calls run on
+the current stream, allocate their outputs and workspaces from torch, and never synchronise.
 """
 
 from __future__ import annotations
@@ -27,6 +27,7 @@ import struct
 from functools import lru_cache
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 from torch.autograd.graph import increment_version
 
@@ -160,6 +161,12 @@ def _moved_on(carried: torch.Tensor) -> None:
 
 
 def _needs_grad(*values) -> bool:
+    """Whether a backward has to be recorded.  Forward-mode derivatives, which no operator
+    here gives, are refused: their tensors do not say that they require one."""
+    if forward_ad._current_level >= 0:               # only then can a tensor carry one
+        for value in values:
+            if value is not None and forward_ad.unpack_dual(value).tangent is not None:
+                raise ValueError("the signal operators give no forward-mode derivatives")
     if torch.is_grad_enabled():
         for value in values:
             if value is not None and value.requires_grad:

@@ -318,3 +318,16 @@ def test_small_tiles_of_whole_and_many_stages(gpu, shape):
         y = check_product(x, weight, bias, dtype)
         for _ in range(3):
             assert torch.equal(mx_product(x, weight, bias=bias, dtype=dtype), y)
+
+
+def test_forward_mode_derivatives_are_refused(gpu):
+    from torch.autograd import forward_ad
+
+    x, weight, bias = rows(gpu, 60, 4, 64), mx_quantize(rows(gpu, 61, 5, 64)), rows(gpu, 62, 5)
+    with forward_ad.dual_level():
+        dual, dual_bias = (forward_ad.make_dual(v, torch.ones_like(v)) for v in (x, bias))
+        for call in (lambda: mx_quantize(dual), lambda: mx_product(dual, weight),
+                     lambda: mx_product(x, weight, bias=dual_bias)):
+            with pytest.raises(ValueError, match="forward-mode"):
+                call()
+        mx_product(x, weight, bias=bias)

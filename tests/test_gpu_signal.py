@@ -610,3 +610,32 @@ def test_growth_of_small_states_over_a_chunk(gpu):
     operands["x"].zero_()
     operands["state"] = (draw(1, N, S).abs() + 0.1) * 1e-30
     check_scan(operands, None, True, draw(T, 1, N) * 1e-30, draw(1, N, S) * 1e-30)
+
+
+def test_forward_mode_derivatives_are_refused(gpu):
+    """There are none: a tensor that carries one is refused, not taken without it."""
+    from torch.autograd import forward_ad
+
+    draw = Draw(gpu, 91)
+    conv = conv_operands(draw, 4, 2, 6, 3, torch.float32)
+    scan = scan_operands(draw, 4, 2, 6, 5, 2, torch.float32)
+    tick = {k: v[0] if k in ("x", "delta", "z", "B", "C") else v for k, v in scan.items()}
+    calls = [(causal_conv, conv), (selective_scan, scan), (selective_scan_step, tick),
+             (causal_conv_step, {**conv, "x": conv["x"][0]})]
+    with forward_ad.dual_level():
+        for fn, operands in calls:
+            for name, value in operands.items():
+                dual = forward_ad.make_dual(value, torch.ones_like(value))
+                for grad in (True, False):
+                    with torch.set_grad_enabled(grad), pytest.raises(ValueError, match="forward-mode"):
+                        fn(**{**operands, name: dual})
+            fn(**operands)                              # plain tensors stay welcome there
+
+
+def test_forward_mode_derivatives_of_lower_precision_parameters_are_refused(gpu):
+    from torch.autograd import forward_ad
+
+    draw = Draw(gpu, 92)
+    x, weight = draw(4, 2, 6, dtype=torch.bfloat16), draw(6, 3, dtype=torch.bfloat16)
+    with forward_ad.dual_level(), pytest.raises(ValueError, match="forward-mode"):
+        causal_conv(x, forward_ad.make_dual(weight, torch.ones_like(weight)))
