@@ -180,6 +180,15 @@ __device__ __forceinline__ void lane_row(const T* table, int64_t n, int q, int32
   }
 }
 
+// A rate A as the exponent of two that a unit of time brings.  What lies below float32 then,
+// minus infinity for one (a state that forgets at once), is its lowest value: a time step of
+// zero, as ticks past a column's end have, times that is zero, and not NaN.
+__device__ __forceinline__ float exponent_rate(float rate) {
+  constexpr float kLowest = -3.402823466e38f;
+  const float exponent = rate * kLog2e;
+  return exponent < kLowest ? kLowest : exponent;
+}
+
 // A lane's R floats of a padded [line][N][4R] workspace at a workgroup's channels.
 template <int R>
 struct LaneStates {

@@ -64,7 +64,7 @@ __global__ __launch_bounds__(kThreads) void scan_forward(ScanShape s, ScanIn<T> 
   float rate[R], h[R];
   lane_row<R>(in.rates, n, q, s.states, own, rate);
 #pragma unroll
-  for (int r = 0; r < R; ++r) rate[r] *= kLog2e;
+  for (int r = 0; r < R; ++r) rate[r] = exponent_rate(rate[r]);
   if (kEnds) {
 #pragma unroll
     for (int r = 0; r < R; ++r) h[r] = 0.0f;
@@ -180,7 +180,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(ScanShape s, uint32_t bl
   const int64_t channel = at >> (31 - __builtin_clz(padded)), lines = s.batch * s.channels;
   const int64_t line = b * s.channels + channel;
   const bool real = state < static_cast<uint32_t>(s.states);
-  const float rate = real ? rates[channel * s.states + state] * kLog2e : 0.0f;
+  const float rate = real ? exponent_rate(rates[channel * s.states + state]) : 0.0f;
   float carry = real && start ? start[line * s.states + state] : 0.0f;
   const int chunks = static_cast<int>(s.chunks);
   constexpr int kAhead = 16;
@@ -232,7 +232,7 @@ __global__ __launch_bounds__(kThreads) void scan_step(ScanShape s, ScanIn<T> in,
   float sum = 0.0f;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    h[r] = fmaf(__builtin_amdgcn_exp2f(dt * (rate[r] * kLog2e)), h[r], dt * x * write[r]);
+    h[r] = fmaf(__builtin_amdgcn_exp2f(dt * exponent_rate(rate[r])), h[r], dt * x * write[r]);
     sum = fmaf(read[r], h[r], sum);
   }
   if (s.states == 4 * R) {

@@ -74,7 +74,7 @@ __global__ __launch_bounds__(kThreads) void scan_adjoint_ends(ScanShape s, ScanI
   lane_row<R>(in.rates, n, q, s.states, own, rate);
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    rate[r] *= kLog2e;
+    rate[r] = exponent_rate(rate[r]);
     g[r] = 0.0f;
   }
   const float bias = in.delta_bias && lane < p.own ? in.delta_bias[p.n0 + lane] : 0.0f;
@@ -170,7 +170,7 @@ __global__ __launch_bounds__(kThreads, 2) void scan_backward(ScanShape s, ScanIn
   }
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    rate[r] *= kLog2e;
+    rate[r] = exponent_rate(rate[r]);
     drate[r] = 0.0f;
     if (!own) g[r] = 0.0f;
   }

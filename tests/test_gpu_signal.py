@@ -13,6 +13,8 @@ once to their type.
 
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -639,3 +641,42 @@ def test_forward_mode_derivatives_of_lower_precision_parameters_are_refused(gpu)
     x, weight = draw(4, 2, 6, dtype=torch.bfloat16), draw(6, 3, dtype=torch.bfloat16)
     with forward_ad.dual_level(), pytest.raises(ValueError, match="forward-mode"):
         causal_conv(x, forward_ad.make_dual(weight, torch.ones_like(weight)))
+
+
+@pytest.mark.parametrize("T", [1, 16, 20, 260])
+def test_rates_of_minus_infinity(gpu, T):
+    """They forget at once: the state is the last tick's input, in the signal's form (whose last
+    tile may reach past the end, and whose time may be cut into chunks) as in the steps'."""
+    draw, B, N, S = Draw(gpu, 93), 3, 6, 5
+    operands = scan_operands(draw, T, B, N, S, 2, torch.float32)
+    operands["A"][::2, 1:3] = -math.inf
+    operands["A"][1, 0] = -3e38
+    check_scan(operands)
+    y, _ = selective_scan(**operands)
+    lengths = torch.tensor([T, T // 2, 0], dtype=torch.int32, device=gpu)
+    short, final = selective_scan(**operands, lengths=lengths)
+    assert torch.equal(short[:, 0], y[:, 0]) and torch.equal(final[2], operands["state"][2])
+    half = {k: v[:T // 2, 1:2] if k in ("x", "delta", "z", "B", "C") else v
+            for k, v in operands.items()}
+    half["state"] = operands["state"][1:2]
+    alone = so.scan(**half)[0]["state"]
+    size = so.scan(**half, magnitude=True)[0]["state"]
+    close(final[1:2], alone, size, 70 * T + 20, "state of a column's own length")
+    state = operands["state"].clone()
+    for t in range(min(T, 3)):
+        selective_scan_step(**{k: v[t] if k in ("x", "delta", "z", "B", "C") else v
+                               for k, v in operands.items() if k != "state"}, state=state)
+    assert torch.isfinite(state).all()
+
+    # The gradients that the limit has: of x and B, and of the first state.
+    if T > 100:
+        return
+    names = ("x", "B", "C", "state")
+    inputs = {k: v.clone().requires_grad_() if k in names else v for k, v in operands.items()}
+    dy, dfinal = draw(T, B, N), draw(B, N, S)
+    y, final = selective_scan(**inputs)
+    got = torch.autograd.grad((y, final), [inputs[k] for k in names], (dy, dfinal))
+    grads = so.scan(**operands, dy=dy, dfinal=dfinal)[1]
+    size = so.scan(**operands, dy=dy, dfinal=dfinal, magnitude=True)[1]
+    for name, value in zip(names, got):
+        close(value, grads[name], size[name], 2 * (70 * T + 20) + S + 60 + N, f"d{name}")
