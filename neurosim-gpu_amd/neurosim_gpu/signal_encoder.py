@@ -55,9 +55,10 @@ class _Encoder:
     def _project(self, name: str, x: torch.Tensor) -> torch.Tensor:
         raise NotImplementedError
 
-    def initial(self, batch: int) -> tuple[torch.Tensor, torch.Tensor]:
-        """The carried (history, state) before a signal: zeros."""
-        return (torch.zeros(self.taps - 1, batch, self.channels, device=self.device),
+    def initial(self, batch: int, dtype: torch.dtype = torch.float32
+                ) -> tuple[torch.Tensor, torch.Tensor]:
+        """The carried (history, state) before a signal of type ``dtype``: zeros."""
+        return (torch.zeros(self.taps - 1, batch, self.channels, dtype=dtype, device=self.device),
                 torch.zeros(batch, self.channels, self.states, device=self.device))
 
     def _scan_inputs(self, x: torch.Tensor):
@@ -71,7 +72,8 @@ class _Encoder:
     def drives(self, signal: torch.Tensor, carried=None, lengths: torch.Tensor | None = None):
         """Drives [T, B, N] of a signal [T, B, F], and the carried (history, state) after it."""
         p = self.parameters
-        history, state = self.initial(signal.shape[1]) if carried is None else carried
+        history, state = (self.initial(signal.shape[1], signal.dtype) if carried is None
+                          else carried)
         x, gate = self._project("project_in", signal).chunk(2, -1)
         x, history = causal_conv(x, p["conv_weight"], p["conv_bias"], history=history,
                                  lengths=lengths)

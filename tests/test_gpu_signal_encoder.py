@@ -106,3 +106,24 @@ def test_refusals(gpu):
         SignalEncoder(4, 10, 8, groups=3, device=gpu)
     with pytest.raises(ValueError, match="positive"):
         SignalEncoder(0, 10, 8, device=gpu)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_signals_of_fewer_bits_are_served(gpu, dtype):
+    """The carried history has the signal's type, also where the encoder makes it.  The bounds
+    are those of float32 signals, with the type's rounding in place of float32's."""
+    encoder = make(gpu).quantized()
+    x = signal(gpu, 20, 4).to(dtype)
+    with torch.no_grad():
+        whole, (history, state) = encoder.drives(x)
+        first, carried = encoder.drives(x[:7])
+        second, _ = encoder.drives(x[7:], carried)
+        carried = encoder.initial(4, dtype)
+        ticks = torch.stack([encoder.step(v, carried) for v in x])
+    assert whole.dtype == history.dtype == dtype and state.dtype == torch.float32
+    assert (carried[0] - history).abs().max() <= 2.0 ** -7 * history.abs().max()   # one rounding
+    scale = float(whole.float().abs().max())
+    for other in (torch.cat((first, second)), ticks):
+        apart = (other.float() - whole.float()).abs()
+        assert float((apart <= 0.02 * scale).float().mean()) >= 0.9
+        assert float(apart.max()) <= 0.25 * scale
