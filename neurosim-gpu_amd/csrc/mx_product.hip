@@ -716,17 +716,13 @@ constexpr int kWaves = kThreads / 64;
 // A workgroup's wavefronts share a strip of 16 columns, a part of K each.
 template <class T>
 __global__ __launch_bounds__(kThreads) void product_rows(MxView a, MxView b, const float* bias,
-                                                         T* out, int64_t stride, uint32_t groups,
-                                                         uint32_t splits, float* partials) {
+                                                         T* out, int64_t stride) {
   __shared__ v4f sums[kWaves][64];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-  const uint32_t split = uniform(blockIdx.x / groups), group = blockIdx.x - split * groups;
-  const int64_t n0 = static_cast<int64_t>(group) * 16;
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * 16;
   const RowPanel pa = row_panel(a, 0, lane), pb = row_panel(b, n0, lane);
   const int blocks = static_cast<int>(a.blocks), stages = (blocks + 7) / 8;
-  const uint32_t parts = splits * kWaves, part = split * kWaves + wave;
-  const int per = static_cast<int>(uniform((stages + parts - 1) / parts));
-  const int first = static_cast<int>(part) * per;
+  const int per = (stages + kWaves - 1) / kWaves, first = wave * per;
   const int stop = first + per < stages ? first + per : stages;
 
   v4f sum = {};
@@ -759,12 +755,8 @@ __global__ __launch_bounds__(kThreads) void product_rows(MxView a, MxView b, con
 #pragma unroll
   for (int w = 0; w < kWaves; ++w)
     total += reinterpret_cast<const float*>(&sums[w][from])[column & 3];
-  if (m < a.rows && n < b.rows) {
-    if (splits > 1)
-      partials[(split * a.rows + m) * b.rows + n] = total;
-    else
-      out[m * stride + n] = static_cast<T>(total + (bias ? bias[n] : 0.0f));
-  }
+  if (m < a.rows && n < b.rows)
+    out[m * stride + n] = static_cast<T>(total + (bias ? bias[n] : 0.0f));
 }
 
 // The parts of K added in order, eight requested at a time.
@@ -818,27 +810,19 @@ Kernel kernel_of(int64_t m, int64_t n, int64_t k) {
   return (m + 255) / 256 * ((n + 255) / 256) >= 192 ? Kernel::kLarge : Kernel::kSmall;
 }
 
-// Parts that K is cut into where workgroups are few.  A part's sums are written, read again
-// and cost a launch (4 us), so parts are long: rows, what a wavefront requests ahead; tiles,
-// eight stages, sixteen where the tiles alone give every compute unit one.  us, whole / cut:
+// Parts that the small tiles cut K into where they are few.  A part's sums are written, read
+// again and cost a launch (4 us), so parts are long: about seven stages, sixteen where the tiles
+// alone give every compute unit one.  (product_rows, whose wavefronts share K, gains nothing:
+// 8 x 2000 by 8192 whole 7.6, in two parts 11.5; 16 x 8000 by 8192 13.0 / 16.3.)  us, whole / cut:
 // 256 x 4096 by 4096 11.4 / 16.2 (2 parts of 8 stages), 1024 x 1024 by 8192 24.3 / 21.7 (2 of
 // 16), 64 x 8192 by 8192 18.1 (2 of 16) / 15.4 (4 of 8), 33 x 1000 by 50,000 15.5 (16 of 13) /
 // 14 (28 of 7).
 int64_t parts_of_k(int64_t m, int64_t n, int64_t k) {
   if (m <= 0 || n <= 0 || k <= 0) return 1;
-  const Kernel kernel = kernel_of(m, n, k);
-  if (kernel == Kernel::kLarge) return 1;
-  const int64_t stages = (k + 255) / 256;
-  int64_t parts, most;
-  if (kernel == Kernel::kRows) {
-    parts = 4096 / ((n + 15) / 16 * kWaves);
-    most = stages / (kWaves * kRowsAhead);
-  } else {
-    const int64_t tiles = (m + 63) / 64 * ((n + 63) / 64);
-    parts = 512 / tiles;
-    most = stages / (tiles >= 256 ? 16 : 7);
-  }
-  if (parts > most) parts = most;
+  if (kernel_of(m, n, k) != Kernel::kSmall) return 1;
+  const int64_t stages = (k + 255) / 256, tiles = (m + 63) / 64 * ((n + 63) / 64);
+  const int64_t most = stages / (tiles >= 256 ? 16 : 7);
+  const int64_t parts = 512 / tiles < most ? 512 / tiles : most;
   if (parts <= 1) return 1;
   const int64_t per = (stages + parts - 1) / parts;   // no empty part
   return (stages + per - 1) / per;
@@ -901,11 +885,10 @@ int run_large(const ns_mx_product_args* p, void* words, hipStream_t stream) {
 }
 
 template <class T>
-int run_rows(const ns_mx_product_args* p, int64_t parts, float* partials, hipStream_t stream) {
-  const int64_t strips = (p->b.rows + 15) / 16;
-  product_rows<T><<<dim3(static_cast<unsigned>(strips * parts)), dim3(kThreads), 0, stream>>>(
-      view(p->a), view(p->b), p->bias, static_cast<T*>(p->out), p->stride,
-      static_cast<uint32_t>(strips), static_cast<uint32_t>(parts), partials);
+int run_rows(const ns_mx_product_args* p, hipStream_t stream) {
+  const int64_t strips = (p->b.rows + 15) / 16;            // fewer than 1024 (kernel_of)
+  product_rows<T><<<dim3(static_cast<unsigned>(strips)), dim3(kThreads), 0, stream>>>(
+      view(p->a), view(p->b), p->bias, static_cast<T*>(p->out), p->stride);
   return launched("product");
 }
 
@@ -915,7 +898,7 @@ int run_kernel(const ns_mx_product_args* p, int64_t parts, float* partials, hipS
   switch (p->a.columns || kernel == Kernel::kRows ? kernel : Kernel::kSmall) {
     case Kernel::kLarge: return run_large<T>(p, partials, stream);
     case Kernel::kSmall: return run_tiles<Small, T>(p, parts, partials, stream);
-    default: return run_rows<T>(p, parts, partials, stream);
+    default: return run_rows<T>(p, stream);
   }
 }
 

@@ -331,3 +331,14 @@ def test_forward_mode_derivatives_are_refused(gpu):
             with pytest.raises(ValueError, match="forward-mode"):
                 call()
         mx_product(x, weight, bias=bias)
+
+
+@pytest.mark.parametrize("shape", [(1, 300, 8192), (16, 17, 8000), (3, 1000, 7937), (8, 2000, 8100)])
+def test_few_rows_with_the_longest_sums(gpu, shape):
+    """Up to 16 rows with K near 8192, the longest that one workgroup sums by itself: no
+    workspace, one launch."""
+    M, N, K = shape
+    assert microscaled._library().ns_mx_product_bytes(M, N, K, 0) == 0
+    x, weight = mx_quantize(rows(gpu, 63, M, K)), mx_quantize(rows(gpu, 64, N, K) / K ** 0.5)
+    for dtype in TYPES:
+        check_product(x, weight, rows(gpu, 65, N), dtype)
