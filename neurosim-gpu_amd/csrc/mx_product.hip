@@ -811,12 +811,14 @@ Kernel kernel_of(int64_t m, int64_t n, int64_t k) {
 }
 
 // Parts that the small tiles cut K into where they are few.  A part's sums are written, read
-// again and cost a launch (4 us), so parts are long: about seven stages, sixteen where the tiles
-// alone give every compute unit one.  (product_rows, whose wavefronts share K, gains nothing:
-// 8 x 2000 by 8192 whole 7.6, in two parts 11.5; 16 x 8000 by 8192 13.0 / 16.3.)  us, whole / cut:
-// 256 x 4096 by 4096 11.4 / 16.2 (2 parts of 8 stages), 1024 x 1024 by 8192 24.3 / 21.7 (2 of
-// 16), 64 x 8192 by 8192 18.1 (2 of 16) / 15.4 (4 of 8), 33 x 1000 by 50,000 15.5 (16 of 13) /
-// 14 (28 of 7).
+// again and cost a launch (4 us), so parts are long: seven stages or more, sixteen where the
+// tiles alone give every compute unit one.  (product_rows, whose wavefronts share K, gains
+// nothing: 8 x 2000 by 8192 whole 7.5, in two parts 11.6; 16 x 8000 by 8192 12.8 / 16.3.)  us,
+// whole / cut: 256 x 4096 by 4096 11.4 / 16.2 (2 parts of 8 stages), 1024 x 1024 by 8192 24.3 /
+// 21.7 (2 of 16), 64 x 8192 by 8192 18.1 (2 of 16) / 15.4 (4 of 8), 33 x 1000 by 50,000 15.5 (16
+// of 13) / 14 (28 of 7).  Seven stages at least against eight: 33 x 1000 by 60,000 13.8 / 14.2,
+// by 50,000 13.0 / 13.3, by 30,000 11.8 / 11.8; 33 x 2000 by 30,000 12.7 / 13.3, by 60,000 18.1 /
+// 18.1; 33 x 500 by 16,384 to 60,000, 64 x 8192 by 8192 and 100 x 2000 by 16,384 the same.
 int64_t parts_of_k(int64_t m, int64_t n, int64_t k) {
   if (m <= 0 || n <= 0 || k <= 0) return 1;
   if (kernel_of(m, n, k) != Kernel::kSmall) return 1;
