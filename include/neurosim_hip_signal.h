@@ -106,9 +106,9 @@ typedef struct ns_scan_args {
   float* partials;             /* workspace (ns_scan_plan) */
 } ns_scan_args;
 
-/* What a scan of this shape needs, `backward` or forward: sizes[0] time chunks worth scanning
- * side by side (1: none), and the floats of `ends` [1] (0 for one chunk), `checkpoints` [2]
- * and `partials` [3] with that many chunks. */
+/* What a scan of this shape needs: sizes[0] time chunks worth scanning side by side (1: none),
+ * the same in both directions, and with that many chunks the floats of `ends` [1] (0 for one
+ * chunk), of `checkpoints` [2], and of the `backward`'s `partials` [3] (0 for a forward). */
 int ns_scan_plan(int64_t ticks, int64_t batch, int64_t channels, int64_t groups, int32_t states,
                  int32_t backward, int64_t* sizes);
 int ns_scan_forward(const ns_scan_args* args, void* stream);

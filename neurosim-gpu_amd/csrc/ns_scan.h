@@ -223,7 +223,6 @@ inline ScanIn<T> scan_in(const ns_scan_args* a) {
 ScanShape scan_shape(const ns_scan_args* a);
 int check_shape(const ns_scan_args* a);
 int check_scan(const ns_scan_args* a);
-int64_t worth_chunks(const ns_scan_args* a, bool backward);
 int64_t scan_part_floats(const ns_scan_args* a);   // of ns_scan_backward's partials
 int scan_grid(const ScanShape& s, dim3* grid);
 // Turns each chunk's own end state (from zero) and decay into the state it starts from, or,

@@ -259,7 +259,7 @@ __global__ __launch_bounds__(kThreads) void scan_step(ScanShape s, ScanIn<T> in,
 // Few tiles over many blocks do not pay: 256 blocks, forward with 1 and 4 chunks, 400 ticks
 // 64 and 60, 128 ticks 23 and 31.  With 512 blocks one chunk is faster than two, 369 / 1039
 // against 499 / 1254: every further pass costs the update again.
-int64_t worth_chunks(const ns_scan_args* a) {
+static int64_t worth_chunks(const ns_scan_args* a) {
   if (a->ticks <= 0 || a->batch <= 0) return 1;
   const int64_t per = a->channels / a->groups;
   const int64_t blocks = a->groups * ((per + kScanChannels - 1) / kScanChannels) * a->batch;
@@ -411,7 +411,7 @@ int ns_scan_plan(int64_t ticks, int64_t batch, int64_t channels, int64_t groups,
   sizes[0] = s.chunks;
   sizes[1] = s.chunks > 1 ? s.chunks * lines * (4 * r + 1) : 0;
   sizes[2] = (ticks + tile - 1) / tile * lines * 4 * r;
-  sizes[3] = ns::scan_part_floats(&a);
+  sizes[3] = backward ? ns::scan_part_floats(&a) : 0;
   return NS_OK;
 }
 

@@ -42,8 +42,8 @@ TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # NS_TYPE_*
 _CONV = struct.Struct("=3q4i Q2q 2Q Q2q Q Q2q Q2q Q2q Q2q Q2q Q2q 2Q")
 _CONV_FORWARD = struct.Struct("=3q4i Q2q 2Q Q2q Q Q2q Q2q 112x")
 # ns_scan_args: shape; x, delta, z, y; B, C; A, D, delta_bias, state, out_state, lengths,
-# checkpoints, ends; dy; dout_state; dx, ddelta, dz, dB, dC; dstate, gradients of A, D and
-# delta_bias, partials.
+# checkpoints, ends; dy; dout_state; dx, ddelta, dz, dB, dC; dstate, dparameters (those of A, D
+# and delta_bias in one piece), partials.
 _SCAN = struct.Struct("=4q4i Q2q Q2q Q2q Q2q Q2q Q2q 8Q Q2q Q Q2q Q2q Q2q Q2q Q2q 3Q")
 _SCAN_FORWARD = struct.Struct("=4q4i Q2q Q2q Q2q Q2q Q2q Q2q 8Q 176x")
 _ABSENT = (0, 0, 0)
