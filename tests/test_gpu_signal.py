@@ -680,3 +680,17 @@ def test_rates_of_minus_infinity(gpu, T):
     size = so.scan(**operands, dy=dy, dfinal=dfinal, magnitude=True)[1]
     for name, value in zip(names, got):
         close(value, grads[name], size[name], 2 * (70 * T + 20) + S + 60 + N, f"d{name}")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,S,G,chunks", [(140, 16, 2, 19), (66, 24, 1, 25), (18, 40, 3, 75), (198, 7, 3, 19)])
+def test_scan_in_many_chunks_of_time(gpu, N, S, G, chunks, dtype):
+    """More chunks than the join asks for at a time, and no multiple of that; several groups and
+    workgroups to a group, the last of them partly empty; columns that end inside a chunk, at
+    a chunk's first tick, and before the first tick."""
+    draw, T, B = Draw(gpu, 100 + S), 600, 4
+    assert signal_ops._plan((T, B, N), G, S, True)[0] == chunks and chunks % 16
+    operands = scan_operands(draw, T, B, N, S, G, dtype)
+    ticks = -(-T // chunks)
+    lengths = torch.tensor([T, 333, 0, 5 * ticks], device=gpu) if S != 40 else None
+    check_scan(operands, lengths, True, draw(T, B, N, dtype=dtype), draw(B, N, S))
