@@ -8,7 +8,8 @@
  * data[t*stride_t + b*stride_b + n].  All signals of a call share one element type.
  * `lengths` (optional, device int32[B]) gives each column's own number of ticks,
  * clamped to [0, T]: later ticks of that column give zeros and change nothing, and
- * what their inputs hold is never used.
+ * what their inputs hold is never used.  What a call writes overlaps nothing that it
+ * reads, but for the history or state that a step moves on in place.
  */
 #ifndef NEUROSIM_HIP_SIGNAL_H
 #define NEUROSIM_HIP_SIGNAL_H

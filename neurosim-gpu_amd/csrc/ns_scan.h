@@ -6,7 +6,9 @@
 // q*R .. q*R + R-1 (S padded to 4R with rates, B and C of zero: such states stay zero).
 // Four lanes per channel rather than one give four times the wavefronts without a
 // second pass over time, and leave a lane few enough states that the backward keeps a
-// whole tile of them in registers; the price is two DPP adds per tick to join y.
+// whole tile of them in registers; the price is two DPP adds per tick to join y.  The lanes of
+// channels that a group lacks idle: T=512, B=8, N=1024, S=16 in bf16 takes 53 us in one group,
+// 51 in 16 (of 64 channels), 97 in 64 (of 16), 980 in 1024 (of one).
 //
 // Time goes in tiles of kTile<R> ticks.  All threads first do a tile's elementwise work,
 // each (tick, channel) once, and leave dt, dt*x (and what else the ticks need) in LDS as

@@ -10,7 +10,7 @@
 //
 // Tiles run from the last to the first.  The forward left h before every tile, so a tile's
 // states are scanned again from there and kept with their decays in registers (no exp in
-// the way back), then the adjoint runs down the tile.  Bound by the vector ALU, 75-80% busy:
+// the way back), then the adjoint runs down the tile.  Bound by the vector ALU, 74% busy:
 // T=2048, B=8, N=4096, S=16 in bf16 takes 1050 us, and 25 for the sums of dB and dC.
 //
 // dB and dC are sums over a group's channels.  A wavefront holds 16 channels: per four ticks
