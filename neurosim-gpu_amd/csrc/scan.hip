@@ -7,11 +7,11 @@
 // and one of the sum, against 8 bytes (bf16) per (tick, channel): the vector ALU bounds it, at
 // 16 states by about two to one over HBM.  T=2048, B=8, N=4096, S=16 in bf16: 377 us, of which
 // those six slots alone take 192 at the card's 33.5e12 lanes/s and the elementwise part (two
-// exp, a log, a reciprocal and their like per tick and channel) about 80: the ALU is 67% busy, with
-// two wavefronts a SIMD (512 workgroups); the chunked scan below, with eight, keeps it 89-96%
-// busy, but walks twice.  (With inputs two
-// tiles ahead 412, with the elementwise part of a thread's items overlapping 377; a tile's
-// ticks beside the next one's elementwise part, in two halves of LDS, 375 and so left out.)
+// exp, a log, a reciprocal and their like per tick and channel) about 80: the ALU is 67% busy,
+// with two wavefronts a SIMD (512 workgroups); the chunked scan below, with eight, keeps it
+// 89-96% busy, but walks twice.  (With inputs two tiles ahead 412, with the elementwise part of
+// a thread's items overlapping 377; a tile's ticks beside the next one's elementwise part, in
+// two halves of LDS, 375 and so left out.)
 //
 // Few columns and channels leave most of the card idle, so time is then cut into chunks
 // scanned side by side: a first pass gives every chunk's end state from zero and its
