@@ -1,7 +1,7 @@
 /*
  * neurosim_hip_signal.h -- C ABI of the signal operators around the tick: the short
- * causal convolution per channel and the selective state space scan, each for whole
- * signals, for one tick, and backwards.  Conventions (status codes, ns_last_error,
+ * causal convolution per channel, the selective state space scan and the gated linear
+ * recurrence, each for whole signals, for one tick, and backwards.  Conventions (status codes, ns_last_error,
  * caller's stream, no allocation, no synchronisation) are those of neurosim_hip.h.
  *
  * A signal is [T, B, N]: ticks, columns, channels, element (t, b, n) at
@@ -116,6 +116,42 @@ int ns_scan_forward(const ns_scan_args* args, void* stream);
 /* One tick (ticks == 1, no lengths): `out_state` is the state itself, updated in place. */
 int ns_scan_step(const ns_scan_args* args, void* stream);
 int ns_scan_backward(const ns_scan_args* args, void* stream);
+
+/* Gated linear recurrence, one state per channel:
+ *   s = sigmoid(forget), i = sigmoid(write), a = exp(-rates[n] s)
+ *   h[t,b,n] = a h[t-1] + sqrt(1 - a^2) i x,   y = h silu(z)   (z optional)
+ * Rates are not negative (a negative one counts as 0). */
+typedef struct ns_recurrence_args {
+  int64_t ticks, batch, channels;
+  int32_t type;                /* NS_TYPE_* of all signals (states and rates float32) */
+  int32_t chunks;              /* time chunks walked side by side (ns_recurrence_plan) */
+  ns_signal x, forget, write, z, y;
+  const float* rates;          /* [N] */
+  const float* state;          /* h before the first tick [B][N], or NULL: zeros */
+  float* out_state;            /* h after each column's last tick [B][N], or NULL */
+  const int32_t* lengths;
+  float* checkpoints;          /* optional workspace (ns_recurrence_plan): states kept for
+                                  ns_recurrence_backward */
+  float* ends;                 /* workspace (ns_recurrence_plan; chunks > 1) */
+  /* ns_recurrence_backward only (checkpoints required): */
+  ns_signal dy;
+  const float* dout_state;     /* gradient of out_state, or NULL: zeros */
+  ns_signal dx, dforget, dwrite, dz;   /* dz present exactly if z is */
+  float* dstate;               /* gradient of state [B][N], or NULL */
+  float* drates;               /* [N] */
+  float* partials;             /* workspace (ns_recurrence_plan) */
+} ns_recurrence_args;
+
+/* What a recurrence of this shape needs: sizes[0] time chunks worth walking side by side (1:
+ * none), and with that many the floats of `ends` [1] (0 for one chunk), of `checkpoints` [2] and of
+ * ns_recurrence_backward's `partials` [3]. */
+int ns_recurrence_plan(int64_t ticks, int64_t batch, int64_t channels, int32_t type,
+                       int64_t* sizes);
+int ns_recurrence_forward(const ns_recurrence_args* args, void* stream);
+/* One tick (ticks == 1, no lengths): `out_state` is the state itself, updated in place. */
+int ns_recurrence_step(const ns_recurrence_args* args, void* stream);
+/* Gradients, with sums in a fixed order (no atomics). */
+int ns_recurrence_backward(const ns_recurrence_args* args, void* stream);
 
 #ifdef __cplusplus
 }

@@ -19,7 +19,8 @@ from .native_compartmental import NativeDendriticMatrixRuntime, NativeDendriticP
 from .precision import PRECISIONS, encode_sparse_weights, quantize_dequantize
 from .rollout import MatrixRollout
 from .runtime import DenseOracle, HybridPELSRuntime, MatrixRuntime, RuntimeStats
-from .signal_ops import causal_conv, causal_conv_step, selective_scan, selective_scan_step
+from .signal_ops import (causal_conv, causal_conv_step, gated_recurrence, gated_recurrence_step,
+                         selective_scan, selective_scan_step)
 from .topology import SparseTopology, random_topology, topology_to
 from .topology_io import load_topology, save_topology, topology_from_dict, topology_to_dict
 
@@ -30,7 +31,8 @@ __all__ = [
     "Dynamics", "HybridPELSRuntime", "MXTensor", "MatrixRollout", "MatrixRuntime",
     "NativeDendriticMatrixRuntime", "NativeDendriticPELSRuntime", "PRECISIONS", "RuntimeStats",
     "SparseTopology", "capture_runtime", "causal_conv", "causal_conv_step",
-    "encode_sparse_weights", "load_native_extension", "load_runtime_checkpoint", "load_topology",
+    "encode_sparse_weights", "gated_recurrence", "gated_recurrence_step", "load_native_extension",
+    "load_runtime_checkpoint", "load_topology",
     "mx_dequantize", "mx_product", "mx_quantize", "quantize_dequantize", "random_topology",
     "restore_runtime", "save_runtime_checkpoint", "save_topology", "selective_scan",
     "selective_scan_step", "topology_from_dict", "topology_to", "topology_to_dict",

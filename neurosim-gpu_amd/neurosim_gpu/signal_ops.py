@@ -1,4 +1,4 @@
-"""The signal operators around the tick: causal convolution and selective scan.
+"""The signal operators around the tick: causal convolution, selective scan, gated recurrence.
 
 A signal is a [T, B, N] tensor: ticks, columns, channels, in the order of a rollout's
 staged drives (a [B, T, N] tensor goes in as its ``transpose(0, 1)``, read in place).
@@ -9,15 +9,19 @@ float32 and each output is rounded once.
 * ``selective_scan``: per channel S leaky integrators whose time step, input weights and
   read-out follow the signal,
   ``h[t] = exp(dt A) h[t-1] + dt x B[t]``, ``y[t] = (C[t] . h[t] + D x) silu(z)`` with
-  ``dt = softplus(delta + delta_bias)``.
+  ``dt = softplus(delta + delta_bias)``;
+* ``gated_recurrence``: per channel one state with a gate on what it forgets and one on what
+  it takes in, ``h[t] = a h[t-1] + sqrt(1 - a^2) sigmoid(write) x``, ``y[t] = h[t] silu(z)``
+  with ``a = exp(-rates sigmoid(forget))``.
 
-Both take and return the state that carries a signal on (``history``, ``state``), give
+All take and return the state that carries a signal on (``history``, ``state``), give
 native gradients of every tensor input (forward-mode derivatives are refused), and have a
 one-tick form that updates the carried state in place.  ``lengths`` gives columns their own
 number of ticks: past it outputs and gradients are zero, the carried state stays that of the
 column's last tick, and what the inputs hold there is never used.  The kernels are
-csrc/conv.hip, scan.hip, scan_grad.hip behind include/neurosim_hip_signal.h; calls run on
-the current stream, allocate their outputs and workspaces from torch, and never synchronise.
+csrc/conv.hip, scan.hip, scan_grad.hip, recur.hip and recur_grad.hip behind
+include/neurosim_hip_signal.h; calls run on the current stream, allocate their outputs and
+workspaces from torch, and never synchronise.
 """
 
 from __future__ import annotations
@@ -46,6 +50,10 @@ _CONV_FORWARD = struct.Struct("=3q4i Q2q 2Q Q2q Q Q2q Q2q 112x")
 # and delta_bias in one piece), partials.
 _SCAN = struct.Struct("=4q4i Q2q Q2q Q2q Q2q Q2q Q2q 8Q Q2q Q Q2q Q2q Q2q Q2q Q2q 3Q")
 _SCAN_FORWARD = struct.Struct("=4q4i Q2q Q2q Q2q Q2q Q2q Q2q 8Q 176x")
+# ns_recurrence_args: shape; x, forget, write, z, y; rates, state, out_state, lengths,
+# checkpoints, ends; dy; dout_state; dx, dforget, dwrite, dz; dstate, drates, partials.
+_RECUR = struct.Struct("=3q2i Q2q Q2q Q2q Q2q Q2q 6Q Q2q Q Q2q Q2q Q2q Q2q 3Q")
+_RECUR_FORWARD = struct.Struct("=3q2i Q2q Q2q Q2q Q2q Q2q 6Q 152x")
 _ABSENT = (0, 0, 0)
 
 _i32, _i64, _ptr = ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p
@@ -56,13 +64,16 @@ _Sizes = _i64 * 4
 def _library() -> ctypes.CDLL:
     lib = load_library()
     for name in ("ns_conv_forward", "ns_conv_step", "ns_conv_backward", "ns_scan_forward",
-                 "ns_scan_step", "ns_scan_backward"):
+                 "ns_scan_step", "ns_scan_backward", "ns_recurrence_forward", "ns_recurrence_step",
+                 "ns_recurrence_backward"):
         fn = getattr(lib, name)
         fn.restype, fn.argtypes = ctypes.c_int, [_ptr, _ptr]
     lib.ns_conv_backward_floats.restype = _i64
     lib.ns_conv_backward_floats.argtypes = [_i64, _i64, _i64, _i32, _i32]
     lib.ns_scan_plan.restype = ctypes.c_int
     lib.ns_scan_plan.argtypes = [_i64, _i64, _i64, _i64, _i32, _i32, _ptr]
+    lib.ns_recurrence_plan.restype = ctypes.c_int
+    lib.ns_recurrence_plan.argtypes = [_i64, _i64, _i64, _i32, _ptr]
     return lib
 
 
@@ -469,5 +480,131 @@ def selective_scan_step(x: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B
         B.data_ptr(), 0, B.stride(0), C.data_ptr(), 0, C.stride(0), A.data_ptr(), _address(D),
         _address(delta_bias), state.data_ptr(), state.data_ptr(), 0, 0, 0)
     call(_library().ns_scan_step, x.device, args)
+    _moved_on(state)
+    return y
+
+
+# ---- gated recurrence ----------------------------------------------------------------
+
+def _check_recurrence(x, forget, write, rates, z, state, dims: int) -> None:
+    _check_signal(x, "x", dims)
+    shape, device, dtype = x.shape, x.device, x.dtype
+    _check_like(forget, "forget", shape, device, dtype)
+    _check_like(write, "write", shape, device, dtype)
+    _check_like(rates, "rates", (shape[-1],), device, torch.float32)
+    if z is not None:
+        _check_like(z, "z", shape, device, dtype)
+    if state is not None:
+        _check_like(state, "state", tuple(shape[-2:]), device, torch.float32)
+
+
+def _recurrence_plan(x: torch.Tensor):
+    """(time chunks, floats of the chunks', the states' and the partial sums' workspaces)."""
+    lib, sizes = _library(), _Sizes()
+    code = lib.ns_recurrence_plan(*x.shape, TYPES[x.dtype], ctypes.addressof(sizes))
+    if code:
+        _raise_on(code, lib)
+    return sizes
+
+
+def _recurrence_forward(x, forget, write, z, rates, state, lengths, keep: bool):
+    """(y, final state, kept states or None) of dense operands."""
+    ticks, batch, n = x.shape
+    device = x.device
+    y = _room(x)
+    final = torch.empty((batch, n), dtype=torch.float32, device=device)
+    chunks, ends_floats, kept_floats, _ = _recurrence_plan(x)
+    ends = torch.empty(ends_floats, dtype=torch.float32, device=device) if ends_floats else None
+    kept = torch.empty(kept_floats, dtype=torch.float32, device=device) if keep else None
+    args = _RECUR_FORWARD.pack(
+        ticks, batch, n, TYPES[x.dtype], chunks, *_signal(x), *_signal(forget), *_signal(write),
+        *_signal(z), *_signal(y), rates.data_ptr(), _address(state), final.data_ptr(),
+        _address(lengths), _address(kept), _address(ends))
+    call(_library().ns_recurrence_forward, device, args)
+    return y, final, kept
+
+
+class _GatedRecurrence(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, forget, write, z, rates, state, lengths):
+        signals = tuple(_unit_channels(v) for v in (x, forget, write, z))
+        rates = _dense(rates)
+        y, final, kept = _recurrence_forward(*signals, rates, _dense(state), lengths, True)
+        ctx.save_for_backward(*signals, rates, lengths, kept)
+        ctx.set_materialize_grads(False)
+        return y, final
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dfinal):
+        x, forget, write, z, rates, lengths, kept = ctx.saved_tensors
+        wants, device = ctx.needs_input_grad, x.device
+        ticks, batch, n = x.shape
+        dfinal = _dense(dfinal)
+        if ticks == 0 or batch == 0:                  # no tick: the state passes through
+            zeros = [torch.zeros_like(v) if v is not None and w else None
+                     for v, w in zip((x, forget, write, z, rates), wants)]
+            return (*zeros, dfinal if wants[5] else None, None)
+        dy = torch.zeros_like(x) if dy is None else _unit_channels(dy)
+        chunks, ends_floats, _, part_floats = _recurrence_plan(x)
+        dx, dforget, dwrite = _room(x), _room(forget), _room(write)
+        dz = None if z is None else _room(z)
+        dstate = (torch.empty((batch, n), dtype=torch.float32, device=device)
+                  if wants[5] else None)
+        drates = torch.empty(n, dtype=torch.float32, device=device)
+        work = torch.empty(part_floats + ends_floats, dtype=torch.float32, device=device)
+        args = _RECUR.pack(
+            ticks, batch, n, TYPES[x.dtype], chunks, *_signal(x), *_signal(forget),
+            *_signal(write), *_signal(z), *_ABSENT, rates.data_ptr(), 0, 0, _address(lengths),
+            kept.data_ptr(), work.data_ptr() + 4 * part_floats if ends_floats else 0,
+            *_signal(dy), _address(dfinal), *_signal(dx), *_signal(dforget), *_signal(dwrite),
+            *_signal(dz), _address(dstate), drates.data_ptr(), work.data_ptr())
+        call(_library().ns_recurrence_backward, device, args)
+        grads = (dx, dforget, dwrite, dz, drates, dstate)
+        return (*(g if w else None for g, w in zip(grads, wants)), None)
+
+
+def gated_recurrence(x: torch.Tensor, forget: torch.Tensor, write: torch.Tensor,
+                     rates: torch.Tensor, *, z: torch.Tensor | None = None,
+                     state: torch.Tensor | None = None, lengths: torch.Tensor | None = None
+                     ) -> tuple[torch.Tensor, torch.Tensor]:
+    """Gated linear recurrence of ``x`` [T, B, N], one state per channel.
+
+    ``forget``, ``write`` and the optional output gate ``z`` are [T, B, N], as before their
+    sigmoids and silu; ``rates`` [N] float32 is how fast a channel with an open gate forgets
+    (positive; a negative rate counts as 0, where a gradient leaves out the input's part,
+    which has no bound there).  ``state`` [B, N] float32 is h before the first tick (zeros if
+    absent).
+
+    Returns ``(y, state)``: y [T, B, N] of x's type and h after each column's last tick."""
+    _check_recurrence(x, forget, write, rates, z, state, 3)
+    lengths = _lengths(lengths, x)
+    if _needs_grad(x, forget, write, rates, z, state):
+        return _GatedRecurrence.apply(x, forget, write, z, rates, state, lengths)
+    y, final, _ = _recurrence_forward(*(_unit_channels(v) for v in (x, forget, write, z)),
+                                      _dense(rates), _dense(state), lengths, False)
+    return y, final
+
+
+def gated_recurrence_step(x: torch.Tensor, forget: torch.Tensor, write: torch.Tensor,
+                          rates: torch.Tensor, *, z: torch.Tensor | None = None,
+                          state: torch.Tensor) -> torch.Tensor:
+    """One tick of ``gated_recurrence``: ``x``, ``forget``, ``write``, ``z`` [B, N] to y
+    [B, N]; ``state`` [B, N] (float32, contiguous) is updated in place.  Keeps nothing for
+    gradients; a backward that saved the state as it was refuses."""
+    _check_recurrence(x, forget, write, rates, z, state, 2)
+    if _needs_grad(x, forget, write, rates, z, state):
+        raise ValueError("a step gives no gradients; use gated_recurrence")
+    if state is None or not state.is_contiguous():
+        raise ValueError("state must be a contiguous [B, N] tensor, updated in place")
+    x, forget, write, z = (_unit_channels(v) for v in (x, forget, write, z))
+    rates, (batch, n) = _dense(rates), x.shape
+    y = _room(x)
+    args = _RECUR_FORWARD.pack(
+        1, batch, n, TYPES[x.dtype], 1, x.data_ptr(), 0, x.stride(0), forget.data_ptr(), 0,
+        forget.stride(0), write.data_ptr(), 0, write.stride(0),
+        *(_ABSENT if z is None else (z.data_ptr(), 0, z.stride(0))), y.data_ptr(), 0, n,
+        rates.data_ptr(), state.data_ptr(), state.data_ptr(), 0, 0, 0)
+    call(_library().ns_recurrence_step, x.device, args)
     _moved_on(state)
     return y
