@@ -1,0 +1,78 @@
+// What the forward and the backward of the gated projection share: activations, sizes of
+// tiles, and operands laid out as the tile kernels read them.
+#pragma once
+
+#include "ns_gemm.h"
+#include "neurosim_hip_block.h"
+
+namespace ns {
+
+using LargeGemm = GemmTile<8, 4, 2, 4>;    // 256 x 256
+using MiddleGemm = GemmTile<4, 4, 2, 2>;   // 128 x 128
+using SmallGemm = GemmTile<2, 2, 2, 2>;    // 64 x 64
+
+// x times the normal distribution's mass below x; erfc keeps the relative accuracy of small ones.
+__device__ __forceinline__ float mass_below(float x) { return 0.5f * erfcf(-0.70710678118654752f * x); }
+
+__device__ __forceinline__ float activated(float x, int activation) {
+  return x * (activation == NS_GATE_SILU ? sigmoid(x) : mass_below(x));
+}
+
+struct Activation {
+  float value, slope;
+};
+__device__ __forceinline__ Activation activated_slope(float x, int activation) {
+  if (activation == NS_GATE_SILU) {
+    const float s = sigmoid(x);
+    return Activation{x * s, s * fmaf(x, 1.0f - s, 1.0f)};
+  }
+  const float below = mass_below(x);
+  const float density = 0.39894228040143268f * __builtin_amdgcn_exp2f(-0.5f * kLog2e * x * x);
+  return Activation{x * below, fmaf(x, density, below)};
+}
+
+inline int64_t type_size(int32_t type) { return type == NS_TYPE_F32 ? 4 : 2; }
+// 16-byte pieces of a row of n values, and n up to whole pieces.
+inline int64_t pieces_of(int64_t n, int32_t type) { return (n * type_size(type) + 15) / 16; }
+inline int64_t whole_values(int64_t n, int32_t type) { return pieces_of(n, type) * 16 / type_size(type); }
+
+enum class GemmSize { kSmall, kMiddle, kLarge };
+GemmSize gemm_size(int64_t m, int64_t n, int32_t type);
+
+// Whether the tile kernels read these rows where they lie.
+inline bool plain(const void* data, int64_t stride, int64_t rows, int64_t columns, int32_t type) {
+  const int64_t e = type_size(type);
+  return reinterpret_cast<uintptr_t>(data) % 16 == 0 && columns * e % 16 == 0 &&
+         (rows <= 1 || (stride * e % 16 == 0 && stride >= columns && stride * e <= kMostStride));
+}
+inline Rows plain_rows(const void* data, int64_t stride, int64_t rows, int64_t columns, int32_t type) {
+  return Rows{static_cast<const uint8_t*>(data),
+              rows <= 1 ? pieces_of(columns, type) * 16 : stride * type_size(type), rows};
+}
+
+// What has to be laid out anew for the forward, and where in the workspace.
+struct PackedForward {
+  bool pack_x, pack_weights;
+  int64_t x, gate, up, bytes;
+};
+inline PackedForward packed_forward(const ns_gated_args* a) {
+  PackedForward w{};
+  const int64_t row = pieces_of(a->columns, a->type) * 16;
+  w.pack_x = !plain(a->x, a->x_stride, a->rows, a->columns, a->type);
+  w.pack_weights = !plain(a->gate, a->gate_stride, a->width, a->columns, a->type) ||
+                   !plain(a->up, a->up_stride, a->width, a->columns, a->type) ||
+                   (a->width > 1 && a->gate_stride != a->up_stride);
+  w.gate = w.pack_x ? a->rows * row : 0;
+  w.up = w.gate + (w.pack_weights ? a->width * row : 0);
+  w.bytes = w.up + (w.pack_weights ? a->width * row : 0);
+  return w;
+}
+
+// Copies rows of `columns` values to `to`, dense and filled up with zeros to whole pieces.
+int pack_rows(Rows* rows, const void* data, int64_t stride, int64_t columns, int32_t type, uint8_t* to,
+              hipStream_t stream);
+
+int check_gated(const ns_gated_args* a);
+bool few_rows(const ns_gated_args* a);
+
+}  // namespace ns

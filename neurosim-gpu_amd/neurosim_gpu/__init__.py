@@ -9,6 +9,7 @@ stand the operators of a signal path, in the same library: causal convolution, s
 scan and products of microscaled 4-bit rows (signal_ops, microscaled, signal_encoder).
 """
 
+from .block_ops import dropout, gated_projection
 from .checkpoint import (capture_runtime, load_runtime_checkpoint, restore_runtime,
                          save_runtime_checkpoint)
 from .compartmental import DendriticDynamics, DendriticMatrixRuntime, DendriticPELSRuntime
@@ -31,7 +32,7 @@ __all__ = [
     "Dynamics", "HybridPELSRuntime", "MXTensor", "MatrixRollout", "MatrixRuntime",
     "NativeDendriticMatrixRuntime", "NativeDendriticPELSRuntime", "PRECISIONS", "RuntimeStats",
     "SparseTopology", "capture_runtime", "causal_conv", "causal_conv_step",
-    "encode_sparse_weights", "gated_recurrence", "gated_recurrence_step", "load_native_extension",
+    "dropout", "encode_sparse_weights", "gated_projection", "gated_recurrence", "gated_recurrence_step", "load_native_extension",
     "load_runtime_checkpoint", "load_topology",
     "mx_dequantize", "mx_product", "mx_quantize", "quantize_dequantize", "random_topology",
     "restore_runtime", "save_runtime_checkpoint", "save_topology", "selective_scan",

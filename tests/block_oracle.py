@@ -58,3 +58,66 @@ def recurrence(x, forget, write, rates, z=None, state=None, lengths=None, dy=Non
         g, after = a[t] * g, before[t]
     grads["state"] = g
     return out, grads
+
+
+def activated(x, activation: str):
+    """(value, slope) of an activation."""
+    if activation == "silu":
+        return silu(x)
+    below = 0.5 * torch.special.erfc(-x * math.sqrt(0.5))
+    return x * below, below + x * torch.exp(-x * x / 2) / math.sqrt(2 * math.pi)
+
+
+def gated(x, gate, up, activation="silu", dy=None):
+    """y and its gradients (without dy: none)."""
+    x, gate, up, dy = (wide(v) for v in (x, gate, up, dy))
+    g, u = x @ gate.t(), x @ up.t()
+    value, slope = activated(g, activation)
+    if dy is None:
+        return value * u, {}
+    dg, du = dy * u * slope, dy * value
+    return value * u, {"x": dg @ gate + du @ up, "gate": dg.t() @ x, "up": du.t() @ x}
+
+
+def gated_bounds(x, gate, up, activation, dy, u, half):
+    """How far y and the gradients may be off for sums in arithmetic of half unit ``u`` and
+    operands rounded to a type of half unit ``half`` (see the tests)."""
+    x, gate, up, dy = (wide(v) for v in (x, gate, up, dy))
+    K = x.shape[1]
+    sums = 2 * (K + 2) * u
+    g, w = x @ gate.t(), x @ up.t()
+    eg, ew = sums * (x.abs() @ gate.abs().t()), sums * (x.abs() @ up.abs().t())
+    value, slope = activated(g, activation)
+    # |f'| <= 1.13 and |f''| <= 0.8 for both.  A value's own operations: silu's exponential is off
+    # by |g| u and its other steps by 5 u; gelu's erfc is off by 8 u and, its argument by 2 u, by
+    # twice g^2 u below zero.  The slope's are off by 16 u of 1 + |g|.
+    ev = 1.13 * eg + (12 + g.abs() + 2 * g * g) * u * value.abs()
+    es = 0.8 * eg + 16 * u * (1 + g.abs())
+    bounds = {"y": ev * (w.abs() + ew) + value.abs() * ew + 2 * u * (value * w).abs()}
+    dg, du = dy * w * slope, dy * value
+    edg = dy.abs() * (ew * slope.abs() + (w.abs() + ew) * es) + 3 * u * dg.abs()
+    edu = dy.abs() * ev + 2 * u * du.abs()
+    edg, edu = edg + half * (dg.abs() + edg), edu + half * (du.abs() + edu)
+    M, F = dy.shape
+    bounds["x"] = (edg @ gate.abs() + edu @ up.abs()
+                   + 2 * (2 * F + 2) * u * (dg.abs() @ gate.abs() + du.abs() @ up.abs()))
+    bounds["gate"] = edg.t() @ x.abs() + 2 * (M + 2) * u * (dg.abs().t() @ x.abs())
+    bounds["up"] = edu.t() @ x.abs() + 2 * (M + 2) * u * (du.abs().t() @ x.abs())
+    return bounds
+
+
+def philox(counter: int, offset: int, seed: int) -> list[int]:
+    """Eight 16-bit numbers of one counter: Philox4x32, 10 rounds, in Python's integers."""
+    word = 0xFFFFFFFF
+    c = [counter & word, counter >> 32 & word, offset & word, offset >> 32 & word]
+    k = [seed & word, seed >> 32 & word]
+    for _ in range(10):
+        p, q = c[0] * 0xD2511F53, c[2] * 0xCD9E8D57
+        c = [(q >> 32) ^ c[1] ^ k[0], q & word, (p >> 32) ^ c[3] ^ k[1], p & word]
+        k = [(k[0] + 0x9E3779B9) & word, (k[1] + 0xBB67AE85) & word]
+    return [part for v in c for part in (v & 0xFFFF, v >> 16)]
+
+
+def kept(count: int, p: float, seed: int, offset: int = 0):
+    numbers = [n for c in range(-(-count // 8)) for n in philox(c, offset, seed)][:count]
+    return torch.tensor([n >= round(p * 65536) for n in numbers], dtype=torch.bool)

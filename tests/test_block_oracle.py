@@ -46,3 +46,26 @@ def test_recurrence_gradients():
                           magnitude=True)[1]
     for name in found:
         assert (grads[name].abs() <= sizes[name] + 1e-12).all(), name
+
+
+def test_gated_gradients():
+    g = torch.Generator().manual_seed(2)
+    for activation in ("silu", "gelu"):
+        operands = {"x": draw(g, 4, 3), "gate": draw(g, 5, 3), "up": draw(g, 5, 3)}
+        dy = draw(g, 4, 5)
+        found = against_differences(lambda v: {"y": bo.gated(**v, activation=activation)[0]},
+                                    operands, {"y": dy})
+        _, grads = bo.gated(**operands, activation=activation, dy=dy)
+        for name, value in found.items():
+            assert (grads[name] - value).abs().max() < 1e-7, name
+
+
+def test_philox_known_answers():
+    """Known answers that the generator's authors publish for Philox4x32 with 10 rounds."""
+    def words(counter, offset, seed):
+        n = bo.philox(counter, offset, seed)
+        return [n[2 * k] | n[2 * k + 1] << 16 for k in range(4)]
+
+    assert words(0, 0, 0) == [0x6627E8D5, 0xE169C58D, 0xBC57AC4C, 0x9B00DBD8]
+    ones = (1 << 64) - 1
+    assert words(ones, ones, ones) == [0x408F276D, 0x41C83B0E, 0xA20BC7C6, 0x6D5451FD]
