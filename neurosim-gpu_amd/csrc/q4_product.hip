@@ -1,0 +1,463 @@
+// Product of float rows and a matrix of 4-bit integers with group scales (gfx950):
+// y[m][n] = sum over groups g of scale[n][g] * sum over k in g of x[m][k] (code[n][k] - zero[n][g]).
+//
+// Bound by the codes' bytes for few rows, so their way through the registers has to be short.
+// The sum over a group runs on the matrix cores with exact operands: a code u is put, by a shift
+// and one and-or, into the mantissa of 16 as the 16-bit number 16 + u, two at a time, and
+// sum x (16 + u) - (16 + zero) sum x is scaled in float32.  16-bit rows go in as they are.  For
+// float32 rows the 16 + zero that is taken off again would cost some bits where x has a mean, so
+// a row goes in as x - c, c its mean over the group, in three bfloat16 parts that together are
+// exact, with a fourth row of ones that gives c its share: sum x (u - zero) =
+// sum (x - c)(u - zero) + c (sum (16 + u) - count (16 + zero)), whose factor of c is exact.
+//
+// In the 16x16x32 instruction the rows of x are the first operand and 16 rows of the weight the
+// second, so a lane's four results are four rows of x (for float32: one row's three parts and the
+// ones) of its own row of the weight, whose codes it loaded and whose scales it needs.
+#include "ns_q4.h"
+#include "ns_gemm.h"
+
+namespace ns {
+namespace {
+
+constexpr int kQ4Waves = 8, kQ4Threads = 64 * kQ4Waves;
+constexpr int kStage = 128;                    // columns a wavefront takes at a time
+constexpr int kRing = 4;                       // stages requested ahead
+
+// Rows of x that 16 rows of the instruction hold.
+template <class T>
+constexpr int kTileRows = sizeof(T) == 4 ? 4 : 16;
+
+// What a workgroup does: CT tiles of x's rows, S strips of 16 rows of the weight per wavefront,
+// NG groups (or parts of one) per stage.
+template <int kCT, int kS, int kNG>
+struct Q4Tile {
+  static constexpr int CT = kCT, S = kS, NG = kNG;
+  static constexpr int chunk = 2048 / CT;      // columns of x in LDS: 64 KiB
+  static constexpr int stages = chunk / kStage, sub = kStage / NG;
+};
+
+struct Q4Place {
+  uint32_t m_tiles, strip_groups, splits, parts;   // parts: wavefronts that share a strip
+  uint32_t chunks, per_split;                      // chunks of columns, and of a split
+};
+
+// Codes 0 .. 3 and 4 .. 7 of a word as four registers of two 16-bit numbers 16 + u: codes i and
+// i + 4 in register i.  The rows of x lie in that order too.
+template <bool kHalf>
+__device__ __forceinline__ v4i sixteen_plus(uint32_t word) {
+  constexpr int at = kHalf ? 6 : 3;            // the place of u in the mantissa
+  constexpr uint32_t mask = kHalf ? 0x03C003C0u : 0x00780078u;
+  constexpr uint32_t sixteen = kHalf ? 0x4C004C00u : 0x41804180u;
+  v4i out;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t moved = 4 * i > at ? word >> (4 * i > at ? 4 * i - at : 0)
+                                      : word << (4 * i > at ? 0 : at - 4 * i);
+    out[i] = static_cast<int>((moved & mask) | sixteen);
+  }
+  return out;
+}
+
+template <class T>
+__device__ __forceinline__ v4f q4_multiply(v4i x, v4i w, v4f sum) {
+  if constexpr (__is_same(T, _Float16)) return multiply_pieces<_Float16>(x, w, sum);
+  else return multiply_pieces<__bf16>(x, w, sum);
+}
+
+// A lane of quarter q has words 0 .. 3 of block q of its row's four; after this, word q of blocks
+// 0 .. 3: a step of the instruction then takes one block, whose group is one.
+__device__ __forceinline__ void swap_lanes_32(uint32_t& a, uint32_t& b) {
+  const auto both = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+  a = both[0];
+  b = both[1];
+}
+__device__ __forceinline__ void swap_lanes_16(uint32_t& a, uint32_t& b) {
+  const auto both = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+  a = both[0];
+  b = both[1];
+}
+__device__ __forceinline__ void deal_blocks(uint32_t (&w)[4]) {
+  swap_lanes_32(w[0], w[2]);
+  swap_lanes_32(w[1], w[3]);
+  swap_lanes_16(w[0], w[1]);
+  swap_lanes_16(w[2], w[3]);
+}
+
+// The sum over kLanes neighbouring lanes, in every one of them.
+template <int kLanes>
+__device__ __forceinline__ float lanes_sum(float v) {
+#pragma unroll
+  for (int step = 1; step < kLanes; step *= 2) v += __shfl_xor(v, step);
+  return v;
+}
+
+template <class G, class T>
+struct Q4Lds {
+  v4i x[G::chunk / 64][16 * G::CT][8];         // pieces of eight columns, at place piece ^ turn(row)
+  float sums[G::chunk / G::sub][16 * G::CT];   // of a row of the instruction over a (sub)group
+  float centre[sizeof(T) == 4 ? G::chunk / G::sub : 1][4 * G::CT];
+};
+
+__device__ __forceinline__ int pair_of(float a, float b) {
+  typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(int, v2bf{static_cast<__bf16>(a), static_cast<__bf16>(b)});
+}
+
+// Puts a chunk of x's rows into LDS.
+template <class G, class T>
+__device__ __forceinline__ void place_rows(const T* x, int64_t stride, int64_t rows, int64_t first,
+                                           int64_t columns, Q4Lds<G, T>& lds) {
+  constexpr int kBlocks = G::chunk / 8, kLanes = G::sub / 8;
+#pragma unroll 1
+  for (int i = threadIdx.x; i < kTileRows<T> * G::CT * kBlocks; i += kQ4Threads) {
+    const int r = i / kBlocks, b = i % kBlocks;
+    if (r >= rows) break;
+    const int64_t k = first + 8 * b, left = columns - k;
+    const T* const from = x + r * stride + k;
+    float v[8];
+    Pack<T, 8> raw;
+    if (left >= 8) {
+      raw = load_pack<T, 8>(from);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) raw.v[j] = j < left ? from[j] : T{};
+    }
+    float sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum += v[j] = static_cast<float>(raw.v[j]);
+    sum = lanes_sum<kLanes>(sum);
+    const int group = b / kLanes, line = b / 8, piece = b % 8;
+    const bool leads = b % kLanes == 0;
+    if constexpr (sizeof(T) == 2) {
+      Pack<T, 8> turned;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) turned.v[2 * j] = raw.v[j], turned.v[2 * j + 1] = raw.v[j + 4];
+      lds.x[line][r][piece ^ turn(r)] = __builtin_bit_cast(v4i, turned);
+      if (leads) lds.sums[group][r] = sum;
+    } else {
+      const int64_t behind = columns - (first + group * G::sub);
+      const float count = behind < G::sub ? (behind > 0 ? static_cast<float>(behind) : 0.0f)
+                                          : static_cast<float>(G::sub);
+      const float centre = count > 0.0f ? sum / count : 0.0f;
+      float rest[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) rest[j] = j < left ? v[j] - centre : 0.0f;
+      const int slot = 16 * (r >> 2) + 4 * (r & 3);
+#pragma unroll
+      for (int part = 0; part < 3; ++part) {
+        float own[8], total = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          own[j] = static_cast<float>(static_cast<__bf16>(rest[j]));
+          rest[j] -= own[j];
+          total += own[j];
+        }
+        lds.x[line][slot + part][piece ^ turn(slot + part)] =
+            v4i{pair_of(own[0], own[4]), pair_of(own[1], own[5]), pair_of(own[2], own[6]),
+                pair_of(own[3], own[7])};
+        total = lanes_sum<kLanes>(total);
+        if (leads) lds.sums[group][slot + part] = total;
+      }
+      float one[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) one[j] = j < left ? 1.0f : 0.0f;
+      lds.x[line][slot + 3][piece ^ turn(slot + 3)] =
+          v4i{pair_of(one[0], one[4]), pair_of(one[1], one[5]), pair_of(one[2], one[6]),
+              pair_of(one[3], one[7])};
+      if (leads) {
+        lds.sums[group][slot + 3] = count;
+        lds.centre[group][r] = centre;
+      }
+    }
+  }
+}
+
+// A wavefront's request of one strip and stage.
+template <int NG>
+struct Q4Stage {
+  uint32_t codes[4];
+  float scale[NG], zero[NG];
+};
+
+template <class G, class T>
+__global__ __launch_bounds__(kQ4Threads) void q4_product(Q4View w, Q4Place p, const T* x,
+                                                         int64_t x_stride, int64_t rows,
+                                                         const float* bias, T* out, int64_t stride,
+                                                         float* partials) {
+  __shared__ union {
+    Q4Lds<G, T> in;
+    v4f sums[kQ4Waves][G::S][G::CT][64];
+  } lds;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), q = lane >> 4;
+  // Each XCD gets a run of workgroups, the rows' tiles of a strip group side by side, so that its
+  // codes are read into one L2.
+  const uint32_t share = gridDim.x / kXcds;
+  uint32_t id = blockIdx.x < share * kXcds ? blockIdx.x % kXcds * share + blockIdx.x / kXcds : blockIdx.x;
+  const uint32_t line = uniform(id / p.m_tiles), m_tile = id - line * p.m_tiles;
+  const uint32_t split = uniform(line / p.strip_groups), strip_group = line - split * p.strip_groups;
+  const uint32_t part = wave % p.parts;
+  const int64_t m0 = static_cast<int64_t>(m_tile) * (kTileRows<T> * G::CT);
+  const int64_t n0 =
+      (static_cast<int64_t>(strip_group) * (kQ4Waves / p.parts) + wave / p.parts) * (16 * G::S);
+
+  const int stages = static_cast<int>((w.blocks + 3) / 4), blocks = static_cast<int>(w.blocks);
+  const int first_chunk = static_cast<int>(split * p.per_split);
+  const int last_chunk = first_chunk + static_cast<int>(p.per_split) < static_cast<int>(p.chunks)
+                             ? first_chunk + static_cast<int>(p.per_split) : static_cast<int>(p.chunks);
+  const int limit = last_chunk * G::stages < stages ? last_chunk * G::stages : stages;
+  const uint32_t per_group = G::NG == 1 ? static_cast<uint32_t>(w.group / kStage) : 1;
+
+  Q4Stage<G::NG> ring[kRing][G::S];
+  const auto load = [&](int stage, Q4Stage<G::NG> (&to)[G::S]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int s = 0; s < G::S; ++s) {
+      const int64_t n = n0 + 16 * s + (lane & 15), row = n < w.rows ? n : w.rows - 1;
+      // Past the last block, x is zero: any codes do.
+      const int block = 4 * stage + q < blocks ? 4 * stage + q : blocks - 1;
+      __builtin_memcpy(to[s].codes, w.codes + (row * blocks + block) * 16, 16);
+      const int64_t line = row * w.groups;
+#pragma unroll
+      for (int g = 0; g < G::NG; ++g) {
+        int64_t group = G::NG == 1 ? static_cast<int64_t>(stage / per_group) : stage * G::NG + g;
+        group = line + (group < w.groups ? group : w.groups - 1);
+        to[s].scale[g] = q4_scale(w, group);
+        to[s].zero[g] = w.zeros ? static_cast<float>(w.zeros[group]) : 8.0f;
+      }
+    }
+  };
+
+  v4f total[G::S][G::CT] = {};
+  const auto compute = [&](int stage, Q4Stage<G::NG> (&from)[G::S]) __attribute__((always_inline)) {
+    const int own = stage % G::stages;                   // in the chunk
+#pragma unroll
+    for (int s = 0; s < G::S; ++s) deal_blocks(from[s].codes);
+#pragma unroll
+    for (int g = 0; g < G::NG; ++g) {
+      v4f sum[G::S][G::CT] = {};
+      constexpr int kSteps = 4 / G::NG;
+#pragma unroll
+      for (int step = 0; step < kSteps; ++step) {
+        const int e = g * kSteps + step;
+        v4i rows_of_x[G::CT];
+#pragma unroll
+        for (int t = 0; t < G::CT; ++t)
+          rows_of_x[t] = lds.in.x[2 * own + e / 2][16 * t + (lane & 15)][(4 * (e & 1) + q) ^ turn(lane & 15)];
+#pragma unroll
+        for (int s = 0; s < G::S; ++s) {
+          const v4i codes = sixteen_plus<__is_same(T, _Float16)>(from[s].codes[e]);
+#pragma unroll
+          for (int t = 0; t < G::CT; ++t) sum[s][t] = q4_multiply<T>(rows_of_x[t], codes, sum[s][t]);
+        }
+      }
+      const int group = own * G::NG + g;
+#pragma unroll
+      for (int t = 0; t < G::CT; ++t) {
+        const v4f taken = *reinterpret_cast<const v4f*>(&lds.in.sums[group][16 * t + 4 * q]);
+        const float centre = sizeof(T) == 4 ? lds.in.centre[group][4 * t + q] : 0.0f;
+#pragma unroll
+        for (int s = 0; s < G::S; ++s) {
+          const float offset = -16.0f - from[s].zero[g], scale = from[s].scale[g];
+          float own_sum[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) own_sum[i] = fmaf(offset, taken[i], sum[s][t][i]);
+          if constexpr (sizeof(T) == 4) {
+            const float parts = (own_sum[2] + own_sum[1]) + own_sum[0];
+            total[s][t][0] = fmaf(scale, fmaf(centre, own_sum[3], parts), total[s][t][0]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) total[s][t][i] = fmaf(scale, own_sum[i], total[s][t][i]);
+          }
+        }
+      }
+    }
+  };
+
+  // The wavefronts of a strip take its stages in turn; a chunk has a multiple of kRing for each.
+  const int step = static_cast<int>(p.parts);
+  int stage = first_chunk * G::stages + static_cast<int>(part);
+#pragma unroll
+  for (int u = 0; u < kRing; ++u)
+    if (stage + u * step < limit) load(stage + u * step, ring[u]);
+  for (int chunk = first_chunk; chunk < last_chunk; ++chunk) {
+    __syncthreads();
+    place_rows<G, T>(x + m0 * x_stride, x_stride, rows - m0, static_cast<int64_t>(chunk) * G::chunk,
+                     w.columns, lds.in);
+    __syncthreads();
+    for (int end = (chunk + 1) * G::stages; stage < end; stage += kRing * step) {
+#pragma unroll
+      for (int u = 0; u < kRing; ++u) {
+        const int now = stage + u * step;
+        if (now < limit) {
+          compute(now, ring[u]);
+          if (now + kRing * step < limit) load(now + kRing * step, ring[u]);
+        }
+      }
+    }
+  }
+
+  if (p.parts > 1) {
+    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < G::S; ++s)
+#pragma unroll
+      for (int t = 0; t < G::CT; ++t) lds.sums[wave][s][t][lane] = total[s][t];
+    __syncthreads();
+    if (part) return;
+    for (int other = 1; other < step; ++other)
+#pragma unroll
+      for (int s = 0; s < G::S; ++s)
+#pragma unroll
+        for (int t = 0; t < G::CT; ++t) total[s][t] += lds.sums[wave + other][s][t][lane];
+  }
+#pragma unroll
+  for (int s = 0; s < G::S; ++s) {
+    const int64_t n = n0 + 16 * s + (lane & 15);
+    if (n >= w.rows) continue;
+    const float more = bias ? bias[n] : 0.0f;
+#pragma unroll
+    for (int t = 0; t < G::CT; ++t)
+#pragma unroll
+      for (int i = 0; i < (sizeof(T) == 4 ? 1 : 4); ++i) {
+        const int64_t m = m0 + (sizeof(T) == 4 ? 4 * t + q : 16 * t + 4 * q + i);
+        if (m >= rows) continue;
+        if (p.splits > 1) partials[(split * rows + m) * w.rows + n] = total[s][t][i];
+        else out[m * stride + n] = static_cast<T>(total[s][t][i] + more);
+      }
+  }
+}
+
+// The parts of K added in order, eight requested at a time.
+template <class T>
+__global__ __launch_bounds__(kThreads) void add_splits(const float* __restrict__ partials,
+                                                       uint32_t splits, int64_t rows, int64_t columns,
+                                                       const float* bias, T* out, int64_t stride) {
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  if (id >= rows * columns) return;
+  float sum = 0.0f;
+  constexpr uint32_t kAhead = 8;
+  for (uint32_t k = 0; k < splits; k += kAhead) {
+    float v[kAhead];
+#pragma unroll
+    for (uint32_t u = 0; u < kAhead; ++u)
+      v[u] = partials[(k + u < splits ? k + u : k) * rows * columns + id];
+#pragma unroll
+    for (uint32_t u = 0; u < kAhead; ++u) sum += k + u < splits ? v[u] : 0.0f;
+  }
+  const int64_t m = id / columns, n = id - m * columns;
+  out[m * stride + n] = static_cast<T>(sum + (bias ? bias[n] : 0.0f));
+}
+
+// y = bias where there is nothing to sum.
+template <class T>
+__global__ __launch_bounds__(kThreads) void bias_rows(int64_t rows, int64_t columns, const float* bias,
+                                                      T* out, int64_t stride) {
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  if (id >= rows * columns) return;
+  const int64_t m = id / columns, n = id - m * columns;
+  out[m * stride + n] = static_cast<T>(bias ? bias[n] : 0.0f);
+}
+
+int launched(const char* what) {
+  const hipError_t err = hipGetLastError();
+  return err == hipSuccess ? NS_OK : fail_launch(what, err);
+}
+
+// How a product is cut: tiles of x's rows per workgroup, wavefronts that share a strip, and
+// parts of K that workgroups share, so that 2048 wavefronts or more stream codes.
+struct Q4Plan {
+  int tiles, strips;
+  Q4Place place;
+  int64_t groups;              // workgroups
+};
+Q4Plan q4_plan(int64_t m, int64_t n, int64_t k, int32_t type) {
+  Q4Plan plan{};
+  const int64_t per_tile = type == NS_TYPE_F32 ? 4 : 16, tiles = (m + per_tile - 1) / per_tile;
+  plan.tiles = tiles <= 1 ? 1 : tiles <= 2 ? 2 : 4;
+  plan.strips = plan.tiles == 1 ? 1 : 2;
+  const int64_t m_tiles = (tiles + plan.tiles - 1) / plan.tiles;
+  const int64_t strips = (n + 16 * plan.strips - 1) / (16 * plan.strips);
+  const int64_t columns = 2048 / plan.tiles, chunks = (k + columns - 1) / columns;
+  int64_t parts = 1;
+  while (parts * 2 <= 4 / plan.tiles && m_tiles * strips * parts < 2048) parts *= 2;
+  const int64_t waves = m_tiles * strips * parts;
+  int64_t splits = waves < 2048 ? 2048 / waves : 1;
+  splits = splits < chunks ? splits : chunks;
+  const int64_t per = splits > 0 ? (chunks + splits - 1) / splits : 1;
+  splits = per > 0 ? (chunks + per - 1) / per : 1;         // no empty part
+  const int64_t strip_groups = (strips * parts + kQ4Waves - 1) / kQ4Waves;
+  plan.groups = m_tiles * strip_groups * splits;
+  plan.place = Q4Place{static_cast<uint32_t>(m_tiles), static_cast<uint32_t>(strip_groups),
+                       static_cast<uint32_t>(splits), static_cast<uint32_t>(parts),
+                       static_cast<uint32_t>(chunks), static_cast<uint32_t>(per)};
+  return plan;
+}
+
+template <class G, class T>
+int run_tile(const ns_q4_product_args* a, const Q4Plan& plan, hipStream_t stream) {
+  q4_product<G, T><<<dim3(static_cast<unsigned>(plan.groups)), dim3(kQ4Threads), 0, stream>>>(
+      q4_view(a->weight), plan.place, static_cast<const T*>(a->x), a->x_stride, a->rows, a->bias,
+      static_cast<T*>(a->out), a->stride, a->workspace);
+  return launched("4-bit product");
+}
+
+template <class T, int kNG>
+int run_groups(const ns_q4_product_args* a, const Q4Plan& plan, hipStream_t stream) {
+  switch (plan.tiles) {
+    case 1: return run_tile<Q4Tile<1, 1, kNG>, T>(a, plan, stream);
+    case 2: return run_tile<Q4Tile<2, 2, kNG>, T>(a, plan, stream);
+    default: return run_tile<Q4Tile<4, 2, kNG>, T>(a, plan, stream);
+  }
+}
+
+template <class T>
+int run(const ns_q4_product_args* a, hipStream_t stream) {
+  const int64_t m = a->rows, n = a->weight.rows, results = (m * n + kThreads - 1) / kThreads;
+  if (results > INT32_MAX) return fail("the product is too large for one launch");
+  if (a->weight.columns == 0) {
+    bias_rows<T><<<dim3(static_cast<unsigned>(results)), dim3(kThreads), 0, stream>>>(
+        m, n, a->bias, static_cast<T*>(a->out), a->stride);
+    return launched("4-bit product");
+  }
+  const Q4Plan plan = q4_plan(m, n, a->weight.columns, a->type);
+  if (plan.groups > INT32_MAX) return fail("the product is too large for one launch");
+  if (plan.place.splits > 1 && !a->workspace) return fail("the product needs its workspace");
+  int rc;
+  switch (a->weight.group) {
+    case 32: rc = run_groups<T, 4>(a, plan, stream); break;
+    case 64: rc = run_groups<T, 2>(a, plan, stream); break;
+    default: rc = run_groups<T, 1>(a, plan, stream); break;
+  }
+  if (rc || plan.place.splits == 1) return rc;
+  add_splits<T><<<dim3(static_cast<unsigned>(results)), dim3(kThreads), 0, stream>>>(
+      a->workspace, plan.place.splits, m, n, a->bias, static_cast<T*>(a->out), a->stride);
+  return launched("4-bit product parts");
+}
+
+}  // namespace
+}  // namespace ns
+
+extern "C" {
+
+int64_t ns_q4_product_floats(int64_t m, int64_t n, int64_t k, int32_t type) {
+  if (m <= 0 || n <= 0 || k <= 0) return 0;
+  const ns::Q4Plan plan = ns::q4_plan(m, n, k, type);
+  return plan.place.splits > 1 ? plan.place.splits * m * n : 0;
+}
+
+int ns_q4_product(const ns_q4_product_args* a, void* stream) {
+  ns::clear_error();
+  if (!a) return ns::fail("product arguments are required");
+  if (int rc = ns::check_q4(a->weight)) return rc;
+  if (a->rows < 0) return ns::fail("rows must not be negative");
+  if (a->rows == 0 || a->weight.rows == 0) return NS_OK;
+  if ((a->weight.columns && !a->x) || !a->out) return ns::fail("x and the output are required");
+  auto queue = static_cast<hipStream_t>(stream);
+  switch (a->type) {
+    case NS_TYPE_F32: return ns::run<float>(a, queue);
+    case NS_TYPE_BF16: return ns::run<__bf16>(a, queue);
+    case NS_TYPE_F16: return ns::run<_Float16>(a, queue);
+    default: return ns::fail("unknown element type");
+  }
+}
+
+}  // extern "C"

@@ -14,6 +14,7 @@ from .checkpoint import (capture_runtime, load_runtime_checkpoint, restore_runti
                          save_runtime_checkpoint)
 from .compartmental import DendriticDynamics, DendriticMatrixRuntime, DendriticPELSRuntime
 from .dynamics import Dynamics
+from .group_scaled import Q4Tensor, q4_dequantize, q4_product, q4_quantize
 from .microscaled import MXTensor, mx_dequantize, mx_product, mx_quantize
 from .native import load_native_extension
 from .native_compartmental import NativeDendriticMatrixRuntime, NativeDendriticPELSRuntime
@@ -30,11 +31,12 @@ __version__ = "0.1.0"
 __all__ = [
     "DendriticDynamics", "DendriticMatrixRuntime", "DendriticPELSRuntime", "DenseOracle",
     "Dynamics", "HybridPELSRuntime", "MXTensor", "MatrixRollout", "MatrixRuntime",
-    "NativeDendriticMatrixRuntime", "NativeDendriticPELSRuntime", "PRECISIONS", "RuntimeStats",
+    "NativeDendriticMatrixRuntime", "NativeDendriticPELSRuntime", "PRECISIONS", "Q4Tensor", "RuntimeStats",
     "SparseTopology", "capture_runtime", "causal_conv", "causal_conv_step",
     "dropout", "encode_sparse_weights", "gated_projection", "gated_recurrence", "gated_recurrence_step", "load_native_extension",
     "load_runtime_checkpoint", "load_topology",
-    "mx_dequantize", "mx_product", "mx_quantize", "quantize_dequantize", "random_topology",
+    "mx_dequantize", "mx_product", "mx_quantize", "q4_dequantize", "q4_product", "q4_quantize",
+    "quantize_dequantize", "random_topology",
     "restore_runtime", "save_runtime_checkpoint", "save_topology", "selective_scan",
     "selective_scan_step", "topology_from_dict", "topology_to", "topology_to_dict",
 ]

@@ -121,3 +121,44 @@ def philox(counter: int, offset: int, seed: int) -> list[int]:
 def kept(count: int, p: float, seed: int, offset: int = 0):
     numbers = [n for c in range(-(-count // 8)) for n in philox(c, offset, seed)][:count]
     return torch.tensor([n >= round(p * 65536) for n in numbers], dtype=torch.bool)
+
+
+def q4_codes(x, group: int, symmetric: bool, dtype):
+    """(codes, scales, zeros) of rows, step by step as the format says: float32 arithmetic, whose
+    division is exactly rounded, and scales rounded to their type."""
+    x = x.detach().float().cpu()
+    rows, columns = x.shape
+    groups = -(-columns // group)
+    wide_x = torch.zeros(rows, groups * group)
+    wide_x[:, :columns] = x
+    parts = wide_x.view(rows, groups, group)
+    low, high = parts.amin(-1).clamp(max=0), parts.amax(-1).clamp(min=0)
+    finite = torch.isfinite(parts).all(-1)
+    scale = torch.maximum(high, -low) / 7 if symmetric else high / 15 - low / 15
+    scale = scale.to(dtype).float()
+    good = finite & torch.isfinite(scale)
+    some = good & (scale > 0)
+    safe = torch.where(some, scale, torch.ones_like(scale))
+    zero = torch.full_like(scale, 8.0) if symmetric else torch.where(
+        some, torch.round(-low / safe).clamp(0, 15), torch.zeros_like(scale))
+    zero_of = zero.unsqueeze(-1)
+    codes = torch.where(some.unsqueeze(-1), (torch.round(parts / safe.unsqueeze(-1)) + zero_of)
+                        .clamp(0, 15), torch.where(good.unsqueeze(-1), zero_of, 0.0))
+    codes = torch.nan_to_num(codes).view(rows, -1)[:, :columns]
+    scale = torch.where(good, scale, torch.full_like(scale, math.nan))
+    return codes.to(torch.uint8), scale.to(dtype), zero.to(torch.uint8)
+
+
+def q4_pack(codes):
+    """Codes [N, K] as bytes [N, ceil(K/32) * 16]."""
+    rows, columns = codes.shape
+    room = torch.zeros(rows, -(-columns // 32) * 32, dtype=torch.uint8)
+    room[:, :columns] = codes
+    return room[:, 0::2] | (room[:, 1::2] << 4)
+
+
+def q4_values(codes, scales, zeros, group: int):
+    """Values [N, K] in float64 (zeros None: 8)."""
+    columns = codes.shape[1]
+    spread = lambda v: v.double().cpu().repeat_interleave(group, 1)[:, :columns]  # noqa: E731
+    return (codes.double().cpu() - (8.0 if zeros is None else spread(zeros))) * spread(scales)

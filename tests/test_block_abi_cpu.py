@@ -11,7 +11,7 @@ from pathlib import Path
 
 import pytest
 
-from neurosim_gpu import block_ops, native, signal_ops
+from neurosim_gpu import block_ops, group_scaled, native, signal_ops
 
 ROOT = Path(__file__).resolve().parents[1]
 INCLUDE = ROOT / "include"
@@ -167,3 +167,56 @@ def test_recurrence_refusals(lib):
                          (dict(kept=16, z=present), "dz is given"),
                          (dict(kept=16, ticks=200, chunks=2), "workspace")):
         assert text in message(lib, "ns_recurrence_backward", args(**change)), change
+
+
+@pytest.mark.skipif(shutil.which("gcc") is None, reason="gcc is not installed")
+def test_packed_4_bit_structs_have_the_header_s_layout(tmp_path):
+    source = tmp_path / "layout.c"
+    source.write_text("""
+#include <stddef.h>
+#include <stdio.h>
+#include "neurosim_hip_q4.h"
+int main(void) {
+  printf("%zu %zu\\n", sizeof(ns_q4_matrix), offsetof(ns_q4_matrix, scale_type));
+  printf("%zu %zu %zu\\n", sizeof(ns_q4_product_args), offsetof(ns_q4_product_args, workspace),
+         offsetof(ns_q4_product_args, type));
+  return 0;
+}
+""")
+    subprocess.run(["gcc", f"-I{INCLUDE}", str(source), "-o", str(tmp_path / "layout")], check=True)
+    lines = subprocess.run([str(tmp_path / "layout")], capture_output=True, text=True,
+                           check=True).stdout.split("\n")
+    matrix, product = ([int(v) for v in line.split()] for line in lines[:2])
+    assert matrix == [group_scaled._MATRIX.size, 48]
+    assert product == [group_scaled._PRODUCT.size, group_scaled._PRODUCT.size - 8,
+                       group_scaled._PRODUCT.size - 16]
+
+
+def test_4_bit_refusals(lib):
+    def matrix(rows=4, columns=64, group=32, codes=16, scales=16, scale_type=1):
+        return rows, columns, group, codes, scales, 0, scale_type
+
+    def product(m=2, x=16, out=16, type=0, **more):
+        return group_scaled._PRODUCT.pack(*matrix(**more), m, x, 64, 0, out, 4, type, 0)
+
+    changes = ((dict(rows=-1), "negative"), (dict(columns=(1 << 23) + 1), "at most"),
+               (dict(group=16), "32, 64"), (dict(group=192), "32, 64"), (dict(codes=0), "required"),
+               (dict(scales=0), "required"), (dict(codes=8), "aligned"), (dict(scale_type=9), "scales"))
+    for change, text in changes:
+        assert text in message(lib, "ns_q4_product", product(**change)), change
+        for fn in (lib.ns_q4_quantize, lib.ns_q4_dequantize):
+            fn.restype, fn.argtypes = ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64,
+                                                     ctypes.c_int32, ctypes.c_void_p]
+            assert fn(group_scaled._MATRIX.pack(*matrix(**change)), 16, 64, 0, None) != 0
+            assert text in lib.ns_last_error().decode(), change
+    for change, text in ((dict(m=-1), "negative"), (dict(x=0), "required"), (dict(out=0), "required"),
+                         (dict(type=5), "element type"), (dict(columns=50_000, rows=100), "workspace")):
+        assert text in message(lib, "ns_q4_product", product(**change)), change
+
+
+def test_4_bit_workspaces(lib):
+    """Workgroups share K, and need a workspace, only where the weight's rows are few."""
+    fn = lib.ns_q4_product_floats
+    fn.restype, fn.argtypes = ctypes.c_int64, [ctypes.c_int64] * 3 + [ctypes.c_int32]
+    assert fn(1, 50_000, 1024, 0) == 0 and fn(0, 5, 5, 0) == 0 and fn(5, 0, 5, 0) == 0
+    assert fn(33, 1000, 50_000, 1) % (33 * 1000) == 0 and fn(33, 1000, 50_000, 1) > 33 * 1000
