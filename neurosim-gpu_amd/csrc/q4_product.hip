@@ -4,11 +4,12 @@
 // Bound by the codes' bytes for few rows, so their way through the registers has to be short.
 // The sum over a group runs on the matrix cores with exact operands: a code u is put, by a shift
 // and one and-or, into the mantissa of 16 as the 16-bit number 16 + u, two at a time, and
-// sum x (16 + u) - (16 + zero) sum x is scaled in float32.  16-bit rows go in as they are.  For
-// float32 rows the 16 + zero that is taken off again would cost some bits where x has a mean, so
-// a row goes in as x - c, c its mean over the group, in three bfloat16 parts that together are
-// exact, with a fourth row of ones that gives c its share: sum x (u - zero) =
-// sum (x - c)(u - zero) + c (sum (16 + u) - count (16 + zero)), whose factor of c is exact.
+// sum x (16 + u) - (16 + zero) sum x is scaled in float32, the sums of x coming from the same
+// instruction with ones as weights.  16-bit rows go in as they are.  For float32 rows the 16 +
+// zero that is taken off again would cost some bits where x has a mean, so a row goes in as
+// x - c, c its mean over the group, in three bfloat16 parts that together are exact, with a
+// fourth row of ones that gives c its share: sum x (u - zero) = sum (x - c)(u - zero) +
+// c (sum (16 + u) - count (16 + zero)), whose factor of c is exact.
 //
 // In the 16x16x32 instruction the rows of x are the first operand and 16 rows of the weight the
 // second, so a lane's four results are four rows of x (for float32: one row's three parts and the
@@ -94,7 +95,6 @@ __device__ __forceinline__ float lanes_sum(float v) {
 template <class G, class T>
 struct Q4Lds {
   v4i x[G::chunk / 64][16 * G::CT][8];         // pieces of eight columns, at place piece ^ turn(row)
-  float sums[G::chunk / G::sub][16 * G::CT];   // of a row of the instruction over a (sub)group
   float centre[sizeof(T) == 4 ? G::chunk / G::sub : 1][4 * G::CT];
 };
 
@@ -103,60 +103,75 @@ __device__ __forceinline__ int pair_of(float a, float b) {
   return __builtin_bit_cast(int, v2bf{static_cast<__bf16>(a), static_cast<__bf16>(b)});
 }
 
-// Puts a chunk of x's rows into LDS.
+// A thread's pieces of a chunk of x's rows, on their way to LDS.
 template <class G, class T>
-__device__ __forceinline__ void place_rows(const T* x, int64_t stride, int64_t rows, int64_t first,
-                                           int64_t columns, Q4Lds<G, T>& lds) {
-  constexpr int kBlocks = G::chunk / 8, kLanes = G::sub / 8;
-#pragma unroll 1
-  for (int i = threadIdx.x; i < kTileRows<T> * G::CT * kBlocks; i += kQ4Threads) {
-    const int r = i / kBlocks, b = i % kBlocks;
-    if (r >= rows) break;
-    const int64_t k = first + 8 * b, left = columns - k;
-    const T* const from = x + r * stride + k;
-    float v[8];
-    Pack<T, 8> raw;
-    if (left >= 8) {
-      raw = load_pack<T, 8>(from);
-    } else {
+struct Q4Rows {
+  static constexpr int blocks = G::chunk / 8;              // of a row
+  static constexpr int count = kTileRows<T> * G::CT * blocks / kQ4Threads;
+  static_assert(kTileRows<T> * G::CT * blocks % kQ4Threads == 0, "whole pieces per thread");
+  Pack<T, 8> v[count];
+};
+
+// Requests them.  Rows that do not exist are not read, nor is the chunk after the last.
+template <class G, class T>
+__device__ __forceinline__ void ask_rows(const T* x, int64_t stride, int64_t rows, int64_t first,
+                                         int64_t columns, Q4Rows<G, T>& to) {
+  using R = Q4Rows<G, T>;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) raw.v[j] = j < left ? from[j] : T{};
+  for (int u = 0; u < R::count; ++u) {
+    const int i = threadIdx.x + u * kQ4Threads, r = i / R::blocks, b = i % R::blocks;
+    const int64_t left = columns - first - 8 * b;
+    const T* const from = x + r * stride + first + 8 * b;
+    to.v[u] = Pack<T, 8>{};
+    if (r < rows && left >= 8) {
+      to.v[u] = load_pack<T, 8>(from);
+    } else if (r < rows && left > 0) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j < left) to.v[u].v[j] = from[j];
     }
-    float sum = 0.0f;
+  }
+}
+
+// Puts them into LDS.
+template <class G, class T>
+__device__ __forceinline__ void place_rows(const Q4Rows<G, T>& rows_of_x, int64_t rows, int64_t first,
+                                           int64_t columns, Q4Lds<G, T>& lds) {
+  using R = Q4Rows<G, T>;
+  constexpr int kLanes = G::sub / 8;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) sum += v[j] = static_cast<float>(raw.v[j]);
-    sum = lanes_sum<kLanes>(sum);
+  for (int u = 0; u < R::count; ++u) {
+    const int i = threadIdx.x + u * kQ4Threads, r = i / R::blocks, b = i % R::blocks;
+    if (r >= rows) break;
+    const Pack<T, 8>& raw = rows_of_x.v[u];
     const int group = b / kLanes, line = b / 8, piece = b % 8;
-    const bool leads = b % kLanes == 0;
     if constexpr (sizeof(T) == 2) {
       Pack<T, 8> turned;
 #pragma unroll
       for (int j = 0; j < 4; ++j) turned.v[2 * j] = raw.v[j], turned.v[2 * j + 1] = raw.v[j + 4];
       lds.x[line][r][piece ^ turn(r)] = __builtin_bit_cast(v4i, turned);
-      if (leads) lds.sums[group][r] = sum;
     } else {
-      const int64_t behind = columns - (first + group * G::sub);
+      const int64_t left = columns - first - 8 * b, behind = columns - (first + group * G::sub);
       const float count = behind < G::sub ? (behind > 0 ? static_cast<float>(behind) : 0.0f)
                                           : static_cast<float>(G::sub);
-      const float centre = count > 0.0f ? sum / count : 0.0f;
-      float rest[8];
+      float sum = 0.0f, rest[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) rest[j] = j < left ? v[j] - centre : 0.0f;
+      for (int j = 0; j < 8; ++j) sum += raw.v[j];
+      const float centre = count > 0.0f ? lanes_sum<kLanes>(sum) / count : 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) rest[j] = j < left ? raw.v[j] - centre : 0.0f;
       const int slot = 16 * (r >> 2) + 4 * (r & 3);
 #pragma unroll
       for (int part = 0; part < 3; ++part) {
-        float own[8], total = 0.0f;
+        float own[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           own[j] = static_cast<float>(static_cast<__bf16>(rest[j]));
           rest[j] -= own[j];
-          total += own[j];
         }
         lds.x[line][slot + part][piece ^ turn(slot + part)] =
             v4i{pair_of(own[0], own[4]), pair_of(own[1], own[5]), pair_of(own[2], own[6]),
                 pair_of(own[3], own[7])};
-        total = lanes_sum<kLanes>(total);
-        if (leads) lds.sums[group][slot + part] = total;
       }
       float one[8];
 #pragma unroll
@@ -164,20 +179,71 @@ __device__ __forceinline__ void place_rows(const T* x, int64_t stride, int64_t r
       lds.x[line][slot + 3][piece ^ turn(slot + 3)] =
           v4i{pair_of(one[0], one[4]), pair_of(one[1], one[5]), pair_of(one[2], one[6]),
               pair_of(one[3], one[7])};
-      if (leads) {
-        lds.sums[group][slot + 3] = count;
-        lds.centre[group][r] = centre;
-      }
+      if (b % kLanes == 0) lds.centre[group][r] = centre;
     }
   }
 }
 
-// A wavefront's request of one strip and stage.
+// A wavefront's request of one strip and stage: scales and zeros as they are in memory, so that
+// nothing waits for them before they are used.
+template <int NG>
+struct Q4Scales {
+  uint32_t scale[NG], zeros;                     // of 32 bits each, or of 16 side by side; bytes
+};
 template <int NG>
 struct Q4Stage {
   uint32_t codes[4];
-  float scale[NG], zero[NG];
+  Q4Scales<NG> by;
 };
+
+// Scales and zeros of groups first .. first + NG - 1 of a row that begins at `at`; past its last
+// group, where x is zero, that one's.
+template <int NG>
+__device__ __forceinline__ void load_scales(const Q4View& w, int64_t at, int first, Q4Scales<NG>& to) {
+  const int groups = static_cast<int>(w.groups);
+  to.zeros = 0x08080808u;
+  if (w.scale_type == NS_TYPE_F32 || first + NG > groups) {
+#pragma unroll
+    for (int g = 0; g < NG; ++g) to.scale[g] = 0;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      const int64_t own = at + (first + g < groups ? first + g : groups - 1);
+      if (w.scale_type == NS_TYPE_F32)
+        to.scale[g] = static_cast<const uint32_t*>(w.scales)[own];
+      else
+        to.scale[g / 2] |= static_cast<uint32_t>(static_cast<const uint16_t*>(w.scales)[own]) << (g % 2 * 16);
+    }
+    if (w.zeros) {
+      to.zeros = 0;
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+        to.zeros |= static_cast<uint32_t>(w.zeros[at + (first + g < groups ? first + g : groups - 1)]) << (8 * g);
+    }
+  } else {
+    to.scale[0] = 0;
+    __builtin_memcpy(to.scale, static_cast<const uint16_t*>(w.scales) + at + first, 2 * NG);
+    if (w.zeros) {
+      to.zeros = 0;
+      __builtin_memcpy(&to.zeros, w.zeros + at + first, NG);
+    }
+  }
+}
+
+template <int NG>
+__device__ __forceinline__ uint32_t raw_scale(const Q4Scales<NG>& s, int g, int32_t type) {
+  const uint32_t half = g & 1 ? s.scale[g / 2] >> 16 : s.scale[g / 2] & 0xFFFFu;
+  return type == NS_TYPE_F32 ? s.scale[g] : half;
+}
+template <int NG>
+__device__ __forceinline__ float zero_offset(const Q4Scales<NG>& s, int g) {
+  return -16.0f - static_cast<float>(s.zeros >> (8 * g) & 255u);
+}
+
+__device__ __forceinline__ float scale_value(uint32_t raw, int32_t type) {
+  if (type == NS_TYPE_F32) return __builtin_bit_cast(float, raw);
+  if (type == NS_TYPE_BF16) return __builtin_bit_cast(float, raw << 16);
+  return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(raw)));
+}
 
 template <class G, class T>
 __global__ __launch_bounds__(kQ4Threads) void q4_product(Q4View w, Q4Place p, const T* x,
@@ -207,25 +273,29 @@ __global__ __launch_bounds__(kQ4Threads) void q4_product(Q4View w, Q4Place p, co
   const int limit = last_chunk * G::stages < stages ? last_chunk * G::stages : stages;
   const uint32_t per_group = G::NG == 1 ? static_cast<uint32_t>(w.group / kStage) : 1;
 
+  // A lane's rows of the weight.
+  const uint8_t* codes[G::S];
+  int64_t scales[G::S];                          // places of their first scales
+#pragma unroll
+  for (int s = 0; s < G::S; ++s) {
+    const int64_t n = n0 + 16 * s + (lane & 15), row = n < w.rows ? n : w.rows - 1;
+    codes[s] = w.codes + row * blocks * 16;
+    scales[s] = row * w.groups;
+  }
   Q4Stage<G::NG> ring[kRing][G::S];
   const auto load = [&](int stage, Q4Stage<G::NG> (&to)[G::S]) __attribute__((always_inline)) {
+    // Past the last block, x is zero: any codes do.
+    const int block = 4 * stage + q < blocks ? 4 * stage + q : blocks - 1;
+    const int first = G::NG == 1 ? static_cast<int>(stage / per_group) : stage * G::NG;
 #pragma unroll
     for (int s = 0; s < G::S; ++s) {
-      const int64_t n = n0 + 16 * s + (lane & 15), row = n < w.rows ? n : w.rows - 1;
-      // Past the last block, x is zero: any codes do.
-      const int block = 4 * stage + q < blocks ? 4 * stage + q : blocks - 1;
-      __builtin_memcpy(to[s].codes, w.codes + (row * blocks + block) * 16, 16);
-      const int64_t line = row * w.groups;
-#pragma unroll
-      for (int g = 0; g < G::NG; ++g) {
-        int64_t group = G::NG == 1 ? static_cast<int64_t>(stage / per_group) : stage * G::NG + g;
-        group = line + (group < w.groups ? group : w.groups - 1);
-        to[s].scale[g] = q4_scale(w, group);
-        to[s].zero[g] = w.zeros ? static_cast<float>(w.zeros[group]) : 8.0f;
-      }
+      __builtin_memcpy(to[s].codes, codes[s] + static_cast<uint32_t>(block) * 16, 16);
+      load_scales<G::NG>(w, scales[s], first, to[s].by);
     }
   };
 
+  constexpr int kOnes = __is_same(T, _Float16) ? 0x3C003C00 : 0x3F803F80;
+  const v4i ones = {kOnes, kOnes, kOnes, kOnes};
   v4f total[G::S][G::CT] = {};
   const auto compute = [&](int stage, Q4Stage<G::NG> (&from)[G::S]) __attribute__((always_inline)) {
     const int own = stage % G::stages;                   // in the chunk
@@ -233,15 +303,17 @@ __global__ __launch_bounds__(kQ4Threads) void q4_product(Q4View w, Q4Place p, co
     for (int s = 0; s < G::S; ++s) deal_blocks(from[s].codes);
 #pragma unroll
     for (int g = 0; g < G::NG; ++g) {
-      v4f sum[G::S][G::CT] = {};
+      v4f sum[G::S][G::CT] = {}, taken[G::CT] = {};
       constexpr int kSteps = 4 / G::NG;
 #pragma unroll
       for (int step = 0; step < kSteps; ++step) {
         const int e = g * kSteps + step;
         v4i rows_of_x[G::CT];
 #pragma unroll
-        for (int t = 0; t < G::CT; ++t)
+        for (int t = 0; t < G::CT; ++t) {
           rows_of_x[t] = lds.in.x[2 * own + e / 2][16 * t + (lane & 15)][(4 * (e & 1) + q) ^ turn(lane & 15)];
+          taken[t] = q4_multiply<T>(rows_of_x[t], ones, taken[t]);
+        }
 #pragma unroll
         for (int s = 0; s < G::S; ++s) {
           const v4i codes = sixteen_plus<__is_same(T, _Float16)>(from[s].codes[e]);
@@ -251,37 +323,42 @@ __global__ __launch_bounds__(kQ4Threads) void q4_product(Q4View w, Q4Place p, co
       }
       const int group = own * G::NG + g;
 #pragma unroll
-      for (int t = 0; t < G::CT; ++t) {
-        const v4f taken = *reinterpret_cast<const v4f*>(&lds.in.sums[group][16 * t + 4 * q]);
-        const float centre = sizeof(T) == 4 ? lds.in.centre[group][4 * t + q] : 0.0f;
+      for (int s = 0; s < G::S; ++s) {
+        const float offset = zero_offset(from[s].by, g);
+        const float scale = scale_value(raw_scale(from[s].by, g, w.scale_type), w.scale_type);
 #pragma unroll
-        for (int s = 0; s < G::S; ++s) {
-          const float offset = -16.0f - from[s].zero[g], scale = from[s].scale[g];
+        for (int t = 0; t < G::CT; ++t) {
           float own_sum[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) own_sum[i] = fmaf(offset, taken[i], sum[s][t][i]);
+          for (int i = 0; i < 4; ++i) own_sum[i] = fmaf(offset, taken[t][i], sum[s][t][i]);
           if constexpr (sizeof(T) == 4) {
             const float parts = (own_sum[2] + own_sum[1]) + own_sum[0];
-            total[s][t][0] = fmaf(scale, fmaf(centre, own_sum[3], parts), total[s][t][0]);
+            const float whole = fmaf(lds.in.centre[group][4 * t + q], own_sum[3], parts);
+            total[s][t][0] = fmaf(scale, whole, total[s][t][0]);
           } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) total[s][t][i] = fmaf(scale, own_sum[i], total[s][t][i]);
           }
         }
       }
+      // One group after the other: side by side they do not fit the registers.
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
 
   // The wavefronts of a strip take its stages in turn; a chunk has a multiple of kRing for each.
   const int step = static_cast<int>(p.parts);
   int stage = first_chunk * G::stages + static_cast<int>(part);
+  const T* const own_x = x + m0 * x_stride;
 #pragma unroll
   for (int u = 0; u < kRing; ++u)
     if (stage + u * step < limit) load(stage + u * step, ring[u]);
   for (int chunk = first_chunk; chunk < last_chunk; ++chunk) {
-    __syncthreads();
-    place_rows<G, T>(x + m0 * x_stride, x_stride, rows - m0, static_cast<int64_t>(chunk) * G::chunk,
-                     w.columns, lds.in);
+    const int64_t first = static_cast<int64_t>(chunk) * G::chunk;
+    Q4Rows<G, T> rows_of_x;
+    ask_rows<G, T>(own_x, x_stride, rows - m0, first, w.columns, rows_of_x);
+    if (chunk > first_chunk) __syncthreads();              // all have read the one before
+    place_rows<G, T>(rows_of_x, rows - m0, first, w.columns, lds.in);
     __syncthreads();
     for (int end = (chunk + 1) * G::stages; stage < end; stage += kRing * step) {
 #pragma unroll
@@ -326,6 +403,128 @@ __global__ __launch_bounds__(kQ4Threads) void q4_product(Q4View w, Q4Place p, co
   }
 }
 
+// Up to 16 rows of 16 bits go from memory to registers: a workgroup's wavefronts share S strips
+// and take their stages in turn, so each reads its own part of x, without LDS or barriers but
+// for the sums at the end.
+constexpr int kRowRing = 3;
+
+template <int NG, int S>
+struct Q4RowStage {
+  v4i x[4];
+  Q4Stage<NG> w[S];
+};
+
+template <class T, int NG, int S>
+__global__ __launch_bounds__(kQ4Threads) void q4_rows(Q4View w, Q4Place p, const T* x, int64_t x_stride,
+                                                      int64_t rows, const float* bias, T* out,
+                                                      int64_t stride, float* partials) {
+  __shared__ v4f sums[kQ4Waves][S][64];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), q = lane >> 4;
+  const uint32_t split = uniform(blockIdx.x / p.strip_groups), strip_group = blockIdx.x - split * p.strip_groups;
+  const int part = static_cast<int>(wave % p.parts), step = static_cast<int>(p.parts);
+  const int64_t n0 = (static_cast<int64_t>(strip_group) * (kQ4Waves / p.parts) + wave / p.parts) * (16 * S);
+  const int blocks = static_cast<int>(w.blocks), stages = (blocks + 3) / 4;
+  const int begin = static_cast<int>(split * p.per_split);
+  const int limit = begin + static_cast<int>(p.per_split) < stages ? begin + static_cast<int>(p.per_split) : stages;
+  const uint32_t per_group = NG == 1 ? static_cast<uint32_t>(w.group / kStage) : 1;
+  const int64_t m = (lane & 15) < rows ? lane & 15 : rows - 1;
+  const T* const own_x = x + m * x_stride + 8 * q;
+  const uint8_t* codes[S];
+  int64_t scales[S];
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    const int64_t n = n0 + 16 * s + (lane & 15), row = n < w.rows ? n : w.rows - 1;
+    codes[s] = w.codes + row * blocks * 16;
+    scales[s] = row * w.groups;
+  }
+  const int whole = static_cast<int>(w.columns / kStage);  // stages that lie within the columns
+  Q4RowStage<NG, S> ring[kRowRing];
+  const auto load = [&](int stage, Q4RowStage<NG, S>& to) __attribute__((always_inline)) {
+    const int block = 4 * stage + q < blocks ? 4 * stage + q : blocks - 1;
+    const int first = NG == 1 ? static_cast<int>(stage / per_group) : stage * NG;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      __builtin_memcpy(to.w[s].codes, codes[s] + static_cast<uint32_t>(block) * 16, 16);
+      load_scales<NG>(w, scales[s], first, to.w[s].by);
+    }
+    const T* const from = own_x + static_cast<int64_t>(stage) * kStage;
+    if (stage < whole) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) __builtin_memcpy(&to.x[e], from + 32 * e, 16);
+    } else {
+      const int left = static_cast<int>(w.columns - static_cast<int64_t>(stage) * kStage) - 8 * q;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        Pack<T, 8> v;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v.v[j] = 32 * e + j < left ? from[32 * e + j] : T{};
+        to.x[e] = __builtin_bit_cast(v4i, v);
+      }
+    }
+  };
+  constexpr int kOnes = __is_same(T, _Float16) ? 0x3C003C00 : 0x3F803F80;
+  const v4i ones = {kOnes, kOnes, kOnes, kOnes};
+  v4f total[S] = {};
+  const auto compute = [&](Q4RowStage<NG, S>& from) __attribute__((always_inline)) {
+#pragma unroll
+    for (int s = 0; s < S; ++s) deal_blocks(from.w[s].codes);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      v4f sum[S] = {}, taken = {};
+#pragma unroll
+      for (int e = g * (4 / NG); e < (g + 1) * (4 / NG); ++e) {
+        // Values 0 .. 7 in the order that sixteen_plus leaves the codes in.
+        v4i v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          v[i] = static_cast<int>(__builtin_amdgcn_perm(
+              static_cast<uint32_t>(from.x[e][2 + i / 2]), static_cast<uint32_t>(from.x[e][i / 2]),
+              i & 1 ? 0x07060302u : 0x05040100u));
+        taken = q4_multiply<T>(v, ones, taken);
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+          sum[s] = q4_multiply<T>(v, sixteen_plus<__is_same(T, _Float16)>(from.w[s].codes[e]), sum[s]);
+      }
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        const float offset = zero_offset(from.w[s].by, g);
+        const float scale = scale_value(raw_scale(from.w[s].by, g, w.scale_type), w.scale_type);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) total[s][i] = fmaf(scale, fmaf(offset, taken[i], sum[s][i]), total[s][i]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+#pragma unroll
+  for (int u = 0; u < kRowRing; ++u)
+    if (begin + part + u * step < limit) load(begin + part + u * step, ring[u]);
+  for (int stage = begin + part; stage < limit; stage += kRowRing * step) {
+#pragma unroll
+    for (int u = 0; u < kRowRing; ++u) {
+      const int now = stage + u * step;
+      if (now < limit) {
+        compute(ring[u]);
+        if (now + kRowRing * step < limit) load(now + kRowRing * step, ring[u]);
+      }
+    }
+  }
+#pragma unroll
+  for (int s = 0; s < S; ++s) sums[wave][s][lane] = total[s];
+  __syncthreads();
+  // The workgroup's strips, 256 results each, a column of the weight's rows by its threads.
+  for (int id = threadIdx.x; id < static_cast<int>(kQ4Waves / p.parts) * S * 256; id += kQ4Threads) {
+    const int strip = id >> 8, column = id & 15, row = id >> 4 & 15, first = strip / S * step;
+    const int from = (row >> 2) * 16 + column;             // the lane that holds it
+    const int64_t n = static_cast<int64_t>(strip_group) * (kQ4Waves / p.parts) * (16 * S) + 16 * strip + column;
+    if (row >= rows || n >= w.rows) continue;
+    float value = 0.0f;
+    for (int k = 0; k < step; ++k)
+      value += reinterpret_cast<const float*>(&sums[first + k][strip % S][from])[row & 3];
+    if (p.splits > 1) partials[(split * rows + row) * w.rows + n] = value;
+    else out[row * stride + n] = static_cast<T>(value + (bias ? bias[n] : 0.0f));
+  }
+}
+
 // The parts of K added in order, eight requested at a time.
 template <class T>
 __global__ __launch_bounds__(kThreads) void add_splits(const float* __restrict__ partials,
@@ -362,14 +561,39 @@ int launched(const char* what) {
   return err == hipSuccess ? NS_OK : fail_launch(what, err);
 }
 
-// How a product is cut: tiles of x's rows per workgroup, wavefronts that share a strip, and
-// parts of K that workgroups share, so that 2048 wavefronts or more stream codes.
+// How a product is cut: tiles of x's rows per workgroup (0: q4_rows), strips per wavefront,
+// wavefronts that share a strip, and parts of K that workgroups share, so that 2048 wavefronts or
+// more stream codes.
 struct Q4Plan {
   int tiles, strips;
   Q4Place place;
   int64_t groups;              // workgroups
 };
+
+Q4Plan rows_plan(int64_t n, int64_t k) {
+  Q4Plan plan{};
+  const int64_t stages = (k + kStage - 1) / kStage;
+  plan.strips = n > 16 * 256 ? 2 : 1;
+  const int64_t strips = (n + 16 * plan.strips - 1) / (16 * plan.strips);
+  int64_t parts = 1;
+  while (parts < kQ4Waves && stages >= 4 * parts) parts *= 2;
+  const int64_t strip_groups = (strips * parts + kQ4Waves - 1) / kQ4Waves;
+  int64_t splits = 1;
+  if (strip_groups < 128) {
+    splits = 512 / strip_groups;
+    splits = splits < stages / (4 * parts) ? splits : stages / (4 * parts);
+    splits = splits > 1 ? splits : 1;
+  }
+  const int64_t per = (stages + splits - 1) / splits;
+  splits = (stages + per - 1) / per;                       // no empty part
+  plan.groups = strip_groups * splits;
+  plan.place = Q4Place{1, static_cast<uint32_t>(strip_groups), static_cast<uint32_t>(splits),
+                       static_cast<uint32_t>(parts), 0, static_cast<uint32_t>(per)};
+  return plan;
+}
+
 Q4Plan q4_plan(int64_t m, int64_t n, int64_t k, int32_t type) {
+  if (type != NS_TYPE_F32 && m <= 16) return rows_plan(n, k);
   Q4Plan plan{};
   const int64_t per_tile = type == NS_TYPE_F32 ? 4 : 16, tiles = (m + per_tile - 1) / per_tile;
   plan.tiles = tiles <= 1 ? 1 : tiles <= 2 ? 2 : 4;
@@ -400,13 +624,24 @@ int run_tile(const ns_q4_product_args* a, const Q4Plan& plan, hipStream_t stream
   return launched("4-bit product");
 }
 
+template <class T, int kNG, int kS>
+int run_rows(const ns_q4_product_args* a, const Q4Plan& plan, hipStream_t stream) {
+  q4_rows<T, kNG, kS><<<dim3(static_cast<unsigned>(plan.groups)), dim3(kQ4Threads), 0, stream>>>(
+      q4_view(a->weight), plan.place, static_cast<const T*>(a->x), a->x_stride, a->rows, a->bias,
+      static_cast<T*>(a->out), a->stride, a->workspace);
+  return launched("4-bit product");
+}
+
 template <class T, int kNG>
 int run_groups(const ns_q4_product_args* a, const Q4Plan& plan, hipStream_t stream) {
-  switch (plan.tiles) {
-    case 1: return run_tile<Q4Tile<1, 1, kNG>, T>(a, plan, stream);
-    case 2: return run_tile<Q4Tile<2, 2, kNG>, T>(a, plan, stream);
-    default: return run_tile<Q4Tile<4, 2, kNG>, T>(a, plan, stream);
+  if constexpr (sizeof(T) == 2) {
+    if (plan.tiles == 0)
+      return plan.strips == 1 ? run_rows<T, kNG, 1>(a, plan, stream) : run_rows<T, kNG, 2>(a, plan, stream);
+  } else {
+    if (plan.tiles == 1) return run_tile<Q4Tile<1, 1, kNG>, T>(a, plan, stream);
   }
+  if (plan.tiles == 2) return run_tile<Q4Tile<2, 2, kNG>, T>(a, plan, stream);
+  return run_tile<Q4Tile<4, 2, kNG>, T>(a, plan, stream);
 }
 
 template <class T>

@@ -225,7 +225,7 @@ __global__ __launch_bounds__(kGradThreads) void recur_backward(RecurShape s, Rec
     meet[turn][wave][lane] = mine;
     __syncthreads();
     float behind[V];
-#pragma unroll
+#pragma unroll 4
     for (int w = kWaves - 1; w >= 0; --w) {
       const TwoWays<V> other = meet[turn][w][lane];
 #pragma unroll
@@ -318,12 +318,12 @@ int run_backward(const ns_recurrence_args* a, hipStream_t stream) {
   return sum_partials(a->partials, s.chunks * s.batch, s.channels, a->drates, stream);
 }
 
+// One channel a lane: two of them, with half the ticks, do not fit the 128 registers that 16
+// wavefronts leave (2048 x 8 x 4096 in bf16 with its forward 1632 us; with one 495; with 8
+// wavefronts of 8 ticks each 544 to 573).
 template <class T>
 int run(const ns_recurrence_args* a, hipStream_t stream) {
-  const bool wide = recur_lane_channels(a) == 2;
-  if (a->z.data)
-    return wide ? run_backward<T, 2, true>(a, stream) : run_backward<T, 1, true>(a, stream);
-  return wide ? run_backward<T, 2, false>(a, stream) : run_backward<T, 1, false>(a, stream);
+  return a->z.data ? run_backward<T, 1, true>(a, stream) : run_backward<T, 1, false>(a, stream);
 }
 
 }  // namespace
