@@ -18,7 +18,7 @@ struct HalfTile {
 };
 
 template <class G, class T>
-__global__ __launch_bounds__(G::threads) void gated_tiles(Rows x, Rows gate, Rows up, uint32_t pieces,
+__global__ __launch_bounds__(G::threads, 512 / G::threads) void gated_tiles(Rows x, Rows gate, Rows up, uint32_t pieces,
                                                           int activation, T* y, int64_t stride,
                                                           float* pre, uint32_t tiles_m,
                                                           uint32_t tiles_n) {
@@ -29,7 +29,7 @@ __global__ __launch_bounds__(G::threads) void gated_tiles(Rows x, Rows gate, Row
     Strip<H, float> kept;
   };
   __shared__ union {
-    v4i stages[2 * G::rows * 8];
+    v4i stages[G::stages * G::rows * 8];
     OwnStrips strips[G::WM * G::WN];
   } lds;
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
@@ -212,7 +212,9 @@ int run(const ns_gated_args* a, hipStream_t stream) {
   }
   const auto pieces = static_cast<uint32_t>(pieces_of(a->columns, a->type));
   switch (gemm_size(a->rows, 2 * a->width, a->type)) {
-    case GemmSize::kLarge: return run_tiles<LargeGemm, T>(a, x, gate, up, pieces, stream);
+    case GemmSize::kLarge:
+      if constexpr (sizeof(T) == 2) return run_tiles<LargeGemm, T>(a, x, gate, up, pieces, stream);
+      [[fallthrough]];
     case GemmSize::kMiddle: return run_tiles<MiddleGemm, T>(a, x, gate, up, pieces, stream);
     default: return run_tiles<SmallGemm, T>(a, x, gate, up, pieces, stream);
   }

@@ -32,26 +32,60 @@ __global__ __launch_bounds__(kThreads) void pack_kernel(const T* from, int64_t s
   store_pack<T, kValues>(to + id * kValues, v);
 }
 
+// A square of values on its way from rows to columns: both ways in 16-byte pieces, eight (of
+// float32 sixteen) lanes to a line.
+template <class T>
+struct Square {
+  static constexpr int V = 16 / sizeof(T), lanes = kSide / V, lines = kThreads / lanes;
+  T at[kSide][kSide + 4 / sizeof(T)];
+};
+
+// Stores columns c0 .. of the square, of which `columns` exist, as rows of `to` from r0 on, up to
+// `filled`, whole pieces.
+template <class T>
+__device__ __forceinline__ void store_turned(const Square<T>& square, T* to, int64_t stride, int64_t r0,
+                                             int64_t filled, int64_t c0, int64_t columns) {
+  using S = Square<T>;
+  const int r = threadIdx.x % S::lanes * S::V;
+#pragma unroll
+  for (int k = 0; k < kSide; k += S::lines) {
+    const int c = k + threadIdx.x / S::lanes;
+    if (r0 + r >= filled || c0 + c >= columns) continue;
+    Pack<T, S::V> v;
+#pragma unroll
+    for (int j = 0; j < S::V; ++j) v.v[j] = square.at[r + j][c];
+    store_pack<T, S::V>(to + (c0 + c) * stride + r0 + r, v);
+  }
+}
+
 // to[c][r] = from[r][c] for r < rows, c < columns, and zeros for rows <= r < filled.
 template <class T>
 __global__ __launch_bounds__(kThreads) void transpose_kernel(const T* from, int64_t stride, int64_t rows,
                                                              int64_t columns, int64_t filled, T* to,
                                                              int64_t to_stride, uint32_t tiles_c) {
-  __shared__ T tile[kSide][kSide + 4 / sizeof(T)];
+  using S = Square<T>;
+  __shared__ S square;
   const uint32_t tile_r = uniform(blockIdx.x / tiles_c), tile_c = blockIdx.x - tile_r * tiles_c;
   const int64_t r0 = static_cast<int64_t>(tile_r) * kSide, c0 = static_cast<int64_t>(tile_c) * kSide;
-  const int side = threadIdx.x % kSide, line = threadIdx.x / kSide;
+  const int side = threadIdx.x % S::lanes * S::V;
 #pragma unroll
-  for (int k = 0; k < kSide; k += kThreads / kSide) {
-    const int64_t r = r0 + line + k, c = c0 + side;
-    tile[line + k][side] = r < rows && c < columns ? from[r * stride + c] : T{};
+  for (int k = 0; k < kSide; k += S::lines) {
+    const int line = k + threadIdx.x / S::lanes;
+    const int64_t r = r0 + line, left = columns - c0 - side;
+    const T* const in = from + r * stride + c0 + side;
+    Pack<T, S::V> v{};
+    if (r < rows && left >= S::V) {
+      v = load_pack<T, S::V>(in);
+    } else if (r < rows) {
+#pragma unroll
+      for (int j = 0; j < S::V; ++j)
+        if (j < left) v.v[j] = in[j];
+    }
+#pragma unroll
+    for (int j = 0; j < S::V; ++j) square.at[line][side + j] = v.v[j];
   }
   __syncthreads();
-#pragma unroll
-  for (int k = 0; k < kSide; k += kThreads / kSide) {
-    const int64_t r = r0 + side, c = c0 + line + k;
-    if (r < filled && c < columns) to[c * to_stride + r] = tile[side][line + k];
-  }
+  store_turned<T>(square, to, to_stride, r0, filled, c0, columns);
 }
 
 // dg and du: as rows [M][2 F'], du behind dg, and as columns [2 F][M'], each padded with zeros to
@@ -61,48 +95,59 @@ __global__ __launch_bounds__(kThreads) void gate_gradients(const float* pre, con
                                                            int64_t rows, int64_t width, int activation,
                                                            T* by_row, int64_t row_half, T* by_column,
                                                            int64_t filled, uint32_t tiles_f) {
-  __shared__ T tile[2][kSide][kSide + 4 / sizeof(T)];
+  using S = Square<T>;
+  __shared__ S square[2];
   const uint32_t tile_m = uniform(blockIdx.x / tiles_f), tile_f = blockIdx.x - tile_m * tiles_f;
   const int64_t m0 = static_cast<int64_t>(tile_m) * kSide, f0 = static_cast<int64_t>(tile_f) * kSide;
-  const int side = threadIdx.x % kSide, line = threadIdx.x / kSide;
-  const int64_t plane = rows * width;
+  const int side = threadIdx.x % S::lanes * S::V;
+  const int64_t plane = rows * width, f = f0 + side, left = width - f;
 #pragma unroll
-  for (int k = 0; k < kSide; k += kThreads / kSide) {
-    const int64_t m = m0 + line + k, f = f0 + side;
-    float dg = 0.0f, du = 0.0f;
-    if (m < rows && f < width) {
-      const float up = static_cast<float>(dy[m * dy_stride + f]);
-      const Activation a = activated_slope(pre[m * width + f], activation);
-      dg = up * pre[plane + m * width + f] * a.slope;
-      du = up * a.value;
+  for (int k = 0; k < kSide; k += S::lines) {
+    const int line = k + threadIdx.x / S::lanes;
+    const int64_t m = m0 + line;
+    Pack<float, S::V> gate{}, raised{};
+    Pack<T, S::V> up{}, g, u;
+    if (m < rows && left >= S::V) {
+      gate = load_pack<float, S::V>(pre + m * width + f);
+      raised = load_pack<float, S::V>(pre + plane + m * width + f);
+      up = load_pack<T, S::V>(dy + m * dy_stride + f);
+    } else if (m < rows) {
+#pragma unroll
+      for (int j = 0; j < S::V; ++j) {
+        if (j >= left) continue;
+        gate.v[j] = pre[m * width + f + j];
+        raised.v[j] = pre[plane + m * width + f + j];
+        up.v[j] = dy[m * dy_stride + f + j];
+      }
     }
-    const T g = static_cast<T>(dg), u = static_cast<T>(du);
-    tile[0][line + k][side] = g;
-    tile[1][line + k][side] = u;
+#pragma unroll
+    for (int j = 0; j < S::V; ++j) {
+      // Zeros where there is nothing: rows and columns of padding stay zero.
+      const Activation a = activated_slope(gate.v[j], activation);
+      const float own = static_cast<float>(up.v[j]);
+      g.v[j] = static_cast<T>(own * raised.v[j] * a.slope);
+      u.v[j] = static_cast<T>(own * a.value);
+      square[0].at[line][side + j] = g.v[j];
+      square[1].at[line][side + j] = u.v[j];
+    }
     if (by_row && m < rows && f < row_half) {
-      by_row[m * 2 * row_half + f] = g;
-      by_row[m * 2 * row_half + row_half + f] = u;
+      store_pack<T, S::V>(by_row + m * 2 * row_half + f, g);
+      store_pack<T, S::V>(by_row + m * 2 * row_half + row_half + f, u);
     }
   }
   if (!by_column) return;
   __syncthreads();
-#pragma unroll
-  for (int k = 0; k < kSide; k += kThreads / kSide) {
-    const int64_t m = m0 + side, f = f0 + line + k;
-    if (m < filled && f < width) {
-      by_column[f * filled + m] = tile[0][side][line + k];
-      by_column[(width + f) * filled + m] = tile[1][side][line + k];
-    }
-  }
+  store_turned<T>(square[0], by_column, filled, m0, filled, f0, width);
+  store_turned<T>(square[1], by_column + width * filled, filled, m0, filled, f0, width);
 }
 
 // out = a b^T, one workgroup per tile.
 template <class G, class T>
-__global__ __launch_bounds__(G::threads) void gemm_tiles(Rows a, Rows b, uint32_t pieces, T* out,
+__global__ __launch_bounds__(G::threads, 512 / G::threads) void gemm_tiles(Rows a, Rows b, uint32_t pieces, T* out,
                                                          int64_t stride, uint32_t tiles_m,
                                                          uint32_t tiles_n) {
   __shared__ union {
-    v4i stages[2 * G::rows * 8];
+    v4i stages[G::stages * G::rows * 8];
     Strip<G, T> strip[G::WM * G::WN];
   } lds;
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
@@ -164,7 +209,9 @@ template <class T>
 int product(const Rows& a, const Rows& b, int64_t pieces, int32_t type, T* out, int64_t stride,
             hipStream_t stream) {
   switch (gemm_size(a.rows, b.rows, type)) {
-    case GemmSize::kLarge: return product_of<LargeGemm, T>(a, b, pieces, out, stride, stream);
+    case GemmSize::kLarge:
+      if constexpr (sizeof(T) == 2) return product_of<LargeGemm, T>(a, b, pieces, out, stride, stream);
+      [[fallthrough]];
     case GemmSize::kMiddle: return product_of<MiddleGemm, T>(a, b, pieces, out, stride, stream);
     default: return product_of<SmallGemm, T>(a, b, pieces, out, stride, stream);
   }
@@ -250,11 +297,27 @@ int pack_rows(Rows* rows, const void* data, int64_t stride, int64_t columns, int
                              : run_pack<_Float16>(rows, data, stride, columns, pieces, to, stream);
 }
 
-// Tiles as large as still give most of the card's 256 compute units one.
+// The size whose rounds of tiles over the 256 compute units take the least time.  In units of 0.1
+// us for 32 stages (2048 columns of 16 bits): a round of large tiles 45 to 51 us; of middle ones
+// 16.2 with two on a compute unit and 24 alone; of small ones 6.2 where there are many, 22 with
+// two on a compute unit and 14 alone, where a stage's way from memory to LDS takes longer than its
+// products.  float32 multiplies at a sixteenth of the rate, so tiles alone count: 60 and 15.7, and
+// large ones gain nothing.  us, small / middle / large, of M x K to F in bf16: 64 x 4096 to 8192
+// 28.8 / 58.8 / 91; 256 x 1024 to 4096 9.9 / 13.2 / 23.5; 512 x 4096 to 4096 50 / 41.8 / 72.6; 2048^3
+// 51 / 32.4 / 40.6; 3000 x 700 to 5000 89 / 68 / 61; 4096^3 406 / 259 / 205; in float32 3885 x 1031 to
+// 1500 248 / 233.
 GemmSize gemm_size(int64_t m, int64_t n, int32_t type) {
   const auto tiles = [=](int64_t side) { return (m + side - 1) / side * ((n + side - 1) / side); };
-  if (type != NS_TYPE_F32 && tiles(256) >= 192) return GemmSize::kLarge;
-  return tiles(128) >= 192 ? GemmSize::kMiddle : GemmSize::kSmall;
+  const auto rounds = [](int64_t count, int64_t at_once) { return (count + at_once - 1) / at_once; };
+  const int64_t few = tiles(64), some = tiles(128);
+  if (type == NS_TYPE_F32)
+    return 600 * rounds(some, 256) <= 157 * rounds(few, 256) ? GemmSize::kMiddle : GemmSize::kSmall;
+  const auto most = [](int64_t a, int64_t b) { return a > b ? a : b; };
+  const int64_t small = most(few <= 256 ? 140 : 220, 62 * rounds(few, 256));
+  const int64_t middle = most(240 * rounds(some, 512), 162 * rounds(some, 256));
+  const int64_t large = 450 * rounds(tiles(256), 256);
+  if (large <= middle && large <= small) return GemmSize::kLarge;
+  return middle <= small ? GemmSize::kMiddle : GemmSize::kSmall;
 }
 
 }  // namespace ns

@@ -40,10 +40,10 @@ struct Rows {
 };
 constexpr int64_t kMostStride = 1 << 23;   // a tile's rows are addressed in 31 bits
 
-// Geometry of a tile: WM x WN wavefronts, each MI x NJ results of 16x16.
-template <int kMI, int kNJ, int kWM, int kWN>
+// Geometry of a tile: WM x WN wavefronts, each MI x NJ results of 16x16; `stages` of them in LDS.
+template <int kMI, int kNJ, int kWM, int kWN, int kStages>
 struct GemmTile {
-  static constexpr int MI = kMI, NJ = kNJ, WM = kWM, WN = kWN;
+  static constexpr int MI = kMI, NJ = kNJ, WM = kWM, WN = kWN, stages = kStages;
   static constexpr int rows_m = 16 * MI * WM, rows_n = 16 * NJ * WN, rows = rows_m + rows_n;
   static constexpr int threads = 64 * WM * WN;
   static constexpr int loads = rows * 8 / threads;          // 16-byte pieces per thread and stage
@@ -173,9 +173,9 @@ __device__ __forceinline__ void gemm_columns(GemmFragments<G>& f, const GemmBase
     gemm_columns<G, T, kPair, kAsk, J + 1>(f, from, next, p, b, at, to, sum);
 }
 
-// The sums of a workgroup's tile over pieces [0, pieces) of its rows.  `stages` is the LDS of two
-// stages.  While a stage's second step is multiplied, the first of the next one is read, and
-// the stage after that is requested into the place that all have read to its end: one barrier a
+// The sums of a workgroup's tile over pieces [0, pieces) of its rows.  `stages` is the LDS of
+// G::stages stages.  While a stage's second step is multiplied, the first of the next one is read,
+// and a stage to come is requested into the place that all have read to its end: one barrier a
 // stage, after its first step.
 template <class G, class T, bool kPair>
 __device__ __forceinline__ void gemm_tile(GemmPlace p, const Second<kPair>& b, v4i* stages,
@@ -187,22 +187,25 @@ __device__ __forceinline__ void gemm_tile(GemmPlace p, const Second<kPair>& b, v
   p.piece = (p.lane & 7) ^ turn(p.row);
   const int count = static_cast<int>(p.pieces + 7) / 8;
   GemmFragments<G> even, odd;
-  request_stage<G, kPair>(p, b, p.piece, lds);
-  request_stage<G, kPair>(p, b, p.piece + 8, lds + kStage);
-  wait_barrier<wait_loads(G::loads)>();
+#pragma unroll
+  for (int k = 0; k < G::stages; ++k) request_stage<G, kPair>(p, b, p.piece + 8 * k, lds + k * kStage);
+  wait_barrier<wait_loads((G::stages - 1) * G::loads)>();
   const GemmBase begin = gemm_base<G>(lds, 0, wm, wn, p.lane);
 #pragma unroll
   for (int i = 0; i < G::MI; ++i) even.a[i] = read_code(begin.a, i);
 #pragma unroll
   for (int j = 0; j < G::NJ; ++j) even.b[j] = read_code(begin.b, j);
   // Stages past the last read as zeros and are not multiplied.
+  uint32_t now = lds;
   for (int stage = 0; stage < count; ++stage) {
-    const uint32_t now = lds + (stage & 1 ? kStage : 0), then = lds + (stage & 1 ? 0 : kStage);
+    const uint32_t then = now + kStage < lds + G::stages * kStage ? now + kStage : lds;
     gemm_columns<G, T, kPair, false>(even, gemm_base<G>(now, 1, wm, wn, p.lane), odd, p, b, 0, 0, sum);
-    // This stage is read by all, and the next one has arrived for all.
-    wait_barrier<0>();
+    // This stage is read by all, and the next one has arrived for all; those behind it may be on
+    // their way.
+    wait_barrier<wait_loads_and_lds((G::stages - 2) * G::loads)>();
     gemm_columns<G, T, kPair, true>(odd, gemm_base<G>(then, 0, wm, wn, p.lane), even, p, b,
-                                    p.piece + 8 * (stage + 2), now, sum);
+                                    p.piece + 8 * (stage + G::stages), now, sum);
+    now = then;
   }
   wait_barrier<0>();                                       // before LDS is used anew
 }

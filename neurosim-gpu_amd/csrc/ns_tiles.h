@@ -55,6 +55,8 @@ __device__ __forceinline__ void wait_all() { __builtin_amdgcn_s_waitcnt(0); }
 
 // s_waitcnt: vmcnt in bits 0-3 and 14-15, expcnt 4-6, lgkmcnt 8-11.
 constexpr int wait_loads(int n) { return (n & 15) | (n >> 4) << 14 | 7 << 4 | 15 << 8; }
+// The same, and all of LDS's answers.
+constexpr int wait_loads_and_lds(int n) { return (n & 15) | (n >> 4) << 14 | 7 << 4; }
 template <int kWait>
 __device__ __forceinline__ void wait_barrier() {
   asm volatile("" ::: "memory");

@@ -22,7 +22,7 @@ namespace {
 
 constexpr int kQ4Waves = 8, kQ4Threads = 64 * kQ4Waves;
 constexpr int kStage = 128;                    // columns a wavefront takes at a time
-constexpr int kRing = 4;                       // stages requested ahead
+constexpr int kRing = 1;                       // stages requested ahead
 
 // Rows of x that 16 rows of the instruction hold.
 template <class T>
@@ -406,7 +406,7 @@ __global__ __launch_bounds__(kQ4Threads) void q4_product(Q4View w, Q4Place p, co
 // Up to 16 rows of 16 bits go from memory to registers: a workgroup's wavefronts share S strips
 // and take their stages in turn, so each reads its own part of x, without LDS or barriers but
 // for the sums at the end.
-constexpr int kRowRing = 3;
+constexpr int kRowRing = 2;
 
 template <int NG, int S>
 struct Q4RowStage {
