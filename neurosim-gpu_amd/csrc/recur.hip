@@ -266,21 +266,34 @@ int run_types(const ns_recurrence_args* a, bool step, void* stream) {
   return run<_Float16>(a, step, queue);
 }
 
-// Time chunks worth walking side by side: enough to fill the card, two tiles each at least.
+int64_t recur_blocks(const ns_recurrence_args* a, int lane_channels) {
+  return (a->channels + 64 * lane_channels - 1) / (64 * lane_channels);
+}
+
+// Time chunks worth walking side by side: enough to fill the card, two tiles each at least.  Bf16,
+// us, in one chunk and in chunks: T=2000, B=4, N=4096 (256 workgroups) 89 / 122; T=200, B=4, N=600
+// (40 workgroups, 4 tiles) 13.6 / 20.6.
 int64_t worth_recur_chunks(const ns_recurrence_args* a) {
   if (a->ticks <= 0 || a->batch <= 0) return 1;
-  const int64_t wide = 64 * recur_lane_channels(a);
-  const int64_t blocks = (a->channels + wide - 1) / wide * a->batch;
+  const int64_t blocks = recur_blocks(a, recur_lane_channels(a)) * a->batch;
   const int64_t tiles = (a->ticks + kRecurTile - 1) / kRecurTile;
-  if (blocks >= 256) return 1;
+  if (blocks >= 192 || tiles < 12) return 1;
   const int64_t chunks = 1024 / blocks < tiles / 2 ? 1024 / blocks : tiles / 2;
   return chunks < 2 ? 1 : chunks;
 }
 
 }  // namespace
 
+// Two channels of 16 bits to a lane where workgroups are many all the same, or where time is cut
+// into chunks and there is enough of it for the wider loads to count.  Us, with one and with two:
+// T=16384, B=1, N=2048 150 / 126; T=4096, B=4, N=1024 81 / 70; but T=2000, B=1, N=600 16.6 / 22.4, T=16000,
+// B=1, N=100 18.4 / 24.5, T=2000, B=4, N=4096 in one chunk 89 and in chunks of two 122.
 int recur_lane_channels(const ns_recurrence_args* a) {
-  return a->type != NS_TYPE_F32 && a->channels > 1 ? 2 : 1;
+  if (a->type == NS_TYPE_F32 || a->channels < 2) return 1;
+  if (recur_blocks(a, 2) * a->batch >= 256) return 2;
+  if (recur_blocks(a, 1) * a->batch >= 192) return 1;
+  constexpr int64_t kMany = 1 << 23;
+  return a->batch > 0 && a->ticks * a->channels >= (kMany + a->batch - 1) / a->batch ? 2 : 1;
 }
 
 RecurShape recur_shape(const ns_recurrence_args* a, int lane_channels) {
@@ -288,7 +301,7 @@ RecurShape recur_shape(const ns_recurrence_args* a, int lane_channels) {
   s.ticks = a->ticks;
   s.batch = a->batch;
   s.channels = a->channels;
-  s.blocks = (a->channels + 64 * lane_channels - 1) / (64 * lane_channels);
+  s.blocks = recur_blocks(a, lane_channels);
   const int64_t tiles = (a->ticks + kRecurTile - 1) / kRecurTile;
   const int64_t wanted = a->chunks > 1 ? a->chunks : 1;
   const int64_t per = tiles > 0 ? (tiles + wanted - 1) / wanted : 1;

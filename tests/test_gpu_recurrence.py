@@ -26,7 +26,8 @@ TYPES = [torch.float32, torch.bfloat16, torch.float16]
 NAMES = ("x", "forget", "write", "rates", "z", "state")
 SHAPES = [  # T, B, N
     (1, 1, 1), (1, 3, 2), (7, 2, 1), (63, 1, 129), (64, 2, 65), (65, 3, 33), (130, 2, 257),
-    (128, 5, 64), (300, 1, 40), (513, 2, 130), (9, 16, 3),
+    (128, 5, 64), (300, 1, 40), (513, 2, 130), (9, 16, 3), (512, 1, 9), (1030, 1, 17),
+    (70, 256, 3), (130, 90, 257), (64, 256, 1), (5, 300, 2), (200, 256, 2),
 ]
 
 
@@ -65,11 +66,56 @@ def test_signals_and_gradients(gpu, shape, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-def test_many_chunks(gpu, dtype):
-    """A long signal of few channels: more chunks than a workgroup has wavefronts."""
+@pytest.mark.parametrize("shape", [(2500, 1, 37), (800, 2, 130), (2050, 1, 4200)])
+def test_chunks(gpu, shape, dtype):
+    """Long signals of few channels, whose time is cut into chunks, the last with two channels of
+    16 bits to a lane."""
     draw = Draw(gpu, 3)
-    T, B, N = 2500, 1, 37
+    T, B, N = shape
     check(operands(draw, T, B, N, dtype), None, draw(T, B, N, dtype=dtype), draw(B, N))
+
+
+@pytest.mark.parametrize("lengths", [None, [17500, 16384, 9001]])
+def test_more_chunks_than_wavefronts(gpu, lengths):
+    """Many chunks.  Rates of 0.5 at least and gates of sigmoid(-1) at least let a channel
+    forget by exp(-0.13) a tick, so terms older than 300 ticks, below exp(-40) of the others,
+    count for nothing, and the bounds are those of 300 ticks."""
+    draw = Draw(gpu, 13)
+    T, B, N = 17500, 3, 2                        # 136 chunks
+    values = operands(draw, T, B, N, torch.float32)
+    values["rates"] = values["rates"].clamp(min=0.5)
+    values["forget"] = values["forget"].clamp(min=-1)
+    lengths = None if lengths is None else torch.tensor(lengths, device=gpu)
+    dy, dfinal = draw(T, B, N), draw(B, N)
+    inputs = leaves(values)
+    y, final = gated_recurrence(**inputs, lengths=lengths)
+    kw = dict(lengths=lengths, dy=dy, dfinal=dfinal)
+    want, grads = bo.recurrence(**values, **kw)
+    size, grad_size = bo.recurrence(**values, **kw, magnitude=True)
+    close(y, want["y"], size["y"], 30 * 300 + 50, "y")
+    close(final, want["state"], size["state"], 30 * 300 + 35, "state")
+    for name, value in gradients((y, final), inputs, (dy, dfinal)).items():
+        summands = T * B if name == "rates" else 2
+        # dstate has passed every tick of its column.
+        passed = 60 * T if name == "state" else 60 * 300
+        close(value, grads[name], grad_size[name], passed + 150 + summands, f"d{name}")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_lengths_of_many_columns(gpu, dtype):
+    """Many columns, each walked by workgroups of its own in one chunk."""
+    draw = Draw(gpu, 15)
+    T, B, N = 140, 256, 3
+    values = operands(draw, T, B, N, dtype)
+    lengths = torch.randint(0, T + 1, (B,), generator=draw.g, dtype=torch.int32).to(gpu)
+    lengths[:6] = torch.tensor([0, 1, 63, 64, 65, T], dtype=torch.int32)
+    dy = draw(T, B, N, dtype=dtype)
+    past = torch.arange(T, device=gpu)[:, None] >= lengths
+    for v in (values["x"], values["forget"], values["write"], values["z"], dy):
+        v[past] = float("nan")
+    y, _, got = check(values, lengths, dy, draw(B, N))
+    for value in (y, *(got[k] for k in ("x", "forget", "write", "z"))):
+        assert not value[past].any()
 
 
 @pytest.mark.parametrize("kind", [torch.int32, torch.int64])
