@@ -270,15 +270,15 @@ int64_t recur_blocks(const ns_recurrence_args* a, int lane_channels) {
   return (a->channels + 64 * lane_channels - 1) / (64 * lane_channels);
 }
 
-// Time chunks worth walking side by side: enough to fill the card, two tiles each at least.  Bf16,
+// Time chunks worth walking side by side: enough to fill the card, four tiles each at least.  Bf16,
 // us, in one chunk and in chunks: T=2000, B=4, N=4096 (256 workgroups) 89 / 122; T=200, B=4, N=600
-// (40 workgroups, 4 tiles) 13.6 / 20.6.
+// (40 workgroups) 13.6 / 20.6 (both with tiles of 64 ticks).
 int64_t worth_recur_chunks(const ns_recurrence_args* a) {
   if (a->ticks <= 0 || a->batch <= 0) return 1;
   const int64_t blocks = recur_blocks(a, recur_lane_channels(a)) * a->batch;
   const int64_t tiles = (a->ticks + kRecurTile - 1) / kRecurTile;
-  if (blocks >= 192 || tiles < 12) return 1;
-  const int64_t chunks = 1024 / blocks < tiles / 2 ? 1024 / blocks : tiles / 2;
+  if (blocks >= 192 || tiles < 24) return 1;
+  const int64_t chunks = 1024 / blocks < tiles / 4 ? 1024 / blocks : tiles / 4;
   return chunks < 2 ? 1 : chunks;
 }
 

@@ -13,7 +13,7 @@
 namespace ns {
 namespace {
 
-constexpr int kWaves = 16, kRun = kRecurTile / kWaves;
+constexpr int kWaves = 8, kRun = kRecurTile / kWaves;
 constexpr int kGradThreads = 64 * kWaves;
 
 template <class T, int V>
@@ -318,9 +318,8 @@ int run_backward(const ns_recurrence_args* a, hipStream_t stream) {
   return sum_partials(a->partials, s.chunks * s.batch, s.channels, a->drates, stream);
 }
 
-// One channel a lane: two of them, with half the ticks, do not fit the 128 registers that 16
-// wavefronts leave (2048 x 8 x 4096 in bf16 with its forward 1632 us; with one 495; with 8
-// wavefronts of 8 ticks each 544 to 573).
+// One channel a lane: two of them do not fit the 128 registers that leave a compute unit two
+// workgroups (2048 x 8 x 4096 in bf16 with its forward, on 16 wavefronts, 1632 us against 495).
 template <class T>
 int run(const ns_recurrence_args* a, hipStream_t stream) {
   return a->z.data ? run_backward<T, 1, true>(a, stream) : run_backward<T, 1, false>(a, stream);

@@ -67,23 +67,23 @@ def plan(lib, *shape):
 
 
 def test_recurrence_plans(lib):
-    """Tiles have 64 ticks.  Time is cut into chunks, of two whole tiles at least and none empty,
+    """Tiles have 32 ticks.  Time is cut into chunks, of four whole tiles at least and none empty,
     only where workgroups are few and tiles many."""
-    assert plan(lib, 2048, 8, 4096, 1) == (0, [1, 0, 32 * 8 * 4096, 8 * 4096])
+    assert plan(lib, 2048, 8, 4096, 1) == (0, [1, 0, 64 * 8 * 4096, 8 * 4096])
     for ticks, batch, n, type in ((16384, 1, 2048, 1), (200, 1, 5, 0), (64, 1, 5, 0), (9000, 3, 64, 0),
                                   (0, 2, 4, 0), (700, 0, 4, 0), (40000, 1, 3, 2), (1000, 192, 3, 0),
                                   (1000, 191, 3, 0), (1000, 128, 129, 1), (767, 1, 4, 0), (704, 1, 4, 0)):
         code, (chunks, ends, kept, parts) = plan(lib, ticks, batch, n, type)
-        tiles, lines = (ticks + 63) // 64, batch * n
-        assert code == 0 and 1 <= chunks <= max(1, tiles // 2)
-        if tiles < 12 or -(-n // 128) * batch >= 192:
+        tiles, lines = (ticks + 31) // 32, batch * n
+        assert code == 0 and 1 <= chunks <= max(1, tiles // 4)
+        if tiles < 24 or -(-n // 128) * batch >= 192:
             assert chunks == 1
         if chunks > 1:
             per = -(-tiles // chunks)
             assert (chunks - 1) * per < tiles
         assert ends == (2 * chunks * lines if chunks > 1 else 0)
         assert kept == tiles * lines and parts == chunks * lines
-    assert plan(lib, 16384, 1, 2048, 1)[1][0] > 16 and plan(lib, 767, 1, 4, 0)[1][0] == 6
+    assert plan(lib, 16384, 1, 2048, 1)[1][0] > 16 and plan(lib, 737, 1, 4, 0)[1][0] == 6
     for bad in ((-1, 1, 1, 0), (1, -1, 1, 0), (1, 1, 0, 0), (1, 1, 1, 9), (1 << 31, 1, 1, 0)):
         assert plan(lib, *bad)[0] != 0, bad
 

@@ -25,7 +25,7 @@ pytestmark = pytest.mark.gpu
 TYPES = [torch.float32, torch.bfloat16, torch.float16]
 NAMES = ("x", "forget", "write", "rates", "z", "state")
 SHAPES = [  # T, B, N
-    (1, 1, 1), (1, 3, 2), (7, 2, 1), (63, 1, 129), (64, 2, 65), (65, 3, 33), (130, 2, 257),
+    (1, 1, 1), (1, 3, 2), (7, 2, 1), (31, 2, 5), (32, 1, 66), (33, 1, 3), (63, 1, 129), (64, 2, 65), (65, 3, 33), (130, 2, 257),
     (128, 5, 64), (300, 1, 40), (513, 2, 130), (9, 16, 3), (512, 1, 9), (1030, 1, 17),
     (70, 256, 3), (130, 90, 257), (64, 256, 1), (5, 300, 2), (200, 256, 2),
 ]
@@ -108,7 +108,7 @@ def test_lengths_of_many_columns(gpu, dtype):
     T, B, N = 140, 256, 3
     values = operands(draw, T, B, N, dtype)
     lengths = torch.randint(0, T + 1, (B,), generator=draw.g, dtype=torch.int32).to(gpu)
-    lengths[:6] = torch.tensor([0, 1, 63, 64, 65, T], dtype=torch.int32)
+    lengths[:6] = torch.tensor([0, 1, 31, 32, 33, T], dtype=torch.int32)
     dy = draw(T, B, N, dtype=dtype)
     past = torch.arange(T, device=gpu)[:, None] >= lengths
     for v in (values["x"], values["forget"], values["write"], values["z"], dy):
@@ -126,7 +126,7 @@ def test_lengths(gpu, kind, dtype):
     draw = Draw(gpu, 5)
     T, B, N = 700, 8, 21
     values = operands(draw, T, B, N, dtype)
-    lengths = torch.tensor([0, 1, 63, 64, 65, 333, T, T + 9], dtype=kind, device=gpu)
+    lengths = torch.tensor([0, 1, 31, 32, 65, 333, T, T + 9], dtype=kind, device=gpu)
     dy = draw(T, B, N, dtype=dtype)
     for b, end in enumerate(lengths.tolist()):
         for k in ("x", "forget", "write", "z"):
