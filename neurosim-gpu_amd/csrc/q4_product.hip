@@ -33,7 +33,7 @@ constexpr int kTileRows = sizeof(T) == 4 ? 4 : 16;
 template <int kCT, int kS, int kNG>
 struct Q4Tile {
   static constexpr int CT = kCT, S = kS, NG = kNG;
-  static constexpr int chunk = 2048 / CT;      // columns of x in LDS: 64 KiB
+  static constexpr int chunk = CT <= 2 ? 2048 / CT : 512;   // columns of x in LDS: 64 KiB at most
   static constexpr int stages = chunk / kStage, sub = kStage / NG;
 };
 
@@ -341,8 +341,13 @@ __global__ __launch_bounds__(kQ4Threads) void q4_product(Q4View w, Q4Place p, co
           }
         }
       }
-      // One group after the other: side by side they do not fit the registers.
-      __builtin_amdgcn_sched_barrier(0);
+      // Four groups one after the other: side by side they do not fit the registers.
+      if constexpr (G::NG == 4) {
+#pragma unroll
+        for (int s = 0; s < G::S; ++s)
+#pragma unroll
+          for (int t = 0; t < G::CT; ++t) asm volatile("" : "+v"(total[s][t]) :: "memory");
+      }
     }
   };
 
@@ -492,7 +497,9 @@ __global__ __launch_bounds__(kQ4Threads) void q4_rows(Q4View w, Q4Place p, const
 #pragma unroll
         for (int i = 0; i < 4; ++i) total[s][i] = fmaf(scale, fmaf(offset, taken[i], sum[s][i]), total[s][i]);
       }
-      __builtin_amdgcn_sched_barrier(0);
+      // One group after the other, in few registers.
+#pragma unroll
+      for (int s = 0; s < S; ++s) asm volatile("" : "+v"(total[s]) :: "memory");
     }
   };
 #pragma unroll
@@ -596,11 +603,15 @@ Q4Plan q4_plan(int64_t m, int64_t n, int64_t k, int32_t type) {
   if (type != NS_TYPE_F32 && m <= 16) return rows_plan(n, k);
   Q4Plan plan{};
   const int64_t per_tile = type == NS_TYPE_F32 ? 4 : 16, tiles = (m + per_tile - 1) / per_tile;
-  plan.tiles = tiles <= 1 ? 1 : tiles <= 2 ? 2 : 4;
-  plan.strips = plan.tiles == 1 ? 1 : 2;
+  plan.tiles = tiles <= 2 ? static_cast<int>(tiles) : tiles == 3 && type != NS_TYPE_F32 ? 3 : 4;
   const int64_t m_tiles = (tiles + plan.tiles - 1) / plan.tiles;
+  const int64_t columns = plan.tiles <= 2 ? 2048 / plan.tiles : 512, chunks = (k + columns - 1) / columns;
+  // Two strips a wavefront halve what is read of x from LDS for each, but also the wavefronts.  Us,
+  // one / two, bf16: 40 x 4096 to 4096 15.3 / 18.5, 32 x 2048 to 4096 13.8 / 16.2, 64 x 4096 to 8192 27.4 /
+  // 26.7, 33 x 50,000 to 1000 34 / 28; float32: 8 x 8192 to 4096 17.4 / 15.5, 20 x 4096 to 4096 18.4 / 17.6.
+  const bool few = type != NS_TYPE_F32 && m_tiles * ((n + 15) / 16) * chunks <= 2048;
+  plan.strips = plan.tiles == 1 || few ? 1 : 2;
   const int64_t strips = (n + 16 * plan.strips - 1) / (16 * plan.strips);
-  const int64_t columns = 2048 / plan.tiles, chunks = (k + columns - 1) / columns;
   int64_t parts = 1;
   while (parts * 2 <= 4 / plan.tiles && m_tiles * strips * parts < 2048) parts *= 2;
   const int64_t waves = m_tiles * strips * parts;
@@ -637,6 +648,12 @@ int run_groups(const ns_q4_product_args* a, const Q4Plan& plan, hipStream_t stre
   if constexpr (sizeof(T) == 2) {
     if (plan.tiles == 0)
       return plan.strips == 1 ? run_rows<T, kNG, 1>(a, plan, stream) : run_rows<T, kNG, 2>(a, plan, stream);
+    if (plan.tiles == 3)
+      return plan.strips == 1 ? run_tile<Q4Tile<3, 1, kNG>, T>(a, plan, stream)
+                              : run_tile<Q4Tile<3, 2, kNG>, T>(a, plan, stream);
+    if (plan.strips == 1)
+      return plan.tiles == 2 ? run_tile<Q4Tile<2, 1, kNG>, T>(a, plan, stream)
+                             : run_tile<Q4Tile<4, 1, kNG>, T>(a, plan, stream);
   } else {
     if (plan.tiles == 1) return run_tile<Q4Tile<1, 1, kNG>, T>(a, plan, stream);
   }
