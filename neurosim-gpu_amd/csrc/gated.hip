@@ -17,6 +17,36 @@ struct HalfTile {
   static constexpr int MI = G::MI, NJ = G::NJ / 2;
 };
 
+// A wavefront's results from row m, column f on, of `rows` x `width`: both products where they are
+// kept, and y.  The two strips may be one place: a wavefront uses them one after the other.
+template <class G, class T>
+__device__ __forceinline__ void store_gated(const v4f (&sum)[G::MI][G::NJ], int activation, T* y,
+                                            int64_t stride, float* pre, int64_t m, int64_t f, int64_t rows,
+                                            int64_t width, int lane, Strip<HalfTile<G>, T>& strip,
+                                            Strip<HalfTile<G>, float>& kept) {
+  using H = HalfTile<G>;
+  v4f part[H::MI][H::NJ];
+  if (pre) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+#pragma unroll
+      for (int i = 0; i < H::MI; ++i)
+#pragma unroll
+        for (int j = 0; j < H::NJ; ++j) part[i][j] = sum[i][j + half * H::NJ];
+      store_tiles<H, float, false>(pre + half * rows * width + m * width + f, width, part, nullptr, rows - m,
+                                   width - f, lane, kept);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < H::MI; ++i)
+#pragma unroll
+    for (int j = 0; j < H::NJ; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        part[i][j][r] = activated(sum[i][j][r], activation) * sum[i][j + H::NJ][r];
+  store_tiles<H, T, false>(y + m * stride + f, stride, part, nullptr, rows - m, width - f, lane, strip);
+}
+
 template <class G, class T>
 __global__ __launch_bounds__(G::threads, 512 / G::threads) void gated_tiles(Rows x, Rows gate, Rows up, uint32_t pieces,
                                                           int activation, T* y, int64_t stride,
@@ -49,29 +79,35 @@ __global__ __launch_bounds__(G::threads, 512 / G::threads) void gated_tiles(Rows
   gemm_tile<G, T, true>(p, b, lds.stages, sum);
 
   const int64_t m = m0 + 16 * (wave / G::WN) * G::MI, f = f0 + 16 * (wave % G::WN) * H::NJ;
-  const int64_t rows = x.rows - m, columns = gate.rows - f;
-  v4f part[H::MI][H::NJ];
-  if (pre) {
-    const int64_t plane = x.rows * gate.rows;
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-#pragma unroll
-      for (int i = 0; i < H::MI; ++i)
-#pragma unroll
-        for (int j = 0; j < H::NJ; ++j) part[i][j] = sum[i][j + half * H::NJ];
-      store_tiles<H, float, false>(pre + half * plane + m * gate.rows + f, gate.rows, part, nullptr,
-                                   rows, columns, lane, lds.strips[wave].kept);
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < H::MI; ++i)
-#pragma unroll
-    for (int j = 0; j < H::NJ; ++j)
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        part[i][j][r] = activated(sum[i][j][r], activation) * sum[i][j + H::NJ][r];
-  store_tiles<H, T, false>(y + m * stride + f, stride, part, nullptr, rows, columns, lane,
-                           lds.strips[wave].y);
+  store_gated<G, T>(sum, activation, y, stride, pre, m, f, x.rows, gate.rows, lane, lds.strips[wave].y,
+                    lds.strips[wave].kept);
+}
+
+// The same for float32 rows in thirds.
+template <class G>
+__global__ __launch_bounds__(G::threads) void gated_split(Rows x, Rows gate, Rows up, uint32_t blocks,
+                                                          int activation, float* y, int64_t stride,
+                                                          float* pre, uint32_t tiles_m, uint32_t tiles_n) {
+  using H = HalfTile<G>;
+  __shared__ union {
+    uint8_t stages[G::stages * G::stage_bytes];
+    Strip<H, float> strips[G::waves];
+    v4i aligned;
+  } lds;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const TilePlace tile = tile_place(tiles_m, tiles_n);
+  const int64_t m0 = static_cast<int64_t>(tile.m) * G::rows_m;
+  const int64_t f0 = static_cast<int64_t>(tile.n) * (G::rows_n / 2);
+  const uint32_t pieces = blocks * (kThirds / 16);
+  const SplitPlace<G> p = split_place<G, true>(
+      lane, wave, blocks, rows_buffer(x, m0, G::rows_m, pieces), static_cast<uint32_t>(x.stride),
+      rows_buffer(gate, f0, G::rows_n / 2, pieces), rows_buffer(up, f0, G::rows_n / 2, pieces),
+      static_cast<uint32_t>(gate.stride));
+  v4f sum[G::MI][G::NJ] = {};
+  split_tile<G>(p, lds.stages, sum);
+  const int64_t m = m0 + 16 * (wave / G::WN) * G::MI, f = f0 + 16 * (wave % G::WN) * H::NJ;
+  store_gated<G, float>(sum, activation, y, stride, pre, m, f, x.rows, gate.rows, lane, lds.strips[wave],
+                        lds.strips[wave]);
 }
 
 // Up to 16 rows of x: bound by the weights' bytes, each read once.  A workgroup takes 16
@@ -183,15 +219,38 @@ int run_rows(const ns_gated_args* a, hipStream_t stream) {
   return launched("gated projection");
 }
 
+template <class G>
+int tiles_of(const ns_gated_args* a, dim3* grid, uint32_t* tiles_m, uint32_t* tiles_n) {
+  const int64_t high = (a->rows + G::rows_m - 1) / G::rows_m;
+  const int64_t wide = (a->width + G::rows_n / 2 - 1) / (G::rows_n / 2);
+  if (high > INT32_MAX / 4 / wide) return fail("the projection is too large for one launch");
+  *grid = dim3(static_cast<unsigned>(high * wide));
+  *tiles_m = static_cast<uint32_t>(high);
+  *tiles_n = static_cast<uint32_t>(wide);
+  return NS_OK;
+}
+
 template <class G, class T>
-int run_tiles(const ns_gated_args* a, const Rows& x, const Rows& gate, const Rows& up, uint32_t pieces,
+int run_tiles(const ns_gated_args* a, const Rows& x, const Rows& gate, const Rows& up, int64_t pieces,
               hipStream_t stream) {
-  const int64_t tiles_m = (a->rows + G::rows_m - 1) / G::rows_m;
-  const int64_t tiles_n = (a->width + G::rows_n / 2 - 1) / (G::rows_n / 2);
-  if (tiles_m > INT32_MAX / 4 / tiles_n) return fail("the projection is too large for one launch");
-  gated_tiles<G, T><<<dim3(static_cast<unsigned>(tiles_m * tiles_n)), dim3(G::threads), 0, stream>>>(
-      x, gate, up, pieces, a->activation, static_cast<T*>(a->y), a->y_stride, a->pre,
-      static_cast<uint32_t>(tiles_m), static_cast<uint32_t>(tiles_n));
+  dim3 grid;
+  uint32_t tiles_m, tiles_n;
+  if (int rc = tiles_of<G>(a, &grid, &tiles_m, &tiles_n)) return rc;
+  gated_tiles<G, T><<<grid, dim3(G::threads), 0, stream>>>(
+      x, gate, up, static_cast<uint32_t>(pieces), a->activation, static_cast<T*>(a->y), a->y_stride, a->pre,
+      tiles_m, tiles_n);
+  return launched("gated projection");
+}
+
+template <class G>
+int run_split(const ns_gated_args* a, const Rows& x, const Rows& gate, const Rows& up, int64_t pieces,
+              hipStream_t stream) {
+  dim3 grid;
+  uint32_t tiles_m, tiles_n;
+  if (int rc = tiles_of<G>(a, &grid, &tiles_m, &tiles_n)) return rc;
+  gated_split<G><<<grid, dim3(G::threads), 0, stream>>>(
+      x, gate, up, static_cast<uint32_t>(pieces / (kThirds / 16)), a->activation, static_cast<float*>(a->y),
+      a->y_stride, a->pre, tiles_m, tiles_n);
   return launched("gated projection");
 }
 
@@ -200,24 +259,27 @@ int run(const ns_gated_args* a, hipStream_t stream) {
   if (few_rows(a)) return run_rows<T>(a, stream);
   const PackedForward w = packed_forward(a);
   auto* space = static_cast<uint8_t*>(a->workspace);
-  Rows x = plain_rows(a->x, a->x_stride, a->rows, a->columns, a->type);
-  Rows gate = plain_rows(a->gate, a->gate_stride, a->width, a->columns, a->type);
-  Rows up = plain_rows(a->up, a->up_stride, a->width, a->columns, a->type);
+  const int64_t k = a->columns;
+  Rows x = plain_rows(a->x, a->x_stride, a->rows, k, a->type);
+  Rows gate = plain_rows(a->gate, a->gate_stride, a->width, k, a->type);
+  Rows up = plain_rows(a->up, a->up_stride, a->width, k, a->type);
   if (w.pack_x)
-    if (int rc = pack_rows(&x, a->x, a->x_stride, a->columns, a->type, space + w.x, stream)) return rc;
+    if (int rc = pack_rows(&x, a->x, a->x_stride, k, a->type, w.thirds, space + w.x, stream)) return rc;
   if (w.pack_weights) {
-    if (int rc = pack_rows(&gate, a->gate, a->gate_stride, a->columns, a->type, space + w.gate, stream))
+    if (int rc = pack_rows(&gate, a->gate, a->gate_stride, k, a->type, w.thirds, space + w.gate, stream))
       return rc;
-    if (int rc = pack_rows(&up, a->up, a->up_stride, a->columns, a->type, space + w.up, stream)) return rc;
+    if (int rc = pack_rows(&up, a->up, a->up_stride, k, a->type, w.thirds, space + w.up, stream)) return rc;
   }
-  const auto pieces = static_cast<uint32_t>(pieces_of(a->columns, a->type));
-  switch (gemm_size(a->rows, 2 * a->width, a->type)) {
-    case GemmSize::kLarge:
-      if constexpr (sizeof(T) == 2) return run_tiles<LargeGemm, T>(a, x, gate, up, pieces, stream);
-      [[fallthrough]];
-    case GemmSize::kMiddle: return run_tiles<MiddleGemm, T>(a, x, gate, up, pieces, stream);
-    default: return run_tiles<SmallGemm, T>(a, x, gate, up, pieces, stream);
+  const GemmSize size = gemm_size(a->rows, 2 * a->width, a->type, w.thirds);
+  if constexpr (sizeof(T) == 4) {
+    if (w.thirds)
+      return size == GemmSize::kMiddle ? run_split<MiddleSplit>(a, x, gate, up, w.pieces, stream)
+                                       : run_split<SmallSplit>(a, x, gate, up, w.pieces, stream);
+  } else {
+    if (size == GemmSize::kLarge) return run_tiles<LargeGemm, T>(a, x, gate, up, w.pieces, stream);
   }
+  return size == GemmSize::kMiddle ? run_tiles<MiddleGemm, T>(a, x, gate, up, w.pieces, stream)
+                                   : run_tiles<SmallGemm, T>(a, x, gate, up, w.pieces, stream);
 }
 
 }  // namespace

@@ -3,9 +3,9 @@
 //   dg = dy u f'(g),  du = dy f(g)
 //   dx = [dg du] [gate; up],  [dgate; dup] = [dg du]^T x
 // The sums of dx run over columns of y, those of the weights over rows of x, and the tile
-// kernels read their operands along the sum.  So dg and du, rounded once, are written both
-// ways by the pass that computes them, and x and the weights are transposed first: passes
-// over memory that cost some tenth of the products.
+// kernels read their operands along the sum.  So dg and du, rounded once to the operands' type, are
+// written both ways by the pass that computes them, and x and the weights are transposed first:
+// passes over memory that cost some tenth of the products.
 #include "ns_gated.h"
 
 namespace ns {
@@ -32,88 +32,118 @@ __global__ __launch_bounds__(kThreads) void pack_kernel(const T* from, int64_t s
   store_pack<T, kValues>(to + id * kValues, v);
 }
 
-// A square of values on its way from rows to columns: both ways in 16-byte pieces, eight (of
-// float32 sixteen) lanes to a line.
+// float32 rows in thirds; a lane per eight columns.
+__global__ __launch_bounds__(kThreads) void thirds_kernel(const float* from, int64_t stride, int64_t rows,
+                                                          int64_t columns, uint32_t blocks, uint8_t* to) {
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x, lanes = 4 * blocks;
+  if (id >= rows * lanes) return;
+  const int64_t row = id / lanes, first = (id - row * lanes) * 8;
+  const float* const in = from + row * stride;
+  float v[8];
+  if (first + 8 <= columns) {
+    const Pack<float, 8> all = load_pack<float, 8>(in + first);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = all.v[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = first + j < columns ? in[first + j] : 0.0f;
+  }
+  store_thirds(to + row * blocks * kThirds, first, v);
+}
+
+// A square of values on its way from rows to columns: both ways eight values a lane, eight lanes to
+// a line.
+constexpr int kWide = 8, kSquareLanes = kSide / kWide, kLines = kThreads / kSquareLanes;
 template <class T>
 struct Square {
-  static constexpr int V = 16 / sizeof(T), lanes = kSide / V, lines = kThreads / lanes;
   T at[kSide][kSide + 4 / sizeof(T)];
 };
 
-// Stores columns c0 .. of the square, of which `columns` exist, as rows of `to` from r0 on, up to
-// `filled`, whole pieces.
+// Eight values from column k on (a multiple of 8) of a laid-out row that starts at `row`: in thirds
+// for float32.
 template <class T>
-__device__ __forceinline__ void store_turned(const Square<T>& square, T* to, int64_t stride, int64_t r0,
-                                             int64_t filled, int64_t c0, int64_t columns) {
-  using S = Square<T>;
-  const int r = threadIdx.x % S::lanes * S::V;
+__device__ __forceinline__ void store_laid(uint8_t* row, int64_t k, const Pack<T, kWide>& v) {
+  if constexpr (sizeof(T) == 4)
+    store_thirds(row, k, v.v);
+  else
+    *reinterpret_cast<v4i*>(row + 2 * k) = __builtin_bit_cast(v4i, v);
+}
+
+// Stores columns c0 .. of the square, of which `columns` exist, as laid-out rows of `to`, `stride`
+// bytes apart, from column r0 on, up to `filled`, whole pieces.
+template <class T>
+__device__ __forceinline__ void store_turned(const Square<T>& square, uint8_t* to, int64_t stride,
+                                             int64_t r0, int64_t filled, int64_t c0, int64_t columns) {
+  const int r = threadIdx.x % kSquareLanes * kWide;
 #pragma unroll
-  for (int k = 0; k < kSide; k += S::lines) {
-    const int c = k + threadIdx.x / S::lanes;
+  for (int k = 0; k < kSide; k += kLines) {
+    const int c = k + threadIdx.x / kSquareLanes;
     if (r0 + r >= filled || c0 + c >= columns) continue;
-    Pack<T, S::V> v;
+    Pack<T, kWide> v;
 #pragma unroll
-    for (int j = 0; j < S::V; ++j) v.v[j] = square.at[r + j][c];
-    store_pack<T, S::V>(to + (c0 + c) * stride + r0 + r, v);
+    for (int j = 0; j < kWide; ++j) v.v[j] = square.at[r + j][c];
+    store_laid<T>(to + (c0 + c) * stride, r0 + r, v);
   }
 }
 
-// to[c][r] = from[r][c] for r < rows, c < columns, and zeros for rows <= r < filled.
+// Laid-out rows of what are columns of `from`: value r of row c is from[r][c] for r < rows, zero for
+// rows <= r < filled; rows begin at `to`, `stride` bytes apart.
 template <class T>
-__global__ __launch_bounds__(kThreads) void transpose_kernel(const T* from, int64_t stride, int64_t rows,
-                                                             int64_t columns, int64_t filled, T* to,
-                                                             int64_t to_stride, uint32_t tiles_c) {
-  using S = Square<T>;
-  __shared__ S square;
+__global__ __launch_bounds__(kThreads) void transpose_kernel(const T* from, int64_t from_stride,
+                                                             int64_t rows, int64_t columns,
+                                                             int64_t filled, uint8_t* to, int64_t stride,
+                                                             uint32_t tiles_c) {
+  __shared__ Square<T> square;
   const uint32_t tile_r = uniform(blockIdx.x / tiles_c), tile_c = blockIdx.x - tile_r * tiles_c;
   const int64_t r0 = static_cast<int64_t>(tile_r) * kSide, c0 = static_cast<int64_t>(tile_c) * kSide;
-  const int side = threadIdx.x % S::lanes * S::V;
+  const int side = threadIdx.x % kSquareLanes * kWide;
 #pragma unroll
-  for (int k = 0; k < kSide; k += S::lines) {
-    const int line = k + threadIdx.x / S::lanes;
+  for (int k = 0; k < kSide; k += kLines) {
+    const int line = k + threadIdx.x / kSquareLanes;
     const int64_t r = r0 + line, left = columns - c0 - side;
-    const T* const in = from + r * stride + c0 + side;
-    Pack<T, S::V> v{};
-    if (r < rows && left >= S::V) {
-      v = load_pack<T, S::V>(in);
+    const T* const in = from + r * from_stride + c0 + side;
+    Pack<T, kWide> v{};
+    if (r < rows && left >= kWide) {
+      v = load_pack<T, kWide>(in);
     } else if (r < rows) {
 #pragma unroll
-      for (int j = 0; j < S::V; ++j)
+      for (int j = 0; j < kWide; ++j)
         if (j < left) v.v[j] = in[j];
     }
 #pragma unroll
-    for (int j = 0; j < S::V; ++j) square.at[line][side + j] = v.v[j];
+    for (int j = 0; j < kWide; ++j) square.at[line][side + j] = v.v[j];
   }
   __syncthreads();
-  store_turned<T>(square, to, to_stride, r0, filled, c0, columns);
+  store_turned<T>(square, to, stride, r0, filled, c0, columns);
 }
 
-// dg and du: as rows [M][2 F'], du behind dg, and as columns [2 F][M'], each padded with zeros to
-// whole pieces (F', M').
+// dg and du: as laid-out rows [M][2 F'], du behind dg, and as columns [2 F][M'], each padded with
+// zeros to whole pieces (F', M').
 template <class T>
 __global__ __launch_bounds__(kThreads) void gate_gradients(const float* pre, const T* dy, int64_t dy_stride,
                                                            int64_t rows, int64_t width, int activation,
-                                                           T* by_row, int64_t row_half, T* by_column,
-                                                           int64_t filled, uint32_t tiles_f) {
-  using S = Square<T>;
-  __shared__ S square[2];
+                                                           uint8_t* by_row, int64_t row_half,
+                                                           int64_t row_stride, uint8_t* by_column,
+                                                           int64_t filled, int64_t column_stride,
+                                                           uint32_t tiles_f) {
+  __shared__ Square<T> square[2];
   const uint32_t tile_m = uniform(blockIdx.x / tiles_f), tile_f = blockIdx.x - tile_m * tiles_f;
   const int64_t m0 = static_cast<int64_t>(tile_m) * kSide, f0 = static_cast<int64_t>(tile_f) * kSide;
-  const int side = threadIdx.x % S::lanes * S::V;
+  const int side = threadIdx.x % kSquareLanes * kWide;
   const int64_t plane = rows * width, f = f0 + side, left = width - f;
 #pragma unroll
-  for (int k = 0; k < kSide; k += S::lines) {
-    const int line = k + threadIdx.x / S::lanes;
+  for (int k = 0; k < kSide; k += kLines) {
+    const int line = k + threadIdx.x / kSquareLanes;
     const int64_t m = m0 + line;
-    Pack<float, S::V> gate{}, raised{};
-    Pack<T, S::V> up{}, g, u;
-    if (m < rows && left >= S::V) {
-      gate = load_pack<float, S::V>(pre + m * width + f);
-      raised = load_pack<float, S::V>(pre + plane + m * width + f);
-      up = load_pack<T, S::V>(dy + m * dy_stride + f);
+    Pack<float, kWide> gate{}, raised{};
+    Pack<T, kWide> up{}, g, u;
+    if (m < rows && left >= kWide) {
+      gate = load_pack<float, kWide>(pre + m * width + f);
+      raised = load_pack<float, kWide>(pre + plane + m * width + f);
+      up = load_pack<T, kWide>(dy + m * dy_stride + f);
     } else if (m < rows) {
 #pragma unroll
-      for (int j = 0; j < S::V; ++j) {
+      for (int j = 0; j < kWide; ++j) {
         if (j >= left) continue;
         gate.v[j] = pre[m * width + f + j];
         raised.v[j] = pre[plane + m * width + f + j];
@@ -121,7 +151,7 @@ __global__ __launch_bounds__(kThreads) void gate_gradients(const float* pre, con
       }
     }
 #pragma unroll
-    for (int j = 0; j < S::V; ++j) {
+    for (int j = 0; j < kWide; ++j) {
       // Zeros where there is nothing: rows and columns of padding stay zero.
       const Activation a = activated_slope(gate.v[j], activation);
       const float own = static_cast<float>(up.v[j]);
@@ -131,14 +161,14 @@ __global__ __launch_bounds__(kThreads) void gate_gradients(const float* pre, con
       square[1].at[line][side + j] = u.v[j];
     }
     if (by_row && m < rows && f < row_half) {
-      store_pack<T, S::V>(by_row + m * 2 * row_half + f, g);
-      store_pack<T, S::V>(by_row + m * 2 * row_half + row_half + f, u);
+      store_laid<T>(by_row + m * row_stride, f, g);
+      store_laid<T>(by_row + m * row_stride, row_half + f, u);
     }
   }
   if (!by_column) return;
   __syncthreads();
-  store_turned<T>(square[0], by_column, filled, m0, filled, f0, width);
-  store_turned<T>(square[1], by_column + width * filled, filled, m0, filled, f0, width);
+  store_turned<T>(square[0], by_column, column_stride, m0, filled, f0, width);
+  store_turned<T>(square[1], by_column + width * column_stride, column_stride, m0, filled, f0, width);
 }
 
 // out = a b^T, one workgroup per tile.
@@ -169,6 +199,32 @@ __global__ __launch_bounds__(G::threads, 512 / G::threads) void gemm_tiles(Rows 
                            lds.strip[wave]);
 }
 
+// The same for float32 rows in thirds.
+template <class G>
+__global__ __launch_bounds__(G::threads) void split_tiles(Rows a, Rows b, uint32_t blocks, float* out,
+                                                          int64_t stride, uint32_t tiles_m,
+                                                          uint32_t tiles_n) {
+  __shared__ union {
+    uint8_t stages[G::stages * G::stage_bytes];
+    Strip<G, float> strip[G::waves];
+    v4i aligned;
+  } lds;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const TilePlace tile = tile_place(tiles_m, tiles_n);
+  const int64_t m0 = static_cast<int64_t>(tile.m) * G::rows_m;
+  const int64_t n0 = static_cast<int64_t>(tile.n) * G::rows_n;
+  const uint32_t pieces = blocks * (kThirds / 16);
+  const v4i second = rows_buffer(b, n0, G::rows_n, pieces);
+  const SplitPlace<G> p = split_place<G, false>(lane, wave, blocks, rows_buffer(a, m0, G::rows_m, pieces),
+                                                static_cast<uint32_t>(a.stride), second, second,
+                                                static_cast<uint32_t>(b.stride));
+  v4f sum[G::MI][G::NJ] = {};
+  split_tile<G>(p, lds.stages, sum);
+  const int64_t m = m0 + 16 * (wave / G::WN) * G::MI, n = n0 + 16 * (wave % G::WN) * G::NJ;
+  store_tiles<G, float, false>(out + m * stride + n, stride, sum, nullptr, a.rows - m, b.rows - n, lane,
+                               lds.strip[wave]);
+}
+
 int launched(const char* what) {
   const hipError_t err = hipGetLastError();
   return err == hipSuccess ? NS_OK : fail_launch(what, err);
@@ -182,13 +238,13 @@ int tile_grid(int64_t tiles_m, int64_t tiles_n, dim3* grid) {
 }
 
 template <class T>
-int transpose(const void* from, int64_t stride, int64_t rows, int64_t columns, int64_t filled, T* to,
-              int64_t to_stride, hipStream_t stream) {
+int transpose(const void* from, int64_t from_stride, int64_t rows, int64_t columns, int64_t filled,
+              uint8_t* to, int64_t stride, hipStream_t stream) {
   const int64_t tiles_r = (filled + kSide - 1) / kSide, tiles_c = (columns + kSide - 1) / kSide;
   dim3 grid;
   if (int rc = tile_grid(tiles_r, tiles_c, &grid)) return rc;
-  transpose_kernel<T><<<grid, dim3(kThreads), 0, stream>>>(static_cast<const T*>(from), stride, rows,
-                                                           columns, filled, to, to_stride,
+  transpose_kernel<T><<<grid, dim3(kThreads), 0, stream>>>(static_cast<const T*>(from), from_stride, rows,
+                                                           columns, filled, to, stride,
                                                            static_cast<uint32_t>(tiles_c));
   return launched("transposition");
 }
@@ -197,78 +253,87 @@ template <class G, class T>
 int product_of(const Rows& a, const Rows& b, int64_t pieces, T* out, int64_t stride, hipStream_t stream) {
   const int64_t tiles_m = (a.rows + G::rows_m - 1) / G::rows_m;
   const int64_t tiles_n = (b.rows + G::rows_n - 1) / G::rows_n;
+  const auto count_m = static_cast<uint32_t>(tiles_m), count_n = static_cast<uint32_t>(tiles_n);
   dim3 grid;
   if (int rc = tile_grid(tiles_m, tiles_n, &grid)) return rc;
-  gemm_tiles<G, T><<<grid, dim3(G::threads), 0, stream>>>(a, b, static_cast<uint32_t>(pieces), out,
-                                                          stride, static_cast<uint32_t>(tiles_m),
-                                                          static_cast<uint32_t>(tiles_n));
+  if constexpr (sizeof(T) == 4)
+    split_tiles<G><<<grid, dim3(G::threads), 0, stream>>>(
+        a, b, static_cast<uint32_t>(pieces / (kThirds / 16)), out, stride, count_m, count_n);
+  else
+    gemm_tiles<G, T><<<grid, dim3(G::threads), 0, stream>>>(a, b, static_cast<uint32_t>(pieces), out, stride,
+                                                            count_m, count_n);
   return launched("product");
 }
 
 template <class T>
 int product(const Rows& a, const Rows& b, int64_t pieces, int32_t type, T* out, int64_t stride,
             hipStream_t stream) {
-  switch (gemm_size(a.rows, b.rows, type)) {
-    case GemmSize::kLarge:
-      if constexpr (sizeof(T) == 2) return product_of<LargeGemm, T>(a, b, pieces, out, stride, stream);
-      [[fallthrough]];
-    case GemmSize::kMiddle: return product_of<MiddleGemm, T>(a, b, pieces, out, stride, stream);
-    default: return product_of<SmallGemm, T>(a, b, pieces, out, stride, stream);
+  const GemmSize size = gemm_size(a.rows, b.rows, type, sizeof(T) == 4);
+  if constexpr (sizeof(T) == 4) {
+    return size == GemmSize::kMiddle ? product_of<MiddleSplit, T>(a, b, pieces, out, stride, stream)
+                                     : product_of<SmallSplit, T>(a, b, pieces, out, stride, stream);
+  } else {
+    switch (size) {
+      case GemmSize::kLarge: return product_of<LargeGemm, T>(a, b, pieces, out, stride, stream);
+      case GemmSize::kMiddle: return product_of<MiddleGemm, T>(a, b, pieces, out, stride, stream);
+      default: return product_of<SmallGemm, T>(a, b, pieces, out, stride, stream);
+    }
   }
 }
 
-// The backward's workspace.
+// The backward's workspace: dg and du as laid-out rows of 2 F' values and as columns of M', the
+// weights transposed (rows of 2 F'), x transposed (rows of M').
 struct BackwardSpace {
   int64_t half, filled;                    // F' and M'
-  int64_t by_row, by_column, weights, x, bytes;
+  int64_t row_bytes, column_bytes;         // of rows of 2 F', and of M'
+  int64_t by_column, weights, x, bytes;
 };
 BackwardSpace backward_space(const ns_gated_args* a) {
   BackwardSpace w{};
-  const int64_t e = type_size(a->type);
-  w.half = whole_values(a->width, a->type);
-  w.filled = whole_values(a->rows, a->type);
-  w.by_column = a->dx ? a->rows * 2 * w.half * e : 0;
-  w.weights = w.by_column + (a->dweights ? 2 * a->width * w.filled * e : 0);
-  w.x = w.weights + (a->dx ? a->columns * 2 * w.half * e : 0);
-  w.bytes = w.x + (a->dweights ? a->columns * w.filled * e : 0);
+  const bool thirds = a->type == NS_TYPE_F32;
+  w.half = whole_values(a->width, thirds);
+  w.filled = whole_values(a->rows, thirds);
+  w.row_bytes = pieces_of(2 * w.half, a->type, thirds) * 16;
+  w.column_bytes = pieces_of(w.filled, a->type, thirds) * 16;
+  w.by_column = a->dx ? a->rows * w.row_bytes : 0;
+  w.weights = w.by_column + (a->dweights ? 2 * a->width * w.column_bytes : 0);
+  w.x = w.weights + (a->dx ? a->columns * w.row_bytes : 0);
+  w.bytes = w.x + (a->dweights ? a->columns * w.column_bytes : 0);
   return w;
 }
 
 template <class T>
 int run_backward(const ns_gated_args* a, hipStream_t stream) {
   const BackwardSpace w = backward_space(a);
-  auto* space = static_cast<uint8_t*>(a->workspace);
-  T* const by_row = a->dx ? reinterpret_cast<T*>(space + w.by_row) : nullptr;
-  T* const by_column = a->dweights ? reinterpret_cast<T*>(space + w.by_column) : nullptr;
-  T* const weights = reinterpret_cast<T*>(space + w.weights);
-  T* const x = reinterpret_cast<T*>(space + w.x);
-  const int64_t e = sizeof(T), tiles_m = (w.filled + kSide - 1) / kSide;
-  const int64_t tiles_f = (w.half + kSide - 1) / kSide;
+  auto* const space = static_cast<uint8_t*>(a->workspace);
+  uint8_t* const by_row = a->dx ? space : nullptr;
+  uint8_t* const by_column = a->dweights ? space + w.by_column : nullptr;
+  uint8_t* const weights = space + w.weights;
+  uint8_t* const x = space + w.x;
+  const int64_t tiles_m = (w.filled + kSide - 1) / kSide, tiles_f = (w.half + kSide - 1) / kSide;
   dim3 grid;
   if (int rc = tile_grid(tiles_m, tiles_f, &grid)) return rc;
   gate_gradients<T><<<grid, dim3(kThreads), 0, stream>>>(
-      a->pre, static_cast<const T*>(a->dy), a->dy_stride, a->rows, a->width, a->activation, by_row,
-      w.half, by_column, w.filled, static_cast<uint32_t>(tiles_f));
+      a->pre, static_cast<const T*>(a->dy), a->dy_stride, a->rows, a->width, a->activation, by_row, w.half,
+      w.row_bytes, by_column, w.filled, w.column_bytes, static_cast<uint32_t>(tiles_f));
   if (int rc = launched("gate gradients")) return rc;
   if (a->dx) {
-    if (int rc = transpose<T>(a->gate, a->gate_stride, a->width, a->columns, w.half, weights, 2 * w.half,
+    if (int rc = transpose<T>(a->gate, a->gate_stride, a->width, a->columns, w.half, weights, w.row_bytes,
                               stream))
       return rc;
-    if (int rc = transpose<T>(a->up, a->up_stride, a->width, a->columns, w.half, weights + w.half,
-                              2 * w.half, stream))
+    if (int rc = transpose<T>(a->up, a->up_stride, a->width, a->columns, w.half,
+                              weights + w.row_bytes / 2, w.row_bytes, stream))
       return rc;
-    const Rows left{reinterpret_cast<const uint8_t*>(by_row), 2 * w.half * e, a->rows};
-    const Rows right{reinterpret_cast<const uint8_t*>(weights), 2 * w.half * e, a->columns};
-    if (int rc = product<T>(left, right, 2 * w.half * e / 16, a->type, static_cast<T*>(a->dx), a->columns,
+    const Rows left{by_row, w.row_bytes, a->rows}, right{weights, w.row_bytes, a->columns};
+    if (int rc = product<T>(left, right, w.row_bytes / 16, a->type, static_cast<T*>(a->dx), a->columns,
                             stream))
       return rc;
   }
   if (a->dweights) {
-    if (int rc = transpose<T>(a->x, a->x_stride, a->rows, a->columns, w.filled, x, w.filled, stream))
+    if (int rc = transpose<T>(a->x, a->x_stride, a->rows, a->columns, w.filled, x, w.column_bytes, stream))
       return rc;
-    const Rows left{reinterpret_cast<const uint8_t*>(by_column), w.filled * e, 2 * a->width};
-    const Rows right{reinterpret_cast<const uint8_t*>(x), w.filled * e, a->columns};
-    return product<T>(left, right, w.filled * e / 16, a->type, static_cast<T*>(a->dweights), a->columns,
+    const Rows left{by_column, w.column_bytes, 2 * a->width}, right{x, w.column_bytes, a->columns};
+    return product<T>(left, right, w.column_bytes / 16, a->type, static_cast<T*>(a->dweights), a->columns,
                       stream);
   }
   return NS_OK;
@@ -282,17 +347,27 @@ int run_pack(Rows* rows, const void* data, int64_t stride, int64_t columns, int6
   pack_kernel<T><<<dim3(static_cast<unsigned>(groups)), dim3(kThreads), 0, stream>>>(
       static_cast<const T*>(data), stride, rows->rows, columns, static_cast<uint32_t>(pieces),
       reinterpret_cast<T*>(to));
-  rows->data = to;
-  rows->stride = pieces * 16;
+  return launched("rows' layout");
+}
+
+int run_thirds(Rows* rows, const void* data, int64_t stride, int64_t columns, int64_t pieces, uint8_t* to,
+               hipStream_t stream) {
+  const int64_t blocks = pieces / (kThirds / 16), groups = (rows->rows * 4 * blocks + kThreads - 1) / kThreads;
+  if (groups > INT32_MAX) return fail("the projection is too large for one launch");
+  thirds_kernel<<<dim3(static_cast<unsigned>(groups)), dim3(kThreads), 0, stream>>>(
+      static_cast<const float*>(data), stride, rows->rows, columns, static_cast<uint32_t>(blocks), to);
   return launched("rows' layout");
 }
 
 }  // namespace
 
-int pack_rows(Rows* rows, const void* data, int64_t stride, int64_t columns, int32_t type, uint8_t* to,
-              hipStream_t stream) {
-  const int64_t pieces = pieces_of(columns, type);
+int pack_rows(Rows* rows, const void* data, int64_t stride, int64_t columns, int32_t type, bool thirds,
+              uint8_t* to, hipStream_t stream) {
+  const int64_t pieces = pieces_of(columns, type, thirds);
+  rows->data = to;
+  rows->stride = pieces * 16;
   if (pieces == 0) return NS_OK;
+  if (thirds) return run_thirds(rows, data, stride, columns, pieces, to, stream);
   return type == NS_TYPE_F32 ? run_pack<float>(rows, data, stride, columns, pieces, to, stream)
                              : run_pack<_Float16>(rows, data, stride, columns, pieces, to, stream);
 }
@@ -301,17 +376,20 @@ int pack_rows(Rows* rows, const void* data, int64_t stride, int64_t columns, int
 // us for 32 stages (2048 columns of 16 bits): a round of large tiles 45 to 51 us; of middle ones
 // 16.2 with two on a compute unit and 24 alone; of small ones 6.2 where there are many, 22 with
 // two on a compute unit and 14 alone, where a stage's way from memory to LDS takes longer than its
-// products.  float32 multiplies at a sixteenth of the rate, so tiles alone count: 60 and 15.7, and
-// large ones gain nothing.  us, small / middle / large, of M x K to F in bf16: 64 x 4096 to 8192
+// products.  float32 in thirds, 32 columns at a time, is bound by its products, and tiles alone
+// count: 34 and 12.9 for 32 stages of 32 columns; as it is, at a sixteenth of bfloat16's rate, 60 and
+// 15.7.  us, small / middle / large, of M x K to F in bf16: 64 x 4096 to 8192
 // 28.8 / 58.8 / 91; 256 x 1024 to 4096 9.9 / 13.2 / 23.5; 512 x 4096 to 4096 50 / 41.8 / 72.6; 2048^3
 // 51 / 32.4 / 40.6; 3000 x 700 to 5000 89 / 68 / 61; 4096^3 406 / 259 / 205; in float32 3885 x 1031 to
 // 1500 248 / 233.
-GemmSize gemm_size(int64_t m, int64_t n, int32_t type) {
+GemmSize gemm_size(int64_t m, int64_t n, int32_t type, bool thirds) {
   const auto tiles = [=](int64_t side) { return (m + side - 1) / side * ((n + side - 1) / side); };
   const auto rounds = [](int64_t count, int64_t at_once) { return (count + at_once - 1) / at_once; };
   const int64_t few = tiles(64), some = tiles(128);
-  if (type == NS_TYPE_F32)
-    return 600 * rounds(some, 256) <= 157 * rounds(few, 256) ? GemmSize::kMiddle : GemmSize::kSmall;
+  if (type == NS_TYPE_F32) {
+    const int64_t middle = (thirds ? 340 : 600) * rounds(some, 256);
+    return middle <= (thirds ? 129 : 157) * rounds(few, 256) ? GemmSize::kMiddle : GemmSize::kSmall;
+  }
   const auto most = [](int64_t a, int64_t b) { return a > b ? a : b; };
   const int64_t small = most(few <= 256 ? 140 : 220, 62 * rounds(few, 256));
   const int64_t middle = most(240 * rounds(some, 512), 162 * rounds(some, 256));

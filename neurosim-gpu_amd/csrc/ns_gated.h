@@ -2,7 +2,7 @@
 // tiles, and operands laid out as the tile kernels read them.
 #pragma once
 
-#include "ns_gemm.h"
+#include "ns_split.h"
 #include "neurosim_hip_block.h"
 
 namespace ns {
@@ -12,6 +12,8 @@ namespace ns {
 using LargeGemm = GemmTile<8, 4, 2, 4, 2>;    // 256 x 256
 using MiddleGemm = GemmTile<4, 4, 2, 2, 2>;   // 128 x 128
 using SmallGemm = GemmTile<2, 2, 2, 2, 4>;    // 64 x 64
+using MiddleSplit = SplitTile<4, 4, 2, 2, 3>; // 128 x 128
+using SmallSplit = SplitTile<2, 2, 2, 2, 2>;  // 64 x 64
 
 // x times the normal distribution's mass below x; erfc keeps the relative accuracy of small ones.
 __device__ __forceinline__ float mass_below(float x) { return 0.5f * erfcf(-0.70710678118654752f * x); }
@@ -34,12 +36,14 @@ __device__ __forceinline__ Activation activated_slope(float x, int activation) {
 }
 
 inline int64_t type_size(int32_t type) { return type == NS_TYPE_F32 ? 4 : 2; }
-// 16-byte pieces of a row of n values, and n up to whole pieces.
-inline int64_t pieces_of(int64_t n, int32_t type) { return (n * type_size(type) + 15) / 16; }
-inline int64_t whole_values(int64_t n, int32_t type) { return pieces_of(n, type) * 16 / type_size(type); }
+// n up to whole pieces, and the 16-byte pieces of a laid-out row of n values, as they are or in thirds.
+inline int64_t whole_values(int64_t n, bool thirds) { return thirds ? (n + 31) / 32 * 32 : (n + 7) / 8 * 8; }
+inline int64_t pieces_of(int64_t n, int32_t type, bool thirds) {
+  return thirds ? (n + 31) / 32 * (kThirds / 16) : (n * type_size(type) + 15) / 16;
+}
 
 enum class GemmSize { kSmall, kMiddle, kLarge };
-GemmSize gemm_size(int64_t m, int64_t n, int32_t type);
+GemmSize gemm_size(int64_t m, int64_t n, int32_t type, bool thirds);
 
 // Whether the tile kernels read these rows where they lie.
 inline bool plain(const void* data, int64_t stride, int64_t rows, int64_t columns, int32_t type) {
@@ -49,19 +53,33 @@ inline bool plain(const void* data, int64_t stride, int64_t rows, int64_t column
 }
 inline Rows plain_rows(const void* data, int64_t stride, int64_t rows, int64_t columns, int32_t type) {
   return Rows{static_cast<const uint8_t*>(data),
-              rows <= 1 ? pieces_of(columns, type) * 16 : stride * type_size(type), rows};
+              rows <= 1 ? pieces_of(columns, type, false) * 16 : stride * type_size(type), rows};
+}
+
+// Whether a forward lays float32 rows out in thirds, three passes over the operands that few rows
+// or small products do not repay.  Us, as they are / in thirds, M x K to F: 64 x 4096 to 4096 72 / 177,
+// 256 x 2048 to 2048 37.8 / 59.6, 512 x 2048 to 2048 68 / 70, 1000 x 500 to 1000 20.7 / 29.4, 700 x 3000 to 900
+// 98 / 90, 1024 x 1024 to 2048 67 / 56, 2048^3 243 / 168.
+inline bool in_thirds(const ns_gated_args* a) {
+  constexpr int64_t kRepays = 200, kProducts = 1500000000;
+  const int64_t results = a->rows * a->width;
+  return a->type == NS_TYPE_F32 && results >= kRepays * (a->rows + 2 * a->width) &&
+         results >= kProducts / (a->columns > 0 ? a->columns : kProducts);
 }
 
 // What has to be laid out anew for the forward, and where in the workspace.
 struct PackedForward {
-  bool pack_x, pack_weights;
+  bool thirds, pack_x, pack_weights;
+  int64_t pieces;                          // of a row
   int64_t x, gate, up, bytes;
 };
 inline PackedForward packed_forward(const ns_gated_args* a) {
   PackedForward w{};
-  const int64_t row = pieces_of(a->columns, a->type) * 16;
-  w.pack_x = !plain(a->x, a->x_stride, a->rows, a->columns, a->type);
-  w.pack_weights = !plain(a->gate, a->gate_stride, a->width, a->columns, a->type) ||
+  w.thirds = in_thirds(a);
+  w.pieces = pieces_of(a->columns, a->type, w.thirds);
+  const int64_t row = w.pieces * 16;
+  w.pack_x = w.thirds || !plain(a->x, a->x_stride, a->rows, a->columns, a->type);
+  w.pack_weights = w.thirds || !plain(a->gate, a->gate_stride, a->width, a->columns, a->type) ||
                    !plain(a->up, a->up_stride, a->width, a->columns, a->type) ||
                    (a->width > 1 && a->gate_stride != a->up_stride);
   w.gate = w.pack_x ? a->rows * row : 0;
@@ -70,9 +88,9 @@ inline PackedForward packed_forward(const ns_gated_args* a) {
   return w;
 }
 
-// Copies rows of `columns` values to `to`, dense and filled up with zeros to whole pieces.
-int pack_rows(Rows* rows, const void* data, int64_t stride, int64_t columns, int32_t type, uint8_t* to,
-              hipStream_t stream);
+// Copies rows of `columns` values to `to`, dense and filled up with zeros, as they are or in thirds.
+int pack_rows(Rows* rows, const void* data, int64_t stride, int64_t columns, int32_t type, bool thirds,
+              uint8_t* to, hipStream_t stream);
 
 int check_gated(const ns_gated_args* a);
 bool few_rows(const ns_gated_args* a);

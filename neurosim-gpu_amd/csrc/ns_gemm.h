@@ -38,7 +38,7 @@ struct Rows {
   int64_t stride;              // bytes from row to row, a multiple of 16, below kMostStride
   int64_t rows;
 };
-constexpr int64_t kMostStride = 1 << 23;   // a tile's rows are addressed in 31 bits
+constexpr int64_t kMostStride = 1 << 23;   // 256 rows of a tile are addressed in 31 bits
 
 // Geometry of a tile: WM x WN wavefronts, each MI x NJ results of 16x16; `stages` of them in LDS.
 template <int kMI, int kNJ, int kWM, int kWN, int kStages>

@@ -102,8 +102,10 @@ def gated_projection(x: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, *,
     """``f(x @ gate.T) * (x @ up.T)`` of ``x`` [..., K], ``gate`` and ``up`` [F, K] (K and F up
     to 2^20), all of one type; the result is [..., F].  ``activation`` f is "silu" or "gelu"
     (of the normal distribution function, not its tanh form).  Call it with a batch's ticks
-    or with a single one; up to 16 rows are bound by the weights' bytes.  A call with
-    gradients takes up to 2^21 rows and keeps both products in float32 for its backward."""
+    or with a single one; up to 16 rows are bound by the weights' bytes.  Large float32 calls,
+    and all float32 gradients, are multiplied in three bfloat16 parts at float32's precision;
+    an infinity in x or a weight then makes its row or column NaN.  A call with gradients takes
+    up to 2^21 rows and keeps both products in float32 for its backward."""
     if activation not in ACTIVATIONS:
         raise ValueError("activation must be 'silu' or 'gelu'")
     if not isinstance(x, torch.Tensor) or x.dim() < 1 or x.dtype not in TYPES:

@@ -84,7 +84,10 @@ def gated_bounds(x, gate, up, activation, dy, u, half):
     operands rounded to a type of half unit ``half`` (see the tests)."""
     x, gate, up, dy = (wide(v) for v in (x, gate, up, dy))
     K = x.shape[1]
-    sums = 2 * (K + 2) * u
+    # Float32 operands go in as three parts, six products of which are summed: six times the
+    # additions, and 2 u of a product left out.
+    times = 6 if half == 0 else 1
+    sums = 2 * times * (K + 2) * u
     g, w = x @ gate.t(), x @ up.t()
     eg, ew = sums * (x.abs() @ gate.abs().t()), sums * (x.abs() @ up.abs().t())
     value, slope = activated(g, activation)
@@ -100,9 +103,9 @@ def gated_bounds(x, gate, up, activation, dy, u, half):
     edg, edu = edg + half * (dg.abs() + edg), edu + half * (du.abs() + edu)
     M, F = dy.shape
     bounds["x"] = (edg @ gate.abs() + edu @ up.abs()
-                   + 2 * (2 * F + 2) * u * (dg.abs() @ gate.abs() + du.abs() @ up.abs()))
-    bounds["gate"] = edg.t() @ x.abs() + 2 * (M + 2) * u * (dg.abs().t() @ x.abs())
-    bounds["up"] = edu.t() @ x.abs() + 2 * (M + 2) * u * (du.abs().t() @ x.abs())
+                   + 2 * times * (2 * F + 2) * u * (dg.abs() @ gate.abs() + du.abs() @ up.abs()))
+    bounds["gate"] = edg.t() @ x.abs() + 2 * times * (M + 2) * u * (dg.abs().t() @ x.abs())
+    bounds["up"] = edu.t() @ x.abs() + 2 * times * (M + 2) * u * (du.abs().t() @ x.abs())
     return bounds
 
 

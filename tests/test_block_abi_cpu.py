@@ -133,7 +133,11 @@ def test_gated_workspaces(lib):
     assert bytes_(40, 64, 30, 1, x_stride=8) == 40 * 128          # overlapping rows
     assert bytes_(40, 63, 30, 1) == (40 + 60) * 128
     assert bytes_(40, 64, 30, 1, gate_stride=72) == 60 * 128       # two strides
-    assert bytes_(40, 64, 30, 0, x_stride=(1 << 21) + 4) == 40 * 256
+    assert bytes_(40, 64, 30, 1, x_stride=(1 << 22) + 8) == 40 * 128
+    assert bytes_(40, 64, 30, 0) == 0 and bytes_(40, 65, 30, 0) == (40 + 60) * 272
+    assert bytes_(5000, 1024, 320, 0) == (5000 + 640) * 32 * 192  # many in float32: in thirds
+    assert bytes_(5000, 1025, 320, 0) == (5000 + 640) * 33 * 192
+    assert bytes_(5000, 64, 320, 0) == 0 and bytes_(100, 8192, 3200, 0) == 0
     assert bytes_(0, 64, 30, 1) == 0
 
 

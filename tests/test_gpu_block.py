@@ -2,7 +2,8 @@
 
 Tolerances of the projection (block_oracle.gated_bounds).  With u = 2^-24, a sum of K products
 in float32 is off by at most 2 (K + 2) u times the sum of their sizes (2 u an addition, since the
-matrix cores may cut off instead of rounding).  The activation carries its argument's error
+matrix cores may cut off instead of rounding), six times that in float32, whose products are
+summed in six parts (and the three left out are at most 2 u of a product).  The activation carries its argument's error
 times its slope, and its own operations.  The gradients' operands dg and du are rounded to
 the operands' type, half a unit each, which passes through their products like the errors
 before.  Outputs are then rounded once to their type.
@@ -69,10 +70,10 @@ def test_gated_projection(gpu, shape, dtype):
     check_gated(operands(draw, M, K, F, dtype), "silu" if K % 2 else "gelu", draw(M, F, dtype=dtype))
 
 
-@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("shape", [(2100, 72, 2800), (40, 2100, 2820), (4120, 2900, 20)])
 def test_large_tiles(gpu, shape, dtype):
-    """256 x 256 tiles: of the forward, of the weights' gradients, of x's."""
+    """The largest tiles: of the forward, of the weights' gradients, of x's."""
     draw = Draw(gpu, 3)
     M, K, F = shape
     check_gated(operands(draw, M, K, F, dtype), "silu", draw(M, F, dtype=dtype))
@@ -96,12 +97,11 @@ def test_kept_products_leave_the_result_alone(gpu, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("rows", [7, 150])
-def test_gated_strides(gpu, rows, dtype):
+@pytest.mark.parametrize("rows,K,F", [(7, 130, 44), (150, 130, 44), (1500, 2500, 410)])
+def test_gated_strides(gpu, rows, K, F, dtype):
     """Rows at any stride and alignment, a shared row, more dimensions, dense or not: the same
     bits as dense copies."""
     draw = Draw(gpu, rows)
-    K, F = 130, 44
     dense = operands(draw, rows, K, F, dtype)
     dy = draw(rows, F, dtype=dtype)
 
@@ -130,6 +130,72 @@ def test_gated_strides(gpu, rows, dtype):
     assert torch.equal(gated_projection(**shared), gated_projection(**plain))
     cubes = {**dense, "x": dense["x"].view(1, rows, K)}
     assert torch.equal(gated_projection(**cubes), want[0].detach().view(1, rows, F))
+
+
+def test_many_float32_rows(gpu):
+    """A float32 forward in thirds, odd sizes each way."""
+    draw = Draw(gpu, 6)
+    M, K, F = 1290, 2301, 525
+    check_gated(operands(draw, M, K, F, torch.float32), "gelu", draw(M, F))
+
+
+@pytest.mark.parametrize("rows,width", [(5, 2), (200, 2), (4100, 400)])
+def test_float32_is_multiplied_as_float32(gpu, rows, width):
+    """Values whose parts matter: all 24 bits set, far apart in size, as large and as small as
+    float32 has them.  Against float64, a product is off by its own rounding and the three parts
+    left out, a sum of two by one rounding more: 2^-22 of the sizes is more than both.  What
+    float32 has no number for, 3.4e38 times more than one, is an infinity of its sign."""
+    g = torch.Generator().manual_seed(3)
+    pad = torch.nn.functional.pad if width > 300 else (lambda v, _: v)
+    x = torch.randn(rows, 2, generator=g)
+    x[0] = torch.tensor([1 + 2.0 ** -23, 0.0])
+    x[1] = torch.tensor([2.0 - 2.0 ** -23, 0.0])
+    x[2] = torch.tensor([3.4e38, 0.0])           # rounds past the largest bfloat16
+    x[3] = torch.tensor([1e-30, 1e10])
+    up = torch.tensor([[1 + 2.0 ** -22, 2.0 ** -12 + 2.0 ** -30], [0.75, -1.0]])
+    up = torch.cat((up, torch.randn(width - 2, 2, generator=g)))
+    gate = torch.zeros_like(up)
+    # Columns of zeros make the products many enough to be worth thirds.
+    inputs = [pad(v, (500, 500)).to(gpu).requires_grad_() for v in (x, gate, up)]
+    y = gated_projection(*inputs)
+    pre = y.grad_fn.saved_tensors[3][1]
+    want = x.double() @ up.double().t()
+    size = x.double().abs() @ up.double().abs().t()
+    pre, past = pre.cpu(), want.abs() > torch.finfo(torch.float32).max
+    assert torch.equal(pre[past], torch.where(want[past] > 0, torch.inf, -torch.inf).float())
+    pre, want, size = pre[~past], want[~past], size[~past]
+    assert ((pre.double() - want).abs() <= 2.0 ** -22 * size + 2.0 ** -126).all()
+
+
+@pytest.mark.parametrize("rows,dtype", [(9, torch.float32), (90, torch.float32), (9, torch.bfloat16),
+                                        (90, torch.bfloat16)])
+def test_infinities_stay_infinities(gpu, rows, dtype):
+    """An infinity of x in a row makes infinities of its products with nonzero weights."""
+    draw = Draw(gpu, 5)
+    values = operands(draw, rows, 70, 20, dtype)
+    clean = gated_projection(**values)
+    values["x"][4, 69] = float("inf")
+    kept = gated_projection(**leaves(values))
+    pre = kept.grad_fn.saved_tensors[3]
+    assert torch.equal(pre[:, 4], torch.stack([torch.where(values[k][:, 69] > 0, torch.inf, -torch.inf)
+                                               for k in ("gate", "up")]))
+    y = gated_projection(**values)
+    y[4] = clean[4]
+    assert torch.equal(y, clean)
+
+
+def test_infinities_of_many_float32_rows(gpu):
+    """Multiplied in parts of either sign, an infinity is none of a sign: its row or column is not
+    finite, and no other one is touched."""
+    draw = Draw(gpu, 5)
+    values = operands(draw, 2000, 2500, 310, torch.float32)
+    clean = gated_projection(**values)
+    values["x"][4, 2499] = float("inf")
+    values["up"][7, 3] = float("-inf")
+    y = gated_projection(**values)
+    assert not torch.isfinite(y[4]).any() and not torch.isfinite(y[:, 7]).any()
+    y[4], y[:, 7] = clean[4], clean[:, 7]
+    assert torch.equal(y, clean)
 
 
 @pytest.mark.parametrize("sizes", [(0, 5, 4), (3, 5, 0), (3, 0, 4), (30, 0, 4)])
