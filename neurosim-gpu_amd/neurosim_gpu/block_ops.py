@@ -6,7 +6,7 @@
   it is used and never stored; optionally added to a residual in the same pass.
 
 float32, bfloat16 and float16 are taken; sums are float32 and each output is rounded once.
-Forward-mode derivatives are refused.  The kernels are csrc/gated.hip, gated_grad.hip and
+Forward-mode derivatives are refused, and so is a backward under graph capture.  The kernels are csrc/gated.hip, gated_grad.hip and
 dropout.hip behind include/neurosim_hip_block.h; calls run on the current stream, allocate
 their outputs and workspaces from torch, and never synchronise.
 """
@@ -22,7 +22,7 @@ from torch.autograd.function import once_differentiable
 
 from .microscaled import _float_rows, _rows
 from .native import load_library
-from .signal_ops import TYPES, _address, _needs_grad, call
+from .signal_ops import TYPES, _address, _needs_grad, call, refuse_capture
 
 ACTIVATIONS = {"silu": 0, "gelu": 1}       # NS_GATE_*
 _MAX_ROWS = 1 << 21                        # NS_GATED_MAX_ROWS
@@ -82,6 +82,7 @@ class _GatedProjection(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
+        refuse_capture("gated_projection")
         x, gate, up, pre = ctx.saved_tensors
         wants, lib, (rows, columns), width = ctx.needs_input_grad, _library(), x.shape, gate.shape[0]
         if not rows or not columns or not width:
@@ -159,6 +160,7 @@ class _Dropout(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
+        refuse_capture("dropout")
         (drawn,), (threshold, seed, offset) = ctx.saved_tensors, ctx.rest
         dx = (_drop(dy.contiguous(), None, threshold, seed if drawn is None else drawn, offset)
               if ctx.needs_input_grad[0] else None)

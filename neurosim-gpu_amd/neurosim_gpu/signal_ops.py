@@ -185,6 +185,13 @@ def _needs_grad(*values) -> bool:
     return False
 
 
+def refuse_capture(what: str) -> None:
+    """A backward that is captured into a graph while an eager graph of the same leaves lives
+    ends the process inside the runtime: none of these is captured."""
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"the backward of {what} cannot be captured into a graph")
+
+
 # ---- convolution ---------------------------------------------------------------------
 
 _ACTIVATIONS = {None: 0, "silu": 1}
@@ -537,6 +544,7 @@ class _GatedRecurrence(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dfinal):
+        refuse_capture("gated_recurrence")
         x, forget, write, z, rates, lengths, kept = ctx.saved_tensors
         wants, device = ctx.needs_input_grad, x.device
         ticks, batch, n = x.shape
@@ -576,7 +584,8 @@ def gated_recurrence(x: torch.Tensor, forget: torch.Tensor, write: torch.Tensor,
     which has no bound there).  ``state`` [B, N] float32 is h before the first tick (zeros if
     absent).
 
-    Returns ``(y, state)``: y [T, B, N] of x's type and h after each column's last tick."""
+    Returns ``(y, state)``: y [T, B, N] of x's type and h after each column's last tick.
+    Calls may be captured into a graph, their backward may not (it raises)."""
     _check_recurrence(x, forget, write, rates, z, state, 3)
     lengths = _lengths(lengths, x)
     if _needs_grad(x, forget, write, rates, z, state):

@@ -16,7 +16,7 @@ import torch
 
 import block_oracle as bo
 from test_gpu_signal import HALF_ULP, SMALLEST, U, Draw, leaves
-from neurosim_gpu import dropout, gated_projection
+from neurosim_gpu import dropout, gated_projection, gated_recurrence
 
 pytestmark = pytest.mark.gpu
 
@@ -374,3 +374,16 @@ def test_dropout_refusals(gpu):
             (dict(x=x, p=0.1, seed=1, residual=x.half()), "like x")):
         with pytest.raises(ValueError, match=message):
             dropout(**args)
+
+
+def test_no_backward_under_capture(gpu, monkeypatch):
+    """Refused from the query alone: no stream is captured here."""
+    x = torch.ones(3, 4, device=gpu, requires_grad=True)
+    w = torch.ones(5, 4, device=gpu)
+    signal = torch.ones(2, 1, 4, device=gpu, requires_grad=True)
+    outs = {"dropout": dropout(x, 0.1, seed=1), "gated_projection": gated_projection(x, w, w),
+            "gated_recurrence": gated_recurrence(signal, signal, signal, torch.ones(4, device=gpu))[0]}
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    for name, out in outs.items():
+        with pytest.raises(RuntimeError, match=f"{name} cannot be captured"):
+            out.sum().backward()
