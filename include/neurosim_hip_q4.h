@@ -5,7 +5,7 @@
  * allocation, no synchronisation) are those of neurosim_hip.h.
  *
  * Format: a row of K values is cut into groups of `group` consecutive values (32, 64, or a
- * multiple of 128; the last one may be short).  A value is (code - zero) * scale with codes of
+ * multiple of 128 up to NS_Q4_MAX_COLUMNS; the last one may be short).  A value is (code - zero) * scale with codes of
  * 0 .. 15, two a byte (even value in the low nibble), rows filled up to whole 16 bytes
  * (ceil(K/32) of them); one scale of a float type and one byte `zero` per group (no zeros: 8).
  * Quantising, with lo = min(0, min x), hi = max(0, max x): scale = hi/15 - lo/15 rounded to its
@@ -45,7 +45,8 @@ int ns_q4_dequantize(const ns_q4_matrix* matrix, void* out, int64_t stride, int3
                      void* stream);
 
 /* y[m][n] = sum_k x[m][k] weight[n][k] + bias[n], products and sums in float32 or finer,
- * rounded to `type`.  A row of x that holds an infinity or a NaN gives NaN. */
+ * rounded to `type`.  A row of x that holds an infinity or a NaN gives NaN, and one with values
+ * beyond 2^115, 128 of which times a code pass float32, may. */
 typedef struct ns_q4_product_args {
   ns_q4_matrix weight;
   int64_t rows;                /* M */

@@ -31,8 +31,8 @@ inline Q4View q4_view(const ns_q4_matrix& m) {
 inline int check_q4(const ns_q4_matrix& m) {
   if (m.rows < 0 || m.columns < 0) return fail("rows and columns must not be negative");
   if (m.columns > NS_Q4_MAX_COLUMNS) return fail("a 4-bit row has at most %d columns", NS_Q4_MAX_COLUMNS);
-  if (m.group != 32 && m.group != 64 && (m.group <= 0 || m.group % 128))
-    return fail("a group has 32, 64 or a multiple of 128 columns");
+  if (m.group != 32 && m.group != 64 && (m.group <= 0 || m.group % 128 || m.group > NS_Q4_MAX_COLUMNS))
+    return fail("a group has 32, 64 or a multiple of 128 columns, up to %d", NS_Q4_MAX_COLUMNS);
   if (m.scale_type != NS_TYPE_F32 && m.scale_type != NS_TYPE_BF16 && m.scale_type != NS_TYPE_F16)
     return fail("unknown element type of the scales");
   if (m.rows && m.columns && (!m.codes || !m.scales)) return fail("codes and scales are required");

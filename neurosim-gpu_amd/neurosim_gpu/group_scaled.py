@@ -50,8 +50,9 @@ def _library() -> ctypes.CDLL:
 
 
 def _check_group(group, columns: int) -> None:
-    if not isinstance(group, int) or (group not in (32, 64) and (group <= 0 or group % 128)):
-        raise ValueError("a group has 32, 64 or a multiple of 128 columns")
+    if (not isinstance(group, int) or group > _MAX_COLUMNS
+            or (group not in (32, 64) and (group <= 0 or group % 128))):
+        raise ValueError(f"a group has 32, 64 or a multiple of 128 columns, up to {_MAX_COLUMNS}")
     if columns > _MAX_COLUMNS:
         raise ValueError(f"a 4-bit row has at most {_MAX_COLUMNS} columns")
 
@@ -143,7 +144,8 @@ def q4_dequantize(value: Q4Tensor, dtype: torch.dtype = torch.float32) -> torch.
 def q4_product(x: torch.Tensor, weight: Q4Tensor, *, bias: torch.Tensor | None = None) -> torch.Tensor:
     """``x @ weight.T + bias``: x [..., K] (float32, bfloat16 or float16), weight [N, K] of 4-bit
     groups, result [..., N] of x's type.  Products are exact and sums float32; the result is
-    rounded once.  A row of x that holds an infinity or a NaN gives NaN."""
+    rounded once.  A row of x that holds an infinity or a NaN gives NaN, and one with values
+    beyond 2^115, 128 of which times a code pass float32, may."""
     if not isinstance(weight, Q4Tensor) or weight.codes.dim() != 2:
         raise ValueError("weight must be a Q4Tensor of [N, K]")
     if not isinstance(x, torch.Tensor) or x.dim() < 1 or x.dtype not in TYPES:

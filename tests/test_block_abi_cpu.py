@@ -208,7 +208,8 @@ def test_4_bit_refusals(lib):
         return group_scaled._PRODUCT.pack(*matrix(**more), m, x, 64, 0, out, 4, type, 0)
 
     changes = ((dict(rows=-1), "negative"), (dict(columns=(1 << 23) + 1), "at most"),
-               (dict(group=16), "32, 64"), (dict(group=192), "32, 64"), (dict(codes=0), "required"),
+               (dict(group=16), "32, 64"), (dict(group=192), "32, 64"), (dict(group=1 << 39), "up to"),
+               (dict(group=(1 << 23) + 128), "up to"), (dict(codes=0), "required"),
                (dict(scales=0), "required"), (dict(codes=8), "aligned"), (dict(scale_type=9), "scales"))
     for change, text in changes:
         assert text in message(lib, "ns_q4_product", product(**change)), change
