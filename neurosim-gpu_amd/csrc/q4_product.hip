@@ -11,6 +11,11 @@
 // fourth row of ones that gives c its share: sum x (u - zero) = sum (x - c)(u - zero) +
 // c (sum (16 + u) - count (16 + zero)), whose factor of c is exact.
 //
+// What bounds it now: requests.  One of 16 rows, 64 bytes each, takes a compute unit some 50 cycles
+// whatever it brings, and the instruction's layout asks for such ones, of the codes (33.5 MB of 16 x
+// 8192 to 8192: 17.2 us, 2.0 TB/s; without x, 13.1) and of x; 1 x 1024 to 50,000 10.7 us, of which
+// the call's way through the host takes 9; 33 x 50,000 to 1000 24.8, 5 of them to add 49 parts of K.
+//
 // In the 16x16x32 instruction the rows of x are the first operand and 16 rows of the weight the
 // second, so a lane's four results are four rows of x (for float32: one row's three parts and the
 // ones) of its own row of the weight, whose codes it loaded and whose scales it needs.
@@ -28,13 +33,23 @@ constexpr int kRing = 1;                       // stages requested ahead
 template <class T>
 constexpr int kTileRows = sizeof(T) == 4 ? 4 : 16;
 
+// Columns of x in LDS at a time: room for two workgroups on a compute unit, with their factors (20 x
+// 1024 to 50,000 in bf16 16.0 us, with 1024 columns 22.9).
+constexpr int chunk_columns(int tiles) { return tiles == 1 ? 1024 : 512; }
+
 // What a workgroup does: CT tiles of x's rows, S strips of 16 rows of the weight per wavefront,
 // NG groups (or parts of one) per stage.
 template <int kCT, int kS, int kNG>
 struct Q4Tile {
   static constexpr int CT = kCT, S = kS, NG = kNG;
-  static constexpr int chunk = CT <= 2 ? 2048 / CT : 512;   // columns of x in LDS: 64 KiB at most
+  static constexpr int chunk = chunk_columns(CT);
   static constexpr int stages = chunk / kStage, sub = kStage / NG;
+  // Two tiles and strips leave a compute unit's registers to two workgroups, which hide each other's
+  // waits; the others request the next chunk of x while one is multiplied, where registers last.  Us,
+  // that way and the other: 20 x 1024 to 50,000 in bf16 16.1 / 22.4, 8 x 1024 to 50,000 in float32 16.7 /
+  // 18.4, though 24 x 8192 to 8192 in groups of 32 26.7 / 25.2; 33 x 50,000 to 1000 26.0 / 24.8.
+  static constexpr bool kTwo = CT == 2 && S == 2;
+  static constexpr bool kNext = !kTwo && (CT * S < 8 || NG == 1);
 };
 
 struct Q4Place {
@@ -92,10 +107,21 @@ __device__ __forceinline__ float lanes_sum(float v) {
   return v;
 }
 
+// What a group's sums are multiplied with, and what their offset is: -(16 + zero).
+struct Q4Factors {
+  float scale, offset;
+};
+
 template <class G, class T>
-struct Q4Lds {
+struct Q4Centres {};
+template <class G>
+struct Q4Centres<G, float> {
+  float centre[G::chunk / G::sub][4 * G::CT];
+};
+template <class G, class T>
+struct Q4Lds : Q4Centres<G, T> {
   v4i x[G::chunk / 64][16 * G::CT][8];         // pieces of eight columns, at place piece ^ turn(row)
-  float centre[sizeof(T) == 4 ? G::chunk / G::sub : 1][4 * G::CT];
+  Q4Factors factors[G::stages * 16 * G::S * kQ4Waves][G::NG];
 };
 
 __device__ __forceinline__ int pair_of(float a, float b) {
@@ -184,16 +210,10 @@ __device__ __forceinline__ void place_rows(const Q4Rows<G, T>& rows_of_x, int64_
   }
 }
 
-// A wavefront's request of one strip and stage: scales and zeros as they are in memory, so that
-// nothing waits for them before they are used.
+// Scales and zeros as they are in memory, so that nothing waits for them before they are used.
 template <int NG>
 struct Q4Scales {
   uint32_t scale[NG], zeros;                     // of 32 bits each, or of 16 side by side; bytes
-};
-template <int NG>
-struct Q4Stage {
-  uint32_t codes[4];
-  Q4Scales<NG> by;
 };
 
 // Scales and zeros of groups first .. first + NG - 1 of a row that begins at `at`; past its last
@@ -245,8 +265,52 @@ __device__ __forceinline__ float scale_value(uint32_t raw, int32_t type) {
   return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(raw)));
 }
 
+// A workgroup's factors come through LDS, laid there by threads that read a row's neighbouring
+// ones: read where they are used, 2 to 8 bytes of 16 rows at a time, they take as long as the codes
+// (1 x 8192 to 8192, groups of 128, in bf16 16.7 us, so 12.6).  By stage, then row, rows turned by
+// the stage so that neighbouring threads store to different banks; of 2^shift stages from `base` on,
+// `rows` rows (a power of two) from `row` on, kEach of them a thread.
+struct Q4Table {
+  int64_t row;
+  int rows, shift, base, last;                   // of the last stage there is
+  uint32_t per_group;                            // stages of a group, where it has some
+};
+
+template <int NG>
+__device__ __forceinline__ int factors_place(const Q4Table& t, int stage, int row) {
+  const int turn = 1 << t.shift < 32 / NG ? 32 / NG >> t.shift : 1;
+  return (stage << __builtin_ctz(t.rows)) + (row ^ (stage * turn & (t.rows - 1)));
+}
+
+template <int NG, int kEach>
+__device__ __forceinline__ void ask_factors(const Q4View& w, const Q4Table& t, Q4Scales<NG> (&to)[kEach]) {
+#pragma unroll
+  for (int u = 0; u < kEach; ++u) {
+    const int id = threadIdx.x + u * kQ4Threads, stage = t.base + (id & ((1 << t.shift) - 1));
+    const int64_t n = t.row + (id >> t.shift), row = n < w.rows ? n : w.rows - 1;
+    const int at = stage < t.last ? stage : t.last;
+    if (u * kQ4Threads < t.rows << t.shift)
+      load_scales<NG>(w, row * w.groups, NG == 1 ? static_cast<int>(at / t.per_group) : at * NG, to[u]);
+  }
+}
+
+template <int NG, int kEach>
+__device__ __forceinline__ void place_factors(const Q4View& w, const Q4Table& t, const Q4Scales<NG> (&from)[kEach],
+                                              Q4Factors (*to)[NG]) {
+#pragma unroll
+  for (int u = 0; u < kEach; ++u) {
+    const int id = threadIdx.x + u * kQ4Threads;
+    if (id >= t.rows << t.shift) break;
+    Q4Factors* const place = to[factors_place<NG>(t, id & ((1 << t.shift) - 1), id >> t.shift)];
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+      place[g] = Q4Factors{scale_value(raw_scale(from[u], g, w.scale_type), w.scale_type),
+                           zero_offset(from[u], g)};
+  }
+}
+
 template <class G, class T>
-__global__ __launch_bounds__(kQ4Threads) void q4_product(Q4View w, Q4Place p, const T* x,
+__global__ __launch_bounds__(kQ4Threads, G::kTwo ? 4 : 2) void q4_product(Q4View w, Q4Place p, const T* x,
                                                          int64_t x_stride, int64_t rows,
                                                          const float* bias, T* out, int64_t stride,
                                                          float* partials) {
@@ -275,32 +339,36 @@ __global__ __launch_bounds__(kQ4Threads) void q4_product(Q4View w, Q4Place p, co
 
   // A lane's rows of the weight.
   const uint8_t* codes[G::S];
-  int64_t scales[G::S];                          // places of their first scales
 #pragma unroll
   for (int s = 0; s < G::S; ++s) {
     const int64_t n = n0 + 16 * s + (lane & 15), row = n < w.rows ? n : w.rows - 1;
     codes[s] = w.codes + row * blocks * 16;
-    scales[s] = row * w.groups;
   }
-  Q4Stage<G::NG> ring[kRing][G::S];
-  const auto load = [&](int stage, Q4Stage<G::NG> (&to)[G::S]) __attribute__((always_inline)) {
+  uint32_t ring[kRing][G::S][4];
+  const auto load = [&](int stage, uint32_t (&to)[G::S][4]) __attribute__((always_inline)) {
     // Past the last block, x is zero: any codes do.
     const int block = 4 * stage + q < blocks ? 4 * stage + q : blocks - 1;
-    const int first = G::NG == 1 ? static_cast<int>(stage / per_group) : stage * G::NG;
 #pragma unroll
-    for (int s = 0; s < G::S; ++s) {
-      __builtin_memcpy(to[s].codes, codes[s] + static_cast<uint32_t>(block) * 16, 16);
-      load_scales<G::NG>(w, scales[s], first, to[s].by);
-    }
+    for (int s = 0; s < G::S; ++s)
+      __builtin_memcpy(to[s], codes[s] + static_cast<uint32_t>(block) * 16, 16);
   };
+  // The factors of the workgroup's rows.
+  const int own_rows = kQ4Waves / static_cast<int>(p.parts) * (16 * G::S);
+  const int first_row = static_cast<int>(wave / p.parts) * (16 * G::S);
+  Q4Table table{static_cast<int64_t>(strip_group) * own_rows, own_rows, __builtin_ctz(G::stages), 0, limit - 1,
+                per_group};
 
   constexpr int kOnes = __is_same(T, _Float16) ? 0x3C003C00 : 0x3F803F80;
   const v4i ones = {kOnes, kOnes, kOnes, kOnes};
   v4f total[G::S][G::CT] = {};
-  const auto compute = [&](int stage, Q4Stage<G::NG> (&from)[G::S]) __attribute__((always_inline)) {
+  const auto compute = [&](int stage, uint32_t (&from)[G::S][4]) __attribute__((always_inline)) {
     const int own = stage % G::stages;                   // in the chunk
+    const Q4Factors* by[G::S];
 #pragma unroll
-    for (int s = 0; s < G::S; ++s) deal_blocks(from[s].codes);
+    for (int s = 0; s < G::S; ++s)
+      by[s] = lds.in.factors[factors_place<G::NG>(table, own, first_row + 16 * s + (lane & 15))];
+#pragma unroll
+    for (int s = 0; s < G::S; ++s) deal_blocks(from[s]);
 #pragma unroll
     for (int g = 0; g < G::NG; ++g) {
       v4f sum[G::S][G::CT] = {}, taken[G::CT] = {};
@@ -316,7 +384,7 @@ __global__ __launch_bounds__(kQ4Threads) void q4_product(Q4View w, Q4Place p, co
         }
 #pragma unroll
         for (int s = 0; s < G::S; ++s) {
-          const v4i codes = sixteen_plus<__is_same(T, _Float16)>(from[s].codes[e]);
+          const v4i codes = sixteen_plus<__is_same(T, _Float16)>(from[s][e]);
 #pragma unroll
           for (int t = 0; t < G::CT; ++t) sum[s][t] = q4_multiply<T>(rows_of_x[t], codes, sum[s][t]);
         }
@@ -324,8 +392,7 @@ __global__ __launch_bounds__(kQ4Threads) void q4_product(Q4View w, Q4Place p, co
       const int group = own * G::NG + g;
 #pragma unroll
       for (int s = 0; s < G::S; ++s) {
-        const float offset = zero_offset(from[s].by, g);
-        const float scale = scale_value(raw_scale(from[s].by, g, w.scale_type), w.scale_type);
+        const float offset = by[s][g].offset, scale = by[s][g].scale;
 #pragma unroll
         for (int t = 0; t < G::CT; ++t) {
           float own_sum[4];
@@ -358,13 +425,22 @@ __global__ __launch_bounds__(kQ4Threads) void q4_product(Q4View w, Q4Place p, co
 #pragma unroll
   for (int u = 0; u < kRing; ++u)
     if (stage + u * step < limit) load(stage + u * step, ring[u]);
+  Q4Rows<G, T> rows_of_x;
+  Q4Scales<G::NG> raw[G::stages * 16 * G::S * kQ4Waves / kQ4Threads];
+  const auto ask = [&](int chunk) __attribute__((always_inline)) {
+    ask_rows<G, T>(own_x, x_stride, rows - m0, static_cast<int64_t>(chunk) * G::chunk, w.columns, rows_of_x);
+    table.base = chunk * G::stages;
+    ask_factors<G::NG>(w, table, raw);
+  };
+  if (G::kNext) ask(first_chunk);
   for (int chunk = first_chunk; chunk < last_chunk; ++chunk) {
     const int64_t first = static_cast<int64_t>(chunk) * G::chunk;
-    Q4Rows<G, T> rows_of_x;
-    ask_rows<G, T>(own_x, x_stride, rows - m0, first, w.columns, rows_of_x);
+    if (!G::kNext) ask(chunk);
     if (chunk > first_chunk) __syncthreads();              // all have read the one before
     place_rows<G, T>(rows_of_x, rows - m0, first, w.columns, lds.in);
+    place_factors<G::NG>(w, table, raw, lds.in.factors);
     __syncthreads();
+    if (G::kNext && chunk + 1 < last_chunk) ask(chunk + 1);
     for (int end = (chunk + 1) * G::stages; stage < end; stage += kRing * step) {
 #pragma unroll
       for (int u = 0; u < kRing; ++u) {
@@ -409,25 +485,30 @@ __global__ __launch_bounds__(kQ4Threads) void q4_product(Q4View w, Q4Place p, co
 }
 
 // Up to 16 rows of 16 bits go from memory to registers: a workgroup's wavefronts share S strips
-// and take their stages in turn, so each reads its own part of x, without LDS or barriers but
-// for the sums at the end.
-constexpr int kRowRing = 2;
+// and take their stages in turn, so each reads its own part of x, without barriers but for the
+// factors and for the sums at the end.
+constexpr int kRowRing = 1, kFactorStages = 8 * kQ4Waves;
 
 template <int NG, int S>
 struct Q4RowStage {
   v4i x[4];
-  Q4Stage<NG> w[S];
+  uint32_t codes[S][4];
 };
 
 template <class T, int NG, int S>
 __global__ __launch_bounds__(kQ4Threads) void q4_rows(Q4View w, Q4Place p, const T* x, int64_t x_stride,
                                                       int64_t rows, const float* bias, T* out,
                                                       int64_t stride, float* partials) {
-  __shared__ v4f sums[kQ4Waves][S][64];
+  __shared__ union {
+    Q4Factors factors[kFactorStages * 16 * S][NG];
+    v4f sums[kQ4Waves][S][64];
+  } lds;
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), q = lane >> 4;
   const uint32_t split = uniform(blockIdx.x / p.strip_groups), strip_group = blockIdx.x - split * p.strip_groups;
   const int part = static_cast<int>(wave % p.parts), step = static_cast<int>(p.parts);
-  const int64_t n0 = (static_cast<int64_t>(strip_group) * (kQ4Waves / p.parts) + wave / p.parts) * (16 * S);
+  const int own_rows = kQ4Waves / step * (16 * S);         // of the workgroup
+  const int64_t group_row = static_cast<int64_t>(strip_group) * own_rows;
+  const int first_row = wave / step * (16 * S);
   const int blocks = static_cast<int>(w.blocks), stages = (blocks + 3) / 4;
   const int begin = static_cast<int>(split * p.per_split);
   const int limit = begin + static_cast<int>(p.per_split) < stages ? begin + static_cast<int>(p.per_split) : stages;
@@ -435,23 +516,18 @@ __global__ __launch_bounds__(kQ4Threads) void q4_rows(Q4View w, Q4Place p, const
   const int64_t m = (lane & 15) < rows ? lane & 15 : rows - 1;
   const T* const own_x = x + m * x_stride + 8 * q;
   const uint8_t* codes[S];
-  int64_t scales[S];
 #pragma unroll
   for (int s = 0; s < S; ++s) {
-    const int64_t n = n0 + 16 * s + (lane & 15), row = n < w.rows ? n : w.rows - 1;
+    const int64_t n = group_row + first_row + 16 * s + (lane & 15), row = n < w.rows ? n : w.rows - 1;
     codes[s] = w.codes + row * blocks * 16;
-    scales[s] = row * w.groups;
   }
   const int whole = static_cast<int>(w.columns / kStage);  // stages that lie within the columns
   Q4RowStage<NG, S> ring[kRowRing];
   const auto load = [&](int stage, Q4RowStage<NG, S>& to) __attribute__((always_inline)) {
     const int block = 4 * stage + q < blocks ? 4 * stage + q : blocks - 1;
-    const int first = NG == 1 ? static_cast<int>(stage / per_group) : stage * NG;
 #pragma unroll
-    for (int s = 0; s < S; ++s) {
-      __builtin_memcpy(to.w[s].codes, codes[s] + static_cast<uint32_t>(block) * 16, 16);
-      load_scales<NG>(w, scales[s], first, to.w[s].by);
-    }
+    for (int s = 0; s < S; ++s)
+      __builtin_memcpy(to.codes[s], codes[s] + static_cast<uint32_t>(block) * 16, 16);
     const T* const from = own_x + static_cast<int64_t>(stage) * kStage;
     if (stage < whole) {
 #pragma unroll
@@ -467,12 +543,21 @@ __global__ __launch_bounds__(kQ4Threads) void q4_rows(Q4View w, Q4Place p, const
       }
     }
   };
+  // Factors of up to 8 `step` stages at a time; no more than there are stages of (a power of two).
+  int shift = __builtin_ctz(kFactorStages / kQ4Waves * p.parts);
+  while (shift > 0 && 1 << (shift - 1) >= limit - begin) --shift;
+  const int span = 1 << shift;
+  Q4Table table{group_row, own_rows, shift, begin, limit - 1, per_group};
   constexpr int kOnes = __is_same(T, _Float16) ? 0x3C003C00 : 0x3F803F80;
   const v4i ones = {kOnes, kOnes, kOnes, kOnes};
   v4f total[S] = {};
-  const auto compute = [&](Q4RowStage<NG, S>& from) __attribute__((always_inline)) {
+  const auto compute = [&](Q4RowStage<NG, S>& from, int place) __attribute__((always_inline)) {
+    const Q4Factors* by[S];
 #pragma unroll
-    for (int s = 0; s < S; ++s) deal_blocks(from.w[s].codes);
+    for (int s = 0; s < S; ++s)
+      by[s] = lds.factors[factors_place<NG>(table, place, first_row + 16 * s + (lane & 15))];
+#pragma unroll
+    for (int s = 0; s < S; ++s) deal_blocks(from.codes[s]);
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       v4f sum[S] = {}, taken = {};
@@ -488,14 +573,14 @@ __global__ __launch_bounds__(kQ4Threads) void q4_rows(Q4View w, Q4Place p, const
         taken = q4_multiply<T>(v, ones, taken);
 #pragma unroll
         for (int s = 0; s < S; ++s)
-          sum[s] = q4_multiply<T>(v, sixteen_plus<__is_same(T, _Float16)>(from.w[s].codes[e]), sum[s]);
+          sum[s] = q4_multiply<T>(v, sixteen_plus<__is_same(T, _Float16)>(from.codes[s][e]), sum[s]);
       }
 #pragma unroll
       for (int s = 0; s < S; ++s) {
-        const float offset = zero_offset(from.w[s].by, g);
-        const float scale = scale_value(raw_scale(from.w[s].by, g, w.scale_type), w.scale_type);
+        const Q4Factors own = by[s][g];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) total[s][i] = fmaf(scale, fmaf(offset, taken[i], sum[s][i]), total[s][i]);
+        for (int i = 0; i < 4; ++i)
+          total[s][i] = fmaf(own.scale, fmaf(own.offset, taken[i], sum[s][i]), total[s][i]);
       }
       // One group after the other, in few registers.
 #pragma unroll
@@ -505,28 +590,38 @@ __global__ __launch_bounds__(kQ4Threads) void q4_rows(Q4View w, Q4Place p, const
 #pragma unroll
   for (int u = 0; u < kRowRing; ++u)
     if (begin + part + u * step < limit) load(begin + part + u * step, ring[u]);
-  for (int stage = begin + part; stage < limit; stage += kRowRing * step) {
+  for (int base = begin; base < limit; base += span) {
+    if (base > begin) __syncthreads();                     // all have read the factors before
+    Q4Scales<NG> raw[kFactorStages * 16 * S / kQ4Threads];
+    table.base = base;
+    ask_factors<NG>(w, table, raw);
+    place_factors<NG>(w, table, raw, lds.factors);
+    __syncthreads();
+    const int end = base + span < limit ? base + span : limit;
+    for (int stage = base + part; stage < end; stage += kRowRing * step) {
 #pragma unroll
-    for (int u = 0; u < kRowRing; ++u) {
-      const int now = stage + u * step;
-      if (now < limit) {
-        compute(ring[u]);
-        if (now + kRowRing * step < limit) load(now + kRowRing * step, ring[u]);
+      for (int u = 0; u < kRowRing; ++u) {
+        const int now = stage + u * step;
+        if (now < end) {
+          compute(ring[u], now - base);
+          if (now + kRowRing * step < limit) load(now + kRowRing * step, ring[u]);
+        }
       }
     }
   }
+  __syncthreads();
 #pragma unroll
-  for (int s = 0; s < S; ++s) sums[wave][s][lane] = total[s];
+  for (int s = 0; s < S; ++s) lds.sums[wave][s][lane] = total[s];
   __syncthreads();
   // The workgroup's strips, 256 results each, a column of the weight's rows by its threads.
-  for (int id = threadIdx.x; id < static_cast<int>(kQ4Waves / p.parts) * S * 256; id += kQ4Threads) {
+  for (int id = threadIdx.x; id < own_rows * 16; id += kQ4Threads) {
     const int strip = id >> 8, column = id & 15, row = id >> 4 & 15, first = strip / S * step;
     const int from = (row >> 2) * 16 + column;             // the lane that holds it
-    const int64_t n = static_cast<int64_t>(strip_group) * (kQ4Waves / p.parts) * (16 * S) + 16 * strip + column;
+    const int64_t n = group_row + 16 * strip + column;
     if (row >= rows || n >= w.rows) continue;
     float value = 0.0f;
     for (int k = 0; k < step; ++k)
-      value += reinterpret_cast<const float*>(&sums[first + k][strip % S][from])[row & 3];
+      value += reinterpret_cast<const float*>(&lds.sums[first + k][strip % S][from])[row & 3];
     if (p.splits > 1) partials[(split * rows + row) * w.rows + n] = value;
     else out[row * stride + n] = static_cast<T>(value + (bias ? bias[n] : 0.0f));
   }
@@ -577,13 +672,19 @@ struct Q4Plan {
   int64_t groups;              // workgroups
 };
 
-Q4Plan rows_plan(int64_t n, int64_t k) {
+Q4Plan rows_plan(int64_t m, int64_t n, int64_t k) {
   Q4Plan plan{};
   const int64_t stages = (k + kStage - 1) / kStage;
-  plan.strips = n > 16 * 256 ? 2 : 1;
+  // More strips a wavefront read x less often, but leave fewer workgroups; with few rows x costs
+  // little.  Us with one / two / four: 8 x 4096 to 8192 10.0 / 9.0 / 12.2, 16 x 8192 to 8192 23.3 / 17.2 / 24.9,
+  // 16 x 4096 to 12,288 19.1 / 15.4 / 13.9, 16 x 4096 to 16,384 22.8 / 15.2 / 14.0, 4 x 2048 to 32,768 15.8 /
+  // 12.2 / 14.1.
+  plan.strips = n <= 16 * 256 ? 1 : m <= 8 || n < 64 * 192 ? 2 : 4;
   const int64_t strips = (n + 16 * plan.strips - 1) / (16 * plan.strips);
   int64_t parts = 1;
-  while (parts < kQ4Waves && stages >= 4 * parts) parts *= 2;
+  // Four stages a wavefront and more: with two 8 x 1024 to 50,000 takes 15.9 us, not 14.3, and 4 x 2048
+  // to 32,768 14.1, not 12.2.
+  while (parts < kQ4Waves && stages >= 8 * parts) parts *= 2;
   const int64_t strip_groups = (strips * parts + kQ4Waves - 1) / kQ4Waves;
   int64_t splits = 1;
   if (strip_groups < 128) {
@@ -600,15 +701,15 @@ Q4Plan rows_plan(int64_t n, int64_t k) {
 }
 
 Q4Plan q4_plan(int64_t m, int64_t n, int64_t k, int32_t type) {
-  if (type != NS_TYPE_F32 && m <= 16) return rows_plan(n, k);
+  if (type != NS_TYPE_F32 && m <= 16) return rows_plan(m, n, k);
   Q4Plan plan{};
   const int64_t per_tile = type == NS_TYPE_F32 ? 4 : 16, tiles = (m + per_tile - 1) / per_tile;
   plan.tiles = tiles <= 2 ? static_cast<int>(tiles) : tiles == 3 && type != NS_TYPE_F32 ? 3 : 4;
   const int64_t m_tiles = (tiles + plan.tiles - 1) / plan.tiles;
-  const int64_t columns = plan.tiles <= 2 ? 2048 / plan.tiles : 512, chunks = (k + columns - 1) / columns;
+  const int64_t columns = chunk_columns(plan.tiles), chunks = (k + columns - 1) / columns;
   // Two strips a wavefront halve what is read of x from LDS for each, but also the wavefronts.  Us,
-  // one / two, bf16: 40 x 4096 to 4096 15.3 / 18.5, 32 x 2048 to 4096 13.8 / 16.2, 64 x 4096 to 8192 27.4 /
-  // 26.7, 33 x 50,000 to 1000 34 / 28; float32: 8 x 8192 to 4096 17.4 / 15.5, 20 x 4096 to 4096 18.4 / 17.6.
+  // one / two, bf16: 40 x 4096 to 4096 13.9 / 16.3, 64 x 2048 to 16,384 25.7 / 25.5, 33 x 50,000 to 1000
+  // 28.2 / 24.8.
   const bool few = type != NS_TYPE_F32 && m_tiles * ((n + 15) / 16) * chunks <= 2048;
   plan.strips = plan.tiles == 1 || few ? 1 : 2;
   const int64_t strips = (n + 16 * plan.strips - 1) / (16 * plan.strips);
@@ -647,7 +748,9 @@ template <class T, int kNG>
 int run_groups(const ns_q4_product_args* a, const Q4Plan& plan, hipStream_t stream) {
   if constexpr (sizeof(T) == 2) {
     if (plan.tiles == 0)
-      return plan.strips == 1 ? run_rows<T, kNG, 1>(a, plan, stream) : run_rows<T, kNG, 2>(a, plan, stream);
+      return plan.strips == 1   ? run_rows<T, kNG, 1>(a, plan, stream)
+             : plan.strips == 2 ? run_rows<T, kNG, 2>(a, plan, stream)
+                                : run_rows<T, kNG, 4>(a, plan, stream);
     if (plan.tiles == 3)
       return plan.strips == 1 ? run_tile<Q4Tile<3, 1, kNG>, T>(a, plan, stream)
                               : run_tile<Q4Tile<3, 2, kNG>, T>(a, plan, stream);

@@ -148,6 +148,18 @@ def test_products(gpu, shape, dtype):
         check_product((draw(M, K) + 0.5).to(dtype), *weight, bias=bias)
 
 
+# Wide weights take more strips a wavefront, by rows; scales come to a workgroup in stretches of 64
+# stages of 128 columns, or of fewer where few wavefronts share a strip.
+@pytest.mark.parametrize("shape", [(16, 12_301, 260), (9, 12_288, 1100), (8, 12_289, 2300), (7, 4200, 1030),
+                                   (16, 4100, 8500), (12, 12_300, 130), (24, 9000, 1100)])
+def test_wide_weights(gpu, shape):
+    M, N, K = shape
+    draw = Draw(gpu, sum(shape))
+    for group, scales in ((32, torch.float32), (64, torch.float16), (128, torch.bfloat16), (384, torch.float32)):
+        dtype = (torch.bfloat16, torch.float16)[group % 3 == 0]
+        check_product((draw(M, K) + 0.5).to(dtype), *weight_of(draw, gpu, N, K, group, group != 64, scales))
+
+
 @pytest.mark.parametrize("scales", TYPES)
 def test_scale_types_and_strange_zeros(gpu, scales):
     draw = Draw(gpu, 5)
