@@ -270,15 +270,16 @@ int64_t recur_blocks(const ns_recurrence_args* a, int lane_channels) {
   return (a->channels + 64 * lane_channels - 1) / (64 * lane_channels);
 }
 
-// Time chunks worth walking side by side: enough to fill the card, four tiles each at least.  Bf16,
-// us, in one chunk and in chunks: T=2000, B=4, N=4096 (256 workgroups) 89 / 122; T=200, B=4, N=600
-// (40 workgroups) 13.6 / 20.6 (both with tiles of 64 ticks).
+// Time chunks worth walking side by side: enough to fill the card twice, four tiles each at least.
+// Bf16, us, in one chunk and in chunks: T=2000, B=4, N=4096 (256 workgroups) 89 / 122; T=200, B=4,
+// N=600 (40 workgroups) 13.6 / 20.6 (both with tiles of 64 ticks).  With 256, 512 and 1024 workgroups:
+// T=16384, B=1, N=2048 132 / 114 / 117, T=65536, B=1, N=512 132 / 117 / 122, T=8192, B=2, N=2048 133 / 118 / 116.
 int64_t worth_recur_chunks(const ns_recurrence_args* a) {
   if (a->ticks <= 0 || a->batch <= 0) return 1;
   const int64_t blocks = recur_blocks(a, recur_lane_channels(a)) * a->batch;
   const int64_t tiles = (a->ticks + kRecurTile - 1) / kRecurTile;
   if (blocks >= 192 || tiles < 24) return 1;
-  const int64_t chunks = 1024 / blocks < tiles / 4 ? 1024 / blocks : tiles / 4;
+  const int64_t chunks = 512 / blocks < tiles / 4 ? 512 / blocks : tiles / 4;
   return chunks < 2 ? 1 : chunks;
 }
 
