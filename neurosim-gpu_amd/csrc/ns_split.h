@@ -8,7 +8,7 @@
 //
 // Rows lie in thirds: for every 32 columns 64 bytes of x0, of x1 and of x2, zeros past the last
 // column.  A stage is one such block of every row of both operands; in LDS a part's 64 bytes of a
-// row follow the next row's, its 16-byte piece k at place k ^ (row/4 % 4).
+// row follow the next row's, its 16-byte piece k at place k ^ third_turn(row).
 #pragma once
 
 #include "ns_gemm.h"
@@ -62,6 +62,10 @@ struct SplitTile {
   static_assert(strips_a * waves == MI * WM && strips_b * waves == NJ * WN, "whole strips");
 };
 
+// 0, 2, 3, 1 for the quarters of 16 rows: so the 16 lanes whose pieces LDS gives at a time, two
+// quarters each of two neighbouring pieces, find them in different banks.
+__device__ __forceinline__ uint32_t third_turn(uint32_t row) { return 0x78u >> (2 * (row >> 2 & 3)) & 3; }
+
 // What a wavefront asks for: 16 rows of a third a request, a piece a lane.
 template <class G>
 struct SplitPlace {
@@ -82,7 +86,7 @@ __device__ __forceinline__ SplitPlace<G> split_place(int lane, int wave, uint32_
   p.wave = wave;
   p.blocks = blocks;
   p.a = a;
-  const uint32_t row = lane >> 2, piece = (lane & 3) ^ (row >> 2 & 3);
+  const uint32_t row = lane >> 2, piece = (lane & 3) ^ third_turn(row);
 #pragma unroll
   for (int s = 0; s < G::strips_a; ++s)
     p.at_a[s] = (16 * (wave + s * G::waves) + row) * stride_a + piece * 16;
@@ -130,7 +134,7 @@ struct SplitBase {
 };
 template <class G>
 __device__ __forceinline__ SplitBase split_base(uint32_t stage, int wm, int wn, int lane) {
-  const uint32_t row = lane & 15, place = (lane >> 4) ^ (row >> 2);
+  const uint32_t row = lane & 15, place = (lane >> 4) ^ third_turn(row);
   const uint32_t at = stage + row * 64 + place * 16;
   SplitBase base{at + wm * (G::MI * 1024), at + G::rows_m * 64 + wn * (G::NJ * 1024)};
   // One register each, here: left to itself the compiler keeps every strip's.
