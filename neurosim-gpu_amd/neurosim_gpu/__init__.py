@@ -6,7 +6,9 @@ SparseTopology / random_topology, precision codecs, checkpoint/resume) and runs
 the native tick as hand-written HIP kernels behind the C ABI declared in
 include/neurosim_hip.h (library: neurosim_gpu/_lib/libneurosim_hip.so).  Around the network
 stand the operators of a signal path, in the same library: causal convolution, selective
-scan and products of microscaled 4-bit rows (signal_ops, microscaled, signal_encoder).
+scan and products of microscaled 4-bit rows (signal_ops, microscaled, signal_encoder), and those
+of a gated block: gated linear recurrence, gated projection, dropout and products with 4-bit
+integer weights (signal_ops, block_ops, group_scaled).
 """
 
 from .block_ops import dropout, gated_projection
@@ -31,10 +33,10 @@ __version__ = "0.1.0"
 __all__ = [
     "DendriticDynamics", "DendriticMatrixRuntime", "DendriticPELSRuntime", "DenseOracle",
     "Dynamics", "HybridPELSRuntime", "MXTensor", "MatrixRollout", "MatrixRuntime",
-    "NativeDendriticMatrixRuntime", "NativeDendriticPELSRuntime", "PRECISIONS", "Q4Tensor", "RuntimeStats",
-    "SparseTopology", "capture_runtime", "causal_conv", "causal_conv_step",
-    "dropout", "encode_sparse_weights", "gated_projection", "gated_recurrence", "gated_recurrence_step", "load_native_extension",
-    "load_runtime_checkpoint", "load_topology",
+    "NativeDendriticMatrixRuntime", "NativeDendriticPELSRuntime", "PRECISIONS", "Q4Tensor",
+    "RuntimeStats", "SparseTopology", "capture_runtime", "causal_conv", "causal_conv_step",
+    "dropout", "encode_sparse_weights", "gated_projection", "gated_recurrence",
+    "gated_recurrence_step", "load_native_extension", "load_runtime_checkpoint", "load_topology",
     "mx_dequantize", "mx_product", "mx_quantize", "q4_dequantize", "q4_product", "q4_quantize",
     "quantize_dequantize", "random_topology",
     "restore_runtime", "save_runtime_checkpoint", "save_topology", "selective_scan",
