@@ -13,8 +13,9 @@
 //
 // What bounds it now: requests.  One of 16 rows, 64 bytes each, takes a compute unit some 50 cycles
 // whatever it brings, and the instruction's layout asks for such ones, of the codes (33.5 MB of 16 x
-// 8192 to 8192: 17.2 us, 2.0 TB/s; without x, 13.1) and of x; 1 x 1024 to 50,000 10.7 us, of which
-// the call's way through the host takes 9; 33 x 50,000 to 1000 24.8, 5 of them to add 49 parts of K.
+// 8192 to 8192: 17.2 us, 2.0 TB/s; without x, 13.1) and of x; 1 x 1024 to 50,000 10.1 us, of which
+// the call's way through the host takes 9.  With more rows, the vector ALU beside the matrix cores:
+// 33 x 50,000 to 1000 24.3, 5 of them to add 49 parts of K, 22.8 before that without any loads.
 //
 // In the 16x16x32 instruction the rows of x are the first operand and 16 rows of the weight the
 // second, so a lane's four results are four rows of x (for float32: one row's three parts and the
@@ -62,8 +63,11 @@ struct Q4Place {
 template <bool kHalf>
 __device__ __forceinline__ v4i sixteen_plus(uint32_t word) {
   constexpr int at = kHalf ? 6 : 3;            // the place of u in the mantissa
-  constexpr uint32_t mask = kHalf ? 0x03C003C0u : 0x00780078u;
+  // The mask in a register: then and and or are one instruction, which takes one constant from
+  // elsewhere (33 x 50,000 to 1000 24.3 us, else 24.8; 1 x 1024 to 50,000 10.1, else 10.7).
+  uint32_t mask = kHalf ? 0x03C003C0u : 0x00780078u;
   constexpr uint32_t sixteen = kHalf ? 0x4C004C00u : 0x41804180u;
+  asm("" : "+v"(mask));
   v4i out;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
