@@ -15,7 +15,7 @@
 // whatever it brings, and the instruction's layout asks for such ones, of the codes (33.5 MB of 16 x
 // 8192 to 8192: 17.2 us, 2.0 TB/s; without x, 13.1) and of x; 1 x 1024 to 50,000 10.1 us, of which
 // the call's way through the host takes 9.  With more rows, the vector ALU beside the matrix cores:
-// 33 x 50,000 to 1000 24.3, 5 of them to add 49 parts of K, 22.8 before that without any loads.
+// 33 x 50,000 to 1000 22.9, some 3 of them to add 49 parts of K; without any loads about 2 less.
 //
 // In the 16x16x32 instruction the rows of x are the first operand and 16 rows of the weight the
 // second, so a lane's four results are four rows of x (for float32: one row's three parts and the
@@ -64,7 +64,7 @@ template <bool kHalf>
 __device__ __forceinline__ v4i sixteen_plus(uint32_t word) {
   constexpr int at = kHalf ? 6 : 3;            // the place of u in the mantissa
   // The mask in a register: then and and or are one instruction, which takes one constant from
-  // elsewhere (33 x 50,000 to 1000 24.3 us, else 24.8; 1 x 1024 to 50,000 10.1, else 10.7).
+  // elsewhere (33 x 50,000 to 1000 then 24.3 us, else 24.8; 1 x 1024 to 50,000 10.1, else 10.7).
   uint32_t mask = kHalf ? 0x03C003C0u : 0x00780078u;
   constexpr uint32_t sixteen = kHalf ? 0x4C004C00u : 0x41804180u;
   asm("" : "+v"(mask));
@@ -631,15 +631,16 @@ __global__ __launch_bounds__(kQ4Threads) void q4_rows(Q4View w, Q4Place p, const
   }
 }
 
-// The parts of K added in order, eight requested at a time.
-template <class T>
-__global__ __launch_bounds__(kThreads) void add_splits(const float* __restrict__ partials,
+// The parts of K added in order, kAhead requested at a time: 32 of many parts (33 x 50,000 to 1000,
+// 49 parts, with 32 / 8 22.9 / 24.3 us), 8 of few (40 x 4096 to 4096, 8 parts, 14.4 / 13.4).
+constexpr int kAddThreads = 64;
+template <class T, uint32_t kAhead>
+__global__ __launch_bounds__(kAddThreads) void add_splits(const float* __restrict__ partials,
                                                        uint32_t splits, int64_t rows, int64_t columns,
                                                        const float* bias, T* out, int64_t stride) {
-  const int64_t id = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * kAddThreads + threadIdx.x;
   if (id >= rows * columns) return;
   float sum = 0.0f;
-  constexpr uint32_t kAhead = 8;
   for (uint32_t k = 0; k < splits; k += kAhead) {
     float v[kAhead];
 #pragma unroll
@@ -787,8 +788,13 @@ int run(const ns_q4_product_args* a, hipStream_t stream) {
     default: rc = run_groups<T, 1>(a, plan, stream); break;
   }
   if (rc || plan.place.splits == 1) return rc;
-  add_splits<T><<<dim3(static_cast<unsigned>(results)), dim3(kThreads), 0, stream>>>(
-      a->workspace, plan.place.splits, m, n, a->bias, static_cast<T*>(a->out), a->stride);
+  const dim3 grid(static_cast<unsigned>((m * n + kAddThreads - 1) / kAddThreads));
+  if (plan.place.splits > 24)
+    add_splits<T, 32><<<grid, dim3(kAddThreads), 0, stream>>>(
+        a->workspace, plan.place.splits, m, n, a->bias, static_cast<T*>(a->out), a->stride);
+  else
+    add_splits<T, 8><<<grid, dim3(kAddThreads), 0, stream>>>(
+        a->workspace, plan.place.splits, m, n, a->bias, static_cast<T*>(a->out), a->stride);
   return launched("4-bit product parts");
 }
 
