@@ -89,24 +89,41 @@ __device__ __forceinline__ void store_turned(const Square<T>& square, uint8_t* t
 
 // Laid-out rows of what are columns of `from`: value r of row c is from[r][c] for r < rows, zero for
 // rows <= r < filled; rows begin at `to`, `stride` bytes apart.
+struct Turn {
+  const void* from;
+  int64_t from_stride, rows, columns, filled;
+  uint8_t* to;
+  int64_t stride;
+  uint32_t tiles_c, end;                   // of its workgroups, in the launch
+};
+// Up to three matrices in one launch.
+struct Turns {
+  Turn of[3];
+  int count;
+};
 template <class T>
-__global__ __launch_bounds__(kThreads) void transpose_kernel(const T* from, int64_t from_stride,
-                                                             int64_t rows, int64_t columns,
-                                                             int64_t filled, uint8_t* to, int64_t stride,
-                                                             uint32_t tiles_c) {
+__global__ __launch_bounds__(kThreads) void transpose_kernel(Turns turns) {
   __shared__ Square<T> square;
-  const uint32_t tile_r = uniform(blockIdx.x / tiles_c), tile_c = blockIdx.x - tile_r * tiles_c;
+  uint32_t id = blockIdx.x;
+  Turn t = turns.of[0];
+#pragma unroll
+  for (int k = 1; k < 3; ++k)
+    if (k < turns.count && blockIdx.x >= turns.of[k - 1].end) {
+      t = turns.of[k];
+      id = blockIdx.x - turns.of[k - 1].end;
+    }
+  const uint32_t tile_r = uniform(id / t.tiles_c), tile_c = id - tile_r * t.tiles_c;
   const int64_t r0 = static_cast<int64_t>(tile_r) * kSide, c0 = static_cast<int64_t>(tile_c) * kSide;
   const int side = threadIdx.x % kSquareLanes * kWide;
 #pragma unroll
   for (int k = 0; k < kSide; k += kLines) {
     const int line = k + threadIdx.x / kSquareLanes;
-    const int64_t r = r0 + line, left = columns - c0 - side;
-    const T* const in = from + r * from_stride + c0 + side;
+    const int64_t r = r0 + line, left = t.columns - c0 - side;
+    const T* const in = static_cast<const T*>(t.from) + r * t.from_stride + c0 + side;
     Pack<T, kWide> v{};
-    if (r < rows && left >= kWide) {
+    if (r < t.rows && left >= kWide) {
       v = load_pack<T, kWide>(in);
-    } else if (r < rows) {
+    } else if (r < t.rows) {
 #pragma unroll
       for (int j = 0; j < kWide; ++j)
         if (j < left) v.v[j] = in[j];
@@ -115,7 +132,7 @@ __global__ __launch_bounds__(kThreads) void transpose_kernel(const T* from, int6
     for (int j = 0; j < kWide; ++j) square.at[line][side + j] = v.v[j];
   }
   __syncthreads();
-  store_turned<T>(square, to, stride, r0, filled, c0, columns);
+  store_turned<T>(square, t.to, t.stride, r0, t.filled, c0, t.columns);
 }
 
 // dg and du: as laid-out rows [M][2 F'], du behind dg, and as columns [2 F][M'], each padded with
@@ -238,15 +255,20 @@ int tile_grid(int64_t tiles_m, int64_t tiles_n, dim3* grid) {
   return NS_OK;
 }
 
-template <class T>
-int transpose(const void* from, int64_t from_stride, int64_t rows, int64_t columns, int64_t filled,
-              uint8_t* to, int64_t stride, hipStream_t stream) {
+int add_turn(Turns* turns, const void* from, int64_t from_stride, int64_t rows, int64_t columns, int64_t filled,
+             uint8_t* to, int64_t stride) {
   const int64_t tiles_r = (filled + kSide - 1) / kSide, tiles_c = (columns + kSide - 1) / kSide;
+  const uint32_t before = turns->count ? turns->of[turns->count - 1].end : 0;
   dim3 grid;
-  if (int rc = tile_grid(tiles_r, tiles_c, &grid)) return rc;
-  transpose_kernel<T><<<grid, dim3(kThreads), 0, stream>>>(static_cast<const T*>(from), from_stride, rows,
-                                                           columns, filled, to, stride,
-                                                           static_cast<uint32_t>(tiles_c));
+  if (int rc = tile_grid(tiles_r, tiles_c, &grid)) return rc;   // a quarter of 2^31 at most, each
+  turns->of[turns->count++] = Turn{from, from_stride, rows, columns, filled, to, stride,
+                                   static_cast<uint32_t>(tiles_c), before + grid.x};
+  return NS_OK;
+}
+
+template <class T>
+int run_turns(const Turns& turns, hipStream_t stream) {
+  transpose_kernel<T><<<dim3(turns.of[turns.count - 1].end), dim3(kThreads), 0, stream>>>(turns);
   return launched("transposition");
 }
 
@@ -318,21 +340,32 @@ int run_backward(const ns_gated_args* a, hipStream_t stream) {
       a->pre, static_cast<const T*>(a->dy), a->dy_stride, a->rows, a->width, a->activation, by_row, w.half,
       w.row_bytes, by_column, w.filled, w.column_bytes, static_cast<uint32_t>(tiles_f));
   if (int rc = launched("gate gradients")) return rc;
+  // Small calls pay by the launch, so x is turned with the weights; a large one is turned when its
+  // product is next, from whose caches it then comes.  Us, all at once / x later: 1000 x 500 to 1000 in
+  // float32 117 / 121, 3885 x 1031 to 1500 517 / 515, 8192 x 4096 to 8192 in bf16 2862 / 2820.
+  constexpr int64_t kSmall = 8 << 20;
+  const bool together = a->rows * a->columns * type_size(a->type) <= kSmall;
+  Turns turns{};
   if (a->dx) {
-    if (int rc = transpose<T>(a->gate, a->gate_stride, a->width, a->columns, w.half, weights, w.row_bytes,
-                              stream))
+    if (int rc = add_turn(&turns, a->gate, a->gate_stride, a->width, a->columns, w.half, weights, w.row_bytes))
       return rc;
-    if (int rc = transpose<T>(a->up, a->up_stride, a->width, a->columns, w.half,
-                              weights + w.row_bytes / 2, w.row_bytes, stream))
+    if (int rc = add_turn(&turns, a->up, a->up_stride, a->width, a->columns, w.half, weights + w.row_bytes / 2,
+                          w.row_bytes))
       return rc;
+    if (a->dweights && together)
+      if (int rc = add_turn(&turns, a->x, a->x_stride, a->rows, a->columns, w.filled, x, w.column_bytes)) return rc;
+    if (int rc = run_turns<T>(turns, stream)) return rc;
     const Rows left{by_row, w.row_bytes, a->rows}, right{weights, w.row_bytes, a->columns};
     if (int rc = product<T>(left, right, w.row_bytes / 16, a->type, static_cast<T*>(a->dx), a->columns,
                             stream))
       return rc;
   }
   if (a->dweights) {
-    if (int rc = transpose<T>(a->x, a->x_stride, a->rows, a->columns, w.filled, x, w.column_bytes, stream))
-      return rc;
+    if (!a->dx || !together) {
+      turns.count = 0;
+      if (int rc = add_turn(&turns, a->x, a->x_stride, a->rows, a->columns, w.filled, x, w.column_bytes)) return rc;
+      if (int rc = run_turns<T>(turns, stream)) return rc;
+    }
     const Rows left{by_column, w.column_bytes, 2 * a->width}, right{x, w.column_bytes, a->columns};
     return product<T>(left, right, w.column_bytes / 16, a->type, static_cast<T*>(a->dweights), a->columns,
                       stream);

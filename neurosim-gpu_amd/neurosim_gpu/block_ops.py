@@ -6,15 +6,16 @@
   it is used and never stored; optionally added to a residual in the same pass.
 
 float32, bfloat16 and float16 are taken; sums are float32 and each output is rounded once.
-Forward-mode derivatives are refused, and so is a backward under graph capture.  The kernels are csrc/gated.hip, gated_grad.hip and
-dropout.hip behind include/neurosim_hip_block.h; calls run on the current stream, allocate
-their outputs and workspaces from torch, and never synchronise.
+Forward-mode derivatives are refused, and so is a backward under graph capture.  The kernels
+are csrc/gated.hip, gated_grad.hip and dropout.hip behind include/neurosim_hip_block.h; calls run
+on the current stream, allocate their outputs and workspaces from torch, and never synchronise.
 """
 
 from __future__ import annotations
 
 import ctypes
 import struct
+import sys
 from functools import lru_cache
 
 import torch
@@ -50,13 +51,20 @@ def _library() -> ctypes.CDLL:
 
 # ---- gated projection ----------------------------------------------------------------
 
-def _gated_args(x, gate, up, activation, y=None, pre=None, dy=None, dx=None, dweights=None,
-                workspace=None) -> bytes:
+def _gated_args(x, gate, up, activation, y=None, pre=None, dy=None, dx=None, dweights=None) -> bytes:
+    """The packed arguments, without a workspace: its size goes by the others."""
     (rows, columns), width = x.shape, gate.shape[0]
     return _GATED.pack(rows, columns, width, TYPES[x.dtype], activation, x.data_ptr(), x.stride(0),
                        gate.data_ptr(), gate.stride(0), up.data_ptr(), up.stride(0), _address(y),
                        width, _address(pre), _address(dy), 0 if dy is None else dy.stride(0),
-                       _address(dx), _address(dweights), _address(workspace))
+                       _address(dx), _address(dweights), 0)
+
+
+def _call_with_workspace(fn, size: int, device, args: bytes) -> None:
+    if size:
+        work = torch.empty(size, dtype=torch.uint8, device=device)
+        args = args[:-8] + work.data_ptr().to_bytes(8, sys.byteorder)     # its last field
+    call(fn, device, args)
 
 
 def _gated_forward(x, gate, up, activation, keep: bool):
@@ -64,10 +72,8 @@ def _gated_forward(x, gate, up, activation, keep: bool):
     lib, (rows, _), width = _library(), x.shape, gate.shape[0]
     y = torch.empty((rows, width), dtype=x.dtype, device=x.device)
     pre = torch.empty((2, rows, width), dtype=torch.float32, device=x.device) if keep else None
-    size = lib.ns_gated_forward_bytes(_gated_args(x, gate, up, activation))
-    work = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
-    call(lib.ns_gated_forward, x.device, _gated_args(x, gate, up, activation, y, pre,
-                                                     workspace=work))
+    args = _gated_args(x, gate, up, activation, y, pre)
+    _call_with_workspace(lib.ns_gated_forward, lib.ns_gated_forward_bytes(args), x.device, args)
     return y, pre
 
 
@@ -91,10 +97,8 @@ class _GatedProjection(torch.autograd.Function):
         dx = torch.empty((rows, columns), dtype=x.dtype, device=x.device) if wants[0] else None
         dweights = (torch.empty((2, width, columns), dtype=x.dtype, device=x.device)
                     if wants[1] or wants[2] else None)
-        operands = x, gate, up, ctx.activation, None, pre, dy, dx, dweights
-        size = lib.ns_gated_backward_bytes(_gated_args(*operands))
-        work = torch.empty(size, dtype=torch.uint8, device=x.device)
-        call(lib.ns_gated_backward, x.device, _gated_args(*operands, work))
+        args = _gated_args(x, gate, up, ctx.activation, None, pre, dy, dx, dweights)
+        _call_with_workspace(lib.ns_gated_backward, lib.ns_gated_backward_bytes(args), x.device, args)
         return (dx, dweights[0] if wants[1] else None, dweights[1] if wants[2] else None, None)
 
 

@@ -387,3 +387,21 @@ def test_no_backward_under_capture(gpu, monkeypatch):
     for name, out in outs.items():
         with pytest.raises(RuntimeError, match=f"{name} cannot be captured"):
             out.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,K,F", [(40, 130, 44), (4400, 1000, 50)])
+def test_gated_gradients_of_some(gpu, rows, K, F, dtype):
+    """Gradients asked for one at a time, or two, are those of all three, bit for bit."""
+    draw = Draw(gpu, rows)
+    values = operands(draw, rows, K, F, dtype)
+    dy = draw(rows, F, dtype=dtype)
+
+    def gradients(names):
+        inputs = {k: v.clone().requires_grad_(k in names) for k, v in values.items()}
+        return torch.autograd.grad(gated_projection(**inputs), [inputs[k] for k in names], dy)
+
+    want = dict(zip(values, gradients(list(values))))
+    for names in (["x"], ["gate"], ["up"], ["gate", "up"], ["x", "up"]):
+        for name, got in zip(names, gradients(names)):
+            assert torch.equal(got, want[name]), names
