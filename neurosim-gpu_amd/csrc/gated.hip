@@ -267,13 +267,13 @@ int run(const ns_gated_args* a, hipStream_t stream) {
   Rows x = plain_rows(a->x, a->x_stride, a->rows, k, a->type);
   Rows gate = plain_rows(a->gate, a->gate_stride, a->width, k, a->type);
   Rows up = plain_rows(a->up, a->up_stride, a->width, k, a->type);
-  if (w.pack_x)
-    if (int rc = pack_rows(&x, a->x, a->x_stride, k, a->type, w.thirds, space + w.x, stream)) return rc;
+  PackJobs jobs{};
+  if (w.pack_x) add_pack(&jobs, &x, a->x, a->x_stride, w.pieces, w.thirds, space + w.x);
   if (w.pack_weights) {
-    if (int rc = pack_rows(&gate, a->gate, a->gate_stride, k, a->type, w.thirds, space + w.gate, stream))
-      return rc;
-    if (int rc = pack_rows(&up, a->up, a->up_stride, k, a->type, w.thirds, space + w.up, stream)) return rc;
+    add_pack(&jobs, &gate, a->gate, a->gate_stride, w.pieces, w.thirds, space + w.gate);
+    add_pack(&jobs, &up, a->up, a->up_stride, w.pieces, w.thirds, space + w.up);
   }
+  if (int rc = run_packs(jobs, k, w.pieces, a->type, w.thirds, stream)) return rc;
   const GemmSize size = gemm_size(a->rows, 2 * a->width, a->type, w.thirds);
   if constexpr (sizeof(T) == 4) {
     if (w.thirds)

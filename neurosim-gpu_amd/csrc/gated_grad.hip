@@ -14,15 +14,29 @@ namespace {
 
 constexpr int kSide = 64;      // of a transposed tile
 
+// The job that lane `id` of a launch belongs to; `id` becomes its place there.
+__device__ __forceinline__ PackJob own_job(const PackJobs& jobs, int64_t& id) {
+  PackJob own = jobs.of[0];
+  int64_t before = 0;
+#pragma unroll
+  for (int k = 1; k < 3; ++k)
+    if (k < jobs.count && id >= jobs.of[k - 1].end) {
+      own = jobs.of[k];
+      before = jobs.of[k - 1].end;
+    }
+  id -= before;
+  return own;
+}
+
 // Rows as they are, zeros behind them up to whole pieces; a lane per piece.
 template <class T>
-__global__ __launch_bounds__(kThreads) void pack_kernel(const T* from, int64_t stride, int64_t rows,
-                                                        int64_t columns, uint32_t pieces, T* to) {
+__global__ __launch_bounds__(kThreads) void pack_kernel(PackJobs jobs, int64_t columns, uint32_t pieces) {
   constexpr int kValues = 16 / sizeof(T);
-  const int64_t id = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  if (id >= rows * pieces) return;
+  int64_t id = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  const PackJob job = own_job(jobs, id);
+  if (id >= job.rows * pieces) return;
   const int64_t row = id / pieces, first = (id - row * pieces) * kValues;
-  const T* const in = from + row * stride;
+  const T* const in = static_cast<const T*>(job.from) + row * job.stride;
   Pack<T, kValues> v;
   if (first + kValues <= columns) {
     v = load_pack<T, kValues>(in + first);
@@ -30,16 +44,17 @@ __global__ __launch_bounds__(kThreads) void pack_kernel(const T* from, int64_t s
 #pragma unroll
     for (int k = 0; k < kValues; ++k) v.v[k] = first + k < columns ? in[first + k] : T{};
   }
-  store_pack<T, kValues>(to + id * kValues, v);
+  store_pack<T, kValues>(reinterpret_cast<T*>(job.to) + id * kValues, v);
 }
 
 // float32 rows in thirds; a lane per eight columns.
-__global__ __launch_bounds__(kThreads) void thirds_kernel(const float* from, int64_t stride, int64_t rows,
-                                                          int64_t columns, uint32_t blocks, uint8_t* to) {
-  const int64_t id = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x, lanes = 4 * blocks;
-  if (id >= rows * lanes) return;
+__global__ __launch_bounds__(kThreads) void thirds_kernel(PackJobs jobs, int64_t columns, uint32_t blocks) {
+  int64_t id = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  const int64_t lanes = 4 * static_cast<int64_t>(blocks);
+  const PackJob job = own_job(jobs, id);
+  if (id >= job.rows * lanes) return;
   const int64_t row = id / lanes, first = (id - row * lanes) * 8;
-  const float* const in = from + row * stride;
+  const float* const in = static_cast<const float*>(job.from) + row * job.stride;
   float v[8];
   if (first + 8 <= columns) {
     const Pack<float, 8> all = load_pack<float, 8>(in + first);
@@ -49,7 +64,7 @@ __global__ __launch_bounds__(kThreads) void thirds_kernel(const float* from, int
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = first + j < columns ? in[first + j] : 0.0f;
   }
-  store_thirds(to + row * blocks * kThirds, first, v);
+  store_thirds(job.to + row * blocks * kThirds, first, v);
 }
 
 // A square of values on its way from rows to columns: both ways eight values a lane, eight lanes to
@@ -373,37 +388,30 @@ int run_backward(const ns_gated_args* a, hipStream_t stream) {
   return NS_OK;
 }
 
-template <class T>
-int run_pack(Rows* rows, const void* data, int64_t stride, int64_t columns, int64_t pieces, uint8_t* to,
-             hipStream_t stream) {
-  const int64_t groups = (rows->rows * pieces + kThreads - 1) / kThreads;
-  if (groups > INT32_MAX) return fail("the projection is too large for one launch");
-  pack_kernel<T><<<dim3(static_cast<unsigned>(groups)), dim3(kThreads), 0, stream>>>(
-      static_cast<const T*>(data), stride, rows->rows, columns, static_cast<uint32_t>(pieces),
-      reinterpret_cast<T*>(to));
-  return launched("rows' layout");
-}
-
-int run_thirds(Rows* rows, const void* data, int64_t stride, int64_t columns, int64_t pieces, uint8_t* to,
-               hipStream_t stream) {
-  const int64_t blocks = pieces / (kThirds / 16), groups = (rows->rows * 4 * blocks + kThreads - 1) / kThreads;
-  if (groups > INT32_MAX) return fail("the projection is too large for one launch");
-  thirds_kernel<<<dim3(static_cast<unsigned>(groups)), dim3(kThreads), 0, stream>>>(
-      static_cast<const float*>(data), stride, rows->rows, columns, static_cast<uint32_t>(blocks), to);
-  return launched("rows' layout");
-}
-
 }  // namespace
 
-int pack_rows(Rows* rows, const void* data, int64_t stride, int64_t columns, int32_t type, bool thirds,
-              uint8_t* to, hipStream_t stream) {
-  const int64_t pieces = pieces_of(columns, type, thirds);
+void add_pack(PackJobs* jobs, Rows* rows, const void* data, int64_t stride, int64_t pieces, bool thirds,
+              uint8_t* to) {
+  const int64_t lanes = thirds ? pieces / (kThirds / 16) * 4 : pieces;     // of a row
+  const int64_t before = jobs->count ? jobs->of[jobs->count - 1].end : 0;
+  jobs->of[jobs->count++] = PackJob{data, stride, rows->rows, to, before + rows->rows * lanes};
   rows->data = to;
   rows->stride = pieces * 16;
-  if (pieces == 0) return NS_OK;
-  if (thirds) return run_thirds(rows, data, stride, columns, pieces, to, stream);
-  return type == NS_TYPE_F32 ? run_pack<float>(rows, data, stride, columns, pieces, to, stream)
-                             : run_pack<_Float16>(rows, data, stride, columns, pieces, to, stream);
+}
+
+int run_packs(const PackJobs& jobs, int64_t columns, int64_t pieces, int32_t type, bool thirds,
+              hipStream_t stream) {
+  const int64_t lanes = jobs.count ? jobs.of[jobs.count - 1].end : 0, groups = (lanes + kThreads - 1) / kThreads;
+  if (groups == 0) return NS_OK;
+  if (groups > INT32_MAX) return fail("the projection is too large for one launch");
+  const dim3 grid(static_cast<unsigned>(groups)), threads(kThreads);
+  if (thirds)
+    thirds_kernel<<<grid, threads, 0, stream>>>(jobs, columns, static_cast<uint32_t>(pieces / (kThirds / 16)));
+  else if (type == NS_TYPE_F32)
+    pack_kernel<float><<<grid, threads, 0, stream>>>(jobs, columns, static_cast<uint32_t>(pieces));
+  else
+    pack_kernel<_Float16><<<grid, threads, 0, stream>>>(jobs, columns, static_cast<uint32_t>(pieces));
+  return launched("rows' layout");
 }
 
 // The size whose rounds of tiles over the 256 compute units take the least time.  In units of 0.1

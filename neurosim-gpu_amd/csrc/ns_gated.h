@@ -88,9 +88,22 @@ inline PackedForward packed_forward(const ns_gated_args* a) {
   return w;
 }
 
-// Copies rows of `columns` values to `to`, dense and filled up with zeros, as they are or in thirds.
-int pack_rows(Rows* rows, const void* data, int64_t stride, int64_t columns, int32_t type, bool thirds,
-              uint8_t* to, hipStream_t stream);
+// Rows to copy, dense and filled up with zeros, as they are or in thirds: up to three matrices of as
+// many columns in one launch, since small calls pay by the launch.
+struct PackJob {
+  const void* from;
+  int64_t stride, rows;
+  uint8_t* to;
+  int64_t end;                             // of its lanes, in the launch
+};
+struct PackJobs {
+  PackJob of[3];
+  int count;
+};
+void add_pack(PackJobs* jobs, Rows* rows, const void* data, int64_t stride, int64_t pieces, bool thirds,
+              uint8_t* to);
+int run_packs(const PackJobs& jobs, int64_t columns, int64_t pieces, int32_t type, bool thirds,
+              hipStream_t stream);
 
 int check_gated(const ns_gated_args* a);
 bool few_rows(const ns_gated_args* a);
