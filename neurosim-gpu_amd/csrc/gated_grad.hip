@@ -6,7 +6,7 @@
 // kernels read their operands along the sum.  So dg and du, rounded once to the operands' type, are
 // written both ways by the pass that computes them, and x and the weights are transposed first:
 // passes over memory that cost some tenth of the products: 8192 x 4096 to 8192 in bf16, products
-// 745 to 840 us each (1.3 to 1.5 PFLOP/s, the matrix cores 73% busy), dg and du 267, transposes 33 to 37.
+// 755 to 850 us each (1.3 to 1.5 PFLOP/s, the matrix cores 73% busy), dg and du 267, transposes 102.
 #include "ns_gated.h"
 
 namespace ns {

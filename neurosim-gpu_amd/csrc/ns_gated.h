@@ -56,10 +56,10 @@ inline Rows plain_rows(const void* data, int64_t stride, int64_t rows, int64_t c
               rows <= 1 ? pieces_of(columns, type, false) * 16 : stride * type_size(type), rows};
 }
 
-// Whether a forward lays float32 rows out in thirds, three passes over the operands that few rows
-// or small products do not repay.  Us, as they are / in thirds, M x K to F: 64 x 4096 to 4096 72 / 177,
-// 256 x 2048 to 2048 37.8 / 59.6, 512 x 2048 to 2048 68 / 70, 1000 x 500 to 1000 20.7 / 29.4, 700 x 3000 to 900
-// 98 / 90, 1024 x 1024 to 2048 67 / 56, 2048^3 243 / 168.
+// Whether a forward lays float32 rows out in thirds, a pass over the operands that few rows or small
+// products do not repay.  Us, as they are / in thirds, M x K to F: 64 x 4096 to 4096 72 / 163, 256 x
+// 2048 to 2048 37.6 / 56.3, 512 x 2048 to 2048 68.0 / 67.3, 1000 x 500 to 1000 20.6 / 24.7, 700 x 3000 to 900
+// 98 / 85, 1024 x 1024 to 2048 67 / 49, 2048^3 243 / 164.
 inline bool in_thirds(const ns_gated_args* a) {
   constexpr int64_t kRepays = 200, kProducts = 1500000000;
   const int64_t results = a->rows * a->width;
