@@ -37,7 +37,9 @@ int ns_dropout(const ns_dropout_args* args, void* stream);
 
 /* Gated projection of M rows of K values to F: g = x gate^T, u = x up^T, y = f(g) u, with
  * f(g) = g sigmoid(g) or g Phi(g), Phi the normal distribution function.  Sums are float32.
- * Rows are dense, at strides in elements. */
+ * Rows are dense, at strides in elements.  A backward rounds dg = dy u f'(g) and du = dy f(g) to
+ * the type before it multiplies them (float16: as multiples of a power of two per row and column,
+ * which keep them in range). */
 #define NS_GATE_SILU 0
 #define NS_GATE_GELU 1
 #define NS_GATED_MAX_COLUMNS (1 << 20)     /* of K and of F */

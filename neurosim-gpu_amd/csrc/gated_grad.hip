@@ -3,9 +3,10 @@
 //   dg = dy u f'(g),  du = dy f(g)
 //   dx = [dg du] [gate; up],  [dgate; dup] = [dg du]^T x
 // The sums of dx run over columns of y, those of the weights over rows of x, and the tile
-// kernels read their operands along the sum.  So dg and du, rounded once to the operands' type, are
-// written both ways by the pass that computes them, and x and the weights are transposed first:
-// passes over memory that cost some tenth of the products: 8192 x 4096 to 8192 in bf16, products
+// kernels read their operands along the sum.  So dg and du, rounded once to the operands' type (the
+// matrix cores multiply 16-bit numbers with 16-bit numbers; two parts of each would double the
+// products), are written both ways by the pass that computes them, and x and the weights are
+// transposed first: passes over memory that cost some tenth of the products: 8192 x 4096 to 8192 in bf16, products
 // 755 to 850 us each (1.3 to 1.5 PFLOP/s, the matrix cores 73% busy), dg and du 267, transposes 102.
 #include "ns_gated.h"
 
@@ -150,6 +151,126 @@ __global__ __launch_bounds__(kThreads) void transpose_kernel(Turns turns) {
   store_turned<T>(square, t.to, t.stride, r0, t.filled, c0, t.columns);
 }
 
+// float16 holds neither a product dy u beyond 65504 nor, to all its bits, one below 2^-14, though the
+// gradients that they are summed to may well be in its range.  So its dg and du are rounded as multiples
+// of a power of two, one for each row of [dg du] (a row of dx) and one for each of their columns (a row
+// of the weights' gradients): that which brings the largest finite one to [2^14, 2^15).  The product's
+// sums are multiplied back in float32.  Where a number is still below float16's normal ones, it is off
+// by at most 2^-39 of the largest.  Finding them costs a pass over what dg and du come from: a training
+// pass of 8192 x 4096 to 8192 2916 -> 3107 us, of 1000 x 500 to 1000 126 -> 135.  bfloat16 has float32's
+// range and needs none of this.
+template <class T>
+constexpr bool kRanged = __is_same(T, _Float16);
+
+// The largest finite sizes, as bits of a float32 (whose order is theirs).
+struct Extremes {
+  uint32_t* row;               // [M], or NULL
+  uint32_t* column;            // [2 F], or NULL
+};
+__device__ __forceinline__ uint32_t size_bits(float v) {
+  const uint32_t bits = __builtin_bit_cast(uint32_t, v) & 0x7FFFFFFFu;
+  return bits < 0x7F800000u ? bits : 0;
+}
+// 2^(14 - e) of a largest size 2^e .. 2^(e+1), at most 2^126, and its inverse.
+__device__ __forceinline__ float into_range(uint32_t largest) {
+  const uint32_t e = largest >> 23 < 15 ? 15 : largest >> 23;
+  return __builtin_bit_cast(float, (268 - e) << 23);
+}
+__device__ __forceinline__ float out_of_range(uint32_t largest) {
+  const uint32_t e = largest >> 23 < 15 ? 15 : largest >> 23;
+  return __builtin_bit_cast(float, (e - 14) << 23);
+}
+
+// Eight neighbouring values of both products and of dy, zeros where there are none.
+template <class T>
+struct GateInputs {
+  Pack<float, kWide> gate, raised;
+  Pack<T, kWide> up;
+};
+template <class T>
+__device__ __forceinline__ GateInputs<T> load_gate_inputs(const float* pre, const T* dy, int64_t dy_stride,
+                                                          int64_t m, int64_t f, int64_t rows,
+                                                          int64_t width) {
+  GateInputs<T> in{};
+  const int64_t plane = rows * width, left = width - f;
+  if (m < rows && left >= kWide) {
+    in.gate = load_pack<float, kWide>(pre + m * width + f);
+    in.raised = load_pack<float, kWide>(pre + plane + m * width + f);
+    in.up = load_pack<T, kWide>(dy + m * dy_stride + f);
+  } else if (m < rows) {
+#pragma unroll
+    for (int j = 0; j < kWide; ++j) {
+      if (j >= left) continue;
+      in.gate.v[j] = pre[m * width + f + j];
+      in.raised.v[j] = pre[plane + m * width + f + j];
+      in.up.v[j] = dy[m * dy_stride + f + j];
+    }
+  }
+  return in;
+}
+
+// dg and du of value j.
+struct GateGradients {
+  float gate, up;
+};
+template <class T>
+__device__ __forceinline__ GateGradients gate_gradients_of(const GateInputs<T>& in, int j, int activation) {
+  const Activation a = activated_slope(in.gate.v[j], activation);
+  const float own = static_cast<float>(in.up.v[j]);
+  return GateGradients{own * in.raised.v[j] * a.slope, own * a.value};
+}
+
+__global__ __launch_bounds__(kThreads) void clear_words(uint32_t* words, int64_t count) {
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  if (id < count) words[id] = 0;
+}
+
+// The extremes of dg and du, a workgroup per square.  The largest of some numbers is the same in any
+// order, so the atomics change no result.
+template <class T>
+__global__ __launch_bounds__(kThreads) void gate_extremes(const float* pre, const T* dy, int64_t dy_stride,
+                                                          int64_t rows, int64_t width, int activation,
+                                                          Extremes to, uint32_t tiles_f) {
+  __shared__ uint32_t own[2][kSide];
+  const uint32_t tile_m = uniform(blockIdx.x / tiles_f), tile_f = blockIdx.x - tile_m * tiles_f;
+  const int64_t m0 = static_cast<int64_t>(tile_m) * kSide, f0 = static_cast<int64_t>(tile_f) * kSide;
+  const int side = threadIdx.x % kSquareLanes * kWide;
+  if (threadIdx.x < 2 * kSide) own[threadIdx.x / kSide][threadIdx.x % kSide] = 0;
+  __syncthreads();
+  uint32_t largest[2][kWide] = {};
+#pragma unroll
+  for (int k = 0; k < kSide; k += kLines) {
+    const int64_t m = m0 + k + threadIdx.x / kSquareLanes;
+    const GateInputs<T> in = load_gate_inputs<T>(pre, dy, dy_stride, m, f0 + side, rows, width);
+    uint32_t of_row = 0;
+#pragma unroll
+    for (int j = 0; j < kWide; ++j) {
+      const GateGradients d = gate_gradients_of<T>(in, j, activation);
+      const uint32_t size[2] = {size_bits(d.gate), size_bits(d.up)};
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        of_row = of_row > size[half] ? of_row : size[half];
+        largest[half][j] = largest[half][j] > size[half] ? largest[half][j] : size[half];
+      }
+    }
+#pragma unroll
+    for (int step = 1; step < kSquareLanes; step *= 2) {
+      const uint32_t other = __shfl_xor(of_row, step);
+      of_row = of_row > other ? of_row : other;
+    }
+    if (to.row && m < rows && threadIdx.x % kSquareLanes == 0) atomicMax(to.row + m, of_row);
+  }
+  if (!to.column) return;
+#pragma unroll
+  for (int half = 0; half < 2; ++half)
+#pragma unroll
+    for (int j = 0; j < kWide; ++j) atomicMax(&own[half][side + j], largest[half][j]);
+  __syncthreads();
+  const int half = threadIdx.x / kSide;
+  const int64_t f = f0 + threadIdx.x % kSide;
+  if (half < 2 && f < width) atomicMax(to.column + half * width + f, own[half][threadIdx.x % kSide]);
+}
+
 // dg and du: as laid-out rows [M][2 F'], du behind dg, and as columns [2 F][M'], each padded with
 // zeros to whole pieces (F', M').
 template <class T>
@@ -158,40 +279,44 @@ __global__ __launch_bounds__(kThreads) void gate_gradients(const float* pre, con
                                                            uint8_t* by_row, int64_t row_half,
                                                            int64_t row_stride, uint8_t* by_column,
                                                            int64_t filled, int64_t column_stride,
-                                                           uint32_t tiles_f) {
+                                                           Extremes extremes, uint32_t tiles_f) {
   __shared__ Square<T> square[2];
   const uint32_t tile_m = uniform(blockIdx.x / tiles_f), tile_f = blockIdx.x - tile_m * tiles_f;
   const int64_t m0 = static_cast<int64_t>(tile_m) * kSide, f0 = static_cast<int64_t>(tile_f) * kSide;
   const int side = threadIdx.x % kSquareLanes * kWide;
-  const int64_t plane = rows * width, f = f0 + side, left = width - f;
+  const int64_t f = f0 + side;
+  float of_column[2][kWide];
+  if constexpr (kRanged<T>) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+#pragma unroll
+      for (int j = 0; j < kWide; ++j)
+        of_column[half][j] =
+            into_range(by_column && f + j < width ? extremes.column[half * width + f + j] : 0);
+  }
 #pragma unroll
   for (int k = 0; k < kSide; k += kLines) {
     const int line = k + threadIdx.x / kSquareLanes;
     const int64_t m = m0 + line;
-    Pack<float, kWide> gate{}, raised{};
-    Pack<T, kWide> up{}, g, u;
-    if (m < rows && left >= kWide) {
-      gate = load_pack<float, kWide>(pre + m * width + f);
-      raised = load_pack<float, kWide>(pre + plane + m * width + f);
-      up = load_pack<T, kWide>(dy + m * dy_stride + f);
-    } else if (m < rows) {
-#pragma unroll
-      for (int j = 0; j < kWide; ++j) {
-        if (j >= left) continue;
-        gate.v[j] = pre[m * width + f + j];
-        raised.v[j] = pre[plane + m * width + f + j];
-        up.v[j] = dy[m * dy_stride + f + j];
-      }
-    }
+    const GateInputs<T> in = load_gate_inputs<T>(pre, dy, dy_stride, m, f, rows, width);
+    float of_row = 1.0f;
+    if constexpr (kRanged<T>) of_row = into_range(by_row && m < rows ? extremes.row[m] : 0);
+    Pack<T, kWide> g, u;
 #pragma unroll
     for (int j = 0; j < kWide; ++j) {
       // Zeros where there is nothing: rows and columns of padding stay zero.
-      const Activation a = activated_slope(gate.v[j], activation);
-      const float own = static_cast<float>(up.v[j]);
-      g.v[j] = static_cast<T>(own * raised.v[j] * a.slope);
-      u.v[j] = static_cast<T>(own * a.value);
-      square[0].at[line][side + j] = g.v[j];
-      square[1].at[line][side + j] = u.v[j];
+      const GateGradients d = gate_gradients_of<T>(in, j, activation);
+      if constexpr (kRanged<T>) {
+        g.v[j] = static_cast<T>(d.gate * of_row);
+        u.v[j] = static_cast<T>(d.up * of_row);
+        square[0].at[line][side + j] = static_cast<T>(d.gate * of_column[0][j]);
+        square[1].at[line][side + j] = static_cast<T>(d.up * of_column[1][j]);
+      } else {
+        g.v[j] = static_cast<T>(d.gate);
+        u.v[j] = static_cast<T>(d.up);
+        square[0].at[line][side + j] = g.v[j];
+        square[1].at[line][side + j] = u.v[j];
+      }
     }
     if (by_row && m < rows && f < row_half) {
       store_laid<T>(by_row + m * row_stride, f, g);
@@ -204,11 +329,11 @@ __global__ __launch_bounds__(kThreads) void gate_gradients(const float* pre, con
   store_turned<T>(square[1], by_column + width * column_stride, column_stride, m0, filled, f0, width);
 }
 
-// out = a b^T, one workgroup per tile.
+// out = a b^T, one workgroup per tile; kRanged types have a's rows' largest sizes and undo their factors.
 template <class G, class T>
 __global__ __launch_bounds__(G::threads, 512 / G::threads) void gemm_tiles(Rows a, Rows b, uint32_t pieces, T* out,
-                                                         int64_t stride, uint32_t tiles_m,
-                                                         uint32_t tiles_n) {
+                                                         int64_t stride, const uint32_t* largest,
+                                                         uint32_t tiles_m, uint32_t tiles_n) {
   __shared__ union {
     v4i stages[G::stages * G::rows * 8];
     Strip<G, T> strip[G::WM * G::WN];
@@ -228,6 +353,15 @@ __global__ __launch_bounds__(G::threads, 512 / G::threads) void gemm_tiles(Rows 
   v4f sum[G::MI][G::NJ] = {};
   gemm_tile<G, T, false>(p, second, lds.stages, sum);
   const int64_t m = m0 + 16 * (wave / G::WN) * G::MI, n = n0 + 16 * (wave % G::WN) * G::NJ;
+  if constexpr (kRanged<T>) {
+#pragma unroll
+    for (int i = 0; i < G::MI; ++i) {
+      const int64_t row = m + 16 * i + (lane & 15);
+      const float back = out_of_range(row < a.rows ? largest[row] : 0);
+#pragma unroll
+      for (int j = 0; j < G::NJ; ++j) sum[i][j] *= back;
+    }
+  }
   store_tiles<G, T, false>(out + m * stride + n, stride, sum, nullptr, a.rows - m, b.rows - n, lane,
                            lds.strip[wave]);
 }
@@ -288,7 +422,8 @@ int run_turns(const Turns& turns, hipStream_t stream) {
 }
 
 template <class G, class T>
-int product_of(const Rows& a, const Rows& b, int64_t pieces, T* out, int64_t stride, hipStream_t stream) {
+int product_of(const Rows& a, const Rows& b, int64_t pieces, T* out, int64_t stride, const uint32_t* largest,
+               hipStream_t stream) {
   const int64_t tiles_m = (a.rows + G::rows_m - 1) / G::rows_m;
   const int64_t tiles_n = (b.rows + G::rows_n - 1) / G::rows_n;
   const auto count_m = static_cast<uint32_t>(tiles_m), count_n = static_cast<uint32_t>(tiles_n);
@@ -299,32 +434,34 @@ int product_of(const Rows& a, const Rows& b, int64_t pieces, T* out, int64_t str
         a, b, static_cast<uint32_t>(pieces / (kThirds / 16)), out, stride, count_m, count_n);
   else
     gemm_tiles<G, T><<<grid, dim3(G::threads), 0, stream>>>(a, b, static_cast<uint32_t>(pieces), out, stride,
-                                                            count_m, count_n);
+                                                            largest, count_m, count_n);
   return launched("product");
 }
 
 template <class T>
 int product(const Rows& a, const Rows& b, int64_t pieces, int32_t type, T* out, int64_t stride,
-            hipStream_t stream) {
+            const uint32_t* largest, hipStream_t stream) {
   const GemmSize size = gemm_size(a.rows, b.rows, type, sizeof(T) == 4);
   if constexpr (sizeof(T) == 4) {
-    return size == GemmSize::kMiddle ? product_of<MiddleSplit, T>(a, b, pieces, out, stride, stream)
-                                     : product_of<SmallSplit, T>(a, b, pieces, out, stride, stream);
+    return size == GemmSize::kMiddle ? product_of<MiddleSplit, T>(a, b, pieces, out, stride, largest, stream)
+                                     : product_of<SmallSplit, T>(a, b, pieces, out, stride, largest, stream);
   } else {
     switch (size) {
-      case GemmSize::kLarge: return product_of<LargeGemm, T>(a, b, pieces, out, stride, stream);
-      case GemmSize::kMiddle: return product_of<MiddleGemm, T>(a, b, pieces, out, stride, stream);
-      default: return product_of<SmallGemm, T>(a, b, pieces, out, stride, stream);
+      case GemmSize::kLarge: return product_of<LargeGemm, T>(a, b, pieces, out, stride, largest, stream);
+      case GemmSize::kMiddle: return product_of<MiddleGemm, T>(a, b, pieces, out, stride, largest, stream);
+      default: return product_of<SmallGemm, T>(a, b, pieces, out, stride, largest, stream);
     }
   }
 }
 
 // The backward's workspace: dg and du as laid-out rows of 2 F' values and as columns of M', the
-// weights transposed (rows of 2 F'), x transposed (rows of M').
+// weights transposed (rows of 2 F'), x transposed (rows of M'), and for float16 the largest sizes of
+// dg's and du's rows and columns.
 struct BackwardSpace {
   int64_t half, filled;                    // F' and M'
   int64_t row_bytes, column_bytes;         // of rows of 2 F', and of M'
-  int64_t by_column, weights, x, bytes;
+  int64_t by_column, weights, x, extremes, bytes;
+  int64_t row_extremes, column_extremes;   // how many
 };
 BackwardSpace backward_space(const ns_gated_args* a) {
   BackwardSpace w{};
@@ -336,7 +473,11 @@ BackwardSpace backward_space(const ns_gated_args* a) {
   w.by_column = a->dx ? a->rows * w.row_bytes : 0;
   w.weights = w.by_column + (a->dweights ? 2 * a->width * w.column_bytes : 0);
   w.x = w.weights + (a->dx ? a->columns * w.row_bytes : 0);
-  w.bytes = w.x + (a->dweights ? a->columns * w.column_bytes : 0);
+  w.extremes = w.x + (a->dweights ? a->columns * w.column_bytes : 0);
+  const bool ranged = a->type == NS_TYPE_F16;
+  w.row_extremes = ranged && a->dx ? a->rows : 0;
+  w.column_extremes = ranged && a->dweights ? 2 * a->width : 0;
+  w.bytes = w.extremes + 4 * (w.row_extremes + w.column_extremes);
   return w;
 }
 
@@ -351,9 +492,22 @@ int run_backward(const ns_gated_args* a, hipStream_t stream) {
   const int64_t tiles_m = (w.filled + kSide - 1) / kSide, tiles_f = (w.half + kSide - 1) / kSide;
   dim3 grid;
   if (int rc = tile_grid(tiles_m, tiles_f, &grid)) return rc;
+  Extremes extremes{};
+  if constexpr (kRanged<T>) {
+    auto* const words = reinterpret_cast<uint32_t*>(space + w.extremes);
+    const int64_t count = w.row_extremes + w.column_extremes;      // 2^22 at most
+    extremes = Extremes{by_row ? words : nullptr, by_column ? words + w.row_extremes : nullptr};
+    clear_words<<<dim3(static_cast<unsigned>((count + kThreads - 1) / kThreads)), dim3(kThreads), 0, stream>>>(
+        words, count);
+    if (int rc = launched("gate gradients' range")) return rc;
+    gate_extremes<T><<<grid, dim3(kThreads), 0, stream>>>(
+        a->pre, static_cast<const T*>(a->dy), a->dy_stride, a->rows, a->width, a->activation, extremes,
+        static_cast<uint32_t>(tiles_f));
+    if (int rc = launched("gate gradients' range")) return rc;
+  }
   gate_gradients<T><<<grid, dim3(kThreads), 0, stream>>>(
       a->pre, static_cast<const T*>(a->dy), a->dy_stride, a->rows, a->width, a->activation, by_row, w.half,
-      w.row_bytes, by_column, w.filled, w.column_bytes, static_cast<uint32_t>(tiles_f));
+      w.row_bytes, by_column, w.filled, w.column_bytes, extremes, static_cast<uint32_t>(tiles_f));
   if (int rc = launched("gate gradients")) return rc;
   // Small calls pay by the launch, so x is turned with the weights; a large one is turned when its
   // product is next, from whose caches it then comes.  Us, all at once / x later: 1000 x 500 to 1000 in
@@ -372,7 +526,7 @@ int run_backward(const ns_gated_args* a, hipStream_t stream) {
     if (int rc = run_turns<T>(turns, stream)) return rc;
     const Rows left{by_row, w.row_bytes, a->rows}, right{weights, w.row_bytes, a->columns};
     if (int rc = product<T>(left, right, w.row_bytes / 16, a->type, static_cast<T*>(a->dx), a->columns,
-                            stream))
+                            extremes.row, stream))
       return rc;
   }
   if (a->dweights) {
@@ -383,7 +537,7 @@ int run_backward(const ns_gated_args* a, hipStream_t stream) {
     }
     const Rows left{by_column, w.column_bytes, 2 * a->width}, right{x, w.column_bytes, a->columns};
     return product<T>(left, right, w.column_bytes / 16, a->type, static_cast<T*>(a->dweights), a->columns,
-                      stream);
+                      extremes.column, stream);
   }
   return NS_OK;
 }

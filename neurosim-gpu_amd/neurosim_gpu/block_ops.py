@@ -5,7 +5,8 @@
 * ``dropout``: elements kept by a counter-based generator, whose mask is computed anew where
   it is used and never stored; optionally added to a residual in the same pass.
 
-float32, bfloat16 and float16 are taken; sums are float32 and each output is rounded once.
+float32, bfloat16 and float16 are taken; sums are float32 and each output is rounded once.  The
+projection's 16-bit gradients multiply dg and du (``gated_projection``) rounded to that type too.
 Forward-mode derivatives are refused, and so is a backward under graph capture.  The kernels
 are csrc/gated.hip, gated_grad.hip and dropout.hip behind include/neurosim_hip_block.h; calls run
 on the current stream, allocate their outputs and workspaces from torch, and never synchronise.
@@ -110,7 +111,11 @@ def gated_projection(x: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, *,
     or with a single one; up to 16 rows are bound by the weights' bytes.  Large float32 calls,
     and all float32 gradients, are multiplied in three bfloat16 parts at float32's precision;
     an infinity in x or a weight then makes its row or column NaN.  A call with gradients takes
-    up to 2^21 rows and keeps both products in float32 for its backward."""
+    up to 2^21 rows and keeps both products in float32 for its backward, whose
+    ``dg = dy u f'(g)`` and ``du = dy f(g)`` (g and u: the two products) are rounded to x's type
+    before they are multiplied: half a unit of a 16-bit type more than float32 between the
+    products would leave.  In float16 they are rounded as multiples of a power of two per row and
+    column, so only the gradients themselves have to be in its range."""
     if activation not in ACTIVATIONS:
         raise ValueError("activation must be 'silu' or 'gelu'")
     if not isinstance(x, torch.Tensor) or x.dim() < 1 or x.dtype not in TYPES:
