@@ -120,7 +120,7 @@ int ns_scan_backward(const ns_scan_args* args, void* stream);
 /* Gated linear recurrence, one state per channel:
  *   s = sigmoid(forget), i = sigmoid(write), a = exp(-rates[n] s)
  *   h[t,b,n] = a h[t-1] + sqrt(1 - a^2) i x,   y = h silu(z)   (z optional)
- * Rates are not negative (a negative one counts as 0). */
+ * Rates are not negative (a negative one counts as 0, and its gradient is 0). */
 typedef struct ns_recurrence_args {
   int64_t ticks, batch, channels;
   int32_t type;                /* NS_TYPE_* of all signals (states and rates float32) */

@@ -7,7 +7,8 @@
 //   dforget = k u (1 - s),  drates = sum of k s
 // The states are walked again from those kept at each tile's start; the adjoint's stretch of
 // ticks has the same decay as the state's, so both meet in LDS at once: one barrier a tile.
-// At u = 0 the term a^2/m, which grows without bound there, is left out.
+// At u = 0 the term a^2/m, which grows without bound there, is left out.  A rate below zero counts
+// as zero, and its gradient is zero.
 //
 // Bound as the forward is: 2048 ticks of 8 x 4096 in bf16 with a gate (1208 MB) 337 us, 3.6 TB/s, the
 // vector ALU 77% busy.
@@ -294,6 +295,10 @@ __global__ __launch_bounds__(kGradThreads) void recur_backward(RecurShape s, Rec
   for (int w = 1; w < kWaves; ++w)
 #pragma unroll
     for (int j = 0; j < V; ++j) sum[j] += meet[0][w][lane].decay[j];
+  // What is computed with a rate below zero does not depend on it.
+  load_floats<V>(in.rates, p, rate);
+#pragma unroll
+  for (int j = 0; j < V; ++j) sum[j] = rate[j] < 0.0f ? 0.0f : sum[j];
   store_floats<V>(partials + p.c * lines + row, p, sum);
 }
 

@@ -580,8 +580,8 @@ def gated_recurrence(x: torch.Tensor, forget: torch.Tensor, write: torch.Tensor,
 
     ``forget``, ``write`` and the optional output gate ``z`` are [T, B, N], as before their
     sigmoids and silu; ``rates`` [N] float32 is how fast a channel with an open gate forgets
-    (positive; a negative rate counts as 0, where a gradient leaves out the input's part,
-    which has no bound there).  ``state`` [B, N] float32 is h before the first tick (zeros if
+    (positive; at a rate of 0 gradients leave out the input's part, which has no bound there,
+    and a negative rate counts as 0 and has a gradient of 0).  ``state`` [B, N] float32 is h before the first tick (zeros if
     absent).
 
     Returns ``(y, state)``: y [T, B, N] of x's type and h after each column's last tick.
