@@ -15,8 +15,8 @@ float32 and each output is rounded once.
   with ``a = exp(-rates sigmoid(forget))``.
 
 All take and return the state that carries a signal on (``history``, ``state``), give
-native gradients of every tensor input (forward-mode derivatives are refused), and have a
-one-tick form that updates the carried state in place.  ``lengths`` gives columns their own
+native gradients of every tensor input (forward-mode derivatives are refused, and so is a
+backward under graph capture), and have a one-tick form that updates the carried state in place.  ``lengths`` gives columns their own
 number of ticks: past it outputs and gradients are zero, the carried state stays that of the
 column's last tick, and what the inputs hold there is never used.  The kernels are
 csrc/conv.hip, scan.hip, scan_grad.hip, recur.hip and recur_grad.hip behind
@@ -187,7 +187,8 @@ def _needs_grad(*values) -> bool:
 
 def refuse_capture(what: str) -> None:
     """A backward that is captured into a graph while an eager graph of the same leaves lives
-    ends the process inside the runtime: none of these is captured."""
+    ends the process inside the runtime, whichever operators it runs through: no operator's
+    backward here is captured."""
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError(f"the backward of {what} cannot be captured into a graph")
 
@@ -244,6 +245,7 @@ class _CausalConv(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dlast):
+        refuse_capture("causal_conv")
         x, weight, bias, history, lengths = ctx.saved_tensors
         wants, device = ctx.needs_input_grad, x.device
         (ticks, batch, channels), taps = x.shape, weight.shape[1]
@@ -408,6 +410,7 @@ class _SelectiveScan(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dfinal):
+        refuse_capture("selective_scan")
         *operands, lengths, kept = ctx.saved_tensors
         x, delta, A, B, C, D, z, delta_bias = operands
         wants, device = ctx.needs_input_grad, x.device
