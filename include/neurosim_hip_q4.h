@@ -44,8 +44,9 @@ int ns_q4_quantize(const ns_q4_matrix* matrix, const void* x, int64_t stride, in
 int ns_q4_dequantize(const ns_q4_matrix* matrix, void* out, int64_t stride, int32_t type,
                      void* stream);
 
-/* y[m][n] = sum_k x[m][k] weight[n][k] + bias[n], products and sums in float32 or finer,
- * rounded to `type`.  A row of x that holds an infinity or a NaN gives NaN, and one with values
+/* y[m][n] = sum_k x[m][k] weight[n][k] + bias[n], sums in float32, rounded to `type`.  The sum of a
+ * group (of 128 columns at most) is off by some 2^-24 of scale (16 + zero) sum |x|, in float32 of
+ * scale (16 + zero) sum |x - their mean|, columns of weight zero among them.  A row of x that holds an infinity or a NaN gives NaN, and one with values
  * beyond 2^115, 128 of which times a code pass float32, may. */
 typedef struct ns_q4_product_args {
   ns_q4_matrix weight;

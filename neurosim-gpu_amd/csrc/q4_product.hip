@@ -1,15 +1,20 @@
 // Product of float rows and a matrix of 4-bit integers with group scales (gfx950):
 // y[m][n] = sum over groups g of scale[n][g] * sum over k in g of x[m][k] (code[n][k] - zero[n][g]).
 //
-// Bound by the codes' bytes for few rows, so their way through the registers has to be short.
-// The sum over a group runs on the matrix cores with exact operands: a code u is put, by a shift
-// and one and-or, into the mantissa of 16 as the 16-bit number 16 + u, two at a time, and
-// sum x (16 + u) - (16 + zero) sum x is scaled in float32, the sums of x coming from the same
-// instruction with ones as weights.  16-bit rows go in as they are.  For float32 rows the 16 +
-// zero that is taken off again would cost some bits where x has a mean, so a row goes in as
-// x - c, c its mean over the group, in three bfloat16 parts that together are exact, with a
-// fourth row of ones that gives c its share: sum x (u - zero) = sum (x - c)(u - zero) +
-// c (sum (16 + u) - count (16 + zero)), whose factor of c is exact.
+// For few rows the codes' bytes are what has to be read, so their way through the registers has to be
+// short.  The sum over a group runs on the matrix cores: a code u is put, by a shift and one
+// and-or, into the mantissa of 16 as the 16-bit number 16 + u, two at a time, and sum x (16 + u) -
+// (16 + zero) sum x is scaled in float32, the sums of x coming from the same instruction with ones
+// as weights.  16-bit rows go in as they are.  For float32 rows the 16 + zero that is taken off
+// again would cost some bits where x has a mean, so a row goes in as x - c, c its mean over the
+// group, rounded to float32 and split into three bfloat16 parts, with a fourth row of ones that
+// gives c its share: sum x (u - zero) = sum (x - c)(u - zero) + c (sum (16 + u) - count (16 +
+// zero)), whose factor of c is exact.
+//
+// Operands and their products are exact, the sums are float32's: a group's is off by some 2^-24 of
+// (16 + zero) sum |x|, for float32 rows of (16 + zero) sum |x - c| (sums go over 128 columns at most).
+// That is some five times what a sum of x (u - zero) would be off by, and counts columns whose
+// weight is zero: one value much larger than its group's others costs them bits there too.
 //
 // What bounds it now: requests.  One of 16 rows, 64 bytes each, takes a compute unit some 50 cycles
 // whatever it brings, and the instruction's layout asks for such ones, of the codes (33.5 MB of 16 x

@@ -102,3 +102,19 @@ def test_products(gpu, dtype, shape):
     for group in groups:
         weight = weight_of(draw, gpu, N, K, group, zeros=(M + group) % 3 > 0)
         check_product((draw(M, K) + 0.5).to(dtype), *weight, bias=draw(N))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M", [2, 6, 30, 70])
+def test_a_large_value_on_a_weight_of_zero(gpu, dtype, M):
+    """It adds nothing to the result, but to its error: within the same bounds, which count |x| (for
+    float32 its distance from the mean) whatever its weight."""
+    draw = Draw(gpu, M)
+    N, K = 90, 700
+    x = draw(M, K).to(dtype)
+    x[:, 130] = 2.0 ** 14
+    for group in GROUPS[:3]:
+        _, codes, scale, zero = weight_of(draw, gpu, N, K, group, zeros=True)
+        codes[:, 130] = zero[:, 130 // group]
+        weight = Q4Tensor(bo.q4_pack(codes).to(gpu), scale.to(gpu), zero.to(gpu), K, group)
+        check_product(x, weight, codes, scale, zero)
