@@ -5,6 +5,7 @@
 // the nine products of two numbers' parts are summed; x1 y2, x2 y1 and x2 y2, left out, are together
 // at most 2^-23 of x y, as much as two roundings of a float32 product.  The matrix cores multiply
 // bfloat16 16 times as fast as float32, so six products take 3/8 of the time of one in float32.
+// Parts below bfloat16's least number, 2^-133, are lost: an x below 2^-109 keeps fewer bits.
 //
 // Rows lie in thirds: for every 32 columns 64 bytes of x0, of x1 and of x2, zeros past the last
 // column.  A stage is one such block of every row of both operands; in LDS a part's 64 bytes of a

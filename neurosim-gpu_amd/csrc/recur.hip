@@ -3,8 +3,9 @@
 //
 // Bound by memory and, nearly as much, by the elementwise part: two sigmoids, an exp2, a root and the
 // series are some 40 slots of the vector ALU a tick and channel, which it is 72 to 76% busy with.
-// 2048 ticks of 8 x 4096 in bf16 with a gate (671 MB) take 155 us, 4.3 TB/s; 16,384 of 2048
-// channels (335 MB) 114: the chunks' ends 48, at 4.2 TB/s, and the outputs 70, at 4.8.
+// 2048 ticks of 8 x 4096 in bf16 with a gate (671 MB) take 148 us in passes back to back (the average
+// of 40; 174 in the first ones), 4.5 TB/s; 16,384 of 2048 channels (335 MB) 114: the chunks' ends 48, at
+// 4.2 TB/s, and the outputs 70, at 4.8.
 #include "ns_recur.h"
 
 namespace ns {

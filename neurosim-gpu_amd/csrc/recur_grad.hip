@@ -10,8 +10,8 @@
 // At u = 0 the term a^2/m, which grows without bound there, is left out.  A rate below zero counts
 // as zero, and its gradient is zero.
 //
-// Bound as the forward is: 2048 ticks of 8 x 4096 in bf16 with a gate (1208 MB) 337 us, 3.6 TB/s, the
-// vector ALU 77% busy.
+// Bound as the forward is: 2048 ticks of 8 x 4096 in bf16 with a gate (1208 MB) 316 us in passes back to
+// back (the average of 40; 385 in the first ones), 3.8 TB/s, the vector ALU 77% busy.
 #include "ns_recur.h"
 
 namespace ns {
