@@ -46,8 +46,9 @@ int ns_q4_dequantize(const ns_q4_matrix* matrix, void* out, int64_t stride, int3
 
 /* y[m][n] = sum_k x[m][k] weight[n][k] + bias[n], sums in float32, rounded to `type`.  The sum of a
  * group (of 128 columns at most) is off by some 2^-24 of scale (16 + zero) sum |x|, in float32 of
- * scale (16 + zero) sum |x - their mean|, columns of weight zero among them.  A row of x that holds an infinity or a NaN gives NaN, and one with values
- * beyond 2^115, 128 of which times a code pass float32, may. */
+ * scale (16 + zero) sum |x - their mean|, columns of weight zero among them.  A row of x that holds
+ * an infinity or a NaN gives NaN, and one with values beyond 2^115, 128 of which times a code pass
+ * float32, may. */
 typedef struct ns_q4_product_args {
   ns_q4_matrix weight;
   int64_t rows;                /* M */

@@ -146,8 +146,9 @@ def q4_product(x: torch.Tensor, weight: Q4Tensor, *, bias: torch.Tensor | None =
     groups, result [..., N] of x's type.  Sums are float32 and the result is rounded once.  A
     group's sum (of 128 columns at most) is off by some 2^-24 of its scale times (16 + zero) times
     the sum of |x|, for float32 rows of |x - their mean|: a value much larger than its
-    neighbours costs them bits even where its own weight is zero.  A row of x that holds an infinity or a NaN gives NaN, and one with values
-    beyond 2^115, 128 of which times a code pass float32, may."""
+    neighbours costs them bits even where its own weight is zero.  A row of x that holds an
+    infinity or a NaN gives NaN, and one with values beyond 2^115, 128 of which times a code
+    pass float32, may."""
     if not isinstance(weight, Q4Tensor) or weight.codes.dim() != 2:
         raise ValueError("weight must be a Q4Tensor of [N, K]")
     if not isinstance(x, torch.Tensor) or x.dim() < 1 or x.dtype not in TYPES:

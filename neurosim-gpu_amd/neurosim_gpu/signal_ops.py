@@ -16,9 +16,10 @@ float32 and each output is rounded once.
 
 All take and return the state that carries a signal on (``history``, ``state``), give
 native gradients of every tensor input (forward-mode derivatives are refused, and so is a
-backward under graph capture), and have a one-tick form that updates the carried state in place.  ``lengths`` gives columns their own
-number of ticks: past it outputs and gradients are zero, the carried state stays that of the
-column's last tick, and what the inputs hold there is never used.  The kernels are
+backward under graph capture), and have a one-tick form that updates the carried state in
+place.  ``lengths`` gives columns their own number of ticks: past it outputs and gradients are
+zero, the carried state stays that of the column's last tick, and what the inputs hold there
+is never used.  The kernels are
 csrc/conv.hip, scan.hip, scan_grad.hip, recur.hip and recur_grad.hip behind
 include/neurosim_hip_signal.h; calls run on the current stream, allocate their outputs and
 workspaces from torch, and never synchronise.
@@ -584,8 +585,8 @@ def gated_recurrence(x: torch.Tensor, forget: torch.Tensor, write: torch.Tensor,
     ``forget``, ``write`` and the optional output gate ``z`` are [T, B, N], as before their
     sigmoids and silu; ``rates`` [N] float32 is how fast a channel with an open gate forgets
     (positive; at a rate of 0 gradients leave out the input's part, which has no bound there,
-    and a negative rate counts as 0 and has a gradient of 0).  ``state`` [B, N] float32 is h before the first tick (zeros if
-    absent).
+    and a negative rate counts as 0 and has a gradient of 0).  ``state`` [B, N] float32 is h
+    before the first tick (zeros if absent).
 
     Returns ``(y, state)``: y [T, B, N] of x's type and h after each column's last tick.
     Calls may be captured into a graph, their backward may not (it raises)."""
